@@ -31,6 +31,9 @@ def main(argv: list[str] | None = None) -> int:
     ap.add_argument("--max-model-len", type=int, default=None, help="longest sequence (default: the model's positions)")
     ap.add_argument("--no-cuda-graph", action="store_true", help="run decode steps kernel by kernel instead of replaying recorded graphs")
     ap.add_argument("--temperature", type=float, default=0.0, help="0: greedy")
+    ap.add_argument("--top-k", type=int, default=0, help="draw from this many of the likeliest tokens (0: all)")
+    ap.add_argument("--top-p", type=float, default=1.0, help="draw from the likeliest tokens that make up this part of the probability")
+    ap.add_argument("--min-p", type=float, default=0.0, help="draw from tokens at least this many times as likely as the likeliest")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--ignore-eos", action="store_true")
     ap.add_argument("--prompt-ids", default=None, help="one prompt given on the command line instead of standard input")
@@ -49,7 +52,8 @@ def main(argv: list[str] | None = None) -> int:
         options.max_model_len = args.max_model_len
     engine = Engine(args.model, options=options)
     params = SamplingParams(max_new_tokens=args.max_new_tokens, temperature=args.temperature, seed=args.seed,
-                            ignore_eos=args.ignore_eos)
+                            ignore_eos=args.ignore_eos, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p)
+    params.validate()
 
     def run(ids: list[int]) -> None:
         def show(token: int, done: bool) -> None:

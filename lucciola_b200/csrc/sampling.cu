@@ -7,31 +7,9 @@
 // counter-based hash of (key of the request, index of the generated token, i),
 // so the token does not depend on what else is in the batch or on how the
 // prompt was cut.  T == 0 is greedy.
-#include "common.cuh"
+#include "sampling.cuh"
 
 namespace lb {
-
-__host__ __device__ __forceinline__ unsigned long long mix64(unsigned long long x) {
-  x ^= x >> 30; x *= 0xBF58476D1CE4E5B9ull;
-  x ^= x >> 27; x *= 0x94D049BB133111EBull;
-  x ^= x >> 31;
-  return x;
-}
-
-// The top 23 bits of a hash as a number strictly inside (0, 1): (b + 0.5) / 2^23.  b + 0.5 has at most 24
-// significant bits, so every value is exact in float32; the smallest is 2^-24 and the largest 1 - 2^-24.  (With
-// 24 bits the largest sum, 16777215.5, would round to 2^24 and give exactly 1, whose score is +infinity.)
-__host__ __device__ __forceinline__ float bits_to_uniform(unsigned int bits23) {
-  return ((float)bits23 + 0.5f) * (1.0f / 8388608.0f);
-}
-
-// Uniform in (0, 1) with 23 bits.
-__host__ __device__ __forceinline__ float hash_uniform(unsigned long long key, unsigned int counter,
-                                                       unsigned int i) {
-  unsigned long long x = mix64(key + 0x9E3779B97F4A7C15ull * (unsigned long long)(counter + 1u));
-  x = mix64(x ^ (0xD6E8FEB86659FD93ull * (unsigned long long)(i + 1u)));
-  return bits_to_uniform((unsigned int)(x >> 41));
-}
 
 __global__ void sample_kernel(int* __restrict__ tokens, const float* __restrict__ logits,
                               const float* __restrict__ temperature,
@@ -48,12 +26,13 @@ __global__ void sample_kernel(int* __restrict__ tokens, const float* __restrict_
   const float inv_t = greedy ? 1.f : 1.f / temp;
   const unsigned long long key = keys ? keys[r] : 0ull;
   const unsigned int counter = counters ? (unsigned int)counters[r] : 0u;
+  const unsigned long long hrow = hash_row(key, counter);
 
   float bv = -INFINITY;
   int bi = 0x7fffffff;
   for (int i = threadIdx.x; i < vocab; i += blockDim.x) {
     float s = row[i];
-    if (!greedy) s = s * inv_t - logf(-logf(hash_uniform(key, counter, (unsigned int)i)));
+    if (!greedy) s = gumbel_score(s, inv_t, bits_to_uniform(hash_bits(hrow, (unsigned int)i)));
     if (s > bv || (s == bv && i < bi)) { bv = s; bi = i; }
   }
   // A NaN never compares greater, so a row of NaNs yields index 0x7fffffff;

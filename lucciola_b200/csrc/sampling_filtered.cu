@@ -1,0 +1,567 @@
+// Sampling from what top-k, top-p and min-p leave of softmax(logits / T), over 32-bit logits [R, V].
+//
+// With M the row's largest logit, z_i = (logit_i - M) / T and w_i = exp(z_i), the row's tokens stand in the order of falling logits,
+// equal ones by index.  Of this order a row keeps the first top_k; of those the ones in front of which the sum of w is below
+// top_p times the sum of all top_k; of those the ones with w >= min_p; and always the first.  All three are prefixes of one order.
+// The token is the kept one with the largest z_i - log(-log(u_i)), u_i the samplers' hash (a draw from the kept ones' softmax).
+//
+// A row belongs to a cluster of CTAs, each with a slice of it in its shared memory: the logits are read once, and what the filters
+// need of the whole row (maximum, sums, borders) goes through distributed shared memory.  Two ways through a row:
+//   * top_k up to SF_SHORT: the k-th largest of the threads' own maxima bounds the k-th largest logit from below (found to within a
+//     bin of a histogram with one entry a thread); the few logits above it go to the cluster's first CTA, which ranks them and
+//     decides everything in 64 bits.
+//   * otherwise, without sorting: the best score among all tokens (of the first top_k, if there is a border to find by digits) is
+//     looked for first, and then whether its token is kept: one sum over the tokens in front of it.  If not, the same again among those;
+//     a drawn token is kept with probability top_p, so that this is rarely repeated more than once or twice.
+// A score needs a hash and two logarithms, so as few tokens as possible get that far: those whose weight is so small that the sum of
+// all not larger is below 1 - top_p, those below min_p, and those that cannot reach the bound below which the best score falls once
+// in 10^8 rows (log of the sum minus 3; such a row is done again without the bound) are left out by their logit alone, and of the
+// rest those whose 1 - u, a lower bound of -log u, is too large already.
+//
+// Which token comes out does not depend on the order of sums, and so not on the batch the row stands in: 32-bit scores and sums decide
+// only where they differ by more than they can be off by, and 64-bit scores and whole-number sums of 64 bits decide the rest.
+#include "sampling.cuh"
+
+#include <atomic>
+
+namespace lb {
+
+constexpr int SF_THREADS = 512;
+constexpr int SF_BINS = 256;
+constexpr int SF_SHORT = 256;            // most top_k of the short way
+constexpr int SF_LIST = 512;             // logits the first CTA ranks, one a thread
+constexpr int SF_MAX_CLUSTER = 8;
+constexpr int SF_SLICE_BYTES = 200 * 1024;     // most logits of a CTA; longer rows are read again where they lie
+constexpr float SF_SCORE_MARGIN = 1.f / 32768.f;     // 32-bit scores z + g lie in [-20, 20] and are off by less than 2^-17
+constexpr float SF_SUM_MARGIN = 1.f / 32768.f;       // 32-bit sums of w, relative: w within 2^-18 where it counts, four at a time in 32 bits
+constexpr float SF_BELOW = 60.f;                     // weights below e^-60 of the largest change no sum of 64 bits
+
+struct FilterParams {
+  int* tokens; const float* logits; const float* temperature; const unsigned long long* keys; const int* counters;
+  const int* top_k; const float* top_p; const float* min_p;
+  long long row_stride; int vocab;
+};
+
+__device__ __forceinline__ uint32_t sf_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t sf_size() { uint32_t r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void sf_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// In two parts, at the start: a peer's shared memory may be written when the peer has begun to run.
+__device__ __forceinline__ void sf_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void sf_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t sf_remote(const void* local, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void sf_st_remote(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ uint32_t sf_ld_remote(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t sf_add_remote(uint32_t addr, uint32_t v) {
+  uint32_t old;
+  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(v) : "memory");
+  return old;
+}
+
+// Values of up to SF_WORDS words a thread, reduced over the cluster; every thread gets the result.  Two sets of slots in turn: a CTA
+// writes a set again only after a barrier that its peers reach when they have read it.
+constexpr int SF_WORDS = 6;
+struct FilterShared {
+  uint32_t warp_part[SF_THREADS / 32][SF_WORDS];
+  uint32_t slot[2][SF_MAX_CLUSTER][SF_WORDS];
+  uint32_t hist[2][SF_BINS];
+  uint32_t scan[SF_THREADS / 32];
+  uint32_t list_n, digit, digit_before;
+  float list_l[SF_LIST]; int list_i[SF_LIST];
+  float rank_l[SF_LIST]; int rank_i[SF_LIST];
+  double warp_sum[SF_THREADS / 32];
+};
+
+struct FilterGroup {                     // what a thread knows of its cluster
+  FilterShared* sh;
+  uint32_t rank, size;
+  int turn;
+};
+
+template <typename T, typename F>
+__device__ __forceinline__ T sf_reduce(FilterGroup& g, T v, F join) {
+  static_assert(sizeof(T) % 4 == 0 && sizeof(T) / 4 <= SF_WORDS, "words of a slot");
+  constexpr int W = sizeof(T) / 4;
+  union U { T t; uint32_t w[W]; __device__ U() {} };
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    U a, b;
+    a.t = v;
+#pragma unroll
+    for (int i = 0; i < W; ++i) b.w[i] = __shfl_xor_sync(0xffffffffu, a.w[i], o);
+    v = join(v, b.t);
+  }
+  if (lane == 0) {
+    U a;
+    a.t = v;
+#pragma unroll
+    for (int i = 0; i < W; ++i) g.sh->warp_part[warp][i] = a.w[i];
+  }
+  __syncthreads();
+  uint32_t (*slot)[SF_WORDS] = g.sh->slot[g.turn & 1];
+  ++g.turn;
+  if (warp == 0) {
+    U a;
+#pragma unroll
+    for (int i = 0; i < W; ++i) a.w[i] = g.sh->warp_part[lane & (SF_THREADS / 32 - 1)][i];
+    v = a.t;
+#pragma unroll
+    for (int o = SF_THREADS / 64; o > 0; o >>= 1) {
+      U b;
+      a.t = v;
+#pragma unroll
+      for (int i = 0; i < W; ++i) b.w[i] = __shfl_xor_sync(0xffffffffu, a.w[i], o);
+      v = join(v, b.t);
+    }
+    if (lane < g.size) {
+      a.t = v;
+#pragma unroll
+      for (int i = 0; i < W; ++i) sf_st_remote(sf_remote(&slot[g.rank][i], lane), a.w[i]);
+    }
+  }
+  sf_cluster_sync();
+  U a;
+#pragma unroll
+  for (int i = 0; i < W; ++i) a.w[i] = slot[0][i];
+  T out = a.t;
+  for (uint32_t c = 1; c < g.size; ++c) {
+    U b;
+#pragma unroll
+    for (int i = 0; i < W; ++i) b.w[i] = slot[c][i];
+    out = join(out, b.t);
+  }
+  return out;
+}
+
+// A histogram of the CTA's threads becomes the cluster's, and the first bin with `want` entries in it or in front of it is found:
+// returns that bin (SF_BINS if there are not that many) and how many entries lie in front of it.  `hist` is this CTA's; complete when
+// every thread has arrived here.
+__device__ __forceinline__ int sf_find_bin(FilterGroup& g, uint32_t* hist, uint32_t want, uint32_t& before) {
+  sf_cluster_sync();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t n = 0;
+  if (tid < SF_BINS)
+    for (uint32_t c = 0; c < g.size; ++c) n += sf_ld_remote(sf_remote(hist + tid, c));
+  uint32_t s = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t t = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += t;
+  }
+  if (lane == 31) g.sh->scan[warp] = s;
+  if (tid == 0) { g.sh->digit = SF_BINS; g.sh->digit_before = 0; }
+  __syncthreads();
+  if (tid < SF_BINS) {
+    for (int w = 0; w < warp; ++w) s += g.sh->scan[w];
+    if (s >= want && s - n < want) { g.sh->digit = tid; g.sh->digit_before = s - n; }
+    if (tid == SF_BINS - 1 && s < want) g.sh->digit_before = s;
+  }
+  __syncthreads();
+  before = g.sh->digit_before;
+  return (int)g.sh->digit;
+}
+
+// Whole numbers in the order of the logits.
+__device__ __forceinline__ uint32_t sf_key(float l) {
+  const uint32_t b = __float_as_uint(l + 0.f);            // -0 as 0: they are equal
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float sf_unkey(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
+// The first of the order's places that are not kept any more; a token is in front of it if its logit is larger, or equal at a smaller index.
+struct Border { float l; int i; };
+__device__ __forceinline__ bool in_front(float l, int i, const Border& b) { return l > b.l || (l == b.l && i < b.i); }
+
+struct Best { float s; int i; float l; float second; };      // best score, its token and logit; the best score of any other token
+struct Best64 { double s; int i; float l; };
+
+template <bool IN_SMEM>
+__global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(FilterParams p) {
+  extern __shared__ __align__(16) float data[];
+  __shared__ FilterShared sh;
+  pdl_trigger();
+  FilterGroup g{&sh, sf_rank(), sf_size(), 0};
+  const int tid = threadIdx.x;
+  const int row = blockIdx.x / g.size;
+  for (int b = tid; b < 2 * SF_BINS; b += SF_THREADS) sh.hist[0][b] = 0;
+  if (tid == 0) sh.list_n = 0;
+  sf_cluster_arrive();
+  pdl_wait(p.logits, p.temperature, p.keys, p.counters, p.top_k, p.top_p, p.min_p);
+
+  // ---- the slice: whole 16-byte words of memory, the first and the last of a row partly filled ----------------------------------
+  const float* row_ptr = p.logits + (long long)row * p.row_stride;
+  const int skew = (int)(((uintptr_t)row_ptr >> 2) & 3);       // the row's first logit is the skew-th of its 16-byte word
+  const float* base = row_ptr - skew;
+  const int words = (p.vocab + skew + 3) >> 2;
+  const int per = (words + (int)g.size - 1) / (int)g.size;
+  const int first = min(words, (int)g.rank * per), nq = min(words, first + per) - first;
+  // word q of the slice from memory; places outside the row are not there (-inf)
+  auto fetch = [&](int q) -> float4 {
+    const int v = 4 * (first + q) - skew;
+    if (v >= 0 && v + 4 <= p.vocab) return __ldcg(reinterpret_cast<const float4*>(base) + first + q);
+    float x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = (v + e >= 0 && v + e < p.vocab) ? __ldcg(row_ptr + v + e) : -INFINITY;
+    return make_float4(x[0], x[1], x[2], x[3]);
+  };
+  auto clean = [](float4 x) {                                  // NaN is as -inf
+    x.x = fmaxf(x.x, -INFINITY); x.y = fmaxf(x.y, -INFINITY); x.z = fmaxf(x.z, -INFINITY); x.w = fmaxf(x.w, -INFINITY);
+    return x;
+  };
+  float4* data4 = reinterpret_cast<float4*>(data);
+  auto word = [&](int q) -> float4 { return IN_SMEM ? data4[q] : clean(fetch(q)); };
+  auto index_of = [&](int q, int e) { return 4 * (first + q) - skew + e; };
+
+  // ---- largest logit ---------------------------------------------------------------------------------------------------------------
+  float mine = -INFINITY;
+  for (int q = tid; q < nq; q += SF_THREADS) {
+    const float4 x = clean(fetch(q));
+    if (IN_SMEM) data4[q] = x;
+    mine = fmaxf(fmaxf(mine, fmaxf(x.x, x.y)), fmaxf(x.z, x.w));
+  }
+  sf_cluster_wait();
+  struct Most { float m, least; };                             // the largest, and the smallest of the threads' largest
+  const Most most = sf_reduce(g, Most{mine, mine > -INFINITY ? mine : INFINITY},
+                              [](Most a, Most b) { return Most{fmaxf(a.m, b.m), fminf(a.least, b.least)}; });
+  const float M = most.m;
+  const float temp = p.temperature ? p.temperature[row] : 0.f;
+  const int k_asked = p.top_k ? p.top_k[row] : 0;
+  const float top_p = p.top_p ? p.top_p[row] : 1.f, min_p = p.min_p ? p.min_p[row] : 0.f;
+  const bool by_k = k_asked > 0 && k_asked < p.vocab, by_p = top_p < 1.f, by_m = min_p > 0.f;
+  auto finish = [&](int token) { if (g.rank == 0 && tid == 0) p.tokens[row] = token; };
+
+  if (!(M > -INFINITY)) { finish(0); return; }
+  if (!(temp > 0.f) || M == INFINITY) {
+    int at = 0x7fffffff;
+    for (int q = tid; q < nq; q += SF_THREADS) {
+      const float4 x = word(q);
+      const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 3; e >= 0; --e) if (v[e] == M) at = min(at, index_of(q, e));
+    }
+    at = sf_reduce(g, at, [](int a, int b) { return min(a, b); });
+    finish(at);
+    return;
+  }
+  const unsigned long long hrow = hash_row(p.keys ? p.keys[row] : 0ull, p.counters ? (unsigned int)p.counters[row] : 0u);
+  if (!by_k && !by_p && !by_m) {
+    // no filter: what sample_kernel computes, so that a row's token does not change with the other rows' filters
+    const float inv = 1.f / temp;
+    struct Plain { float s; int i; };
+    Plain b{-INFINITY, 0x7fffffff};
+    for (int q = tid; q < nq; q += SF_THREADS) {
+      const float4 x = word(q);
+      const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = index_of(q, e);
+        if (!(v[e] > -INFINITY)) continue;
+        const float s = gumbel_score(v[e], inv, bits_to_uniform(hash_bits(hrow, (unsigned int)i)));
+        if (s > b.s || (s == b.s && i < b.i)) b = Plain{s, i};
+      }
+    }
+    b = sf_reduce(g, b, [](Plain a, Plain c) { return (c.s > a.s || (c.s == a.s && c.i < a.i)) ? c : a; });
+    finish(b.i == 0x7fffffff ? 0 : b.i);
+    return;
+  }
+  const double t64 = (double)fminf(temp, 1e30f);
+  const float inv_t = (float)fmin(1.0 / t64, 3e38);            // (M - M) / T stays 0 and -inf / T -inf
+  const float k2 = (float)fmin(1.4426950408889634 / t64, 3e38);
+  auto z64 = [&](float l) { return ((double)l - (double)M) / t64; };
+  auto score64 = [&](float l, int i) {
+    return z64(l) - log(-log(((double)hash_bits(hrow, (unsigned int)i) + 0.5) / 8388608.0));
+  };
+
+  // ---- the short way -------------------------------------------------------------------------------------------------------------------
+  if (by_k && k_asked <= SF_SHORT) {
+    const float low = M - SF_BELOW * fminf(temp, 1e30f), least = fmaxf(most.least, low);
+    const float scale = fminf(0.999f * SF_BINS / (M - least), 1e37f);          // (0 times it is 0)
+    auto place = [&](float l) { return l > -INFINITY ? (M - l) * scale : INFINITY; };      // grows as the logit falls
+    const float at = place(mine);
+    if (at < (float)SF_BINS) atomicAdd(&sh.hist[0][(int)at], 1u);
+    uint32_t before;
+    const int bin = sf_find_bin(g, sh.hist[0], (uint32_t)k_asked, before);
+    // the logits at least as large as the k-th largest of the threads' largest, or, with fewer threads than that, all that weigh anything
+    auto wanted = [&](float l) { return bin < SF_BINS ? place(l) < (float)(bin + 1) : l >= low; };
+    if (wanted(mine)) {                                            // a thread whose largest is behind the end has nothing to send
+      const uint32_t n_addr = sf_remote(&sh.list_n, 0);
+      for (int q = tid; q < nq; q += SF_THREADS) {
+        const float4 x = word(q);
+        const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (wanted(v[e])) {
+            const uint32_t n = sf_add_remote(n_addr, 1u);
+            if (n < SF_LIST) {
+              sf_st_remote(sf_remote(&sh.list_l[n], 0), __float_as_uint(v[e]));
+              sf_st_remote(sf_remote(&sh.list_i[n], 0), (uint32_t)index_of(q, e));
+            }
+          }
+      }
+    }
+    sf_cluster_sync();
+    const uint32_t sent = sf_ld_remote(sf_remote(&sh.list_n, 0));
+    sf_cluster_sync();                                         // nobody reads the first CTA's memory any more
+    if (sent <= SF_LIST) {
+      if (g.rank != 0) return;
+      const int n = (int)sent, kept = min(n, k_asked);
+      if (tid < n) {
+        const float l = sh.list_l[tid];
+        const int i = sh.list_i[tid];
+        int r = 0;
+        for (int j = 0; j < n; ++j) r += in_front(sh.list_l[j], sh.list_i[j], Border{l, i}) ? 1 : 0;
+        sh.rank_l[r] = l;
+        sh.rank_i[r] = i;
+      }
+      __syncthreads();
+      const int lane = tid & 31, warp = tid >> 5;
+      const float l = tid < kept ? sh.rank_l[tid] : 0.f;
+      const int i = tid < kept ? sh.rank_i[tid] : 0x7fffffff;
+      const double w = tid < kept ? exp(z64(l)) : 0.0;
+      double s = w;                                            // sum of w up to and with this place
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double t = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += t;
+      }
+      if (lane == 31) sh.warp_sum[warp] = s;
+      __syncthreads();
+      double total = 0.0;
+      for (int c = 0; c < SF_THREADS / 32; ++c) {
+        if (c == warp) s += total;
+        total += sh.warp_sum[c];
+      }
+      const bool in = tid == 0 || (tid < kept && (!by_p || s - w < (double)top_p * total) && (!by_m || w >= (double)min_p));
+      Best64 b{in ? score64(l, i) : -INFINITY, i, l};
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        Best64 c{__shfl_xor_sync(0xffffffffu, b.s, o), __shfl_xor_sync(0xffffffffu, b.i, o), 0.f};
+        if (c.s > b.s || (c.s == b.s && c.i < b.i)) b = c;
+      }
+      __syncthreads();
+      if (lane == 0) { sh.warp_sum[warp] = b.s; sh.scan[warp] = (uint32_t)b.i; }
+      __syncthreads();
+      if (tid == 0) {
+        for (int c = 1; c < SF_THREADS / 32; ++c) {
+          const double cs = sh.warp_sum[c];
+          const int ci = (int)sh.scan[c];
+          if (cs > b.s || (cs == b.s && ci < b.i)) { b.s = cs; b.i = ci; }
+        }
+        p.tokens[row] = b.i;
+      }
+      return;
+    }
+  }
+
+  // ---- the border of a large top_k, digit by digit: of the logits, then of the index among equal ones ---------------------------------------
+  Border border{-INFINITY, 0};                                 // every token that is there lies in front of it
+  if (by_k) {
+    uint32_t want = (uint32_t)k_asked, key = 0, index = 0;
+    int turn = 0;
+    bool all = false, ties = false;
+    for (int digit = 0; digit < 7 && !all; ++digit) {          // four of the logit, three of the index
+      uint32_t* hist = sh.hist[turn & 1];
+      ++turn;
+      __syncthreads();
+      for (int b = tid; b < SF_BINS; b += SF_THREADS) hist[b] = 0;
+      __syncthreads();
+      const int shift = digit < 4 ? 24 - 8 * digit : 16 - 8 * (digit - 4);
+      for (int q = tid; q < nq; q += SF_THREADS) {
+        const float4 x = word(q);
+        const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (!(v[e] > -INFINITY)) continue;
+          const uint32_t kk = sf_key(v[e]), ii = (uint32_t)index_of(q, e);
+          if (digit < 4) {
+            if (digit == 0 || (kk >> (shift + 8)) == (key >> (shift + 8))) atomicAdd(&hist[255 - ((kk >> shift) & 255)], 1u);
+          } else if (kk == key && (ii >> (shift + 8)) == (index >> (shift + 8))) {
+            atomicAdd(&hist[(ii >> shift) & 255], 1u);
+          }
+        }
+      }
+      uint32_t before;
+      const int bin = sf_find_bin(g, hist, want, before);
+      if (bin == SF_BINS) { all = true; break; }               // fewer tokens than top_k (first digit only)
+      want -= before;
+      if (digit < 4) key |= (uint32_t)(255 - bin) << shift;
+      else index |= (uint32_t)bin << shift;
+      ties = digit >= 4;
+    }
+    if (!all) border = Border{sf_unkey(key), ties ? (int)index + 1 : 0x7fffffff};
+  }
+
+  // ---- rejection ---------------------------------------------------------------------------------------------------------------------------------
+  auto weight = [&](float l) { return exp2_approx((l - M) * k2); };
+  // the sum of the weights in front of a border, and how many there are
+  struct Sum { double s; int n; int pad; };
+  auto sum_in_front = [&](const Border& b) {
+    double s = 0.0;
+    int n = 0;
+    for (int q = tid; q < nq; q += SF_THREADS) {
+      const float4 x = word(q);
+      const float v[4] = {x.x, x.y, x.z, x.w};
+      if (fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)) < b.l) continue;
+      float w4 = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (in_front(v[e], index_of(q, e), b)) { w4 += weight(v[e]); ++n; }
+      s += (double)w4;
+    }
+    return sf_reduce(g, Sum{s, n, 0}, [](Sum a, Sum c) { return Sum{a.s + c.s, a.n + c.n, 0}; });
+  };
+  // the same of two borders in whole numbers, for what the above cannot tell: units of 2^-unit, the sum of a row below 2^63
+  struct Sum64 { unsigned long long inner, outer; };
+  auto sums64 = [&](const Border& inner, const Border& outer) {
+    const double one = ldexp(1.0, 62 - (32 - __clz(p.vocab)));
+    Sum64 s{0ull, 0ull};
+    for (int q = tid; q < nq; q += SF_THREADS) {
+      const float4 x = word(q);
+      const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll 1
+      for (int e = 0; e < 4; ++e) {
+        if (!(v[e] > -INFINITY) || !in_front(v[e], index_of(q, e), outer)) continue;
+        const unsigned long long w = __double2ull_rn(exp(z64(v[e])) * one);
+        s.outer += w;
+        if (in_front(v[e], index_of(q, e), inner)) s.inner += w;
+      }
+    }
+    return sf_reduce(g, s, [](Sum64 a, Sum64 c) { return Sum64{a.inner + c.inner, a.outer + c.outer}; });
+  };
+
+  const Border whole = border;                                 // of all that top_k leaves
+  const double total = sum_in_front(whole).s;
+  double sum = total;                                          // of what is in front of `border`
+  for (;;) {
+    Best best{-INFINITY, 0x7fffffff, 0.f, -INFINITY};
+    const float log_sum = (float)log(sum);
+    for (int bounded = 1; bounded >= 0 && best.i == 0x7fffffff; --bounded) {
+      // the smallest z that may be drawn: of min-p, of top-p, and of what can reach the bound (-log(-log u) is at most 16.64)
+      float zc = -INFINITY;
+      if (by_m) zc = fmaxf(zc, logf(min_p) - 1e-4f);
+      if (by_p) zc = fmaxf(zc, logf(fmaxf((1.f - top_p) / (float)p.vocab, 1e-37f)) + (float)log(total) - 1e-2f);
+      const float bound = log_sum - 3.f;
+      if (bounded) zc = fmaxf(zc, bound - 16.7f);
+      zc = fminf(zc, 0.f);                                     // the first is always kept
+      const float l_cut = M + zc * fminf(temp, 1e30f) - 1e-5f * fabsf(M);
+      const float reach = bounded ? exp2f(-bound * 1.4426951f) * 1.01f : INFINITY;       // -log u < w e^-bound for a score above the bound
+      for (int q = tid; q < nq; q += SF_THREADS) {
+        const float4 x = word(q);
+        const float v[4] = {x.x, x.y, x.z, x.w};
+        const float cut = fmaxf(l_cut, border.l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (!(v[e] >= cut) || !(v[e] > -INFINITY)) continue;
+          const int i = index_of(q, e);
+          if (!in_front(v[e], i, border)) continue;
+          const float u = bits_to_uniform(hash_bits(hrow, (unsigned int)i));
+          if ((1.f - u) > weight(v[e]) * reach) continue;
+          const float s = (v[e] - M) * inv_t - logf(-logf(u));
+          if (s > best.s || (s == best.s && i < best.i)) { best.second = fmaxf(best.second, best.s); best.s = s; best.i = i; best.l = v[e]; }
+          else best.second = fmaxf(best.second, s);
+        }
+      }
+      auto better = [](Best a, Best c) {
+        const bool swap = c.s > a.s || (c.s == a.s && c.i < a.i);
+        const float second = fmaxf(fmaxf(a.second, c.second), fminf(a.s, c.s));
+        return swap ? Best{c.s, c.i, c.l, second} : Best{a.s, a.i, a.l, second};
+      };
+      best = sf_reduce(g, best, better);
+      if (bounded && !(best.s >= bound)) best.i = 0x7fffffff;          // what was left out may be better
+      if (best.i != 0x7fffffff && best.second > best.s - SF_SCORE_MARGIN) {
+        // two scores too near to tell apart: in 64 bits, all that come near the best
+        const float near = best.s - SF_SCORE_MARGIN;
+        Best64 b{-INFINITY, 0x7fffffff, 0.f};
+        for (int q = tid; q < nq; q += SF_THREADS) {
+          const float4 x = word(q);
+          const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll 1
+          for (int e = 0; e < 4; ++e) {
+            const int i = index_of(q, e);
+            if (!(v[e] >= l_cut) || !(v[e] > -INFINITY) || !in_front(v[e], i, border)) continue;
+            const float u = bits_to_uniform(hash_bits(hrow, (unsigned int)i));
+            if ((v[e] - M) * inv_t - logf(-logf(u)) < near) continue;
+            const double s = score64(v[e], i);
+            if (s > b.s || (s == b.s && i < b.i)) b = Best64{s, i, v[e]};
+          }
+        }
+        b = sf_reduce(g, b, [](Best64 a, Best64 c) { return (c.s > a.s || (c.s == a.s && c.i < a.i)) ? c : a; });
+        best.i = b.i;
+        best.l = b.l;
+      }
+    }
+    const Border at{best.l, best.i};
+    bool kept = !by_m || exp(z64(best.l)) >= (double)min_p;
+    const Sum before = by_p || !kept ? sum_in_front(at) : Sum{0.0, 1, 0};
+    if (by_p && kept) {
+      const double room = (double)top_p * total, off = SF_SUM_MARGIN * total;
+      if (fabs(before.s - room) > off) {
+        kept = before.s < room;
+      } else {
+        const Sum64 s = sums64(at, whole);
+        kept = (double)s.inner < (double)top_p * (double)s.outer;
+      }
+    }
+    if (kept || before.n == 0) { finish(best.i); return; }
+    border = at;
+    sum = before.s;
+  }
+}
+
+template <bool IN_SMEM>
+static cudaError_t sf_launch(const FilterParams& p, int rows, int cluster, size_t smem, cudaStream_t stream) {
+  if (IN_SMEM) {
+    static std::atomic<unsigned long long> configured{0ull};   // a bit a device
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    if (!(configured.load() >> (device & 63) & 1ull)) {
+      e = cudaFuncSetAttribute(sample_filtered_kernel<IN_SMEM>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_SLICE_BYTES);
+      if (e != cudaSuccess) return e;
+      configured.fetch_or(1ull << (device & 63));
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)rows * cluster); cfg.blockDim = dim3(SF_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = g_pdl_enabled ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, sample_filtered_kernel<IN_SMEM>, p);
+}
+
+}  // namespace lb
+
+// tokens[r] = the token drawn for logits[r * row_stride .. + vocab); see the head of this file.  temperature (none: greedy), keys,
+// counters, top_k (<= 0 or >= vocab: all), top_p (>= 1: all), min_p (<= 0: all): one a row, each may be null.
+LB_EXPORT int lb_sample_filtered(int* tokens, const float* logits, long long row_stride, const float* temperature,
+                                 const unsigned long long* keys, const int* counters, const int* top_k, const float* top_p,
+                                 const float* min_p, int num_rows, int vocab, cudaStream_t stream) {
+  LB_CHECK_ARG(num_rows >= 0 && vocab > 0 && vocab < (1 << 24) && row_stride >= vocab, "sample_filtered: bad sizes rows=%d vocab=%d (at most %d) row stride=%lld",
+               num_rows, vocab, (1 << 24) - 1, row_stride);
+  if (num_rows == 0) return 0;
+  LB_CHECK_ARG(num_rows <= (1 << 24), "sample_filtered: %d rows, at most %d a launch", num_rows, 1 << 24);
+  const lb::FilterParams p{tokens, logits, temperature, keys, counters, top_k, top_p, min_p, row_stride, vocab};
+  const int words = (vocab + 3 + 3) / 4;
+  int cluster = 1;
+  while (cluster < lb::SF_MAX_CLUSTER && words / cluster > lb::SF_THREADS) cluster *= 2;
+  const size_t smem = (size_t)((words + cluster - 1) / cluster) * 16;
+  const bool fits = smem <= lb::SF_SLICE_BYTES;
+  const cudaError_t e = fits ? lb::sf_launch<true>(p, num_rows, cluster, smem, stream) : lb::sf_launch<false>(p, num_rows, cluster, 0, stream);
+  if (e != cudaSuccess) { lb::set_error("sample_filtered: launch failed: %s", cudaGetErrorString(e)); return 2; }
+  lb::count_launch();
+  return 0;
+}

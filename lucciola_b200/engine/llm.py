@@ -205,10 +205,10 @@ class AsyncEngine:
 
     def generate_async(self, prompt: Sequence[int], max_new_tokens: int,
                        callback: Optional[Callable[[int, bool], None]] = None, temperature: float = 0.0,
-                       seed: int = 0, ignore_eos: bool = False) -> int:
+                       seed: int = 0, ignore_eos: bool = False, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0) -> int:
         """lucciola's call: submit with the sampling parameters spelled out."""
         return self.submit(prompt, SamplingParams(max_new_tokens=max_new_tokens, temperature=temperature, seed=seed,
-                                                  ignore_eos=ignore_eos), callback)
+                                                  ignore_eos=ignore_eos, top_k=top_k, top_p=top_p, min_p=min_p), callback)
 
     def abort(self, rid: int) -> None:
         """Give request `rid` up.  Takes effect between two steps of the engine: what the request holds goes back

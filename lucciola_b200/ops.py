@@ -135,6 +135,7 @@ _SIGNATURES = {
     "lb_expert_tile_rows": [c_int] * 1,
     "lb_latent_flash_ok": [c_int] * 4,
     "lb_sample": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
+    "lb_sample_filtered": [c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
 }
 
 _fn_cache: dict[str, object] = {}
@@ -212,6 +213,12 @@ def _check(t: torch.Tensor, what: str, dtype: torch.dtype | None = None) -> None
         raise KernelError(f"{what} must be contiguous")
     if dtype is not None and t.dtype != dtype:
         raise KernelError(f"{what} must be {dtype}, is {t.dtype}")
+
+
+def _on_current_device(t: torch.Tensor) -> None:
+    """The library launches on the current device: a stream and pointers of another one are refused."""
+    if t.device.index != torch.cuda.current_device():
+        raise KernelError(f"tensors on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
 def current_stream() -> int:
@@ -974,14 +981,40 @@ def gemm_plain(y: torch.Tensor, x: torch.Tensor, w: torch.Tensor, stream: int, p
 
 
 def sample(tokens: torch.Tensor, logits: torch.Tensor, stream: int, temperature: torch.Tensor | None = None,
-           keys: torch.Tensor | None = None, counters: torch.Tensor | None = None) -> None:
-    """tokens[r] = greedy or temperature sample of logits[r, :]; see sampling/sampler.py for the key."""
-    _check(tokens, "token output", torch.int32); _check(logits, "logits", torch.float32)
-    if temperature is not None:
-        _check(temperature, "temperature", torch.float32); _check(keys, "keys", torch.int64)
-        _check(counters, "counters", torch.int32)
+           keys: torch.Tensor | None = None, counters: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
+           top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None) -> None:
+    """tokens[r] = greedy or temperature sample of logits[r, :]; see sampling/sampler.py for the key.
+
+    With any of `top_k` (int32 [R]; 0: all), `top_p` (float32 [R]; 1: all) and `min_p` (float32 [R]; 0: all) a row draws from what
+    they leave: in the order of falling logits (equal ones by index) the first top_k; of those the ones with less than top_p of their
+    whole probability in front of them; of those the ones at least min_p times as likely as the first; the first always.  A row whose
+    filters leave all draws the token it draws without them, and a row with temperature 0 is greedy.  NaN is as -infinity.  The
+    logits' rows may be a column range of wider ones then, and no longer than 2^24 - 1."""
+    if top_k is None and top_p is None and min_p is None:
+        _check(tokens, "token output", torch.int32); _check(logits, "logits", torch.float32)
+        if temperature is not None:
+            _check(temperature, "temperature", torch.float32); _check(keys, "keys", torch.int64)
+            _check(counters, "counters", torch.int32)
+        R, V = logits.shape
+        _call("lb_sample", tokens.data_ptr(), logits.data_ptr(), _ptr(temperature), _ptr(keys), _ptr(counters), R, V, stream)
+        return
+    if not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise KernelError("logits must be float32 rows on the GPU with unit column stride")
     R, V = logits.shape
-    _call("lb_sample", tokens.data_ptr(), logits.data_ptr(), _ptr(temperature), _ptr(keys), _ptr(counters), R, V, stream)
+    if temperature is not None and (keys is None or counters is None):
+        raise KernelError("a draw with temperature needs keys and counters")
+    for t, what, dtype in ((tokens, "token output", torch.int32), (temperature, "temperature", torch.float32), (keys, "keys", torch.int64),
+                           (counters, "counters", torch.int32), (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
+                           (min_p, "min_p", torch.float32)):
+        if t is not None:
+            _check(t, what, dtype)
+            if t.shape != (R,):
+                raise KernelError(f"{what} must be one number a row of {R}, is {tuple(t.shape)}")
+            if t.device != logits.device:
+                raise KernelError(f"{what} is on {t.device}, the logits on {logits.device}")
+    _on_current_device(logits)
+    _call("lb_sample_filtered", tokens.data_ptr(), logits.data_ptr(), logits.stride(0) if R > 1 else max(V, 1), _ptr(temperature), _ptr(keys),
+          _ptr(counters), _ptr(top_k), _ptr(top_p), _ptr(min_p), R, V, stream)
 
 
 _WORKSPACE_ELEMS = 16 * 1024 * 1024      # float32 partials of split products (64 MB)

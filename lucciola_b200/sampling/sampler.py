@@ -3,7 +3,9 @@
 Greedy takes the largest logit, the lowest index among equals.  With a temperature T > 0 the token
 is argmax_i(logit_i / T - log(-log(u_i))) (Gumbel-max: a draw from softmax(logits / T)), where u_i
 is a hash of (key of the request's seed, index of the generated token, i).  The draw therefore
-depends on the request alone, not on the batch it shares a step with."""
+depends on the request alone, not on the batch it shares a step with.  A request's filters (top_k, top_p,
+min_p) leave the argmax fewer tokens; steps in which some request has any run the sampler that knows them,
+in which a request without filters draws the same token as in the other."""
 from __future__ import annotations
 
 from typing import Sequence
@@ -49,6 +51,8 @@ class Sampler:
         stream = torch.cuda.current_stream(self.device).cuda_stream
         if all(p.temperature <= 0 for p in params):
             ops.sample(tokens, logits, stream)
+        elif any(p.filtered for p in params):
+            ops.sample(tokens, logits, stream, *self._filters(params, generated))
         else:
             temps = torch.tensor([p.temperature for p in params], dtype=torch.float32).to(self.device, non_blocking=True)
             keys = np.array([sampling_key(p.seed) for p in params], dtype=np.uint64).view(np.int64)
@@ -62,6 +66,18 @@ class Sampler:
         self._host[:R].copy_(tokens, non_blocking=True)
         self._done.record()
         return R
+
+    def _filters(self, params: Sequence[SamplingParams], generated: Sequence[int]) -> list[torch.Tensor]:
+        """What the filtering sampler takes, in one copy: temperatures, keys, counters, top_k, top_p, min_p."""
+        R = len(params)
+        host = np.empty((7, R), dtype=np.int32)                     # the keys are the first two rows
+        f32 = host.view(np.float32)
+        host[:2].reshape(-1).view(np.uint64)[:] = [sampling_key(p.seed) for p in params]
+        f32[2], host[3], host[4] = [p.temperature for p in params], list(generated), [p.top_k for p in params]
+        f32[5], f32[6] = [p.top_p for p in params], [p.min_p for p in params]
+        dev = torch.from_numpy(host).to(self.device, non_blocking=True)
+        keys = dev[:2].reshape(-1).view(torch.int64)
+        return [dev[2].view(torch.float32), keys, dev[3], dev[4], dev[5].view(torch.float32), dev[6].view(torch.float32)]
 
     def collect(self, handle) -> list[int]:
         if self._done is None:

@@ -1,0 +1,259 @@
+// Attention of a step whose requests share prefixes, on the ordinary pipes: 32-bit queries, keys and values, and bfloat16 ones that the
+// tensor-core kernel does not take.  The plan, the walk and the combination are attention_shared.cuh's.
+//
+// A tile has up to 32 query rows (tokens x heads of a kv head's group; a group of more heads is cut into equal parts that read the same
+// cached head).  Queries, a block of 64 keys and its values lie in shared memory as 32-bit numbers.  256 threads: thread (ty, tx) has
+// rows 2 ty and 2 ty + 1; of the scores the keys tx, tx + 16, tx + 32, tx + 48, of the result the dimensions 4 tx + 64 c .. + 3.  Sixteen
+// threads share a row: its maximum and sum are four shuffles.
+#include "attention_shared.cuh"
+
+#include <atomic>
+
+namespace lb {
+
+constexpr int AP_THREADS = 256;
+constexpr int AP_ROWS = 32;
+
+__device__ __forceinline__ float4 ap_load4(const float* p) { return __ldcg(reinterpret_cast<const float4*>(p)); }
+__device__ __forceinline__ float4 ap_load4(const bf16* p) {
+  const uint2 w = __ldcg(reinterpret_cast<const uint2*>(p));
+  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// floats of dynamic shared memory: queries, keys (rows four further apart, so that the keys of eight threads fall into different banks),
+// values, weights; then the page of every key of the block
+template <int D> constexpr int ap_smem_bytes() { return (AP_ROWS * D + AS_KEYS * (D + 4) + AS_KEYS * D + AP_ROWS * (AS_KEYS + 4) + AS_KEYS) * 4; }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(AP_THREADS) attention_shared_plain_kernel(SharedParams p) {
+  extern __shared__ __align__(16) float ap_smem[];
+  __shared__ SharedPlan plan;
+  float* qs = ap_smem;
+  float* ks = qs + AP_ROWS * D;
+  float* vs = ks + AS_KEYS * (D + 4);
+  float* ps = vs + AS_KEYS * D;
+  int* page = reinterpret_cast<int*>(ps + AP_ROWS * (AS_KEYS + 4));      // offset of each key's row in the pool's page units, -1: not there
+  pdl_trigger();
+  pdl_wait();
+  as_make_plan(p, plan, gridDim.x);
+  as_write_records(p, plan, blockIdx.x, gridDim.x);
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const T* q = reinterpret_cast<const T*>(p.q);
+  const T* kc = reinterpret_cast<const T*>(p.k_cache);
+  const T* vc = reinterpret_cast<const T*>(p.v_cache);
+  const int d = p.dim, G = p.group, cache_heads = p.kv_heads / p.kv_share;
+  long long x = (long long)blockIdx.x * plan.span;
+  const long long x_end = min(x + plan.span, (long long)plan.units * p.kv_heads);
+  while (x < x_end) {
+    const Segment g = as_next(p, plan, blockIdx.x, x, x_end);
+    if (g.blocks == 0) continue;
+    const int rows = g.tokens * G;
+    __syncthreads();
+    for (int i = tid; i < AP_ROWS * (D / 4); i += AP_THREADS) {
+      const int r = i / (D / 4), c = i % (D / 4) * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < rows && c < d) {
+        int token, position;
+        as_token(plan, g, r / G, token, position);
+        v = ap_load4(q + ((size_t)token * p.heads + g.kv_head * G + r % G) * d + c);
+      }
+      *reinterpret_cast<float4*>(qs + r * D + c) = v;
+    }
+    int last[2];                         // the last key each row sees
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      int token;
+      last[e] = -1;
+      if (2 * ty + e < rows) as_token(plan, g, (2 * ty + e) / G, token, last[e]);
+    }
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float o[2][D / 64][4];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) o[e][c][0] = o[e][c][1] = o[e][c][2] = o[e][c][3] = 0.f;
+    const int* bt = p.table + (size_t)g.table_row * p.max_pages;
+    for (int b = g.block; b < g.block + g.blocks; ++b) {
+      const int k0 = (g.key_lo & ~(AS_KEYS - 1)) + b * AS_KEYS;
+      __syncthreads();                   // the block before has been read
+      if (tid < AS_KEYS) {
+        const int key = k0 + tid;
+        int at = -1;
+        if (key >= g.key_lo && key < g.key_hi) {
+          const int pi = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+          at = bt[pi];
+          if (at >= p.num_pages) at = -1;
+        }
+        page[tid] = at;
+      }
+      __syncthreads();
+      for (int i = tid; i < AS_KEYS * (D / 4); i += AP_THREADS) {
+        const int j = i / (D / 4), c = i % (D / 4) * 4, at = page[j];
+        float4 kv = make_float4(0.f, 0.f, 0.f, 0.f), vv = kv;
+        if (at >= 0 && c < d) {
+          const int key = k0 + j, slot = p.page_shift >= 0 ? key & (p.page_size - 1) : key % p.page_size;
+          const size_t off = (((size_t)at * cache_heads + g.kv_head / p.kv_share) * p.page_size + slot) * d + c;
+          kv = ap_load4(kc + off);
+          vv = ap_load4(vc + off);
+        }
+        *reinterpret_cast<float4*>(ks + j * (D + 4) + c) = kv;
+        *reinterpret_cast<float4*>(vs + j * D + c) = vv;
+      }
+      __syncthreads();
+      float s[2][4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) s[e][0] = s[e][1] = s[e][2] = s[e][3] = 0.f;
+#pragma unroll 4
+      for (int c = 0; c < D; c += 4) {
+        const float4 q0 = *reinterpret_cast<const float4*>(qs + 2 * ty * D + c), q1 = *reinterpret_cast<const float4*>(qs + (2 * ty + 1) * D + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float4 k = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * (D + 4) + c);
+          s[0][j] = fmaf(q0.x, k.x, fmaf(q0.y, k.y, fmaf(q0.z, k.z, fmaf(q0.w, k.w, s[0][j]))));
+          s[1][j] = fmaf(q1.x, k.x, fmaf(q1.y, k.y, fmaf(q1.z, k.z, fmaf(q1.w, k.w, s[1][j]))));
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float mx = m[e];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int jj = tx + 16 * j;
+          s[e][j] = (k0 + jj <= last[e] && page[jj] >= 0) ? s[e][j] * p.scale_log2 : -INFINITY;
+          mx = fmaxf(mx, s[e][j]);
+        }
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        const float f = m[e] == -INFINITY ? 0.f : exp2f(m[e] - ref);
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float w = exp2f(s[e][j] - ref);
+          sum += w;
+          ps[(2 * ty + e) * (AS_KEYS + 4) + tx + 16 * j] = w;
+        }
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        m[e] = mx;
+        l[e] = l[e] * f + sum;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) { o[e][c][0] *= f; o[e][c][1] *= f; o[e][c][2] *= f; o[e][c][3] *= f; }
+      }
+      __syncwarp();                      // a row's weights are written and read by one half of a warp
+#pragma unroll 4
+      for (int j = 0; j < AS_KEYS; ++j) {
+        const float w0 = ps[2 * ty * (AS_KEYS + 4) + j], w1 = ps[(2 * ty + 1) * (AS_KEYS + 4) + j];
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          const float4 v = *reinterpret_cast<const float4*>(vs + j * D + 64 * c + 4 * tx);
+          o[0][c][0] = fmaf(w0, v.x, o[0][c][0]); o[0][c][1] = fmaf(w0, v.y, o[0][c][1]); o[0][c][2] = fmaf(w0, v.z, o[0][c][2]); o[0][c][3] = fmaf(w0, v.w, o[0][c][3]);
+          o[1][c][0] = fmaf(w1, v.x, o[1][c][0]); o[1][c][1] = fmaf(w1, v.y, o[1][c][1]); o[1][c][2] = fmaf(w1, v.z, o[1][c][2]); o[1][c][3] = fmaf(w1, v.w, o[1][c][3]);
+        }
+      }
+      __syncwarp();
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = 2 * ty + e;
+      if (r >= rows) continue;
+      if (tx == 0) *reinterpret_cast<float2*>(p.part_ml + (g.row + r) * 2) = make_float2(m[e], l[e]);
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c)
+        if (64 * c + 4 * tx < d)
+          *reinterpret_cast<float4*>(p.part_o + (g.row + r) * d + 64 * c + 4 * tx) = make_float4(o[e][c][0], o[e][c][1], o[e][c][2], o[e][c][3]);
+    }
+  }
+}
+
+static int as_sms() {
+  int device = 0, n = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
+  return n;
+}
+
+// How a launch on the ordinary pipes cuts its rows: heads of a tile, tokens of a tile.
+struct PlainCut { int share, group, tokens; };
+static PlainCut ap_cut(int group) {
+  int share = 1;
+  while (group % share || group / share > AP_ROWS) ++share;
+  const int g = group / share;
+  return {share, g, AP_ROWS / g};
+}
+
+template <typename T, int D>
+static cudaError_t ap_launch(const SharedParams& p, int ctas, cudaStream_t stream) {
+  static std::atomic<unsigned long long> configured{0ull};     // a bit a device
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  if (!(configured.load() >> (device & 63) & 1ull)) {
+    e = cudaFuncSetAttribute(attention_shared_plain_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, ap_smem_bytes<D>());
+    if (e != cudaSuccess) return e;
+    configured.fetch_or(1ull << (device & 63));
+  }
+  e = launch(attention_shared_plain_kernel<T, D>, dim3(ctas), dim3(AP_THREADS), ap_smem_bytes<D>(), stream, p);
+  if (e != cudaSuccess) return e;
+  count_launch();
+  return launch(as_combine_kernel<T>, dim3((unsigned)(((long long)p.T * p.heads + 7) / 8)), dim3(256), 0, stream, p);
+}
+
+}  // namespace lb
+
+// Elements of the two workspaces of a launch: partial results (float32) and the combining kernel's list (int32).
+LB_EXPORT int lb_attention_shared_workspace(int num_tokens, int num_q_heads, int num_kv_heads, int head_dim, int dtype, int page_size,
+                                            long long* floats, long long* ints) {
+  LB_CHECK_ARG(num_tokens >= 0 && num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0 && head_dim > 0, "attention_shared: bad sizes");
+  const int ctas = lb::as_sms();
+  LB_CHECK_ARG(ctas > 0, "attention_shared: no device");
+  const lb::PlainCut cut = lb::ap_cut(num_q_heads / num_kv_heads);
+  const long long rows = 2ll * num_tokens * num_q_heads + (long long)ctas * cut.tokens * cut.group;
+  *floats = rows * (head_dim + 2);
+  *ints = (long long)num_tokens * lb::AS_REC + 8;
+  return 0;
+}
+
+// q, out: [T, heads, dim]; k_cache, v_cache: [pages, kv heads, page_size, dim]; table [S, max_pages], cu_tokens [S + 1], context_lens,
+// prefix_of and prefix_lens [S], all int32.  See attention_shared.cuh.
+LB_EXPORT int lb_attention_shared(int dtype, const void* q, void* out, const void* k_cache, const void* v_cache, const int* table,
+                                  const int* cu_tokens, const int* context_lens, const int* prefix_of, const int* prefix_lens, int num_tokens,
+                                  int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int page_size, int num_pages, int max_pages,
+                                  float scale, float* floats, long long num_floats, int* ints, long long num_ints, cudaStream_t stream) {
+  LB_CHECK_ARG(lb::valid_dtype(dtype), "attention_shared: unknown element type %d", dtype);
+  LB_CHECK_ARG(num_tokens >= 0 && num_seqs >= 0 && num_seqs <= lb::AS_MAX_SEQS, "attention_shared: %d tokens of %d requests, at most %d requests",
+               num_tokens, num_seqs, lb::AS_MAX_SEQS);
+  LB_CHECK_ARG(num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0, "attention_shared: %d query heads on %d kv heads",
+               num_q_heads, num_kv_heads);
+  LB_CHECK_ARG(head_dim > 0 && head_dim <= 256 && head_dim % 8 == 0, "attention_shared: heads of %d, a multiple of 8 up to 256 is needed", head_dim);
+  LB_CHECK_ARG(page_size > 0 && num_pages > 0 && max_pages > 0 && (long long)max_pages * page_size < (1ll << 31) - 64, "attention_shared: %d pages of %d tokens, tables of %d",
+               num_pages, page_size, max_pages);
+  if (num_tokens == 0 || num_seqs == 0) return 0;
+  LB_CHECK_ARG((long long)num_tokens * num_q_heads < (1ll << 30), "attention_shared: %d tokens of %d heads", num_tokens, num_q_heads);
+  LB_CHECK_ARG(((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)floats | (uintptr_t)ints) % 16 == 0,
+               "attention_shared: operands must be 16-byte aligned");
+  long long need_floats = 0, need_ints = 0;
+  if (lb_attention_shared_workspace(num_tokens, num_q_heads, num_kv_heads, head_dim, dtype, page_size, &need_floats, &need_ints)) return 1;
+  LB_CHECK_ARG(floats && ints && num_floats >= need_floats && num_ints >= need_ints,
+               "attention_shared: workspaces of %lld and %lld elements are needed, got %lld and %lld", need_floats, need_ints, num_floats, num_ints);
+  const int ctas = lb::as_sms();
+  const lb::PlainCut cut = lb::ap_cut(num_q_heads / num_kv_heads);
+  lb::SharedParams p;
+  p.q = q; p.out = out; p.k_cache = k_cache; p.v_cache = v_cache; p.table = table; p.max_pages = max_pages; p.num_pages = num_pages;
+  p.cu = cu_tokens; p.ctx = context_lens; p.prefix_of = prefix_of; p.prefix_lens = prefix_lens;
+  p.T = num_tokens; p.S = num_seqs; p.heads = num_q_heads; p.kv_heads = num_kv_heads * cut.share; p.group = cut.group; p.dim = head_dim;
+  p.page_size = page_size; p.page_shift = -1; p.kv_share = cut.share; p.tile_tokens = p.lane_tokens = cut.tokens; p.min_span = 1;
+  for (int b = 0; b < 31; ++b) if ((1 << b) == page_size) p.page_shift = b;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  const long long rows = (need_floats) / (head_dim + 2);
+  p.part_o = floats; p.part_ml = floats + rows * head_dim;
+  p.rec = ints; p.head = ints + (long long)num_tokens * lb::AS_REC;
+  cudaError_t e;
+  if (dtype == LB_F32)
+    e = head_dim <= 64 ? lb::ap_launch<float, 64>(p, ctas, stream) : head_dim <= 128 ? lb::ap_launch<float, 128>(p, ctas, stream) : lb::ap_launch<float, 256>(p, ctas, stream);
+  else
+    e = head_dim <= 64 ? lb::ap_launch<lb::bf16, 64>(p, ctas, stream) : head_dim <= 128 ? lb::ap_launch<lb::bf16, 128>(p, ctas, stream) : lb::ap_launch<lb::bf16, 256>(p, ctas, stream);
+  if (e != cudaSuccess) { lb::set_error("attention_shared: launch failed: %s", cudaGetErrorString(e)); return 2; }
+  lb::count_launch();
+  return 0;
+}

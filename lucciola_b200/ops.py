@@ -123,6 +123,8 @@ _SIGNATURES = {
     "lb_attention_tcgen05": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                              c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_longlong, c_void_p, c_float, c_int, c_void_p,
                              c_void_p],
+    "lb_attention_shared": [c_int] + [c_void_p] * 9 + [c_int] * 8 + [c_float, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p],
+    "lb_attention_shared_workspace": [c_int] * 6 + [c_void_p, c_void_p],
     "lb_latent_flash": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                         c_float, c_void_p, c_int, c_int, c_void_p, c_longlong, c_void_p],
     "lb_latent_gather": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
@@ -1468,6 +1470,63 @@ def _attention_workspace(device: torch.device, elems: int) -> torch.Tensor:
         ws = torch.empty(max(elems, 1 << 20, 2 * ws.numel() if ws is not None else 0), dtype=torch.float32, device=device)
         _attn_ws[key] = ws
     return ws
+
+
+@functools.lru_cache(maxsize=4096)
+def _shared_workspace(device: int, *sizes: int) -> tuple[int, int]:
+    """Elements of the workspaces of attention_shared on this device: float32, int32."""
+    floats, ints = c_longlong(0), c_longlong(0)
+    _call("lb_attention_shared_workspace", *sizes, ctypes.addressof(floats), ctypes.addressof(ints))
+    return floats.value, ints.value
+
+
+def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                     cu_tokens: torch.Tensor, context_lens: torch.Tensor, prefix_of: torch.Tensor, prefix_lens: torch.Tensor, max_q_len: int,
+                     num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int, scale: float, stream: int) -> None:
+    """Causal attention of a step over paged keys and values, the keys that several requests share read once for all of them.
+
+    q, out [T, heads, dim] (float32 or bfloat16); pools [pages, kv heads, page_size, dim]; block_table [S, pages a sequence],
+    cu_tokens [S + 1] and context_lens [S] as in StepContext.  prefix_of[s] (int32 [S]) is the row of the batch whose block table
+    holds the prefix that request s shares (its own row for that request itself, -1: none), prefix_lens[r] (int32 [S]) how many
+    tokens the prefix of row r has: the first prefix_lens[prefix_of[s]] keys of s are read through that row's table, the others
+    through its own.  All of these are device values, read by the kernel, so that a recorded step is replayed with other groups and
+    lengths; `max_q_len` is the most tokens of a request.  Page ids outside the pool are not there: a row that sees no key gives
+    zeros, and rows of q that belong to no request (behind cu_tokens[S]) leave the output as it was.  S is at most 512, a head a multiple of
+    8 up to 256.  Partial results go through memory that the call
+    takes from torch's allocator on the current stream, so calls on several streams do not meet; a stream that is not the current
+    one is told to the allocator."""
+    _check(q, "q"); _check(out, "attention output", q.dtype); _check(k_cache, "k pool", q.dtype); _check(v_cache, "v pool", q.dtype)
+    T, S = q.shape[0], context_lens.shape[0]
+    for t, what, shape in ((cu_tokens, "cu_tokens", (S + 1,)), (context_lens, "context lengths", (S,)), (prefix_of, "prefix_of", (S,)),
+                           (prefix_lens, "prefix_lens", (S,))):
+        _check(t, what, torch.int32)
+        if tuple(t.shape) != shape:
+            raise KernelError(f"{what} is {tuple(t.shape)} for {S} requests")
+    _check(block_table, "block table", torch.int32)
+    if block_table.dim() != 2 or block_table.shape[0] != S:
+        raise KernelError(f"the block table is {tuple(block_table.shape)} for {S} requests")
+    if num_kv_heads <= 0 or num_q_heads % num_kv_heads:
+        raise KernelError(f"{num_q_heads} query heads are not a multiple of {num_kv_heads} kv heads")
+    if tuple(q.shape) != (T, num_q_heads, head_dim) or out.shape != q.shape:
+        raise KernelError(f"q is {tuple(q.shape)} and the output {tuple(out.shape)} for {num_q_heads} heads of {head_dim}")
+    if k_cache.dim() != 4 or tuple(k_cache.shape[1:]) != (num_kv_heads, page_size, head_dim) or v_cache.shape != k_cache.shape:
+        raise KernelError(f"the pools are {tuple(k_cache.shape)} and {tuple(v_cache.shape)} for {num_kv_heads} heads of {head_dim} in pages of {page_size}")
+    for t in (out, k_cache, v_cache, block_table, cu_tokens, context_lens, prefix_of, prefix_lens):
+        if t.device != q.device:
+            raise KernelError(f"operands on {q.device} and {t.device}")
+    _on_current_device(q)
+    if T == 0 or S == 0:
+        return
+    dt = dtype_code(q.dtype)
+    n_floats, n_ints = _shared_workspace(q.device.index, T, num_q_heads, num_kv_heads, head_dim, dt, page_size)
+    floats = torch.empty(n_floats, dtype=torch.float32, device=q.device)
+    ints = torch.empty(n_ints, dtype=torch.int32, device=q.device)
+    if stream != torch.cuda.current_stream(q.device).cuda_stream:
+        other = torch.cuda.ExternalStream(stream, device=q.device)
+        floats.record_stream(other); ints.record_stream(other)
+    _call("lb_attention_shared", dt, q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+          cu_tokens.data_ptr(), context_lens.data_ptr(), prefix_of.data_ptr(), prefix_lens.data_ptr(), T, S, num_q_heads, num_kv_heads,
+          head_dim, page_size, k_cache.shape[0], block_table.shape[1], float(scale), floats.data_ptr(), n_floats, ints.data_ptr(), n_ints, stream)
 
 
 def attention_flash_ok(q: torch.Tensor, num_q_heads: int, num_kv_heads: int, head_dim: int, v_dim: int = 0) -> bool:

@@ -2,6 +2,7 @@
 import math
 
 import numpy as np
+import torch
 
 M64 = (1 << 64) - 1
 
@@ -45,3 +46,33 @@ def draw(logits, temperature, key, counter, top_k=0, top_p=1.0, min_p=0.0) -> in
     kept = kept_tokens(logits, temperature, top_k, top_p, min_p)
     score = (x[kept] - x.max()) / temperature - np.log(-np.log(uniforms(key, counter, len(x))[kept]))
     return int(kept[score == score.max()].min())
+
+
+def shared_attention(q, k_cache, v_cache, table, cu, ctx, prefix_of, prefix_lens, scale):
+    """[T, heads, dim] in 64 bits; rows of no request are NaN.  Key j of request s lies in the table row of its prefix if j is one of the
+    prefix's keys, else in its own; keys whose page is not in the pool are not there."""
+    heads, dim = q.shape[1:]
+    pages, kv_heads, ps = k_cache.shape[:3]
+    out = torch.full(q.shape, math.nan, dtype=torch.float64)
+    for s in range(len(ctx)):
+        n = cu[s + 1] - cu[s]
+        length = min(ctx[s], table.shape[1] * ps)
+        lead = prefix_of[s]
+        keys = []
+        for j in range(length):
+            row = table[lead] if 0 <= lead < len(ctx) and j < prefix_lens[lead] else table[s]
+            page = int(row[j // ps])
+            keys.append((page, j % ps) if 0 <= page < pages else None)
+        for i in range(n):
+            position = ctx[s] - n + i
+            seen = [at for at in keys[:max(position + 1, 0)] if at is not None]
+            t = cu[s] + i
+            if not seen:
+                out[t] = 0.0
+                continue
+            page, slot = torch.tensor(seen).T
+            k = k_cache[page, :, slot].double().repeat_interleave(heads // kv_heads, 1)       # [keys, heads, dim]
+            v = v_cache[page, :, slot].double().repeat_interleave(heads // kv_heads, 1)
+            w = torch.softmax(torch.einsum("hd,jhd->hj", q[t].double(), k) * scale, 1)
+            out[t] = torch.einsum("hj,jhd->hd", w, v)
+    return out

@@ -1,4 +1,4 @@
-// Attention of a step whose requests share prefixes, on the ordinary pipes: 32-bit queries, keys and values, and bfloat16 ones that the
+// Attention of a step whose requests share prefixes: the entry point, and the kernel on the ordinary pipes for 32-bit queries, keys and values, and bfloat16 ones that the
 // tensor-core kernel does not take.  The plan, the walk and the combination are attention_shared.cuh's.
 //
 // A tile has up to 32 query rows (tokens x heads of a kv head's group; a group of more heads is cut into equal parts that read the same
@@ -173,13 +173,18 @@ static int as_sms() {
   return n;
 }
 
-// How a launch on the ordinary pipes cuts its rows: heads of a tile, tokens of a tile.
-struct PlainCut { int share, group, tokens; };
-static PlainCut ap_cut(int group) {
-  int share = 1;
-  while (group % share || group / share > AP_ROWS) ++share;
-  const int g = group / share;
-  return {share, g, AP_ROWS / g};
+// How a launch cuts its rows: kv heads that share a cached one, heads of a tile, tokens of a tile and of a part of one.
+struct SharedCut { bool tc; int share, group, tile_tokens, lane_tokens; };
+static SharedCut as_cut(int dtype, int group, int head_dim, int page_size) {
+  SharedCut c{attention_shared_tc_takes(dtype, group, head_dim, page_size), 1, group, 0, 0};
+  if (c.tc) {
+    attention_shared_tc_cut(group, c.tile_tokens, c.lane_tokens);
+    return c;
+  }
+  while (group % c.share || group / c.share > AP_ROWS) ++c.share;
+  c.group = group / c.share;
+  c.tile_tokens = c.lane_tokens = AP_ROWS / c.group;
+  return c;
 }
 
 template <typename T, int D>
@@ -193,9 +198,11 @@ static cudaError_t ap_launch(const SharedParams& p, int ctas, cudaStream_t strea
     if (e != cudaSuccess) return e;
     configured.fetch_or(1ull << (device & 63));
   }
-  e = launch(attention_shared_plain_kernel<T, D>, dim3(ctas), dim3(AP_THREADS), ap_smem_bytes<D>(), stream, p);
-  if (e != cudaSuccess) return e;
-  count_launch();
+  return launch(attention_shared_plain_kernel<T, D>, dim3(ctas), dim3(AP_THREADS), ap_smem_bytes<D>(), stream, p);
+}
+
+template <typename T>
+static cudaError_t as_combine(const SharedParams& p, cudaStream_t stream) {
   return launch(as_combine_kernel<T>, dim3((unsigned)(((long long)p.T * p.heads + 7) / 8)), dim3(256), 0, stream, p);
 }
 
@@ -207,8 +214,8 @@ LB_EXPORT int lb_attention_shared_workspace(int num_tokens, int num_q_heads, int
   LB_CHECK_ARG(num_tokens >= 0 && num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0 && head_dim > 0, "attention_shared: bad sizes");
   const int ctas = lb::as_sms();
   LB_CHECK_ARG(ctas > 0, "attention_shared: no device");
-  const lb::PlainCut cut = lb::ap_cut(num_q_heads / num_kv_heads);
-  const long long rows = 2ll * num_tokens * num_q_heads + (long long)ctas * cut.tokens * cut.group;
+  const lb::SharedCut cut = lb::as_cut(dtype, num_q_heads / num_kv_heads, head_dim, page_size);
+  const long long rows = 2ll * num_tokens * num_q_heads + (long long)ctas * cut.tile_tokens * cut.group;
   *floats = rows * (head_dim + 2);
   *ints = (long long)num_tokens * lb::AS_REC + 8;
   return 0;
@@ -228,6 +235,7 @@ LB_EXPORT int lb_attention_shared(int dtype, const void* q, void* out, const voi
   LB_CHECK_ARG(head_dim > 0 && head_dim <= 256 && head_dim % 8 == 0, "attention_shared: heads of %d, a multiple of 8 up to 256 is needed", head_dim);
   LB_CHECK_ARG(page_size > 0 && num_pages > 0 && max_pages > 0 && (long long)max_pages * page_size < (1ll << 31) - 64, "attention_shared: %d pages of %d tokens, tables of %d",
                num_pages, page_size, max_pages);
+  LB_CHECK_ARG(scale > 0.f && scale < 1e30f, "attention_shared: a scale of %f, a positive one is needed", (double)scale);
   if (num_tokens == 0 || num_seqs == 0) return 0;
   LB_CHECK_ARG((long long)num_tokens * num_q_heads < (1ll << 30), "attention_shared: %d tokens of %d heads", num_tokens, num_q_heads);
   LB_CHECK_ARG(((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)floats | (uintptr_t)ints) % 16 == 0,
@@ -237,23 +245,29 @@ LB_EXPORT int lb_attention_shared(int dtype, const void* q, void* out, const voi
   LB_CHECK_ARG(floats && ints && num_floats >= need_floats && num_ints >= need_ints,
                "attention_shared: workspaces of %lld and %lld elements are needed, got %lld and %lld", need_floats, need_ints, num_floats, num_ints);
   const int ctas = lb::as_sms();
-  const lb::PlainCut cut = lb::ap_cut(num_q_heads / num_kv_heads);
+  const lb::SharedCut cut = lb::as_cut(dtype, num_q_heads / num_kv_heads, head_dim, page_size);
   lb::SharedParams p;
   p.q = q; p.out = out; p.k_cache = k_cache; p.v_cache = v_cache; p.table = table; p.max_pages = max_pages; p.num_pages = num_pages;
   p.cu = cu_tokens; p.ctx = context_lens; p.prefix_of = prefix_of; p.prefix_lens = prefix_lens;
   p.T = num_tokens; p.S = num_seqs; p.heads = num_q_heads; p.kv_heads = num_kv_heads * cut.share; p.group = cut.group; p.dim = head_dim;
-  p.page_size = page_size; p.page_shift = -1; p.kv_share = cut.share; p.tile_tokens = p.lane_tokens = cut.tokens; p.min_span = 1;
+  p.page_size = page_size; p.page_shift = -1; p.kv_share = cut.share; p.tile_tokens = cut.tile_tokens; p.lane_tokens = cut.lane_tokens;
+  p.min_span = cut.tc ? 4 : 1;
   for (int b = 0; b < 31; ++b) if ((1 << b) == page_size) p.page_shift = b;
   p.scale_log2 = scale * 1.4426950408889634f;
   const long long rows = (need_floats) / (head_dim + 2);
   p.part_o = floats; p.part_ml = floats + rows * head_dim;
   p.rec = ints; p.head = ints + (long long)num_tokens * lb::AS_REC;
   cudaError_t e;
-  if (dtype == LB_F32)
+  if (cut.tc)
+    e = lb::attention_shared_tc(p, ctas, stream);
+  else if (dtype == LB_F32)
     e = head_dim <= 64 ? lb::ap_launch<float, 64>(p, ctas, stream) : head_dim <= 128 ? lb::ap_launch<float, 128>(p, ctas, stream) : lb::ap_launch<float, 256>(p, ctas, stream);
   else
     e = head_dim <= 64 ? lb::ap_launch<lb::bf16, 64>(p, ctas, stream) : head_dim <= 128 ? lb::ap_launch<lb::bf16, 128>(p, ctas, stream) : lb::ap_launch<lb::bf16, 256>(p, ctas, stream);
   if (e != cudaSuccess) { lb::set_error("attention_shared: launch failed: %s", cudaGetErrorString(e)); return 2; }
+  lb::count_launch();
+  e = dtype == LB_F32 ? lb::as_combine<float>(p, stream) : lb::as_combine<lb::bf16>(p, stream);
+  if (e != cudaSuccess) { lb::set_error("attention_shared: launch of the combination failed: %s", cudaGetErrorString(e)); return 2; }
   lb::count_launch();
   return 0;
 }

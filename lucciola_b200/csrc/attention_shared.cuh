@@ -35,6 +35,11 @@ struct SharedParams {
   int* rec; int* head;                   // [T][AS_REC], {units a kv head, units a CTA, rows a kv head, first token, end of the tokens}
 };
 
+// The tensor-core kernel (attention_shared_tc.cu): what it takes, how it cuts rows, its launch.
+bool attention_shared_tc_takes(int dtype, int group, int head_dim, int page_size);
+void attention_shared_tc_cut(int group, int& tile_tokens, int& lane_tokens);
+cudaError_t attention_shared_tc(const SharedParams& p, int ctas, cudaStream_t stream);
+
 struct SharedPlan {
   int q0[AS_MAX_SEQS + 1], ctx[AS_MAX_SEQS];
   int lead[AS_MAX_SEQS];                 // the row whose table holds the prefix this request shares, -1: none

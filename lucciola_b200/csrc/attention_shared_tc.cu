@@ -1,0 +1,401 @@
+// Attention of a step whose requests share prefixes, on the 5th-generation tensor cores (bfloat16, heads of 64 or 128, up to 128 query
+// heads a kv head, pages of 8 tokens and more that are powers of two).  The plan, the walk and the combination are attention_shared.cuh's.
+//
+// One CTA an SM walks its piece of the line of key blocks, segment after segment.  A segment has up to 256 query rows: two tiles, A and
+// B, of up to 128 rows each, on which two sets of warps and two halves of tensor memory work.  The rows of a group's members against its
+// prefix fill both; a segment of one tile (a request's own keys: a handful of rows) goes to A and B in turn, so that the start and the end
+// of one segment pass while the other's products run, and the copies of keys and values run on through all of them.
+//     S = Q K^T      tcgen05.mma, operands from shared memory, two S buffers a tile
+//     P              one thread a query row, online softmax in 32 bits, P (bfloat16) written over S in tensor memory
+//     O += P V       tcgen05.mma, P from tensor memory, V as it lies in the pages; O stays in tensor memory
+// The sum of a row's weights is taken before they are rounded to bfloat16 for P V.  A row's reference value follows its maximum when that
+// has grown by more than 2^8 only (O is rescaled then).
+//
+// Why 128-row tiles even for one request's few rows: a block of 64 keys takes the tensor cores some 500 cycles whatever the rows, and the
+// memory 1400 cycles at its full rate shared by all SMs, so rows that are not there cost nothing; one kernel for both kinds of work is what
+// lets the line be cut evenly.
+//
+// Warps: 0 copies keys, 10 values (cp.async, 16 bytes a thread, swizzled for the tensor cores; four blocks each, three in flight); 1 issues
+// tile A's products and owns the tensor memory, 11 tile B's; 2..5 softmax of A, 6..9 of B.  Each walks the same segments by itself.  All
+// waits are bounded; when one gives up, the CTA records it and every role leaves.
+#include "attention_shared.cuh"
+#include "attention_tcgen05.cuh"
+
+#include <atomic>
+
+namespace lb {
+
+constexpr int SC_STAGES = 4;
+constexpr int SC_IN_FLIGHT = 2;                                // blocks a copying warp has requested beyond the one it waits for
+constexpr int SC_THREADS = 384;
+enum : int { SC_ERR_Q = 401, SC_ERR_KV_FULL = 402, SC_ERR_KV_EMPTY = 403, SC_ERR_S_FULL = 404, SC_ERR_P_FULL = 405, SC_ERR_O_FULL = 406, SC_ERR_O_FREE = 407 };
+
+// Shared memory: queries of A and B | ring of keys | ring of values | barriers.  Rows of 128 bytes (64 elements), 128-byte swizzle, the second
+// 64 elements of a head a half further on.
+template <int D> struct ScLayout {
+  static constexpr int HALVES = D / 64;
+  static constexpr int KV_HALF = AS_KEYS * 128, KV_TILE = HALVES * KV_HALF;
+  static constexpr int Q_TILE = HALVES * TA_HALF_BYTES;
+  static constexpr int K_OFF = 2 * Q_TILE, V_OFF = K_OFF + SC_STAGES * KV_TILE, BAR_OFF = V_OFF + SC_STAGES * KV_TILE;
+  static constexpr int BARS = 4 * SC_STAGES + 2 * 8;
+  static constexpr int BYTES = BAR_OFF + BARS * 8 + 16;
+};
+
+template <int D>
+__global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(SharedParams p) {
+  typedef ScLayout<D> L;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ SharedPlan plan;
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t sbase = ta_smem_u32(smem);
+  const uint32_t bars = sbase + L::BAR_OFF;
+  auto k_full = [&](int s) { return bars + 8u * s; };
+  auto k_empty = [&](int s) { return bars + 8u * (SC_STAGES + s); };
+  auto v_full = [&](int s) { return bars + 8u * (2 * SC_STAGES + s); };
+  auto v_empty = [&](int s) { return bars + 8u * (3 * SC_STAGES + s); };
+  // of tile t and S buffer b: S complete, P written, P V complete; of tile t: queries there, O read
+  auto s_full = [&](int t, int b) { return bars + 8u * (4 * SC_STAGES + t * 8 + b); };
+  auto p_full = [&](int t, int b) { return bars + 8u * (4 * SC_STAGES + t * 8 + 2 + b); };
+  auto pv_done = [&](int t, int b) { return bars + 8u * (4 * SC_STAGES + t * 8 + 4 + b); };
+  auto q_full = [&](int t) { return bars + 8u * (4 * SC_STAGES + t * 8 + 6); };
+  auto o_free = [&](int t) { return bars + 8u * (4 * SC_STAGES + t * 8 + 7); };
+  uint32_t* tmem_slot = (uint32_t*)(smem + L::BAR_OFF + L::BARS * 8);
+  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < SC_STAGES; ++i) {
+      ta_mbar_init(k_full(i), 1); ta_mbar_init(k_empty(i), 2);             // both tiles are through with it: their products have read it, or do not
+      ta_mbar_init(v_full(i), 1); ta_mbar_init(v_empty(i), 2);
+    }
+    for (int t = 0; t < 2; ++t) {
+      for (int b = 0; b < 2; ++b) { ta_mbar_init(s_full(t, b), 1); ta_mbar_init(p_full(t, b), 4); ta_mbar_init(pv_done(t, b), 1); }
+      ta_mbar_init(q_full(t), 4); ta_mbar_init(o_free(t), 4);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ta_smem_u32(tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  as_make_plan(p, plan, gridDim.x);
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;            // columns: tile t's S buffers at t * 128 and t * 128 + 64 (P over their first 32), O at 256 + t * 128
+  as_write_records(p, plan, blockIdx.x, gridDim.x);
+
+  const int G = p.group, per = p.lane_tokens, cta = blockIdx.x;
+  long long x = (long long)cta * plan.span;
+  const long long x_end = min(x + plan.span, (long long)plan.units * p.kv_heads);
+  int blocks_done = 0, singles = 0;            // blocks of all segments so far, segments of one tile so far
+
+  if (warp == 0 || warp == 10) {
+    // ---- copies ------------------------------------------------------------------------------------------------------------------
+    const bool is_v = warp == 10;
+    constexpr int CHUNKS = D / 8, RPI = 32 / CHUNKS, STEPS = AS_KEYS / RPI;      // 16-byte chunks of a row, rows an instruction
+    const int c = lane % CHUNKS, rp = lane / CHUNKS;
+    const uint8_t* pool = (const uint8_t*)(is_v ? p.v_cache : p.k_cache) + c * 16;
+    const uint32_t ring = sbase + (is_v ? L::V_OFF : L::K_OFF) + (uint32_t)(c >> 3) * L::KV_HALF;
+    const int ps = p.page_size, shift = p.page_shift;
+    const size_t page_stride = (size_t)p.kv_heads * ps * (D * 2);
+    bool ok = true;
+    auto hand_over = [&](int i) {              // block i (of all) has landed: visible to the tensor cores, then said so
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) ta_mbar_arrive(is_v ? v_full(i % SC_STAGES) : k_full(i % SC_STAGES));
+    };
+    while (x < x_end && ok) {
+      const Segment g = as_next(p, plan, cta, x, x_end);
+      const int* bt = p.table + (size_t)g.table_row * p.max_pages;
+      const uint8_t* head = pool + (size_t)g.kv_head * ps * (D * 2);
+      const int first_key = (g.key_lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS;
+      // the page of key kb + lane * ps (of kb itself for pages of 64 tokens and more), -1 where no key of this segment lies
+      auto page_of = [&](int kb) -> int {
+        const int key = kb + lane * min(ps, AS_KEYS), size = min(ps, AS_KEYS);
+        if (lane * size >= AS_KEYS || key >= g.key_hi || key + size <= g.key_lo) return -1;
+        const int id = bt[key >> shift];
+        return id < p.num_pages ? id : -1;
+      };
+      int ids = g.blocks > 0 ? page_of(first_key) : -1;
+      for (int b = 0; b < g.blocks; ++b) {
+        const int i = blocks_done + b, s = i % SC_STAGES, kb = first_key + b * AS_KEYS;
+        int go = 1;
+        if (lane == 0) go = ta_mbar_wait_idle(is_v ? v_empty(s) : k_empty(s), (uint32_t)((i / SC_STAGES) & 1) ^ 1u, abort_flag, SC_ERR_KV_EMPTY) ? 1 : 0;
+        go = __shfl_sync(0xffffffffu, go, 0);
+        if (!go) { ok = false; break; }
+        const bool inner = kb >= g.key_lo && kb + AS_KEYS <= g.key_hi;
+        const uint32_t stage = ring + (uint32_t)s * L::KV_TILE;
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j) {
+          const int r = rp + RPI * j, key = kb + r;
+          const int id = __shfl_sync(0xffffffffu, ids, r >> min(shift, 6));
+          const uint32_t bytes = (id >= 0 && (inner || (key >= g.key_lo && key < g.key_hi))) ? 16u : 0u;       // 0: sixteen zeros
+          const uint8_t* src = head + (size_t)max(id, 0) * page_stride + (size_t)(key & (ps - 1)) * (D * 2);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                       ::"r"(stage + (uint32_t)r * 128u + (uint32_t)(((c & 7) ^ (r & 7)) << 4)), "l"(src), "r"(bytes) : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        ids = b + 1 < g.blocks ? page_of(kb + AS_KEYS) : -1;
+        if (i >= SC_IN_FLIGHT) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(SC_IN_FLIGHT) : "memory");
+          hand_over(i - SC_IN_FLIGHT);
+        }
+      }
+      if (ok) blocks_done += g.blocks;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (ok)
+      for (int i = max(blocks_done - SC_IN_FLIGHT, 0); i < blocks_done; ++i) hand_over(i);
+  } else if (warp == 1 || warp == 11) {
+    // ---- products, one thread a tile -------------------------------------------------------------------------------------------------
+    const int t = warp == 1 ? 0 : 1;
+    if (elect_one()) {
+      constexpr uint32_t idesc_qk = ta_idesc(0, AS_KEYS), idesc_pv = ta_idesc(1, D);
+      const uint32_t s_col = tmem + (uint32_t)t * 128u, o_col = tmem + 256u + (uint32_t)t * 128u;
+      const uint32_t qa = sbase + t * L::Q_TILE;
+      int mine = 0, segments = 0;              // this tile's blocks and segments so far
+      bool ok = true;
+      while (x < x_end && ok) {
+        const Segment g = as_next(p, plan, cta, x, x_end);
+        if (g.blocks == 0) continue;
+        const bool two = g.tokens > per;
+        if (!two && (singles++ & 1) != t) {
+          // The other tile's blocks are let pass one by one: a wait tells one turn of the ring from the next only.
+          for (int i = 0; i < g.blocks && ok; ++i) {
+            const int n = blocks_done + i, s = n % SC_STAGES;
+            ok = ta_mbar_wait_idle(k_full(s), (uint32_t)((n / SC_STAGES) & 1), abort_flag, SC_ERR_KV_FULL);
+            if (ok) ta_mbar_arrive(k_empty(s));
+            ok = ok && ta_mbar_wait_idle(v_full(s), (uint32_t)((n / SC_STAGES) & 1), abort_flag, SC_ERR_KV_FULL);
+            if (ok) ta_mbar_arrive(v_empty(s));
+          }
+          blocks_done += g.blocks;
+          continue;
+        }
+        ok = ta_mbar_wait(q_full(t), (uint32_t)(segments & 1), abort_flag, SC_ERR_Q);
+        // S(i) = Q K(i)^T into S buffer (mine + i) & 1
+        auto issue_qk = [&](int i) -> bool {
+          const int n = blocks_done + i, s = n % SC_STAGES, b = (mine + i) & 1;
+          if (!ta_mbar_wait(k_full(s), (uint32_t)((n / SC_STAGES) & 1), abort_flag, SC_ERR_KV_FULL)) return false;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t ka = sbase + L::K_OFF + s * L::KV_TILE;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            ta_umma(s_col + (uint32_t)b * 64u, ta_desc_kmajor(qa + (uint32_t)(k >> 2) * TA_HALF_BYTES + (uint32_t)(k & 3) * 32u),
+                    ta_desc_kmajor(ka + (uint32_t)(k >> 2) * L::KV_HALF + (uint32_t)(k & 3) * 32u), idesc_qk, k != 0);
+          ta_commit(s_full(t, b));
+          ta_commit(k_empty(s));
+          return true;
+        };
+        for (int i = 0; i < 2 && i < g.blocks && ok; ++i) ok = issue_qk(i);
+        for (int i = 0; i < g.blocks && ok; ++i) {
+          const int n = blocks_done + i, s = n % SC_STAGES, b = (mine + i) & 1;
+          ok = ta_mbar_wait(p_full(t, b), (uint32_t)(((mine + i) >> 1) & 1), abort_flag, SC_ERR_P_FULL) &&
+               ta_mbar_wait(v_full(s), (uint32_t)((n / SC_STAGES) & 1), abort_flag, SC_ERR_KV_FULL);
+          if (ok && i == 0 && segments > 0) ok = ta_mbar_wait(o_free(t), (uint32_t)((segments - 1) & 1), abort_flag, SC_ERR_O_FREE);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t va = sbase + L::V_OFF + s * L::KV_TILE;
+#pragma unroll
+          for (int k = 0; k < AS_KEYS / 16; ++k)
+            ta_umma_ts(o_col, s_col + (uint32_t)b * 64u + (uint32_t)k * 8u, ta_desc_mnmajor(va + (uint32_t)k * 16u * 128u, L::KV_HALF), idesc_pv, (i | k) != 0);
+          ta_commit(pv_done(t, b));
+          ta_commit(v_empty(s));
+          if (i + 2 < g.blocks) ok = issue_qk(i + 2);          // where P(i) lies: the tensor cores finish P V(i) first
+        }
+        blocks_done += g.blocks;
+        mine += g.blocks;
+        ++segments;
+      }
+    }
+  } else {
+    // ---- softmax: thread = query row; warp w reads lanes (w % 4) * 32 .. + 31 of tensor memory -----------------------------------------------
+    const int t = warp < 6 ? 0 : 1;
+    const int quarter = warp & 3, r = quarter * 32 + lane;
+    const uint32_t tlane = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_addr = tmem + tlane + (uint32_t)t * 128u, o_addr = tmem + tlane + 256u + (uint32_t)t * 128u;
+    const uint32_t q_row = sbase + t * L::Q_TILE + (uint32_t)r * 128u;
+    const int ps = p.page_size, shift = p.page_shift;
+    int mine = 0;
+    bool ok = true;
+    while (x < x_end && ok) {
+      const Segment g = as_next(p, plan, cta, x, x_end);
+      if (g.blocks == 0) continue;
+      const bool two = g.tokens > per;
+      if (!two && (singles++ & 1) != t) continue;
+      // this row's token, its queries
+      const int i_tok = (two ? t * per : 0) + r / G;
+      const bool valid = r < per * G && i_tok < g.tokens;
+      const bool warp_valid = quarter * 32 < min(g.tokens - (two ? t * per : 0), per) * G;
+      int token = 0, position = 0;
+      if (valid) {
+        as_token(plan, g, i_tok, token, position);
+        const uint8_t* src = (const uint8_t*)p.q + ((size_t)token * p.heads + g.kv_head * G + r % G) * (D * 2);
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                       ::"r"(q_row + (uint32_t)(c >> 3) * TA_HALF_BYTES + (uint32_t)(((c & 7) ^ (r & 7)) << 4)), "l"(src + c * 16) : "memory");
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) ta_mbar_arrive(q_full(t));
+      const int hi = valid ? min(position + 1, g.key_hi) : 0x7fffffff;
+      const int* bt = p.table + (size_t)g.table_row * p.max_pages;
+      float m_ref = -INFINITY, l_run = 0.f;
+      for (int i = 0; i < g.blocks; ++i) {
+        const int j = mine + i, b = j & 1;
+        const int kb = (g.key_lo & ~(AS_KEYS - 1)) + (g.block + i) * AS_KEYS;
+        int id = 0;                            // the page of the block's keys lane * size .. + size - 1, if there are any
+        const int size = min(ps, AS_KEYS), key = kb + lane * size;
+        if (lane * size < AS_KEYS && key < g.key_hi && key + size > g.key_lo) id = bt[key >> shift];
+        ok = ta_mbar_wait(s_full(t, b), (uint32_t)((j >> 1) & 1), abort_flag, SC_ERR_S_FULL);
+        if (!ok) break;
+        if (!warp_valid) {                     // no row of this warp: its rows of P are anything, and nobody reads what comes of them
+          __syncwarp();
+          if (lane == 0) ta_mbar_arrive(p_full(t, b));
+          continue;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t absent = __ballot_sync(0xffffffffu, id < 0 || id >= p.num_pages);
+        const bool need_mask = absent != 0 || kb < g.key_lo || __any_sync(0xffffffffu, kb + AS_KEYS > hi);
+        float xs[AS_KEYS];
+        {
+          uint32_t v[64];
+          ta_tmem_ld64(s_addr + (uint32_t)b * 64u, v);
+#pragma unroll
+          for (int e = 0; e < 64; ++e) xs[e] = __uint_as_float(v[e]);
+        }
+        if (need_mask) {
+          const int sh = min(shift, 6);
+#pragma unroll
+          for (int e = 0; e < AS_KEYS; ++e)
+            if (kb + e >= hi || kb + e < g.key_lo || ((absent >> (e >> sh)) & 1u)) xs[e] = -INFINITY;
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < AS_KEYS; e += 8) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) mx4[u] = ta_max3(mx4[u], xs[e + 2 * u], xs[e + 2 * u + 1]);
+        }
+        const float m_loc = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+        const bool grow = valid && m_loc > m_ref + TA_RESCALE_STEP;      // also true for the first finite maximum (m_ref = -inf)
+        if (__any_sync(0xffffffffu, grow)) {
+          float f = 1.f;
+          if (grow) {
+            if (m_ref != -INFINITY) f = exp2f(m_ref - m_loc);
+            m_ref = m_loc;
+            l_run *= f;
+          }
+          if (i > 0) {
+            ok = ta_mbar_wait(pv_done(t, b ^ 1), (uint32_t)(((j - 1) >> 1) & 1), abort_flag, SC_ERR_O_FULL);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t v[32];
+              ta_tmem_ld32(o_addr + (uint32_t)c, v);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+              ta_tmem_st32(o_addr + (uint32_t)c, v);
+            }
+            ta_tmem_wait_st();
+          }
+        }
+        const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+        const uint64_t scale2 = ta_pack2(p.scale_log2, p.scale_log2), negm2 = ta_pack2(-m_use, -m_use);
+        uint64_t sum2 = ta_pack2(0.f, 0.f);
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          float y0, y1;
+          ta_unpack2(ta_fma2(ta_pack2(xs[2 * e], xs[2 * e + 1]), scale2, negm2), y0, y1);
+          const float p0 = exp2_approx(y0), p1 = exp2_approx(y1);        // 2^-inf = 0 for masked keys
+          sum2 = ta_add2(sum2, ta_pack2(p0, p1));
+          __nv_bfloat162 b2 = __floats2bfloat162_rn(p0, p1);
+          w[e] = *reinterpret_cast<uint32_t*>(&b2);
+        }
+        ta_tmem_st32(s_addr + (uint32_t)b * 64u, w);
+        ta_tmem_wait_st();
+        {
+          float s0, s1;
+          ta_unpack2(sum2, s0, s1);
+          l_run += s0 + s1;
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) ta_mbar_arrive(p_full(t, b));
+      }
+      if (!ok) break;
+      mine += g.blocks;
+      const int j = mine - 1;
+      ok = ta_mbar_wait(pv_done(t, j & 1), (uint32_t)((j >> 1) & 1), abort_flag, SC_ERR_O_FULL);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (warp_valid) {
+        const size_t row = g.row + (size_t)(two ? t * per * G : 0) + r;
+        if (valid) *reinterpret_cast<float2*>(p.part_ml + row * 2) = make_float2(m_ref, l_run);
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t v[32];
+          ta_tmem_ld32(o_addr + (uint32_t)c, v);               // warp-wide: rows without a token take part and write nothing
+          if (valid) {
+            uint4* dst = reinterpret_cast<uint4*>(p.part_o + row * D + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[e] = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          }
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) ta_mbar_arrive(o_free(t));
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+template <int D>
+static cudaError_t sc_launch(const SharedParams& p, int ctas, cudaStream_t stream) {
+  constexpr int smem = ScLayout<D>::BYTES + 1024;
+  static_assert(smem + sizeof(SharedPlan) + 64 <= 227 * 1024, "shared memory of a CTA");
+  static std::atomic<unsigned long long> configured{0ull};     // a bit a device
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  if (!(configured.load() >> (device & 63) & 1ull)) {
+    e = cudaFuncSetAttribute(attention_shared_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    configured.fetch_or(1ull << (device & 63));
+  }
+  return launch(attention_shared_tc_kernel<D>, dim3(ctas), dim3(SC_THREADS), smem, stream, p);
+}
+
+bool attention_shared_tc_takes(int dtype, int group, int head_dim, int page_size) {
+  return dtype == LB_BF16 && (head_dim == 64 || head_dim == 128) && group <= TA_ROWS && page_size >= 8 && (page_size & (page_size - 1)) == 0;
+}
+
+void attention_shared_tc_cut(int group, int& tile_tokens, int& lane_tokens) {
+  lane_tokens = TA_ROWS / group;
+  tile_tokens = 2 * lane_tokens;
+}
+
+cudaError_t attention_shared_tc(const SharedParams& p, int ctas, cudaStream_t stream) {
+  return p.dim == 64 ? sc_launch<64>(p, ctas, stream) : sc_launch<128>(p, ctas, stream);
+}
+
+}  // namespace lb
+
+// Reads and clears the flag a bounded wait of this kernel sets when it gives up (0: none).
+LB_EXPORT int lb_attention_shared_device_error() {
+  int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, lb::g_attention_tc_error, sizeof(int)) != cudaSuccess) return -1;
+  if (v != 0) cudaMemcpyToSymbol(lb::g_attention_tc_error, &zero, sizeof(int));
+  return v;
+}

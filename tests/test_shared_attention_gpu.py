@@ -164,6 +164,16 @@ def test_odd_groups(ops, dtype):
     c.check(ops)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_runs_of_blocks(ops, dim):
+    """More blocks of keys for every CTA than its ring holds, in segments of one tile and of two, long ones beside short ones."""
+    rng = random.Random(dim)
+    requests = [(0, 1, 4096 + rng.randint(1, 2000)) for _ in range(9)] + [(-1, 1, rng.randint(1, 3000)) for _ in range(6)] + \
+               [(1, 20, 1500 + rng.randint(20, 900)) for _ in range(4)] + [(-1, 90, 1200)]
+    rng.shuffle(requests)
+    Batch(16, 8, dim, 16, requests, [4096, 1500], torch.bfloat16).check(ops)
+
+
 def test_large_scores_and_equal_keys(ops):
     """A running maximum that grows from block to block, and one that is the first key's; all keys alike."""
     for sign in (1.0, -1.0):

@@ -37,16 +37,15 @@ __global__ void __launch_bounds__(AP_THREADS) attention_shared_plain_kernel(Shar
   pdl_trigger();
   pdl_wait();
   as_make_plan(p, plan, gridDim.x);
-  as_write_records(p, plan, blockIdx.x, gridDim.x);
+  as_write_records(p, plan, blockIdx.x, gridDim.x, threadIdx.x, AP_THREADS);
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const T* q = reinterpret_cast<const T*>(p.q);
   const T* kc = reinterpret_cast<const T*>(p.k_cache);
   const T* vc = reinterpret_cast<const T*>(p.v_cache);
   const int d = p.dim, G = p.group, cache_heads = p.kv_heads / p.kv_share;
-  long long x = (long long)blockIdx.x * plan.span;
-  const long long x_end = min(x + plan.span, (long long)plan.units * p.kv_heads);
-  while (x < x_end) {
-    const Segment g = as_next(p, plan, blockIdx.x, x, x_end);
+  Walk way = as_begin(p, plan, blockIdx.x);
+  while (way.x < way.x_end) {
+    const Segment g = as_next(p, plan, blockIdx.x, way);
     if (g.blocks == 0) continue;
     const int rows = g.tokens * G;
     __syncthreads();
@@ -73,7 +72,7 @@ __global__ void __launch_bounds__(AP_THREADS) attention_shared_plain_kernel(Shar
     for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) o[e][c][0] = o[e][c][1] = o[e][c][2] = o[e][c][3] = 0.f;
-    const int* bt = p.table + (size_t)g.table_row * p.max_pages;
+    const int* bt = p.table + (size_t)g.request * p.max_pages;
     for (int b = g.block; b < g.block + g.blocks; ++b) {
       const int k0 = (g.key_lo & ~(AS_KEYS - 1)) + b * AS_KEYS;
       __syncthreads();                   // the block before has been read
@@ -162,7 +161,7 @@ __global__ void __launch_bounds__(AP_THREADS) attention_shared_plain_kernel(Shar
 #pragma unroll
       for (int c = 0; c < D / 64; ++c)
         if (64 * c + 4 * tx < d)
-          *reinterpret_cast<float4*>(p.part_o + (g.row + r) * d + 64 * c + 4 * tx) = make_float4(o[e][c][0], o[e][c][1], o[e][c][2], o[e][c][3]);
+          *reinterpret_cast<float4*>(p.part_o + g.row * d + ((16 * c + tx) * rows + r) * 4) = make_float4(o[e][c][0], o[e][c][1], o[e][c][2], o[e][c][3]);
     }
   }
 }
@@ -203,7 +202,7 @@ static cudaError_t ap_launch(const SharedParams& p, int ctas, cudaStream_t strea
 
 template <typename T>
 static cudaError_t as_combine(const SharedParams& p, cudaStream_t stream) {
-  return launch(as_combine_kernel<T>, dim3((unsigned)(((long long)p.T * p.heads + 7) / 8)), dim3(256), 0, stream, p);
+  return launch(as_combine_kernel<T>, dim3(p.T, p.kv_heads), dim3(AS_COMBINE_THREADS), 0, stream, p);
 }
 
 }  // namespace lb
@@ -251,9 +250,14 @@ LB_EXPORT int lb_attention_shared(int dtype, const void* q, void* out, const voi
   p.cu = cu_tokens; p.ctx = context_lens; p.prefix_of = prefix_of; p.prefix_lens = prefix_lens;
   p.T = num_tokens; p.S = num_seqs; p.heads = num_q_heads; p.kv_heads = num_kv_heads * cut.share; p.group = cut.group; p.dim = head_dim;
   p.page_size = page_size; p.page_shift = -1; p.kv_share = cut.share; p.tile_tokens = cut.tile_tokens; p.lane_tokens = cut.lane_tokens;
-  p.min_span = cut.tc ? 4 : 1;
+  p.min_span = cut.tc ? 2 : 1;
   for (int b = 0; b < 31; ++b) if ((1 << b) == page_size) p.page_shift = b;
   p.scale_log2 = scale * 1.4426950408889634f;
+  // units of the whole line, at most
+  const long long tiles = 2ll * ((long long)num_tokens / p.tile_tokens + num_seqs), blocks = (long long)max_pages * page_size / lb::AS_KEYS + 1;
+  LB_CHECK_ARG(tiles * 2 * blocks * p.kv_heads < (1ll << 31) - 65536, "attention_shared: %d tokens of %d requests on tables of %d pages are too much for one launch",
+               num_tokens, num_seqs, max_pages);
+  LB_CHECK_ARG(p.kv_heads <= 65535, "attention_shared: %d kv heads", p.kv_heads);
   const long long rows = (need_floats) / (head_dim + 2);
   p.part_o = floats; p.part_ml = floats + rows * head_dim;
   p.rec = ints; p.head = ints + (long long)num_tokens * lb::AS_REC;

@@ -17,9 +17,9 @@
 
 namespace lb {
 
-constexpr int AS_MAX_SEQS = 512;
+constexpr int AS_MAX_SEQS = 256;
 constexpr int AS_KEYS = 64;
-constexpr int AS_REC = 8;                // integers a token in the combining kernel's list
+constexpr int AS_REC = 12;               // integers a token in the combining kernel's list
 
 struct SharedParams {
   const void* q; void* out;              // [T, heads, dim]
@@ -31,7 +31,9 @@ struct SharedParams {
   int tile_tokens, lane_tokens;          // tokens of a tile; a tile of more than lane_tokens counts twice
   int min_span;                          // least units a CTA takes
   float scale_log2;
-  float* part_o; float* part_ml;         // [rows][dim], [rows][2]
+  // Partial results: 4 consecutive dimensions of all rows of a tile, then the next 4 ([dim / 4][rows][4], so that threads with a row each
+  // write, and threads with a head each read, side by side), and [rows][2]: the reference value (-inf: no key) and the sum.
+  float* part_o; float* part_ml;
   int* rec; int* head;                   // [T][AS_REC], {units a kv head, units a CTA, rows a kv head, first token, end of the tokens}
 };
 
@@ -41,25 +43,27 @@ void attention_shared_tc_cut(int group, int& tile_tokens, int& lane_tokens);
 cudaError_t attention_shared_tc(const SharedParams& p, int ctas, cudaStream_t stream);
 
 struct SharedPlan {
-  int q0[AS_MAX_SEQS + 1], ctx[AS_MAX_SEQS];
-  int lead[AS_MAX_SEQS];                 // the row whose table holds the prefix this request shares, -1: none
+  int4 meta[AS_MAX_SEQS];                // lead (the row whose table holds the prefix that this request shares, -1: none), new tokens,
+                                         // context, tokens of the prefix in this row's table
+  int q0[AS_MAX_SEQS];                   // first token
   int rank[AS_MAX_SEQS];                 // tokens of the group in front of this request's
+  int led[AS_MAX_SEQS];                  // tokens of the group that this row leads
   int member[AS_MAX_SEQS];               // the groups' members, group by group
-  int first_member[AS_MAX_SEQS], members[AS_MAX_SEQS], tokens[AS_MAX_SEQS], prefix[AS_MAX_SEQS];     // of the group led by this row
-  int unit[2 * AS_MAX_SEQS + 1];         // where the entries begin in the line: groups by their leader, then requests
-  int row[2 * AS_MAX_SEQS];              // and in the list of rows
-  int scratch[2 * AS_MAX_SEQS];
-  int units, span, rows;                 // of a kv head; of a CTA; of a kv head
+  int first_member[AS_MAX_SEQS + 1];     // of the group that this row leads
+  int unit[2 * AS_MAX_SEQS], row[2 * AS_MAX_SEQS], place[2 * AS_MAX_SEQS];     // of entry e (groups by their leader, then requests): where it
+                                         // begins in the line, in the list of rows and among the entries that are not empty
+  int2 entry[2 * AS_MAX_SEQS];           // of those: first unit, e
+  int entries, units, span, rows;        // how many; units and rows of a kv head, units of a CTA
 };
 
 __device__ __forceinline__ int as_blocks(int lo, int hi) { return hi > lo ? (hi - (lo & ~(AS_KEYS - 1)) + AS_KEYS - 1) / AS_KEYS : 0; }
-__device__ __forceinline__ int as_visible(const SharedParams& p, int ctx) { return min(ctx, p.max_pages * p.page_size); }
 
 // Units of `tokens` tokens in tiles with `blocks` blocks each.
 __device__ __forceinline__ int as_units(const SharedParams& p, int tokens, int blocks) {
   if (tokens <= 0 || blocks <= 0) return 0;
-  const int full = (tokens - 1) / p.tile_tokens, last = tokens - full * p.tile_tokens;
   const int twice = p.tile_tokens > p.lane_tokens ? 2 : 1;
+  if (tokens <= p.tile_tokens) return blocks * (tokens > p.lane_tokens ? 2 : 1);
+  const int full = (tokens - 1) / p.tile_tokens, last = tokens - full * p.tile_tokens;
   return blocks * (full * twice + (last > p.lane_tokens ? 2 : 1));
 }
 
@@ -81,120 +85,109 @@ __device__ __forceinline__ int as_scan(int* a, int n) {
   return total;
 }
 
-// Made by all threads of a CTA (three warps at least); ends with a barrier.
+// Made by all threads of a CTA (four warps at least); ends with a barrier.
 __device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& pl, int ctas) {
   const int tid = threadIdx.x, n = p.S;
-  for (int s = tid; s <= n; s += blockDim.x) pl.q0[s] = min(max(p.cu[s], 0), p.T);
+  const int most = p.max_pages * p.page_size;
   for (int s = tid; s < n; s += blockDim.x) {
-    const int l = p.prefix_of[s];
-    pl.lead[s] = l >= 0 && l < n ? l : -1;
-    pl.prefix[s] = as_visible(p, max(p.prefix_lens[s], 0));
-    pl.ctx[s] = as_visible(p, max(p.ctx[s], 0));
-  }
-  __syncthreads();
-  if (tid < 32) {                        // never falling, whatever the caller's numbers are
-    int most = 0;
-    for (int i = 0; i <= n; i += 32) {
-      int v = i + tid <= n ? pl.q0[i + tid] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(0xffffffffu, v, o);
-        if (tid >= o) v = max(v, t);
-      }
-      v = max(v, most);
-      if (i + tid <= n) pl.q0[i + tid] = v;
-      most = __shfl_sync(0xffffffffu, v, 31);
-    }
+    const int a = __ldcg(p.cu + s), b = __ldcg(p.cu + s + 1), c = __ldcg(p.ctx + s), l = __ldcg(p.prefix_of + s), f = __ldcg(p.prefix_lens + s);
+    const int q0 = min(max(a, 0), p.T);
+    pl.q0[s] = q0;
+    pl.meta[s] = make_int4(l >= 0 && l < n ? l : -1, max(min(b, p.T) - q0, 0), min(max(c, 0), most), min(max(f, 0), most));
   }
   __syncthreads();
   // Who shares with whom: every request looks at all others (n is a few dozen, a few hundred at most).
   for (int s = tid; s < n; s += blockDim.x) {
-    const int l = pl.lead[s];
-    int rank = 0, tokens = 0, before = 0, all = 0;
-    int led = 0, led_tokens = 0;
+    const int4 me = pl.meta[s];
+    const int l = me.x;
+    int rank = 0, before = 0, all = 0, led = 0, led_tokens = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) {
-      const int lj = pl.lead[j], qj = pl.q0[j + 1] - pl.q0[j];
-      if (l >= 0 && lj == l) {
-        ++all;
-        tokens += qj;
-        if (j < s) { ++before; rank += qj; }
-      }
-      if (lj == s) { ++led; led_tokens += qj; }
+      const int2 o = *reinterpret_cast<const int2*>(&pl.meta[j]);
+      const bool same = o.x == l && l >= 0, mine = o.x == s;
+      all += same ? 1 : 0;
+      before += same && j < s ? 1 : 0;
+      rank += same && j < s ? o.y : 0;
+      led += mine ? 1 : 0;
+      led_tokens += mine ? o.y : 0;
     }
-    pl.rank[s] = rank;
-    pl.members[s] = led;
-    pl.tokens[s] = led_tokens;
-    pl.scratch[s] = before;
+    // A group of one, or a prefix shorter than a block, is not worth a tile of its own.
+    const int prefix = l >= 0 ? pl.meta[l].w : 0;
+    const bool shares = all >= 2 && prefix >= AS_KEYS, leads = led >= 2 && me.w >= AS_KEYS;
+    pl.rank[s] = shares ? rank : -1;
+    pl.led[s] = led_tokens;
+    pl.member[s] = before;               // until the list is made
+    pl.first_member[s] = led;
+    const int ua = leads ? as_units(p, led_tokens, as_blocks(0, me.w)) : 0, ub = as_units(p, me.y, as_blocks(shares ? prefix : 0, me.z));
+    pl.unit[s] = ua; pl.unit[n + s] = ub;
+    pl.row[s] = leads ? led_tokens * p.group : 0; pl.row[n + s] = me.y * p.group;
+    pl.place[s] = ua > 0 ? 1 : 0; pl.place[n + s] = ub > 0 ? 1 : 0;
   }
   __syncthreads();
-  for (int s = tid; s < n; s += blockDim.x) pl.first_member[s] = pl.members[s];
-  __syncthreads();
-  if (tid < 32) as_scan(pl.first_member, n);
-  __syncthreads();
-  for (int s = tid; s < n; s += blockDim.x) {
-    const int l = pl.lead[s];
-    if (l >= 0) pl.member[pl.first_member[l] + pl.scratch[s]] = s;
-  }
-  __syncthreads();
-  // A group of one, or a prefix shorter than a block, is not worth a tile of its own.
-  for (int s = tid; s < n; s += blockDim.x)
-    if (pl.members[s] < 2 || pl.prefix[s] < AS_KEYS) pl.members[s] = 0;
-  __syncthreads();
-  for (int s = tid; s < n; s += blockDim.x) {
-    const int l = pl.lead[s];
-    const bool shares = l >= 0 && pl.members[l] > 0;
-    if (!shares) pl.lead[s] = -1;
-    const int q = pl.q0[s + 1] - pl.q0[s];
-    const bool leads = pl.members[s] > 0;
-    pl.unit[s] = leads ? as_units(p, pl.tokens[s], as_blocks(0, pl.prefix[s])) : 0;
-    pl.row[s] = leads ? pl.tokens[s] * p.group : 0;
-    pl.unit[n + s] = as_units(p, q, as_blocks(shares ? pl.prefix[l] : 0, pl.ctx[s]));
-    pl.row[n + s] = q * p.group;
-  }
-  __syncthreads();
-  if (tid < 32) {
+  const int warp = tid >> 5;
+  if (warp == 0) {
     const int u = as_scan(pl.unit, 2 * n);
-    if (tid == 0) {
-      pl.unit[2 * n] = u;
-      pl.units = u;
-      pl.span = max((int)(((long long)u * p.kv_heads + ctas - 1) / ctas), p.min_span);
-    }
-  } else if (tid < 64) {
+    if (tid == 0) pl.units = u;
+  } else if (warp == 1) {
     const int r = as_scan(pl.row, 2 * n);
-    if (tid == 32) pl.rows = r;
+    if ((tid & 31) == 0) pl.rows = r;
+  } else if (warp == 2) {
+    const int e = as_scan(pl.place, 2 * n);
+    if ((tid & 31) == 0) pl.entries = e;
+  } else if (warp == 3) {
+    const int m = as_scan(pl.first_member, n);
+    if ((tid & 31) == 0) pl.first_member[n] = m;
   }
+  __syncthreads();
+  // cu_tokens that fall would make more rows than there is room for: nothing is done then
+  const int units = pl.rows > 2 * p.T * p.group ? 0 : pl.units;
+  if (tid == 0) pl.span = max((int)(((unsigned)units * (unsigned)p.kv_heads + (unsigned)ctas - 1u) / (unsigned)ctas), p.min_span);
+  for (int e = tid; e < 2 * n; e += blockDim.x) {
+    const int end = e + 1 < 2 * n ? pl.place[e + 1] : pl.entries;
+    if (pl.place[e] < end) pl.entry[pl.place[e]] = make_int2(pl.unit[e], e);
+  }
+  int l = -1, before = 0;
+  for (int s0 = 0; s0 < n; s0 += blockDim.x) {      // (one round: n is at most 256)
+    const int s = s0 + tid;
+    if (s < n) { l = pl.meta[s].x; before = pl.member[s]; }
+    __syncthreads();
+    if (s < n && l >= 0) pl.member[pl.first_member[l] + before] = s;
+    if (s < n && pl.rank[s] < 0) pl.meta[s].x = -1;
+  }
+  if (tid == 0) pl.units = units;
   __syncthreads();
 }
 
-// What the combining kernel has to know of every token: for the prefix and for the request's own keys, the token's first row, the unit of
-// its tile's first block, and how many units further the last block begins (-1: no block).
-__device__ __forceinline__ void as_write_records(const SharedParams& p, const SharedPlan& pl, int cta, int ctas) {
-  if (cta == 0 && threadIdx.x == 0) { p.head[0] = pl.units; p.head[1] = pl.span; p.head[2] = pl.rows; p.head[3] = pl.q0[0]; p.head[4] = pl.q0[p.S]; }
-  for (int s = cta; s < p.S; s += ctas) {
-    const int t0 = pl.q0[s], q = pl.q0[s + 1] - t0, l = pl.lead[s];
-    for (int i = threadIdx.x; i < q; i += blockDim.x) {
-      int r[AS_REC];
-      auto place = [&](int* at, int e, int index, int tokens, int row_blocks, int all_blocks) {
-        const int tile = index / p.tile_tokens, first = tile * p.tile_tokens;
-        const int w = min(tokens - first, p.tile_tokens) > p.lane_tokens ? 2 : 1;
-        const int twice = p.tile_tokens > p.lane_tokens ? 2 : 1;
-        at[0] = pl.row[e] + index * p.group;
-        at[1] = pl.unit[e] + tile * all_blocks * twice;
-        at[2] = row_blocks > 0 ? (row_blocks - 1) * w : -1;
-      };
-      r[0] = r[1] = 0; r[2] = -1;
+// What the combining kernel has to know of every token, for the prefix and for the request's own keys: the first row of the token's
+// tile, the token's first row in the tile, the tile's rows, the unit of its first block, and how many units further the last block begins
+// (-1: no block).  By `threads` threads of each CTA; the CTAs without work come first.
+__device__ __forceinline__ void as_write_records(const SharedParams& p, const SharedPlan& pl, int cta, int ctas, int thread, int threads) {
+  if (cta == 0 && thread == 0) {
+    p.head[0] = pl.units; p.head[1] = pl.span; p.head[2] = pl.rows;
+    p.head[3] = p.S > 0 ? pl.q0[0] : 0;
+    p.head[4] = p.S > 0 ? pl.q0[p.S - 1] + pl.meta[p.S - 1].y : 0;
+  }
+  const int twice = p.tile_tokens > p.lane_tokens ? 2 : 1;
+  for (int s = ctas - 1 - cta; s < p.S; s += ctas) {
+    const int4 me = pl.meta[s];
+    const int t0 = pl.q0[s], q = me.y, l = me.x;
+    const int prefix = l >= 0 ? pl.meta[l].w : 0;
+    for (int i = thread; i < q; i += threads) {
+      int4 a = make_int4(0, 0, 0, 0);
+      int a_last = -1;
       if (l >= 0) {
-        const int nb = as_blocks(0, pl.prefix[l]);
-        place(r, l, pl.rank[s] + i, pl.tokens[l], nb, nb);
+        const int index = pl.rank[s] + i, tokens = pl.led[l], nb = as_blocks(0, prefix);
+        const int tile = index / p.tile_tokens, first = tile * p.tile_tokens, here = min(tokens - first, p.tile_tokens);
+        a = make_int4(pl.row[l] + first * p.group, (index - first) * p.group, here * p.group, pl.unit[l] + tile * nb * twice);
+        a_last = (nb - 1) * (here > p.lane_tokens ? 2 : 1);
       }
-      const int lo = l >= 0 ? pl.prefix[l] : 0;
-      const int tile_end = min((i / p.tile_tokens + 1) * p.tile_tokens, q);
-      const int hi = min(pl.ctx[s], pl.ctx[s] - q + tile_end);      // keys the tile's last token sees
-      place(r + 3, p.S + s, i, q, as_blocks(lo, hi), as_blocks(lo, pl.ctx[s]));
-      r[6] = r[7] = 0;
+      const int tile = i / p.tile_tokens, first = tile * p.tile_tokens, here = min(q - first, p.tile_tokens), e = p.S + s;
+      const int nb = as_blocks(prefix, min(me.z, me.z - q + first + here));      // blocks that the tile's last token sees
+      const int4 b = make_int4(pl.row[e] + first * p.group, (i - first) * p.group, here * p.group,
+                               pl.unit[e] + tile * as_blocks(prefix, me.z) * twice);
+      const int b_last = nb > 0 ? (nb - 1) * (here > p.lane_tokens ? 2 : 1) : -1;
       int4* dst = reinterpret_cast<int4*>(p.rec + (size_t)(t0 + i) * AS_REC);
-      dst[0] = make_int4(r[0], r[1], r[2], r[3]);
-      dst[1] = make_int4(r[4], r[5], r[6], r[7]);
+      dst[0] = a; dst[1] = b; dst[2] = pl.units > 0 ? make_int4(a_last, b_last, 0, 0) : make_int4(-1, -1, 0, 0);
     }
   }
 }
@@ -202,62 +195,86 @@ __device__ __forceinline__ void as_write_records(const SharedParams& p, const Sh
 // A run of blocks of one tile and one kv head.
 struct Segment {
   int kv_head;
-  int table_row;
-  int shared;                            // leader of the group, -1: rows of one request
-  int request;                           // whose rows they are, if not shared
-  int first;                             // shared: rank in the group of the first token; else the first token's place in the request
-  int tokens;
+  int request;                           // the row of the block table; whose tokens they are, if not shared
+  bool shared;                           // tokens of the members of the group that `request` leads
+  int first, tokens;                     // first token (of the group, of the request), and how many
   int key_lo, key_hi;                    // keys of the tile (of all its rows together)
   int block, blocks;                     // first block of the run (of the tile's), and how many (0: none are there)
-  size_t row;                            // where its partial rows begin
+  long long row;                         // where the tile's partial rows begin
 };
 
-// The segment at unit x of the line (0 <= x < units * kv_heads), cut off at x_end; x moves behind it.
-__device__ __forceinline__ Segment as_next(const SharedParams& p, const SharedPlan& pl, int cta, long long& x, long long x_end) {
-  Segment g;
-  g.kv_head = (int)(x / pl.units);
-  const int u = (int)(x - (long long)g.kv_head * pl.units);
-  int a = 0, b = 2 * p.S - 1;            // the last entry that begins at or before u: the one that holds it
-  while (a < b) {
-    const int mid = (a + b + 1) >> 1;
-    if (pl.unit[mid] <= u) a = mid; else b = mid - 1;
+// A CTA's way along the line: where it is, and which entry and tile that is in.
+struct Walk { int x, x_end, kv_head, at, tile; };
+
+__device__ __forceinline__ int as_tile_units(const SharedParams& p, int blocks) { return p.tile_tokens > p.lane_tokens ? 2 * blocks : blocks; }
+__device__ __forceinline__ int as_entry_blocks(const SharedParams& p, const SharedPlan& pl, int e) {
+  if (e < p.S) return as_blocks(0, pl.meta[e].w);
+  const int4 me = pl.meta[e - p.S];
+  return as_blocks(me.x >= 0 ? pl.meta[me.x].w : 0, me.z);
+}
+
+__device__ __forceinline__ Walk as_begin(const SharedParams& p, const SharedPlan& pl, int cta) {
+  Walk w;
+  const int total = pl.units * p.kv_heads;
+  w.x = min(cta * pl.span, total);
+  w.x_end = min(w.x + pl.span, total);
+  w.kv_head = w.at = w.tile = 0;
+  if (w.x < w.x_end) {
+    w.kv_head = (int)((unsigned)w.x / (unsigned)pl.units);
+    const int u = w.x - w.kv_head * pl.units;
+    int a = 0, b = pl.entries - 1;       // the last entry that begins at or before u
+    while (a < b) {
+      const int mid = (a + b + 1) >> 1;
+      if (pl.entry[mid].x <= u) a = mid; else b = mid - 1;
+    }
+    w.at = a;
+    const int2 e = pl.entry[a];
+    w.tile = (int)((unsigned)(u - e.x) / (unsigned)as_tile_units(p, as_entry_blocks(p, pl, e.y)));
   }
-  const bool shared = a < p.S;
-  const int s = shared ? a : a - p.S;
-  const int q = pl.q0[s + 1] - pl.q0[s];
-  const int tokens = shared ? pl.tokens[s] : q;
-  const int lead = shared ? -1 : pl.lead[s];
-  const int lo = lead >= 0 ? pl.prefix[lead] : 0;
-  const int nb = shared ? as_blocks(0, pl.prefix[s]) : as_blocks(lo, pl.ctx[s]);
-  const int twice = p.tile_tokens > p.lane_tokens ? 2 : 1;
-  const int tile = (u - pl.unit[a]) / (nb * twice);
-  const int tile_unit = pl.unit[a] + tile * nb * twice;
-  g.table_row = s;
-  g.shared = shared ? s : -1;
+  return w;
+}
+
+// The segment at w.x (< w.x_end); w moves behind it.
+__device__ __forceinline__ Segment as_next(const SharedParams& p, const SharedPlan& pl, int cta, Walk& w) {
+  Segment g;
+  const int2 e = pl.entry[w.at];
+  g.kv_head = w.kv_head;
+  g.shared = e.y < p.S;
+  const int s = g.shared ? e.y : e.y - p.S;
+  const int4 me = pl.meta[s];
+  const int tokens = g.shared ? pl.led[s] : me.y;
+  const int hi = g.shared ? me.w : me.z;
+  g.key_lo = !g.shared && me.x >= 0 ? pl.meta[me.x].w : 0;
+  const int nb = as_blocks(g.key_lo, hi);
   g.request = s;
-  g.first = tile * p.tile_tokens;
+  g.first = w.tile * p.tile_tokens;
   g.tokens = min(tokens - g.first, p.tile_tokens);
-  const int w = g.tokens > p.lane_tokens ? 2 : 1;
-  g.key_lo = lo;
-  g.key_hi = shared ? pl.prefix[s] : min(pl.ctx[s], pl.ctx[s] - q + g.first + g.tokens);
-  const long long base = (long long)g.kv_head * pl.units + tile_unit;
-  const int there = as_blocks(lo, g.key_hi);           // a portion's earlier tiles see fewer blocks than its last
+  const int two = g.tokens > p.lane_tokens ? 1 : 0;              // units of a block: 1 << two
+  g.key_hi = g.shared ? hi : min(hi, hi - tokens + g.first + g.tokens);
+  const int base = w.kv_head * pl.units + e.x + w.tile * as_tile_units(p, nb);
+  const int there = as_blocks(g.key_lo, g.key_hi);               // a portion's earlier tiles see fewer blocks than its last
   // a block belongs to the CTA in whose piece it begins
-  const int from = (int)((x - base + w - 1) / w);
-  const long long end = min(x_end, base + (long long)nb * w);
-  const int to = min((int)((end - base + w - 1) / w), there);
-  g.block = from;
-  g.blocks = max(to - from, 0);
-  g.row = (size_t)g.kv_head * pl.rows + pl.row[a] + (size_t)g.first * p.group + (size_t)cta * p.tile_tokens * p.group;
-  x = end;
+  const int tile_end = base + (nb << two), end = min(w.x_end, tile_end);
+  g.block = (w.x - base + two) >> two;
+  g.blocks = max(min((end - base + two) >> two, there) - g.block, 0);
+  g.row = (long long)w.kv_head * pl.rows + pl.row[e.y] + g.first * p.group + (long long)cta * p.tile_tokens * p.group;
+  w.x = end;
+  if (end == tile_end) {
+    if (g.first + g.tokens < tokens) {
+      ++w.tile;
+    } else {
+      w.tile = 0;
+      if (++w.at == pl.entries) { w.at = 0; ++w.kv_head; }
+    }
+  }
   return g;
 }
 
 // The i-th token of a segment: its place in the step, and the last key it sees.
 __device__ __forceinline__ void as_token(const SharedPlan& pl, const Segment& g, int i, int& token, int& position) {
   int s = g.request, at = g.first + i;
-  if (g.shared >= 0) {                   // the member whose tokens these are: the last one whose first token is not behind
-    int a = pl.first_member[g.shared], b = a + pl.members[g.shared] - 1;
+  if (g.shared) {                        // the member whose tokens these are: the last one whose first token is not behind
+    int a = pl.first_member[s], b = pl.first_member[s + 1] - 1;
     while (a < b) {
       const int mid = (a + b + 1) >> 1;
       if (pl.rank[pl.member[mid]] <= at) a = mid; else b = mid - 1;
@@ -266,7 +283,8 @@ __device__ __forceinline__ void as_token(const SharedPlan& pl, const Segment& g,
     at -= pl.rank[s];
   }
   token = pl.q0[s] + at;
-  position = pl.ctx[s] - (pl.q0[s + 1] - pl.q0[s]) + at;
+  const int4 me = pl.meta[s];
+  position = me.z - me.y + at;
 }
 
 __device__ __forceinline__ void as_store4(float* dst, float a, float b, float c, float d) { *reinterpret_cast<float4*>(dst) = make_float4(a, b, c, d); }
@@ -275,82 +293,60 @@ __device__ __forceinline__ void as_store4(bf16* dst, float a, float b, float c, 
   *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
 }
 
-// out[t, h] = sum 2^(m - M) o / sum 2^(m - M) l over the partial results of a row, in the order of the line: one warp a row.
-// Partial results with m = -inf weigh nothing and their o is not read.
+// out[t, h] = sum 2^(m - M) o / sum 2^(m - M) l over the partial results of a row, in the order of the line.  A block has one token and kv
+// head; a thread one head of the group (neighbouring threads neighbouring heads: rows that lie side by side) and four dimensions.  The
+// partial results are read eight at a time, all at once; one with m = -inf weighs nothing.
+constexpr int AS_COMBINE_THREADS = 128;
 template <typename T>
-__global__ void __launch_bounds__(256) as_combine_kernel(SharedParams p) {
+__global__ void __launch_bounds__(AS_COMBINE_THREADS) as_combine_kernel(SharedParams p) {
   pdl_trigger();
   const int* rec = p.rec;
   const int* head = p.head;
+  const int t = blockIdx.x, kv = blockIdx.y;
   pdl_wait(rec, head);
-  const int lane = threadIdx.x & 31;
-  const int item = (blockIdx.x * 256 + threadIdx.x) >> 5;
-  if (item >= p.T * p.heads) return;
-  const int t = item / p.heads, h = item % p.heads, kv = h / p.group;
-  if (t < __ldcg(head + 3) || t >= __ldcg(head + 4)) return;         // rows of no request stay as they were
-  const int4 r0 = __ldcg(reinterpret_cast<const int4*>(rec + (size_t)t * AS_REC));
-  const int4 r1 = __ldcg(reinterpret_cast<const int4*>(rec + (size_t)t * AS_REC) + 1);
-  const int units = __ldcg(head), span = __ldcg(head + 1), rows = __ldcg(head + 2);
-  const long long line = (long long)kv * units;
-  // the two runs of partial results: first CTA, number, first row
-  int c0[2], n[2];
-  size_t row[2];
-  const int first_row[2] = {r0.x, r0.w}, unit[2] = {r0.y, r1.x}, last[2] = {r0.z, r1.y};
+  const int4* r = reinterpret_cast<const int4*>(rec + (size_t)t * AS_REC);
+  const int4 a = __ldcg(r), b = __ldcg(r + 1), last = __ldcg(r + 2);
+  const int4 hd = __ldcg(reinterpret_cast<const int4*>(head));
+  if (t < hd.w || t >= __ldcg(head + 4)) return;               // rows of no request stay as they were
+  const unsigned line = (unsigned)kv * (unsigned)hd.x, span = (unsigned)hd.y;
+  const long long step = (long long)p.tile_tokens * p.group;
+  const int ca = (int)((line + a.w) / span), cb = (int)((line + b.w) / span);
+  const int na = last.x < 0 ? 0 : (int)((line + a.w + last.x) / span) - ca + 1, total = na + (last.y < 0 ? 0 : (int)((line + b.w + last.y) / span) - cb + 1);
+  const long long row_a = (long long)kv * hd.z + a.x + ca * step, row_b = (long long)kv * hd.z + b.x + cb * step;
+  const int chunks = p.dim / 4;
+  for (int i = threadIdx.x; i < p.group * chunks; i += AS_COMBINE_THREADS) {
+    const int h = i % p.group, c = i / p.group;
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int z0 = 0; z0 < total; z0 += 8) {
+      float2 ml[8];
+      float4 o[8];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    c0[i] = (int)((line + unit[i]) / span);
-    n[i] = last[i] < 0 ? 0 : (int)((line + unit[i] + last[i]) / span) - c0[i] + 1;
-    row[i] = (size_t)kv * rows + first_row[i] + h % p.group + (size_t)c0[i] * p.tile_tokens * p.group;
-  }
-  const size_t step = (size_t)p.tile_tokens * p.group;
-  const int total = n[0] + n[1];
-  auto row_of = [&](int i) { return i < n[0] ? row[0] + (size_t)i * step : row[1] + (size_t)(i - n[0]) * step; };
-  float M = -INFINITY, L = 0.f;
-  for (int i = lane; i < total; i += 32) M = fmaxf(M, __ldcg(p.part_ml + row_of(i) * 2));
-  M = warp_max(M);
-  T* out = reinterpret_cast<T*>(p.out) + (size_t)item * p.dim;
-  float acc[2][4];                       // dimensions lane * 4 + 128 c .. + 3
-  const int chunks = (p.dim + 127) / 128;
-#pragma unroll
-  for (int c = 0; c < 2; ++c) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.f;
-  if (M > -INFINITY) {
-    for (int i0 = 0; i0 < total; i0 += 32) {
-      const int i = i0 + lane;
-      float w = 0.f;
-      if (i < total) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + row_of(i) * 2));
-        w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
-        L += w * ml.y;
+      for (int u = 0; u < 8; ++u) {
+        const int z = z0 + u;
+        const bool of_a = z < na;
+        const long long tile = of_a ? row_a + z * step : row_b + (z - na) * step;
+        const int in = (of_a ? a.y : b.y) + h, rows = of_a ? a.z : b.z;
+        ml[u] = z < total ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + (tile + in) * 2)) : make_float2(-INFINITY, 0.f);
+        o[u] = z < total ? __ldcg(reinterpret_cast<const float4*>(p.part_o + tile * p.dim + ((long long)c * rows + in) * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
-      const int here = min(32, total - i0);
-      for (int j0 = 0; j0 < here; j0 += 8) {
-        float wj[8];
-        float4 a[8];
+      float m = M;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          if (c >= chunks) break;
-          const int d = lane * 4 + 128 * c;
+      for (int u = 0; u < 8; ++u) m = fmaxf(m, ml[u].x);
+      const float ref = m == -INFINITY ? 0.f : m;
+      const float f = exp2f(M - ref);                          // (0 at first: M = -inf)
+      L *= f; acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+      M = m;
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            wj[u] = __shfl_sync(0xffffffffu, w, (j0 + u) & 31);
-            if (j0 + u >= here) wj[u] = 0.f;
-            a[u] = wj[u] != 0.f && d < p.dim ? __ldcg(reinterpret_cast<const float4*>(p.part_o + row_of(i0 + j0 + u) * p.dim + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
-          }
-#pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            acc[c][0] = fmaf(wj[u], a[u].x, acc[c][0]); acc[c][1] = fmaf(wj[u], a[u].y, acc[c][1]);
-            acc[c][2] = fmaf(wj[u], a[u].z, acc[c][2]); acc[c][3] = fmaf(wj[u], a[u].w, acc[c][3]);
-          }
-        }
+      for (int u = 0; u < 8; ++u) {
+        if (ml[u].x == -INFINITY) continue;
+        const float w = exp2f(ml[u].x - ref);
+        L = fmaf(w, ml[u].y, L);
+        acc.x = fmaf(w, o[u].x, acc.x); acc.y = fmaf(w, o[u].y, acc.y); acc.z = fmaf(w, o[u].z, acc.z); acc.w = fmaf(w, o[u].w, acc.w);
       }
     }
-  }
-  L = warp_sum(L);
-  const float inv = L > 0.f ? 1.f / L : 0.f;
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int d = lane * 4 + 128 * c;
-    if (c < chunks && d < p.dim) as_store4(out + d, acc[c][0] * inv, acc[c][1] * inv, acc[c][2] * inv, acc[c][3] * inv);
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    as_store4(reinterpret_cast<T*>(p.out) + ((size_t)t * p.heads + (size_t)kv * p.group + h) * p.dim + 4 * c, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
   }
 }
 

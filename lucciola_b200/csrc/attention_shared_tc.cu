@@ -16,8 +16,9 @@
 // lets the line be cut evenly.
 //
 // Warps: 0 copies keys, 10 values (cp.async, 16 bytes a thread, swizzled for the tensor cores; four blocks each, three in flight); 1 issues
-// tile A's products and owns the tensor memory, 11 tile B's; 2..5 softmax of A, 6..9 of B.  Each walks the same segments by itself.  All
-// waits are bounded; when one gives up, the CTA records it and every role leaves.
+// tile A's products and owns the tensor memory, 11 tile B's; 2..5 softmax of A, 6..9 of B.  Each walks the same segments by itself.  Barriers tell one
+// turn from the next only, so each tile has barriers of its own for the stages of the rings, and a copying warp speaks to the tiles that
+// read a block.  All waits are bounded; when one gives up, the CTA records it and every role leaves.
 #include "attention_shared.cuh"
 #include "attention_tcgen05.cuh"
 
@@ -27,6 +28,7 @@ namespace lb {
 
 constexpr int SC_STAGES = 4;
 constexpr int SC_IN_FLIGHT = 2;                                // blocks a copying warp has requested beyond the one it waits for
+constexpr int SC_BARS = 4 * SC_STAGES + 8;                     // barriers of a tile
 constexpr int SC_THREADS = 384;
 enum : int { SC_ERR_Q = 401, SC_ERR_KV_FULL = 402, SC_ERR_KV_EMPTY = 403, SC_ERR_S_FULL = 404, SC_ERR_P_FULL = 405, SC_ERR_O_FULL = 406, SC_ERR_O_FREE = 407 };
 
@@ -37,9 +39,31 @@ template <int D> struct ScLayout {
   static constexpr int KV_HALF = AS_KEYS * 128, KV_TILE = HALVES * KV_HALF;
   static constexpr int Q_TILE = HALVES * TA_HALF_BYTES;
   static constexpr int K_OFF = 2 * Q_TILE, V_OFF = K_OFF + SC_STAGES * KV_TILE, BAR_OFF = V_OFF + SC_STAGES * KV_TILE;
-  static constexpr int BARS = 4 * SC_STAGES + 2 * 8;
-  static constexpr int BYTES = BAR_OFF + BARS * 8 + 16;
+  static constexpr int BYTES = BAR_OFF + 2 * SC_BARS * 8 + 16;
 };
+
+// One block of 64 keys (or values) of a kv head from the pages into a stage of the ring, by one warp: a lane copies 16-byte chunk c of the
+// rows rp, rp + RPI, ...  `stage` is the stage's address plus the lane's half and row, xr[u] its swizzled chunk in rows rp + RPI u; `head` points
+// at the lane's chunk and row of the head in page 0; lane i holds the id of the i-th page of the block (-1: no page; pages of more than 64 tokens:
+// `sub` is where in the page the block begins).  Keys outside lo .. hi - 1 and of no page are filled with zeros.
+template <int PS, int D>
+__device__ __forceinline__ void sc_copy_block(uint32_t stage, const uint32_t (&xr)[4], const uint8_t* head, int ids, int kb, int lo, int hi,
+                                              size_t page_stride, int rp, int sub) {
+  constexpr int RPI = 32 / (D / 8), ROW = D * 2;
+  const bool inner = kb >= lo && kb + AS_KEYS <= hi;           // every key of the block may be seen
+#pragma unroll
+  for (int pg = 0; pg < AS_KEYS / PS; ++pg) {
+    const int id = __shfl_sync(0xffffffffu, ids, pg);
+    const uint8_t* src = head + (size_t)max(id, 0) * page_stride + sub * ROW;
+#pragma unroll
+    for (int j = 0; j < PS / RPI; ++j) {
+      const int key = kb + pg * PS + rp + RPI * j;
+      const uint32_t bytes = (id >= 0 && (inner || (key >= lo && key < hi))) ? 16u : 0u;       // 0: sixteen zeros
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                   ::"r"(stage + xr[j & (8 / RPI - 1)] + (uint32_t)((pg * PS + RPI * j) * 128)), "l"(src + j * RPI * ROW), "r"(bytes) : "memory");
+    }
+  }
+}
 
 template <int D>
 __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(SharedParams p) {
@@ -49,27 +73,24 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = ta_smem_u32(smem);
   const uint32_t bars = sbase + L::BAR_OFF;
-  auto k_full = [&](int s) { return bars + 8u * s; };
-  auto k_empty = [&](int s) { return bars + 8u * (SC_STAGES + s); };
-  auto v_full = [&](int s) { return bars + 8u * (2 * SC_STAGES + s); };
-  auto v_empty = [&](int s) { return bars + 8u * (3 * SC_STAGES + s); };
-  // of tile t and S buffer b: S complete, P written, P V complete; of tile t: queries there, O read
-  auto s_full = [&](int t, int b) { return bars + 8u * (4 * SC_STAGES + t * 8 + b); };
-  auto p_full = [&](int t, int b) { return bars + 8u * (4 * SC_STAGES + t * 8 + 2 + b); };
-  auto pv_done = [&](int t, int b) { return bars + 8u * (4 * SC_STAGES + t * 8 + 4 + b); };
-  auto q_full = [&](int t) { return bars + 8u * (4 * SC_STAGES + t * 8 + 6); };
-  auto o_free = [&](int t) { return bars + 8u * (4 * SC_STAGES + t * 8 + 7); };
-  uint32_t* tmem_slot = (uint32_t*)(smem + L::BAR_OFF + L::BARS * 8);
+  // of tile t: keys (values) in stage s there, and read; of S buffer b: S complete, P written, P V complete; queries there, O read
+  auto k_full = [&](int t, int s) { return bars + 8u * (t * SC_BARS + s); };
+  auto k_empty = [&](int t, int s) { return bars + 8u * (t * SC_BARS + SC_STAGES + s); };
+  auto v_full = [&](int t, int s) { return bars + 8u * (t * SC_BARS + 2 * SC_STAGES + s); };
+  auto v_empty = [&](int t, int s) { return bars + 8u * (t * SC_BARS + 3 * SC_STAGES + s); };
+  auto s_full = [&](int t, int b) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + b); };
+  auto p_full = [&](int t, int b) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + 2 + b); };
+  auto pv_done = [&](int t, int b) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + 4 + b); };
+  auto q_full = [&](int t) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + 6); };
+  auto o_free = [&](int t) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + 7); };
+  uint32_t* tmem_slot = (uint32_t*)(smem + L::BAR_OFF + 2 * SC_BARS * 8);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
 
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < SC_STAGES; ++i) {
-      ta_mbar_init(k_full(i), 1); ta_mbar_init(k_empty(i), 2);             // both tiles are through with it: their products have read it, or do not
-      ta_mbar_init(v_full(i), 1); ta_mbar_init(v_empty(i), 2);
-    }
     for (int t = 0; t < 2; ++t) {
+      for (int i = 0; i < 4 * SC_STAGES; ++i) ta_mbar_init(k_full(t, i), 1);
       for (int b = 0; b < 2; ++b) { ta_mbar_init(s_full(t, b), 1); ta_mbar_init(p_full(t, b), 4); ta_mbar_init(pv_done(t, b), 1); }
       ta_mbar_init(q_full(t), 4); ta_mbar_init(o_free(t), 4);
     }
@@ -85,70 +106,80 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   as_make_plan(p, plan, gridDim.x);
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;            // columns: tile t's S buffers at t * 128 and t * 128 + 64 (P over their first 32), O at 256 + t * 128
-  as_write_records(p, plan, blockIdx.x, gridDim.x);
 
   const int G = p.group, per = p.lane_tokens, cta = blockIdx.x;
-  long long x = (long long)cta * plan.span;
-  const long long x_end = min(x + plan.span, (long long)plan.units * p.kv_heads);
-  int blocks_done = 0, singles = 0;            // blocks of all segments so far, segments of one tile so far
+  Walk way = as_begin(p, plan, cta);
+  int singles = 0;                             // segments of one tile so far: they go to tile A and B in turn
+  // the tiles that work on a segment, as bits
+  auto tiles_of = [&](const Segment& g) -> int { return g.tokens > per ? 3 : 1 << (singles++ & 1); };
 
   if (warp == 0 || warp == 10) {
     // ---- copies ------------------------------------------------------------------------------------------------------------------
     const bool is_v = warp == 10;
-    constexpr int CHUNKS = D / 8, RPI = 32 / CHUNKS, STEPS = AS_KEYS / RPI;      // 16-byte chunks of a row, rows an instruction
+    constexpr int CHUNKS = D / 8, RPI = 32 / CHUNKS;           // 16-byte chunks of a row, rows an instruction
     const int c = lane % CHUNKS, rp = lane / CHUNKS;
-    const uint8_t* pool = (const uint8_t*)(is_v ? p.v_cache : p.k_cache) + c * 16;
-    const uint32_t ring = sbase + (is_v ? L::V_OFF : L::K_OFF) + (uint32_t)(c >> 3) * L::KV_HALF;
-    const int ps = p.page_size, shift = p.page_shift;
+    const uint8_t* pool = (const uint8_t*)(is_v ? p.v_cache : p.k_cache) + c * 16 + rp * (D * 2);
+    const uint32_t ring = sbase + (is_v ? L::V_OFF : L::K_OFF) + (uint32_t)(c >> 3) * L::KV_HALF + (uint32_t)rp * 128u;
+    uint32_t xr[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) xr[u] = (uint32_t)(((c & 7) ^ ((rp + RPI * u) & 7)) << 4);
+    const int ps = p.page_size, shift = p.page_shift, size = min(ps, AS_KEYS);
     const size_t page_stride = (size_t)p.kv_heads * ps * (D * 2);
     bool ok = true;
-    auto hand_over = [&](int i) {              // block i (of all) has landed: visible to the tensor cores, then said so
+    int n = 0;                                 // blocks so far
+    uint32_t used = 0, turn[2] = {0, 0};       // of stage s: the tiles that read its block (bits 2 s, 2 s + 1); of tile t, bit s: the parity of its next wait
+    auto hand_over = [&](int i) {              // block i has landed: visible to the tensor cores, then said so to its tiles
+      const int s = i % SC_STAGES;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) ta_mbar_arrive(is_v ? v_full(i % SC_STAGES) : k_full(i % SC_STAGES));
+      if (lane < 2 && ((used >> (2 * s + lane)) & 1u)) ta_mbar_arrive(is_v ? v_full(lane, s) : k_full(lane, s));
     };
-    while (x < x_end && ok) {
-      const Segment g = as_next(p, plan, cta, x, x_end);
-      const int* bt = p.table + (size_t)g.table_row * p.max_pages;
+    while (way.x < way.x_end && ok) {
+      const Segment g = as_next(p, plan, cta, way);
+      if (g.blocks == 0) continue;
+      const uint32_t tiles = (uint32_t)tiles_of(g);
+      const int* bt = p.table + (size_t)g.request * p.max_pages;
       const uint8_t* head = pool + (size_t)g.kv_head * ps * (D * 2);
       const int first_key = (g.key_lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS;
-      // the page of key kb + lane * ps (of kb itself for pages of 64 tokens and more), -1 where no key of this segment lies
+      // lane i: the id of the i-th page of the block at kb, -1 where no key of this segment lies
       auto page_of = [&](int kb) -> int {
-        const int key = kb + lane * min(ps, AS_KEYS), size = min(ps, AS_KEYS);
+        const int key = kb + lane * size;
         if (lane * size >= AS_KEYS || key >= g.key_hi || key + size <= g.key_lo) return -1;
         const int id = bt[key >> shift];
         return id < p.num_pages ? id : -1;
       };
-      int ids = g.blocks > 0 ? page_of(first_key) : -1;
-      for (int b = 0; b < g.blocks; ++b) {
-        const int i = blocks_done + b, s = i % SC_STAGES, kb = first_key + b * AS_KEYS;
+      int ids = page_of(first_key);
+      for (int b = 0; b < g.blocks; ++b, ++n) {
+        const int s = n % SC_STAGES, kb = first_key + b * AS_KEYS;
+        const int next_ids = b + 1 < g.blocks ? page_of(kb + AS_KEYS) : -1;
+        // the tiles that read this stage's last block are through with it
+        const uint32_t before = (used >> (2 * s)) & 3u;
         int go = 1;
-        if (lane == 0) go = ta_mbar_wait_idle(is_v ? v_empty(s) : k_empty(s), (uint32_t)((i / SC_STAGES) & 1) ^ 1u, abort_flag, SC_ERR_KV_EMPTY) ? 1 : 0;
-        go = __shfl_sync(0xffffffffu, go, 0);
-        if (!go) { ok = false; break; }
-        const bool inner = kb >= g.key_lo && kb + AS_KEYS <= g.key_hi;
+        if (lane < 2 && ((before >> lane) & 1u))
+          go = ta_mbar_wait_idle(is_v ? v_empty(lane, s) : k_empty(lane, s), (turn[lane & 1] >> s) & 1u, abort_flag, SC_ERR_KV_EMPTY) ? 1 : 0;
+        if (__any_sync(0xffffffffu, go == 0)) { ok = false; break; }
+        turn[0] ^= (before & 1u) << s;
+        turn[1] ^= (before >> 1) << s;
+        used = (used & ~(3u << (2 * s))) | (tiles << (2 * s));
         const uint32_t stage = ring + (uint32_t)s * L::KV_TILE;
-#pragma unroll
-        for (int j = 0; j < STEPS; ++j) {
-          const int r = rp + RPI * j, key = kb + r;
-          const int id = __shfl_sync(0xffffffffu, ids, r >> min(shift, 6));
-          const uint32_t bytes = (id >= 0 && (inner || (key >= g.key_lo && key < g.key_hi))) ? 16u : 0u;       // 0: sixteen zeros
-          const uint8_t* src = head + (size_t)max(id, 0) * page_stride + (size_t)(key & (ps - 1)) * (D * 2);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                       ::"r"(stage + (uint32_t)r * 128u + (uint32_t)(((c & 7) ^ (r & 7)) << 4)), "l"(src), "r"(bytes) : "memory");
+        switch (ps) {
+          case 8: sc_copy_block<8, D>(stage, xr, head, ids, kb, g.key_lo, g.key_hi, page_stride, rp, 0); break;
+          case 16: sc_copy_block<16, D>(stage, xr, head, ids, kb, g.key_lo, g.key_hi, page_stride, rp, 0); break;
+          case 32: sc_copy_block<32, D>(stage, xr, head, ids, kb, g.key_lo, g.key_hi, page_stride, rp, 0); break;
+          default: sc_copy_block<64, D>(stage, xr, head, ids, kb, g.key_lo, g.key_hi, page_stride, rp, kb & (ps - 1)); break;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        ids = b + 1 < g.blocks ? page_of(kb + AS_KEYS) : -1;
-        if (i >= SC_IN_FLIGHT) {
+        if (n >= SC_IN_FLIGHT) {
           asm volatile("cp.async.wait_group %0;" ::"n"(SC_IN_FLIGHT) : "memory");
-          hand_over(i - SC_IN_FLIGHT);
+          hand_over(n - SC_IN_FLIGHT);
         }
+        ids = next_ids;
       }
-      if (ok) blocks_done += g.blocks;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (ok)
-      for (int i = max(blocks_done - SC_IN_FLIGHT, 0); i < blocks_done; ++i) hand_over(i);
+      for (int i = max(n - SC_IN_FLIGHT, 0); i < n; ++i) hand_over(i);
+    if (is_v) as_write_records(p, plan, cta, gridDim.x, lane, 32);         // while the last blocks are worked on
   } else if (warp == 1 || warp == 11) {
     // ---- products, one thread a tile -------------------------------------------------------------------------------------------------
     const int t = warp == 1 ? 0 : 1;
@@ -156,29 +187,19 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       constexpr uint32_t idesc_qk = ta_idesc(0, AS_KEYS), idesc_pv = ta_idesc(1, D);
       const uint32_t s_col = tmem + (uint32_t)t * 128u, o_col = tmem + 256u + (uint32_t)t * 128u;
       const uint32_t qa = sbase + t * L::Q_TILE;
-      int mine = 0, segments = 0;              // this tile's blocks and segments so far
+      int n0 = 0, mine = 0, segments = 0;      // blocks of all segments so far, this tile's blocks and segments
+      uint32_t k_turn = 0, v_turn = 0;         // bit s: the parity of this tile's next wait for stage s
       bool ok = true;
-      while (x < x_end && ok) {
-        const Segment g = as_next(p, plan, cta, x, x_end);
+      while (way.x < way.x_end && ok) {
+        const Segment g = as_next(p, plan, cta, way);
         if (g.blocks == 0) continue;
-        const bool two = g.tokens > per;
-        if (!two && (singles++ & 1) != t) {
-          // The other tile's blocks are let pass one by one: a wait tells one turn of the ring from the next only.
-          for (int i = 0; i < g.blocks && ok; ++i) {
-            const int n = blocks_done + i, s = n % SC_STAGES;
-            ok = ta_mbar_wait_idle(k_full(s), (uint32_t)((n / SC_STAGES) & 1), abort_flag, SC_ERR_KV_FULL);
-            if (ok) ta_mbar_arrive(k_empty(s));
-            ok = ok && ta_mbar_wait_idle(v_full(s), (uint32_t)((n / SC_STAGES) & 1), abort_flag, SC_ERR_KV_FULL);
-            if (ok) ta_mbar_arrive(v_empty(s));
-          }
-          blocks_done += g.blocks;
-          continue;
-        }
+        if (!((tiles_of(g) >> t) & 1)) { n0 += g.blocks; continue; }
         ok = ta_mbar_wait(q_full(t), (uint32_t)(segments & 1), abort_flag, SC_ERR_Q);
         // S(i) = Q K(i)^T into S buffer (mine + i) & 1
         auto issue_qk = [&](int i) -> bool {
-          const int n = blocks_done + i, s = n % SC_STAGES, b = (mine + i) & 1;
-          if (!ta_mbar_wait(k_full(s), (uint32_t)((n / SC_STAGES) & 1), abort_flag, SC_ERR_KV_FULL)) return false;
+          const int s = (n0 + i) % SC_STAGES, b = (mine + i) & 1;
+          if (!ta_mbar_wait(k_full(t, s), (k_turn >> s) & 1u, abort_flag, SC_ERR_KV_FULL)) return false;
+          k_turn ^= 1u << s;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t ka = sbase + L::K_OFF + s * L::KV_TILE;
 #pragma unroll
@@ -186,26 +207,27 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
             ta_umma(s_col + (uint32_t)b * 64u, ta_desc_kmajor(qa + (uint32_t)(k >> 2) * TA_HALF_BYTES + (uint32_t)(k & 3) * 32u),
                     ta_desc_kmajor(ka + (uint32_t)(k >> 2) * L::KV_HALF + (uint32_t)(k & 3) * 32u), idesc_qk, k != 0);
           ta_commit(s_full(t, b));
-          ta_commit(k_empty(s));
+          ta_commit(k_empty(t, s));
           return true;
         };
         for (int i = 0; i < 2 && i < g.blocks && ok; ++i) ok = issue_qk(i);
         for (int i = 0; i < g.blocks && ok; ++i) {
-          const int n = blocks_done + i, s = n % SC_STAGES, b = (mine + i) & 1;
-          ok = ta_mbar_wait(p_full(t, b), (uint32_t)(((mine + i) >> 1) & 1), abort_flag, SC_ERR_P_FULL) &&
-               ta_mbar_wait(v_full(s), (uint32_t)((n / SC_STAGES) & 1), abort_flag, SC_ERR_KV_FULL);
+          const int s = (n0 + i) % SC_STAGES, b = (mine + i) & 1;
+          ok = ta_mbar_wait(v_full(t, s), (v_turn >> s) & 1u, abort_flag, SC_ERR_KV_FULL);
           if (ok && i == 0 && segments > 0) ok = ta_mbar_wait(o_free(t), (uint32_t)((segments - 1) & 1), abort_flag, SC_ERR_O_FREE);
+          ok = ok && ta_mbar_wait(p_full(t, b), (uint32_t)(((mine + i) >> 1) & 1), abort_flag, SC_ERR_P_FULL);
           if (!ok) break;
+          v_turn ^= 1u << s;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t va = sbase + L::V_OFF + s * L::KV_TILE;
 #pragma unroll
           for (int k = 0; k < AS_KEYS / 16; ++k)
             ta_umma_ts(o_col, s_col + (uint32_t)b * 64u + (uint32_t)k * 8u, ta_desc_mnmajor(va + (uint32_t)k * 16u * 128u, L::KV_HALF), idesc_pv, (i | k) != 0);
           ta_commit(pv_done(t, b));
-          ta_commit(v_empty(s));
+          ta_commit(v_empty(t, s));
           if (i + 2 < g.blocks) ok = issue_qk(i + 2);          // where P(i) lies: the tensor cores finish P V(i) first
         }
-        blocks_done += g.blocks;
+        n0 += g.blocks;
         mine += g.blocks;
         ++segments;
       }
@@ -217,40 +239,54 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     const uint32_t tlane = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_addr = tmem + tlane + (uint32_t)t * 128u, o_addr = tmem + tlane + 256u + (uint32_t)t * 128u;
     const uint32_t q_row = sbase + t * L::Q_TILE + (uint32_t)r * 128u;
-    const int ps = p.page_size, shift = p.page_shift;
-    int mine = 0;
-    bool ok = true;
-    while (x < x_end && ok) {
-      const Segment g = as_next(p, plan, cta, x, x_end);
-      if (g.blocks == 0) continue;
-      const bool two = g.tokens > per;
-      if (!two && (singles++ & 1) != t) continue;
-      // this row's token, its queries
-      const int i_tok = (two ? t * per : 0) + r / G;
-      const bool valid = r < per * G && i_tok < g.tokens;
-      const bool warp_valid = quarter * 32 < min(g.tokens - (two ? t * per : 0), per) * G;
-      int token = 0, position = 0;
-      if (valid) {
-        as_token(plan, g, i_tok, token, position);
-        const uint8_t* src = (const uint8_t*)p.q + ((size_t)token * p.heads + g.kv_head * G + r % G) * (D * 2);
+    const int ps = p.page_size, shift = p.page_shift, size = min(ps, AS_KEYS), bits = min(shift, 6);
+    Segment g;
+    int position = 0, lane_rows = 0, row0 = 0;                 // the last key this row sees; rows of this tile, and where they begin among the segment's
+    // The next segment of this tile, if there is one: its queries are requested, a row a thread.
+    auto next_segment = [&]() -> bool {
+      for (;;) {
+        if (way.x >= way.x_end) return false;
+        g = as_next(p, plan, cta, way);
+        if (g.blocks == 0) continue;
+        const int tiles = tiles_of(g);
+        if (!((tiles >> t) & 1)) continue;
+        const int first = tiles == 3 ? t * per : 0;
+        row0 = first * G;
+        lane_rows = min(g.tokens - first, per) * G;
+        if (r < lane_rows) {
+          const int i = r / G;
+          int token;
+          as_token(plan, g, first + i, token, position);
+          const uint8_t* src = (const uint8_t*)p.q + ((size_t)token * p.heads + g.kv_head * G + (r - i * G)) * (D * 2);
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                       ::"r"(q_row + (uint32_t)(c >> 3) * TA_HALF_BYTES + (uint32_t)(((c & 7) ^ (r & 7)) << 4)), "l"(src + c * 16) : "memory");
+          for (int c = 0; c < D / 8; ++c)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                         ::"r"(q_row + (uint32_t)(c >> 3) * TA_HALF_BYTES + (uint32_t)(((c & 7) ^ (r & 7)) << 4)), "l"(src + c * 16) : "memory");
+        }
+        return true;
       }
+    };
+    auto hand_queries = [&]() {
       asm volatile("cp.async.wait_all;" ::: "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) ta_mbar_arrive(q_full(t));
-      const int hi = valid ? min(position + 1, g.key_hi) : 0x7fffffff;
-      const int* bt = p.table + (size_t)g.table_row * p.max_pages;
+    };
+    int mine = 0;
+    bool ok = true, more = next_segment();
+    if (more) hand_queries();
+    while (more) {
+      const bool valid = r < lane_rows, warp_valid = quarter * 32 < lane_rows;
+      const int hi = valid ? min(position + 1, g.key_hi) : 0x7fffffff, lo = g.key_lo;
+      const int* bt = p.table + (size_t)g.request * p.max_pages;
+      const int blocks = g.blocks;
+      int kb = (lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS;
       float m_ref = -INFINITY, l_run = 0.f;
-      for (int i = 0; i < g.blocks; ++i) {
+      for (int i = 0; i < blocks; ++i, kb += AS_KEYS) {
         const int j = mine + i, b = j & 1;
-        const int kb = (g.key_lo & ~(AS_KEYS - 1)) + (g.block + i) * AS_KEYS;
-        int id = 0;                            // the page of the block's keys lane * size .. + size - 1, if there are any
-        const int size = min(ps, AS_KEYS), key = kb + lane * size;
-        if (lane * size < AS_KEYS && key < g.key_hi && key + size > g.key_lo) id = bt[key >> shift];
+        int id = 0;                            // the i-th page of the block, where there are keys of this segment
+        const int key = kb + lane * size;
+        if (lane * size < AS_KEYS && key < g.key_hi && key + size > lo) id = bt[key >> shift];
         ok = ta_mbar_wait(s_full(t, b), (uint32_t)((j >> 1) & 1), abort_flag, SC_ERR_S_FULL);
         if (!ok) break;
         if (!warp_valid) {                     // no row of this warp: its rows of P are anything, and nobody reads what comes of them
@@ -260,7 +296,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t absent = __ballot_sync(0xffffffffu, id < 0 || id >= p.num_pages);
-        const bool need_mask = absent != 0 || kb < g.key_lo || __any_sync(0xffffffffu, kb + AS_KEYS > hi);
+        const bool need_mask = absent != 0 || kb < lo || __any_sync(0xffffffffu, kb + AS_KEYS > hi);
         float xs[AS_KEYS];
         {
           uint32_t v[64];
@@ -269,10 +305,9 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
           for (int e = 0; e < 64; ++e) xs[e] = __uint_as_float(v[e]);
         }
         if (need_mask) {
-          const int sh = min(shift, 6);
 #pragma unroll
           for (int e = 0; e < AS_KEYS; ++e)
-            if (kb + e >= hi || kb + e < g.key_lo || ((absent >> (e >> sh)) & 1u)) xs[e] = -INFINITY;
+            if (kb + e >= hi || kb + e < lo || ((absent >> (e >> bits)) & 1u)) xs[e] = -INFINITY;
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -329,29 +364,34 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         if (lane == 0) ta_mbar_arrive(p_full(t, b));
       }
       if (!ok) break;
-      mine += g.blocks;
-      const int j = mine - 1;
-      ok = ta_mbar_wait(pv_done(t, j & 1), (uint32_t)((j >> 1) & 1), abort_flag, SC_ERR_O_FULL);
+      mine += blocks;
+      // All products with this tile's queries are done: the next segment's come while this one's result is awaited and written.
+      const long long tile = g.row;
+      const int rows = g.tokens * G, row = row0 + r;
+      more = next_segment();
+      ok = ta_mbar_wait(pv_done(t, (mine - 1) & 1), (uint32_t)(((mine - 1) >> 1) & 1), abort_flag, SC_ERR_O_FULL);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (warp_valid) {
-        const size_t row = g.row + (size_t)(two ? t * per * G : 0) + r;
-        if (valid) *reinterpret_cast<float2*>(p.part_ml + row * 2) = make_float2(m_ref, l_run);
+        if (valid) *reinterpret_cast<float2*>(p.part_ml + (tile + row) * 2) = make_float2(m_ref, l_run);
+        float4* dst = reinterpret_cast<float4*>(p.part_o + tile * D) + row;
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t v[32];
           ta_tmem_ld32(o_addr + (uint32_t)c, v);               // warp-wide: rows without a token take part and write nothing
           if (valid) {
-            uint4* dst = reinterpret_cast<uint4*>(p.part_o + row * D + c);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dst[e] = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+            for (int e = 0; e < 8; ++e)
+              dst[(size_t)((c >> 2) + e) * rows] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]), __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
           }
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) ta_mbar_arrive(o_free(t));
+      if (more) hand_queries();
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();

@@ -1493,7 +1493,7 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     tokens the prefix of row r has: the first prefix_lens[prefix_of[s]] keys of s are read through that row's table, the others
     through its own.  All of these are device values, read by the kernel, so that a recorded step is replayed with other groups and
     lengths; `max_q_len` is the most tokens of a request.  Page ids outside the pool are not there: a row that sees no key gives
-    zeros, and rows of q that belong to no request (behind cu_tokens[S]) leave the output as it was.  S is at most 512, a head a multiple of
+    zeros, and rows of q that belong to no request (behind cu_tokens[S]) leave the output as it was.  S is at most 256, a head a multiple of
     8 up to 256.  Partial results go through memory that the call
     takes from torch's allocator on the current stream, so calls on several streams do not meet; a stream that is not the current
     one is told to the allocator."""

@@ -35,8 +35,8 @@ __global__ void __launch_bounds__(AP_THREADS) attention_shared_plain_kernel(Shar
   float* ps = vs + AS_KEYS * D;
   int* page = reinterpret_cast<int*>(ps + AP_ROWS * (AS_KEYS + 4));      // offset of each key's row in the pool's page units, -1: not there
   pdl_trigger();
+  as_make_plan(p, plan, blockIdx.x, gridDim.x);                // lengths and groups were written before the kernel ahead began
   pdl_wait();
-  as_make_plan(p, plan, gridDim.x);
   as_write_records(p, plan, blockIdx.x, gridDim.x, threadIdx.x, AP_THREADS);
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const T* q = reinterpret_cast<const T*>(p.q);

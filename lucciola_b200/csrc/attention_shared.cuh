@@ -43,10 +43,11 @@ void attention_shared_tc_cut(int group, int& tile_tokens, int& lane_tokens);
 cudaError_t attention_shared_tc(const SharedParams& p, int ctas, cudaStream_t stream);
 
 struct SharedPlan {
-  int4 meta[AS_MAX_SEQS];                // lead (the row whose table holds the prefix that this request shares, -1: none), new tokens,
-                                         // context, tokens of the prefix in this row's table
+  int4 meta[AS_MAX_SEQS];                // prefix_of (-1: none), new tokens, context, tokens of the prefix in this row's table
   int q0[AS_MAX_SEQS];                   // first token
+  int lead[AS_MAX_SEQS];                 // the row whose table holds the prefix that this request shares, -1: none
   int rank[AS_MAX_SEQS];                 // tokens of the group in front of this request's
+  int before[AS_MAX_SEQS];               // members of the group in front of it
   int led[AS_MAX_SEQS];                  // tokens of the group that this row leads
   int member[AS_MAX_SEQS];               // the groups' members, group by group
   int first_member[AS_MAX_SEQS + 1];     // of the group that this row leads
@@ -54,6 +55,7 @@ struct SharedPlan {
                                          // begins in the line, in the list of rows and among the entries that are not empty
   int2 entry[2 * AS_MAX_SEQS];           // of those: first unit, e
   int entries, units, span, rows;        // how many; units and rows of a kv head, units of a CTA
+  int kv_head, at, tile;                 // where this CTA's piece begins
 };
 
 __device__ __forceinline__ int as_blocks(int lo, int hi) { return hi > lo ? (hi - (lo & ~(AS_KEYS - 1)) + AS_KEYS - 1) / AS_KEYS : 0; }
@@ -67,42 +69,50 @@ __device__ __forceinline__ int as_units(const SharedParams& p, int tokens, int b
   return blocks * (full * twice + (last > p.lane_tokens ? 2 : 1));
 }
 
-// An exclusive sum over `n` numbers by one warp, in place; returns the whole.
+// An exclusive sum over `n` numbers by one warp, in place; returns the whole.  A lane has a run of them.
 __device__ __forceinline__ int as_scan(int* a, int n) {
-  const int lane = threadIdx.x & 31;
-  int total = 0;
-  for (int i = 0; i < n; i += 32) {
-    const int v = i + lane < n ? a[i + lane] : 0;
-    int s = v;
+  const int lane = threadIdx.x & 31, per = (n + 31) >> 5, from = min(lane * per, n), to = min(from + per, n);
+  int s = 0;
+  for (int i = from; i < to; ++i) s += a[i];
+  const int mine = s;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += t;
-    }
-    if (i + lane < n) a[i + lane] = total + s - v;
-    total += __shfl_sync(0xffffffffu, s, 31);
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += t;
+  }
+  const int total = __shfl_sync(0xffffffffu, s, 31);
+  s -= mine;
+  for (int i = from; i < to; ++i) {
+    const int v = a[i];
+    a[i] = s;
+    s += v;
   }
   return total;
 }
 
-// Made by all threads of a CTA (four warps at least); ends with a barrier.
-__device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& pl, int ctas) {
+__device__ __forceinline__ int as_tile_units(const SharedParams& p, int blocks) { return p.tile_tokens > p.lane_tokens ? 2 * blocks : blocks; }
+
+// Made by all threads of a CTA (256 at least, a power of two of them or 384); ends with a barrier.  Reads lengths and groups only.
+__device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& pl, int cta, int ctas) {
   const int tid = threadIdx.x, n = p.S;
   const int most = p.max_pages * p.page_size;
-  for (int s = tid; s < n; s += blockDim.x) {
+  if (tid < n) {
+    const int s = tid;
     const int a = __ldcg(p.cu + s), b = __ldcg(p.cu + s + 1), c = __ldcg(p.ctx + s), l = __ldcg(p.prefix_of + s), f = __ldcg(p.prefix_lens + s);
     const int q0 = min(max(a, 0), p.T);
     pl.q0[s] = q0;
     pl.meta[s] = make_int4(l >= 0 && l < n ? l : -1, max(min(b, p.T) - q0, 0), min(max(c, 0), most), min(max(f, 0), most));
   }
   __syncthreads();
-  // Who shares with whom: every request looks at all others (n is a few dozen, a few hundred at most).
-  for (int s = tid; s < n; s += blockDim.x) {
-    const int4 me = pl.meta[s];
+  // Who shares with whom: every request looks at all others (n is a few dozen, a few hundred at most), 1 << k lanes for each.
+  const int k = n <= (int)blockDim.x / 4 ? 2 : n <= (int)blockDim.x / 2 ? 1 : 0;
+  const int s = tid >> k, part = tid & ((1 << k) - 1);
+  if ((s & ~(31 >> k)) < n) {            // whole warps
+    const int4 me = s < n ? pl.meta[s] : make_int4(-1, 0, 0, 0);
     const int l = me.x;
     int rank = 0, before = 0, all = 0, led = 0, led_tokens = 0;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) {
+#pragma unroll 4
+    for (int j = part; j < n; j += 1 << k) {
       const int2 o = *reinterpret_cast<const int2*>(&pl.meta[j]);
       const bool same = o.x == l && l >= 0, mine = o.x == s;
       all += same ? 1 : 0;
@@ -111,23 +121,33 @@ __device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& 
       led += mine ? 1 : 0;
       led_tokens += mine ? o.y : 0;
     }
-    // A group of one, or a prefix shorter than a block, is not worth a tile of its own.
-    const int prefix = l >= 0 ? pl.meta[l].w : 0;
-    const bool shares = all >= 2 && prefix >= AS_KEYS, leads = led >= 2 && me.w >= AS_KEYS;
-    pl.rank[s] = shares ? rank : -1;
-    pl.led[s] = led_tokens;
-    pl.member[s] = before;               // until the list is made
-    pl.first_member[s] = led;
-    const int ua = leads ? as_units(p, led_tokens, as_blocks(0, me.w)) : 0, ub = as_units(p, me.y, as_blocks(shares ? prefix : 0, me.z));
-    pl.unit[s] = ua; pl.unit[n + s] = ub;
-    pl.row[s] = leads ? led_tokens * p.group : 0; pl.row[n + s] = me.y * p.group;
-    pl.place[s] = ua > 0 ? 1 : 0; pl.place[n + s] = ub > 0 ? 1 : 0;
+    for (int o = (1 << k) >> 1; o > 0; o >>= 1) {
+      all += __shfl_xor_sync(0xffffffffu, all, o); before += __shfl_xor_sync(0xffffffffu, before, o); rank += __shfl_xor_sync(0xffffffffu, rank, o);
+      led += __shfl_xor_sync(0xffffffffu, led, o); led_tokens += __shfl_xor_sync(0xffffffffu, led_tokens, o);
+    }
+    if (part == 0 && s < n) {
+      // A group of one, or a prefix shorter than a block, is not worth a tile of its own.
+      const int prefix = l >= 0 ? pl.meta[l].w : 0;
+      const bool shares = all >= 2 && prefix >= AS_KEYS, leads = led >= 2 && me.w >= AS_KEYS;
+      pl.lead[s] = shares ? l : -1;
+      pl.rank[s] = rank;
+      pl.before[s] = before;
+      pl.led[s] = led_tokens;
+      pl.first_member[s] = led;
+      const int ua = leads ? as_units(p, led_tokens, as_blocks(0, me.w)) : 0, ub = as_units(p, me.y, as_blocks(shares ? prefix : 0, me.z));
+      pl.unit[s] = ua; pl.unit[n + s] = ub;
+      pl.row[s] = leads ? led_tokens * p.group : 0; pl.row[n + s] = me.y * p.group;
+      pl.place[s] = ua > 0 ? 1 : 0; pl.place[n + s] = ub > 0 ? 1 : 0;
+    }
   }
   __syncthreads();
   const int warp = tid >> 5;
   if (warp == 0) {
     const int u = as_scan(pl.unit, 2 * n);
-    if (tid == 0) pl.units = u;
+    if (tid == 0) {
+      pl.units = u;
+      pl.span = max((int)(((unsigned)u * (unsigned)p.kv_heads + (unsigned)ctas - 1u) / (unsigned)ctas), p.min_span);
+    }
   } else if (warp == 1) {
     const int r = as_scan(pl.row, 2 * n);
     if ((tid & 31) == 0) pl.rows = r;
@@ -139,24 +159,29 @@ __device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& 
     if ((tid & 31) == 0) pl.first_member[n] = m;
   }
   __syncthreads();
-  // cu_tokens that fall would make more rows than there is room for: nothing is done then
-  const int units = pl.rows > 2 * p.T * p.group ? 0 : pl.units;
-  if (tid == 0) pl.span = max((int)(((unsigned)units * (unsigned)p.kv_heads + (unsigned)ctas - 1u) / (unsigned)ctas), p.min_span);
+  // where this CTA begins: the entry whose units hold its first one
+  const int units = pl.units, x = cta * pl.span;
+  const int kv = units > 0 ? (int)((unsigned)x / (unsigned)units) : 0, u = x - kv * units;
   for (int e = tid; e < 2 * n; e += blockDim.x) {
-    const int end = e + 1 < 2 * n ? pl.place[e + 1] : pl.entries;
-    if (pl.place[e] < end) pl.entry[pl.place[e]] = make_int2(pl.unit[e], e);
+    const bool last = e + 1 == 2 * n;
+    const int at = pl.place[e], end = last ? units : pl.unit[e + 1], from = pl.unit[e];
+    if (at < (last ? pl.entries : pl.place[e + 1])) {
+      pl.entry[at] = make_int2(from, e);
+      if (from <= u && u < end) {
+        const int l = e < n ? -1 : pl.lead[e - n];
+        const int nb = e < n ? as_blocks(0, pl.meta[e].w) : as_blocks(l >= 0 ? pl.meta[l].w : 0, pl.meta[e - n].z);
+        pl.kv_head = kv;
+        pl.at = at;
+        pl.tile = (int)((unsigned)(u - from) / (unsigned)as_tile_units(p, nb));
+      }
+    }
   }
-  int l = -1, before = 0;
-  for (int s0 = 0; s0 < n; s0 += blockDim.x) {      // (one round: n is at most 256)
-    const int s = s0 + tid;
-    if (s < n) { l = pl.meta[s].x; before = pl.member[s]; }
-    __syncthreads();
-    if (s < n && l >= 0) pl.member[pl.first_member[l] + before] = s;
-    if (s < n && pl.rank[s] < 0) pl.meta[s].x = -1;
-  }
-  if (tid == 0) pl.units = units;
+  if (tid < n && pl.meta[tid].x >= 0) pl.member[pl.first_member[pl.meta[tid].x] + pl.before[tid]] = tid;
   __syncthreads();
 }
+
+// cu_tokens that fall would make more rows than there is room for: nothing is done then.
+__device__ __forceinline__ bool as_sound(const SharedParams& p, const SharedPlan& pl) { return pl.rows <= 2 * p.T * p.group; }
 
 // What the combining kernel has to know of every token, for the prefix and for the request's own keys: the first row of the token's
 // tile, the token's first row in the tile, the tile's rows, the unit of its first block, and how many units further the last block begins
@@ -170,7 +195,7 @@ __device__ __forceinline__ void as_write_records(const SharedParams& p, const Sh
   const int twice = p.tile_tokens > p.lane_tokens ? 2 : 1;
   for (int s = ctas - 1 - cta; s < p.S; s += ctas) {
     const int4 me = pl.meta[s];
-    const int t0 = pl.q0[s], q = me.y, l = me.x;
+    const int t0 = pl.q0[s], q = me.y, l = pl.lead[s];
     const int prefix = l >= 0 ? pl.meta[l].w : 0;
     for (int i = thread; i < q; i += threads) {
       int4 a = make_int4(0, 0, 0, 0);
@@ -187,7 +212,7 @@ __device__ __forceinline__ void as_write_records(const SharedParams& p, const Sh
                                pl.unit[e] + tile * as_blocks(prefix, me.z) * twice);
       const int b_last = nb > 0 ? (nb - 1) * (here > p.lane_tokens ? 2 : 1) : -1;
       int4* dst = reinterpret_cast<int4*>(p.rec + (size_t)(t0 + i) * AS_REC);
-      dst[0] = a; dst[1] = b; dst[2] = pl.units > 0 ? make_int4(a_last, b_last, 0, 0) : make_int4(-1, -1, 0, 0);
+      dst[0] = a; dst[1] = b; dst[2] = as_sound(p, pl) ? make_int4(a_last, b_last, 0, 0) : make_int4(-1, -1, 0, 0);
     }
   }
 }
@@ -206,32 +231,10 @@ struct Segment {
 // A CTA's way along the line: where it is, and which entry and tile that is in.
 struct Walk { int x, x_end, kv_head, at, tile; };
 
-__device__ __forceinline__ int as_tile_units(const SharedParams& p, int blocks) { return p.tile_tokens > p.lane_tokens ? 2 * blocks : blocks; }
-__device__ __forceinline__ int as_entry_blocks(const SharedParams& p, const SharedPlan& pl, int e) {
-  if (e < p.S) return as_blocks(0, pl.meta[e].w);
-  const int4 me = pl.meta[e - p.S];
-  return as_blocks(me.x >= 0 ? pl.meta[me.x].w : 0, me.z);
-}
-
 __device__ __forceinline__ Walk as_begin(const SharedParams& p, const SharedPlan& pl, int cta) {
-  Walk w;
-  const int total = pl.units * p.kv_heads;
-  w.x = min(cta * pl.span, total);
-  w.x_end = min(w.x + pl.span, total);
-  w.kv_head = w.at = w.tile = 0;
-  if (w.x < w.x_end) {
-    w.kv_head = (int)((unsigned)w.x / (unsigned)pl.units);
-    const int u = w.x - w.kv_head * pl.units;
-    int a = 0, b = pl.entries - 1;       // the last entry that begins at or before u
-    while (a < b) {
-      const int mid = (a + b + 1) >> 1;
-      if (pl.entry[mid].x <= u) a = mid; else b = mid - 1;
-    }
-    w.at = a;
-    const int2 e = pl.entry[a];
-    w.tile = (int)((unsigned)(u - e.x) / (unsigned)as_tile_units(p, as_entry_blocks(p, pl, e.y)));
-  }
-  return w;
+  if (!as_sound(p, pl)) return Walk{0, 0, 0, 0, 0};
+  const int total = pl.units * p.kv_heads, x = min(cta * pl.span, total);
+  return Walk{x, min(x + pl.span, total), pl.kv_head, pl.at, pl.tile};
 }
 
 // The segment at w.x (< w.x_end); w moves behind it.
@@ -244,7 +247,8 @@ __device__ __forceinline__ Segment as_next(const SharedParams& p, const SharedPl
   const int4 me = pl.meta[s];
   const int tokens = g.shared ? pl.led[s] : me.y;
   const int hi = g.shared ? me.w : me.z;
-  g.key_lo = !g.shared && me.x >= 0 ? pl.meta[me.x].w : 0;
+  const int lead = g.shared ? -1 : pl.lead[s];
+  g.key_lo = lead >= 0 ? pl.meta[lead].w : 0;
   const int nb = as_blocks(g.key_lo, hi);
   g.request = s;
   g.first = w.tile * p.tile_tokens;

@@ -8,8 +8,8 @@
 //     S = Q K^T      tcgen05.mma, operands from shared memory, two S buffers a tile
 //     P              one thread a query row, online softmax in 32 bits, P (bfloat16) written over S in tensor memory
 //     O += P V       tcgen05.mma, P from tensor memory, V as it lies in the pages; O stays in tensor memory
-// The sum of a row's weights is taken before they are rounded to bfloat16 for P V.  A row's reference value follows its maximum when that
-// has grown by more than 2^8 only (O is rescaled then).
+// The sum of a row's weights is taken before they are rounded to bfloat16 for P V.  A row's reference value is the maximum of its first
+// block, and moves (O is rescaled then) when a block's weights against it sum up to 2^15: what the maximum was does not matter to the quotient.
 //
 // Why 128-row tiles even for one request's few rows: a block of 64 keys takes the tensor cores some 500 cycles whatever the rows, and the
 // memory 1400 cycles at its full rate shared by all SMs, so rows that are not there cost nothing; one kernel for both kinds of work is what
@@ -28,9 +28,9 @@ namespace lb {
 
 constexpr int SC_STAGES = 4;
 constexpr int SC_IN_FLIGHT = 2;                                // blocks a copying warp has requested beyond the one it waits for
-constexpr int SC_BARS = 4 * SC_STAGES + 8;                     // barriers of a tile
-constexpr int SC_THREADS = 384;
-enum : int { SC_ERR_Q = 401, SC_ERR_KV_FULL = 402, SC_ERR_KV_EMPTY = 403, SC_ERR_S_FULL = 404, SC_ERR_P_FULL = 405, SC_ERR_O_FULL = 406, SC_ERR_O_FREE = 407 };
+constexpr int SC_BARS = 4 * SC_STAGES + 12;                    // barriers of a tile
+constexpr int SC_THREADS = 640;
+enum : int { SC_ERR_Q = 401, SC_ERR_KV_FULL = 402, SC_ERR_KV_EMPTY = 403, SC_ERR_S_FULL = 404, SC_ERR_P_FULL = 405, SC_ERR_O_FULL = 406, SC_ERR_O_FREE = 407, SC_ERR_PAIR = 408 };
 
 // Shared memory: queries of A and B | ring of keys | ring of values | barriers.  Rows of 128 bytes (64 elements), 128-byte swizzle, the second
 // 64 elements of a head a half further on.
@@ -39,7 +39,16 @@ template <int D> struct ScLayout {
   static constexpr int KV_HALF = AS_KEYS * 128, KV_TILE = HALVES * KV_HALF;
   static constexpr int Q_TILE = HALVES * TA_HALF_BYTES;
   static constexpr int K_OFF = 2 * Q_TILE, V_OFF = K_OFF + SC_STAGES * KV_TILE, BAR_OFF = V_OFF + SC_STAGES * KV_TILE;
-  static constexpr int BYTES = BAR_OFF + 2 * SC_BARS * 8 + 16;
+  static constexpr int PAIR_OFF = BAR_OFF + 2 * SC_BARS * 8 + 16;  // [2 turns][2 tiles][2 halves][128 rows]: what the two warps of a row tell each other
+  static constexpr int BYTES = PAIR_OFF + 2 * 2 * 2 * TA_ROWS * 4;
+};
+
+// What a softmax warp keeps of its way and of the segment at hand in shared memory: its registers are for a block's scores and weights (what
+// does not fit goes to local memory, of which little stays on the SM beside 220 KB of shared memory).
+struct ScWarp {
+  Walk way; int singles;
+  int request, key_hi, rows, row;        // row of the block table, end of the segment's keys; rows of its tile, this warp's first among them
+  long long tile;                        // where the tile's partial rows begin
 };
 
 // One block of 64 keys (or values) of a kv head from the pages into a stage of the ring, by one warp: a lane copies 16-byte chunk c of the
@@ -65,11 +74,23 @@ __device__ __forceinline__ void sc_copy_block(uint32_t stage, const uint32_t (&x
   }
 }
 
+// The lowest n bits (none below 0, all from 32 on).
+__device__ __forceinline__ uint32_t sc_low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+// The caller waits with ta_tmem_wait_st() before it tells anyone.
+__device__ __forceinline__ void sc_tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+
 template <int D>
 __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(SharedParams p) {
   typedef ScLayout<D> L;
   extern __shared__ uint8_t smem_raw[];
   __shared__ SharedPlan plan;
+  __shared__ ScWarp states[SC_THREADS / 32 - 4];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = ta_smem_u32(smem);
   const uint32_t bars = sbase + L::BAR_OFF;
@@ -83,39 +104,42 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   auto pv_done = [&](int t, int b) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + 4 + b); };
   auto q_full = [&](int t) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + 6); };
   auto o_free = [&](int t) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + 7); };
+  auto pair_bar = [&](int t, int q) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + 8 + q); };     // the two warps of 32 rows
   uint32_t* tmem_slot = (uint32_t*)(smem + L::BAR_OFF + 2 * SC_BARS * 8);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  volatile int* holes = (volatile int*)(tmem_slot + 2);       // some key of this CTA's segments lies in no page
 
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
       for (int i = 0; i < 4 * SC_STAGES; ++i) ta_mbar_init(k_full(t, i), 1);
-      for (int b = 0; b < 2; ++b) { ta_mbar_init(s_full(t, b), 1); ta_mbar_init(p_full(t, b), 4); ta_mbar_init(pv_done(t, b), 1); }
-      ta_mbar_init(q_full(t), 4); ta_mbar_init(o_free(t), 4);
+      for (int b = 0; b < 2; ++b) { ta_mbar_init(s_full(t, b), 1); ta_mbar_init(p_full(t, b), 8); ta_mbar_init(pv_done(t, b), 1); }
+      ta_mbar_init(q_full(t), 8); ta_mbar_init(o_free(t), 8);
+      for (int q = 0; q < 4; ++q) ta_mbar_init(pair_bar(t, q), 2);
     }
     *abort_flag = 0;
+    *holes = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ta_smem_u32(tmem_slot)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  pdl_wait();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  as_make_plan(p, plan, gridDim.x);
+  as_make_plan(p, plan, blockIdx.x, gridDim.x);                // lengths and groups were written before the kernel ahead began
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = *tmem_slot;            // columns: tile t's S buffers at t * 128 and t * 128 + 64 (P over their first 32), O at 256 + t * 128
+  pdl_wait();
+  const uint32_t tmem = *tmem_slot;            // columns: tile t's S buffers at t * 128 and t * 128 + 64 (P over the first 16 of each half), O at 256 + t * 128
 
   const int G = p.group, per = p.lane_tokens, cta = blockIdx.x;
   Walk way = as_begin(p, plan, cta);
-  int singles = 0;                             // segments of one tile so far: they go to tile A and B in turn
-  // the tiles that work on a segment, as bits
-  auto tiles_of = [&](const Segment& g) -> int { return g.tokens > per ? 3 : 1 << (singles++ & 1); };
+  // the tiles that work on a segment, as bits: segments of one tile go to tile A and B in turn
+  auto tiles_of = [&](const Segment& g, int& singles) -> int { return g.tokens > per ? 3 : 1 << (singles++ & 1); };
 
-  if (warp == 0 || warp == 10) {
+  if (warp == 0 || warp == 2) {
     // ---- copies ------------------------------------------------------------------------------------------------------------------
-    const bool is_v = warp == 10;
+    const bool is_v = warp == 2;
     constexpr int CHUNKS = D / 8, RPI = 32 / CHUNKS;           // 16-byte chunks of a row, rows an instruction
     const int c = lane % CHUNKS, rp = lane / CHUNKS;
     const uint8_t* pool = (const uint8_t*)(is_v ? p.v_cache : p.k_cache) + c * 16 + rp * (D * 2);
@@ -126,8 +150,8 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     const int ps = p.page_size, shift = p.page_shift, size = min(ps, AS_KEYS);
     const size_t page_stride = (size_t)p.kv_heads * ps * (D * 2);
     bool ok = true;
-    int n = 0;                                 // blocks so far
-    uint32_t used = 0, turn[2] = {0, 0};       // of stage s: the tiles that read its block (bits 2 s, 2 s + 1); of tile t, bit s: the parity of its next wait
+    int n = 0, singles = 0;                    // blocks so far, segments of one tile so far
+    uint32_t used = 0, turn0 = 0, turn1 = 0;   // of stage s: the tiles that read its block (bits 2 s, 2 s + 1); of tiles A and B, bit s: the parity of the next wait
     auto hand_over = [&](int i) {              // block i has landed: visible to the tensor cores, then said so to its tiles
       const int s = i % SC_STAGES;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -137,7 +161,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     while (way.x < way.x_end && ok) {
       const Segment g = as_next(p, plan, cta, way);
       if (g.blocks == 0) continue;
-      const uint32_t tiles = (uint32_t)tiles_of(g);
+      const uint32_t tiles = (uint32_t)tiles_of(g, singles);
       const int* bt = p.table + (size_t)g.request * p.max_pages;
       const uint8_t* head = pool + (size_t)g.kv_head * ps * (D * 2);
       const int first_key = (g.key_lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS;
@@ -146,7 +170,9 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         const int key = kb + lane * size;
         if (lane * size >= AS_KEYS || key >= g.key_hi || key + size <= g.key_lo) return -1;
         const int id = bt[key >> shift];
-        return id < p.num_pages ? id : -1;
+        if (id >= 0 && id < p.num_pages) return id;
+        *holes = 1;                            // before the block is handed over
+        return -1;
       };
       int ids = page_of(first_key);
       for (int b = 0; b < g.blocks; ++b, ++n) {
@@ -156,10 +182,10 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         const uint32_t before = (used >> (2 * s)) & 3u;
         int go = 1;
         if (lane < 2 && ((before >> lane) & 1u))
-          go = ta_mbar_wait_idle(is_v ? v_empty(lane, s) : k_empty(lane, s), (turn[lane & 1] >> s) & 1u, abort_flag, SC_ERR_KV_EMPTY) ? 1 : 0;
+          go = ta_mbar_wait_idle(is_v ? v_empty(lane, s) : k_empty(lane, s), ((lane ? turn1 : turn0) >> s) & 1u, abort_flag, SC_ERR_KV_EMPTY) ? 1 : 0;
         if (__any_sync(0xffffffffu, go == 0)) { ok = false; break; }
-        turn[0] ^= (before & 1u) << s;
-        turn[1] ^= (before >> 1) << s;
+        turn0 ^= (before & 1u) << s;
+        turn1 ^= (before >> 1) << s;
         used = (used & ~(3u << (2 * s))) | (tiles << (2 * s));
         const uint32_t stage = ring + (uint32_t)s * L::KV_TILE;
         switch (ps) {
@@ -180,20 +206,20 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     if (ok)
       for (int i = max(n - SC_IN_FLIGHT, 0); i < n; ++i) hand_over(i);
     if (is_v) as_write_records(p, plan, cta, gridDim.x, lane, 32);         // while the last blocks are worked on
-  } else if (warp == 1 || warp == 11) {
+  } else if (warp == 1 || warp == 3) {
     // ---- products, one thread a tile -------------------------------------------------------------------------------------------------
     const int t = warp == 1 ? 0 : 1;
     if (elect_one()) {
       constexpr uint32_t idesc_qk = ta_idesc(0, AS_KEYS), idesc_pv = ta_idesc(1, D);
       const uint32_t s_col = tmem + (uint32_t)t * 128u, o_col = tmem + 256u + (uint32_t)t * 128u;
       const uint32_t qa = sbase + t * L::Q_TILE;
-      int n0 = 0, mine = 0, segments = 0;      // blocks of all segments so far, this tile's blocks and segments
+      int n0 = 0, mine = 0, segments = 0, singles = 0;       // blocks of all segments so far, this tile's blocks and segments
       uint32_t k_turn = 0, v_turn = 0;         // bit s: the parity of this tile's next wait for stage s
       bool ok = true;
       while (way.x < way.x_end && ok) {
         const Segment g = as_next(p, plan, cta, way);
         if (g.blocks == 0) continue;
-        if (!((tiles_of(g) >> t) & 1)) { n0 += g.blocks; continue; }
+        if (!((tiles_of(g, singles) >> t) & 1)) { n0 += g.blocks; continue; }
         ok = ta_mbar_wait(q_full(t), (uint32_t)(segments & 1), abort_flag, SC_ERR_Q);
         // S(i) = Q K(i)^T into S buffer (mine + i) & 1
         auto issue_qk = [&](int i) -> bool {
@@ -222,7 +248,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
           const uint32_t va = sbase + L::V_OFF + s * L::KV_TILE;
 #pragma unroll
           for (int k = 0; k < AS_KEYS / 16; ++k)
-            ta_umma_ts(o_col, s_col + (uint32_t)b * 64u + (uint32_t)k * 8u, ta_desc_mnmajor(va + (uint32_t)k * 16u * 128u, L::KV_HALF), idesc_pv, (i | k) != 0);
+            ta_umma_ts(o_col, s_col + (uint32_t)b * 64u + (uint32_t)(k >> 1) * 32u + (uint32_t)(k & 1) * 8u, ta_desc_mnmajor(va + (uint32_t)k * 16u * 128u, L::KV_HALF), idesc_pv, (i | k) != 0);
           ta_commit(pv_done(t, b));
           ta_commit(v_empty(t, s));
           if (i + 2 < g.blocks) ok = issue_qk(i + 2);          // where P(i) lies: the tensor cores finish P V(i) first
@@ -233,35 +259,77 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       }
     }
   } else {
-    // ---- softmax: thread = query row; warp w reads lanes (w % 4) * 32 .. + 31 of tensor memory -----------------------------------------------
-    const int t = warp < 6 ? 0 : 1;
-    const int quarter = warp & 3, r = quarter * 32 + lane;
+    // ---- softmax: two threads a query row, one for each half of a block's keys; warp w reads lanes (w % 4) * 32 .. + 31 of tensor memory ---
+    const int t = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t tlane = (uint32_t)(quarter * 32) << 16;
-    const uint32_t s_addr = tmem + tlane + (uint32_t)t * 128u, o_addr = tmem + tlane + 256u + (uint32_t)t * 128u;
-    const uint32_t q_row = sbase + t * L::Q_TILE + (uint32_t)r * 128u;
-    const int ps = p.page_size, shift = p.page_shift, size = min(ps, AS_KEYS), bits = min(shift, 6);
-    Segment g;
-    int position = 0, lane_rows = 0, row0 = 0;                 // the last key this row sees; rows of this tile, and where they begin among the segment's
-    // The next segment of this tile, if there is one: its queries are requested, a row a thread.
+    const uint32_t s_addr = tmem + tlane + (uint32_t)t * 128u + (uint32_t)half * 32u, o_addr = tmem + tlane + 256u + (uint32_t)t * 128u + (uint32_t)half * (D / 2);
+    const uint32_t q_rows = sbase + t * L::Q_TILE + (uint32_t)quarter * 32u * 128u;        // this warp's rows
+    const uint32_t my_pair = pair_bar(t, quarter);
+    float* told = reinterpret_cast<float*>(smem + L::PAIR_OFF) + t * 2 * TA_ROWS + r;      // [turn][.][half][row]
+    int turns = 0;
+    volatile ScWarp* mem = states + (warp - 4);
+    if (lane == 0) {
+      mem->way.x = way.x; mem->way.x_end = way.x_end; mem->way.kv_head = way.kv_head; mem->way.at = way.at; mem->way.tile = way.tile;
+      mem->singles = 0;
+    }
+    __syncwarp();
+    bool ok = true;
+    // Tells the row's other thread x and gets its.  Values of one turn are overwritten two turns later, when both have read them.
+    auto exchange = [&](float x) -> float {
+      float* at = told + (turns & 1) * 4 * TA_ROWS;
+      at[half * TA_ROWS] = x;
+      __syncwarp();
+      if (lane == 0) ta_mbar_arrive(my_pair);
+      if (!ta_mbar_wait(my_pair, (uint32_t)(turns & 1), abort_flag, SC_ERR_PAIR)) { ok = false; return x; }
+      ++turns;
+      return at[(half ^ 1) * TA_ROWS];
+    };
+    // Of the segment at hand: blocks, the first one's first key, the first key and the end of those this row sees (of none, if there is no such
+    // row), and the least end among the warp's rows.
+    int blocks = 0, block_key = 0, lo = 0, hi = 0, hi_all = 0;
+    bool valid = false, warp_valid = false;
+    // The next segment of this tile, if there is one: its queries are requested, half of a warp's rows by each of the two.
     auto next_segment = [&]() -> bool {
+      Walk at_now;
+      at_now.x = mem->way.x; at_now.x_end = mem->way.x_end; at_now.kv_head = mem->way.kv_head; at_now.at = mem->way.at; at_now.tile = mem->way.tile;
+      int singles = mem->singles;
+      __syncwarp();
       for (;;) {
-        if (way.x >= way.x_end) return false;
-        g = as_next(p, plan, cta, way);
+        if (at_now.x >= at_now.x_end) return false;
+        const Segment g = as_next(p, plan, cta, at_now);
         if (g.blocks == 0) continue;
-        const int tiles = tiles_of(g);
+        const int tiles = tiles_of(g, singles);
         if (!((tiles >> t) & 1)) continue;
-        const int first = tiles == 3 ? t * per : 0;
-        row0 = first * G;
-        lane_rows = min(g.tokens - first, per) * G;
-        if (r < lane_rows) {
+        const int first = tiles == 3 ? t * per : 0, lane_rows = min(g.tokens - first, per) * G;
+        valid = r < lane_rows;
+        warp_valid = quarter * 32 < lane_rows;
+        blocks = g.blocks;
+        lo = g.key_lo;
+        block_key = (lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS;
+        hi = 0x7fffffff;
+        int from = -1;                         // this row's place among all rows of the queries
+        if (valid) {
           const int i = r / G;
-          int token;
+          int token, position;
           as_token(plan, g, first + i, token, position);
-          const uint8_t* src = (const uint8_t*)p.q + ((size_t)token * p.heads + g.kv_head * G + (r - i * G)) * (D * 2);
+          from = token * p.heads + g.kv_head * G + (r - i * G);
+          hi = min(position + 1, g.key_hi);
+        }
+        hi_all = __reduce_min_sync(0xffffffffu, hi);
+        if (lane == 0) {
+          mem->way.x = at_now.x; mem->way.kv_head = at_now.kv_head; mem->way.at = at_now.at; mem->way.tile = at_now.tile; mem->singles = singles;
+          mem->request = g.request; mem->key_hi = g.key_hi; mem->rows = g.tokens * G; mem->row = first * G + quarter * 32; mem->tile = g.row;
+        }
+        __syncwarp();
+        constexpr int CHUNKS = D / 8, RPI = 32 / CHUNKS;       // whole rows side by side
+        const int c = lane % CHUNKS;
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c)
+        for (int i = 0; i < 16 / RPI; ++i) {
+          const int rr = half * 16 + i * RPI + lane / CHUNKS, at = __shfl_sync(0xffffffffu, from, rr);
+          if (at >= 0)
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                         ::"r"(q_row + (uint32_t)(c >> 3) * TA_HALF_BYTES + (uint32_t)(((c & 7) ^ (r & 7)) << 4)), "l"(src + c * 16) : "memory");
+                         ::"r"(q_rows + (uint32_t)rr * 128u + (uint32_t)(c >> 3) * TA_HALF_BYTES + (uint32_t)(((c & 7) ^ (rr & 7)) << 4)),
+                           "l"((const uint8_t*)p.q + (size_t)at * (D * 2) + c * 16) : "memory");
         }
         return true;
       }
@@ -273,20 +341,13 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       if (lane == 0) ta_mbar_arrive(q_full(t));
     };
     int mine = 0;
-    bool ok = true, more = next_segment();
+    bool more = next_segment();
     if (more) hand_queries();
     while (more) {
-      const bool valid = r < lane_rows, warp_valid = quarter * 32 < lane_rows;
-      const int hi = valid ? min(position + 1, g.key_hi) : 0x7fffffff, lo = g.key_lo;
-      const int* bt = p.table + (size_t)g.request * p.max_pages;
-      const int blocks = g.blocks;
-      int kb = (lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS;
       float m_ref = -INFINITY, l_run = 0.f;
-      for (int i = 0; i < blocks; ++i, kb += AS_KEYS) {
-        const int j = mine + i, b = j & 1;
-        int id = 0;                            // the i-th page of the block, where there are keys of this segment
-        const int key = kb + lane * size;
-        if (lane * size < AS_KEYS && key < g.key_hi && key + size > lo) id = bt[key >> shift];
+      bool settled = false;                    // every row has a reference
+      for (int i = 0; i < blocks; ++i, block_key += AS_KEYS) {
+        const int j = mine + i, b = j & 1, kb = block_key + half * 32;
         ok = ta_mbar_wait(s_full(t, b), (uint32_t)((j >> 1) & 1), abort_flag, SC_ERR_S_FULL);
         if (!ok) break;
         if (!warp_valid) {                     // no row of this warp: its rows of P are anything, and nobody reads what comes of them
@@ -295,70 +356,99 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
           continue;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t absent = __ballot_sync(0xffffffffu, id < 0 || id >= p.num_pages);
-        const bool need_mask = absent != 0 || kb < lo || __any_sync(0xffffffffu, kb + AS_KEYS > hi);
-        float xs[AS_KEYS];
-        {
-          uint32_t v[64];
-          ta_tmem_ld64(s_addr + (uint32_t)b * 64u, v);
-#pragma unroll
-          for (int e = 0; e < 64; ++e) xs[e] = __uint_as_float(v[e]);
-        }
-        if (need_mask) {
-#pragma unroll
-          for (int e = 0; e < AS_KEYS; ++e)
-            if (kb + e >= hi || kb + e < lo || ((absent >> (e >> bits)) & 1u)) xs[e] = -INFINITY;
-        }
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int e = 0; e < AS_KEYS; e += 8) {
-#pragma unroll
-          for (int u = 0; u < 4; ++u) mx4[u] = ta_max3(mx4[u], xs[e + 2 * u], xs[e + 2 * u + 1]);
-        }
-        const float m_loc = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
-        const bool grow = valid && m_loc > m_ref + TA_RESCALE_STEP;      // also true for the first finite maximum (m_ref = -inf)
-        if (__any_sync(0xffffffffu, grow)) {
-          float f = 1.f;
-          if (grow) {
-            if (m_ref != -INFINITY) f = exp2f(m_ref - m_loc);
-            m_ref = m_loc;
-            l_run *= f;
+        uint32_t seen = 0xffffffffu;           // which of this half's keys the row sees
+        bool masked = kb < lo || kb + 32 > hi_all;
+        if (masked) seen = sc_low_bits(hi - kb) & ~sc_low_bits(lo - kb);
+        if (*holes) {                          // there are pages that are not: a look at this block's
+          const int size = min(p.page_size, 32);
+          const int key = kb + lane * size;
+          const bool here = lane * size < 32 && key < mem->key_hi && key + size > lo;
+          const int id = here ? p.table[(size_t)mem->request * p.max_pages + (key >> p.page_shift)] : 0;
+          uint32_t absent = __ballot_sync(0xffffffffu, id < 0 || id >= p.num_pages);
+          masked |= absent != 0;
+          for (; absent; absent &= absent - 1) {
+            const int first = (__ffs(absent) - 1) * size;
+            seen &= ~(sc_low_bits(first + size) & ~sc_low_bits(first));
           }
-          if (i > 0) {
-            ok = ta_mbar_wait(pv_done(t, b ^ 1), (uint32_t)(((j - 1) >> 1) & 1), abort_flag, SC_ERR_O_FULL);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t v[32];
-              ta_tmem_ld32(o_addr + (uint32_t)c, v);
+        }
+        // Where every row has a reference, its maximum is not looked for: sums of 32 weights that stay below 2^14 say that no score is
+        // far above the reference.  Otherwise the block is done again from the scores, which still lie in tensor memory, with the maximum.
+        uint32_t w[16];
+        float sum;
+        for (bool exact = !settled;; exact = true) {
+          float xs[32];
+          {
+            uint32_t v[32];
+            ta_tmem_ld32(s_addr + (uint32_t)b * 64u, v);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-              ta_tmem_st32(o_addr + (uint32_t)c, v);
+            for (int e = 0; e < 32; ++e) xs[e] = __uint_as_float(v[e]);
+          }
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((seen >> e) & 1u)) xs[e] = -INFINITY;
+          }
+          if (exact) {
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u) mx4[u] = ta_max3(mx4[u], xs[e + 2 * u], xs[e + 2 * u + 1]);
             }
-            ta_tmem_wait_st();
-          }
-        }
-        const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-        const uint64_t scale2 = ta_pack2(p.scale_log2, p.scale_log2), negm2 = ta_pack2(-m_use, -m_use);
-        uint64_t sum2 = ta_pack2(0.f, 0.f);
-        uint32_t w[32];
+            float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+            mx = fmaxf(mx, exchange(mx));
+            if (!ok) break;
+            const float m_loc = mx * p.scale_log2;
+            const bool grow = valid && m_loc > m_ref + TA_RESCALE_STEP;  // also true for the first finite maximum (m_ref = -inf)
+            if (__any_sync(0xffffffffu, grow)) {
+              float f = 1.f;
+              if (grow) {
+                if (m_ref != -INFINITY) f = exp2f(m_ref - m_loc);
+                m_ref = m_loc;
+                l_run *= f;
+              }
+              if (i > 0) {
+                ok = ta_mbar_wait(pv_done(t, b ^ 1), (uint32_t)(((j - 1) >> 1) & 1), abort_flag, SC_ERR_O_FULL);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                for (int c = 0; c < D / 2; c += 32) {          // half of the dimensions each
+                  uint32_t v[32];
+                  ta_tmem_ld32(o_addr + (uint32_t)c, v);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float y0, y1;
-          ta_unpack2(ta_fma2(ta_pack2(xs[2 * e], xs[2 * e + 1]), scale2, negm2), y0, y1);
-          const float p0 = exp2_approx(y0), p1 = exp2_approx(y1);        // 2^-inf = 0 for masked keys
-          sum2 = ta_add2(sum2, ta_pack2(p0, p1));
-          __nv_bfloat162 b2 = __floats2bfloat162_rn(p0, p1);
-          w[e] = *reinterpret_cast<uint32_t*>(&b2);
-        }
-        ta_tmem_st32(s_addr + (uint32_t)b * 64u, w);
-        ta_tmem_wait_st();
-        {
+                  for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                  ta_tmem_st32(o_addr + (uint32_t)c, v);
+                }
+                ta_tmem_wait_st();
+              }
+            }
+            settled = !__any_sync(0xffffffffu, valid && m_ref == -INFINITY);
+          }
+          const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+          const uint64_t scale2 = ta_pack2(p.scale_log2, p.scale_log2), negm2 = ta_pack2(-m_use, -m_use);
+          uint64_t sum2 = ta_pack2(0.f, 0.f);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float y0, y1;
+            ta_unpack2(ta_fma2(ta_pack2(xs[2 * e], xs[2 * e + 1]), scale2, negm2), y0, y1);
+            const float p0 = exp2_approx(y0), p1 = exp2_approx(y1);      // 2^-inf = 0 for masked keys
+            sum2 = ta_add2(sum2, ta_pack2(p0, p1));
+            __nv_bfloat162 b2 = __floats2bfloat162_rn(p0, p1);
+            w[e] = *reinterpret_cast<uint32_t*>(&b2);
+          }
           float s0, s1;
           ta_unpack2(sum2, s0, s1);
-          l_run += s0 + s1;
+          sum = s0 + s1;
+          if (exact) break;
+          // both halves of the keys, for all 32 rows
+          const bool far = __any_sync(0xffffffffu, valid && !(sum < 16384.f));
+          if (exchange(far ? 1.f : 0.f) == 0.f && !far) break;
+          if (!ok) break;
         }
+        if (!ok) break;
+        sc_tmem_st16(s_addr + (uint32_t)b * 64u, w);
+        ta_tmem_wait_st();
+        l_run += sum;
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
         if (lane == 0) ta_mbar_arrive(p_full(t, b));
@@ -366,20 +456,23 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       if (!ok) break;
       mine += blocks;
       // All products with this tile's queries are done: the next segment's come while this one's result is awaited and written.
-      const long long tile = g.row;
-      const int rows = g.tokens * G, row = row0 + r;
+      const long long tile = mem->tile;
+      const int rows = mem->rows, row = mem->row + lane;
+      const bool row_valid = valid, some_valid = warp_valid;
       more = next_segment();
       ok = ta_mbar_wait(pv_done(t, (mine - 1) & 1), (uint32_t)(((mine - 1) >> 1) & 1), abort_flag, SC_ERR_O_FULL);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (warp_valid) {
-        if (valid) *reinterpret_cast<float2*>(p.part_ml + (tile + row) * 2) = make_float2(m_ref, l_run);
-        float4* dst = reinterpret_cast<float4*>(p.part_o + tile * D) + row;
+      if (some_valid) {
+        l_run += exchange(l_run);
+        if (!ok) break;
+        if (row_valid && half == 0) *reinterpret_cast<float2*>(p.part_ml + (tile + row) * 2) = make_float2(m_ref, l_run);
+        float4* dst = reinterpret_cast<float4*>(p.part_o + tile * D) + (size_t)half * (D / 8) * rows + row;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
+        for (int c = 0; c < D / 2; c += 32) {
           uint32_t v[32];
           ta_tmem_ld32(o_addr + (uint32_t)c, v);               // warp-wide: rows without a token take part and write nothing
-          if (valid) {
+          if (row_valid) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               dst[(size_t)((c >> 2) + e) * rows] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]), __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
@@ -404,7 +497,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
 template <int D>
 static cudaError_t sc_launch(const SharedParams& p, int ctas, cudaStream_t stream) {
   constexpr int smem = ScLayout<D>::BYTES + 1024;
-  static_assert(smem + sizeof(SharedPlan) + 64 <= 227 * 1024, "shared memory of a CTA");
+  static_assert(smem + sizeof(SharedPlan) + sizeof(ScWarp) * (SC_THREADS / 32 - 4) + 64 <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<unsigned long long> configured{0ull};     // a bit a device
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);

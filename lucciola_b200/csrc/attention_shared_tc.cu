@@ -15,10 +15,10 @@
 // memory 1400 cycles at its full rate shared by all SMs, so rows that are not there cost nothing; one kernel for both kinds of work is what
 // lets the line be cut evenly.
 //
-// Warps: 0 copies keys, 10 values (cp.async, 16 bytes a thread, swizzled for the tensor cores; four blocks each, three in flight); 1 issues
-// tile A's products and owns the tensor memory, 11 tile B's; 2..5 softmax of A, 6..9 of B.  Each walks the same segments by itself.  Barriers tell one
-// turn from the next only, so each tile has barriers of its own for the stages of the rings, and a copying warp speaks to the tiles that
-// read a block.  All waits are bounded; when one gives up, the CTA records it and every role leaves.
+// Warps: 0 and 4 copy keys, 2 and 5 values (cp.async, 16 bytes a thread, swizzled for the tensor cores; a warp has half of every block, and
+// three blocks in flight); 1 issues tile A's products and owns the tensor memory, 3 tile B's; 6..9 softmax of A, 10..13 of B.  Each walks the
+// same segments by itself.  Barriers tell one turn from the next only, so each tile has barriers of its own for the stages of the rings, and a
+// copying warp speaks to the tiles that read a block.  All waits are bounded; when one gives up, the CTA records it and every role leaves.
 #include "attention_shared.cuh"
 #include "attention_tcgen05.cuh"
 
@@ -28,9 +28,9 @@ namespace lb {
 
 constexpr int SC_STAGES = 4;
 constexpr int SC_IN_FLIGHT = 2;                                // blocks a copying warp has requested beyond the one it waits for
-constexpr int SC_BARS = 4 * SC_STAGES + 12;                    // barriers of a tile
-constexpr int SC_THREADS = 640;
-enum : int { SC_ERR_Q = 401, SC_ERR_KV_FULL = 402, SC_ERR_KV_EMPTY = 403, SC_ERR_S_FULL = 404, SC_ERR_P_FULL = 405, SC_ERR_O_FULL = 406, SC_ERR_O_FREE = 407, SC_ERR_PAIR = 408 };
+constexpr int SC_BARS = 4 * SC_STAGES + 8;                     // barriers of a tile
+constexpr int SC_THREADS = 448, SC_SOFTMAX = 6;                // the first of the softmax warps
+enum : int { SC_ERR_Q = 401, SC_ERR_KV_FULL = 402, SC_ERR_KV_EMPTY = 403, SC_ERR_S_FULL = 404, SC_ERR_P_FULL = 405, SC_ERR_O_FULL = 406, SC_ERR_O_FREE = 407 };
 
 // Shared memory: queries of A and B | ring of keys | ring of values | barriers.  Rows of 128 bytes (64 elements), 128-byte swizzle, the second
 // 64 elements of a head a half further on.
@@ -39,8 +39,7 @@ template <int D> struct ScLayout {
   static constexpr int KV_HALF = AS_KEYS * 128, KV_TILE = HALVES * KV_HALF;
   static constexpr int Q_TILE = HALVES * TA_HALF_BYTES;
   static constexpr int K_OFF = 2 * Q_TILE, V_OFF = K_OFF + SC_STAGES * KV_TILE, BAR_OFF = V_OFF + SC_STAGES * KV_TILE;
-  static constexpr int PAIR_OFF = BAR_OFF + 2 * SC_BARS * 8 + 16;  // [2 turns][2 tiles][2 halves][128 rows]: what the two warps of a row tell each other
-  static constexpr int BYTES = PAIR_OFF + 2 * 2 * 2 * TA_ROWS * 4;
+  static constexpr int BYTES = BAR_OFF + 2 * SC_BARS * 8 + 16;     // and the tensor memory's address and two flags
 };
 
 // What a softmax warp keeps of its way and of the segment at hand in shared memory: its registers are for a block's scores and weights (what
@@ -51,17 +50,17 @@ struct ScWarp {
   long long tile;                        // where the tile's partial rows begin
 };
 
-// One block of 64 keys (or values) of a kv head from the pages into a stage of the ring, by one warp: a lane copies 16-byte chunk c of the
-// rows rp, rp + RPI, ...  `stage` is the stage's address plus the lane's half and row, xr[u] its swizzled chunk in rows rp + RPI u; `head` points
-// at the lane's chunk and row of the head in page 0; lane i holds the id of the i-th page of the block (-1: no page; pages of more than 64 tokens:
-// `sub` is where in the page the block begins).  Keys outside lo .. hi - 1 and of no page are filled with zeros.
+// Half of a block of 64 keys (or values) of a kv head from the pages into a stage of the ring, by one warp: a lane copies 16-byte chunk c of the
+// rows rp, rp + RPI, ... of the half.  `stage` is the half's address plus the lane's part of the head and row, xr[u] its swizzled chunk in rows
+// rp + RPI u; `head` points at the lane's chunk and row of the head in page 0; lane i holds the id of the half's i-th page (-1: no page; pages of more
+// than 32 tokens: `sub` is where in the page the half begins).  Keys outside lo .. hi - 1 and of no page are filled with zeros.
 template <int PS, int D>
-__device__ __forceinline__ void sc_copy_block(uint32_t stage, const uint32_t (&xr)[4], const uint8_t* head, int ids, int kb, int lo, int hi,
-                                              size_t page_stride, int rp, int sub) {
+__device__ __forceinline__ void sc_copy_half(uint32_t stage, const uint32_t (&xr)[4], const uint8_t* head, int ids, int kb, int lo, int hi,
+                                             size_t page_stride, int rp, int sub) {
   constexpr int RPI = 32 / (D / 8), ROW = D * 2;
-  const bool inner = kb >= lo && kb + AS_KEYS <= hi;           // every key of the block may be seen
+  const bool inner = kb >= lo && kb + 32 <= hi;                // every key may be seen
 #pragma unroll
-  for (int pg = 0; pg < AS_KEYS / PS; ++pg) {
+  for (int pg = 0; pg < 32 / PS; ++pg) {
     const int id = __shfl_sync(0xffffffffu, ids, pg);
     const uint8_t* src = head + (size_t)max(id, 0) * page_stride + sub * ROW;
 #pragma unroll
@@ -74,23 +73,15 @@ __device__ __forceinline__ void sc_copy_block(uint32_t stage, const uint32_t (&x
   }
 }
 
-// The lowest n bits (none below 0, all from 32 on).
-__device__ __forceinline__ uint32_t sc_low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
-
-// The caller waits with ta_tmem_wait_st() before it tells anyone.
-__device__ __forceinline__ void sc_tmem_st16(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
-      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
-      : "memory");
-}
+// The lowest n bits (none below 0, all from 64 on).
+__device__ __forceinline__ unsigned long long sc_low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 
 template <int D>
 __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(SharedParams p) {
   typedef ScLayout<D> L;
   extern __shared__ uint8_t smem_raw[];
   __shared__ SharedPlan plan;
-  __shared__ ScWarp states[SC_THREADS / 32 - 4];
+  __shared__ ScWarp states[SC_THREADS / 32 - SC_SOFTMAX];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = ta_smem_u32(smem);
   const uint32_t bars = sbase + L::BAR_OFF;
@@ -104,7 +95,6 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   auto pv_done = [&](int t, int b) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + 4 + b); };
   auto q_full = [&](int t) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + 6); };
   auto o_free = [&](int t) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + 7); };
-  auto pair_bar = [&](int t, int q) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + 8 + q); };     // the two warps of 32 rows
   uint32_t* tmem_slot = (uint32_t*)(smem + L::BAR_OFF + 2 * SC_BARS * 8);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   volatile int* holes = (volatile int*)(tmem_slot + 2);       // some key of this CTA's segments lies in no page
@@ -113,10 +103,12 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
-      for (int i = 0; i < 4 * SC_STAGES; ++i) ta_mbar_init(k_full(t, i), 1);
-      for (int b = 0; b < 2; ++b) { ta_mbar_init(s_full(t, b), 1); ta_mbar_init(p_full(t, b), 8); ta_mbar_init(pv_done(t, b), 1); }
-      ta_mbar_init(q_full(t), 8); ta_mbar_init(o_free(t), 8);
-      for (int q = 0; q < 4; ++q) ta_mbar_init(pair_bar(t, q), 2);
+      for (int i = 0; i < SC_STAGES; ++i) {
+        ta_mbar_init(k_full(t, i), 2); ta_mbar_init(k_empty(t, i), 1);     // two warps copy the halves of a block
+        ta_mbar_init(v_full(t, i), 2); ta_mbar_init(v_empty(t, i), 1);
+      }
+      for (int b = 0; b < 2; ++b) { ta_mbar_init(s_full(t, b), 1); ta_mbar_init(p_full(t, b), 4); ta_mbar_init(pv_done(t, b), 1); }
+      ta_mbar_init(q_full(t), 4); ta_mbar_init(o_free(t), 4);
     }
     *abort_flag = 0;
     *holes = 0;
@@ -130,82 +122,103 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   as_make_plan(p, plan, blockIdx.x, gridDim.x);                // lengths and groups were written before the kernel ahead began
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   pdl_wait();
-  const uint32_t tmem = *tmem_slot;            // columns: tile t's S buffers at t * 128 and t * 128 + 64 (P over the first 16 of each half), O at 256 + t * 128
+  const uint32_t tmem = *tmem_slot;            // columns: tile t's S buffers at t * 128 and t * 128 + 64 (P over their first 32), O at 256 + t * 128
 
   const int G = p.group, per = p.lane_tokens, cta = blockIdx.x;
   Walk way = as_begin(p, plan, cta);
   // the tiles that work on a segment, as bits: segments of one tile go to tile A and B in turn
   auto tiles_of = [&](const Segment& g, int& singles) -> int { return g.tokens > per ? 3 : 1 << (singles++ & 1); };
 
-  if (warp == 0 || warp == 2) {
-    // ---- copies ------------------------------------------------------------------------------------------------------------------
-    const bool is_v = warp == 2;
+  if (warp != 1 && warp != 3 && warp < SC_SOFTMAX) {
+    // ---- copies: warps 0 and 4 the halves of every block of keys, 2 and 5 of values -----------------------------------------------------
+    const bool is_v = warp == 2 || warp == 5;
+    const int half = warp >= 4 ? 1 : 0;
     constexpr int CHUNKS = D / 8, RPI = 32 / CHUNKS;           // 16-byte chunks of a row, rows an instruction
     const int c = lane % CHUNKS, rp = lane / CHUNKS;
     const uint8_t* pool = (const uint8_t*)(is_v ? p.v_cache : p.k_cache) + c * 16 + rp * (D * 2);
-    const uint32_t ring = sbase + (is_v ? L::V_OFF : L::K_OFF) + (uint32_t)(c >> 3) * L::KV_HALF + (uint32_t)rp * 128u;
+    const uint32_t ring = sbase + (is_v ? L::V_OFF : L::K_OFF) + (uint32_t)(c >> 3) * L::KV_HALF + (uint32_t)(half * 32 + rp) * 128u;
     uint32_t xr[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) xr[u] = (uint32_t)(((c & 7) ^ ((rp + RPI * u) & 7)) << 4);
-    const int ps = p.page_size, shift = p.page_shift, size = min(ps, AS_KEYS);
+    const int ps = p.page_size, shift = p.page_shift, size = min(ps, 32);
     const size_t page_stride = (size_t)p.kv_heads * ps * (D * 2);
     bool ok = true;
-    int n = 0, singles = 0;                    // blocks so far, segments of one tile so far
+    int n = 0, handed = 0, singles = 0;        // blocks requested, handed over; segments of one tile
     uint32_t used = 0, turn0 = 0, turn1 = 0;   // of stage s: the tiles that read its block (bits 2 s, 2 s + 1); of tiles A and B, bit s: the parity of the next wait
-    auto hand_over = [&](int i) {              // block i has landed: visible to the tensor cores, then said so to its tiles
-      const int s = i % SC_STAGES;
+    // The block to come: its segment, this half's first key, lane i the id of the half's i-th page (-1: no page, or no key of the segment in it).
+    // It is looked up before the one at hand is copied, across the ends of segments.
+    int left = 0, kb = 0, lo = 0, hi = 0, ids = -1;
+    uint32_t tiles = 0;
+    const int* bt = nullptr;
+    const uint8_t* head = nullptr;
+    auto look_ahead = [&]() -> bool {
+      if (left == 0) {
+        for (;;) {
+          if (way.x >= way.x_end) return false;
+          const Segment g = as_next(p, plan, cta, way);
+          if (g.blocks == 0) continue;
+          tiles = (uint32_t)tiles_of(g, singles);
+          bt = p.table + (size_t)g.request * p.max_pages;
+          head = pool + (size_t)g.kv_head * ps * (D * 2);
+          left = g.blocks; lo = g.key_lo; hi = g.key_hi;
+          kb = (lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS + half * 32;
+          break;
+        }
+      } else {
+        kb += AS_KEYS;
+      }
+      --left;
+      const int key = kb + lane * size;
+      ids = -1;
+      if (lane * size < 32 && key < hi && key + size > lo) {
+        const int id = bt[key >> shift];
+        if (id >= 0 && id < p.num_pages) ids = id;
+        else *holes = 1;                       // before the block is handed over
+      }
+      return true;
+    };
+    auto hand_over = [&]() {                   // the oldest block has landed: visible to the tensor cores, then said so to its tiles
+      const int s = handed++ % SC_STAGES;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane < 2 && ((used >> (2 * s + lane)) & 1u)) ta_mbar_arrive(is_v ? v_full(lane, s) : k_full(lane, s));
     };
-    while (way.x < way.x_end && ok) {
-      const Segment g = as_next(p, plan, cta, way);
-      if (g.blocks == 0) continue;
-      const uint32_t tiles = (uint32_t)tiles_of(g, singles);
-      const int* bt = p.table + (size_t)g.request * p.max_pages;
-      const uint8_t* head = pool + (size_t)g.kv_head * ps * (D * 2);
-      const int first_key = (g.key_lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS;
-      // lane i: the id of the i-th page of the block at kb, -1 where no key of this segment lies
-      auto page_of = [&](int kb) -> int {
-        const int key = kb + lane * size;
-        if (lane * size >= AS_KEYS || key >= g.key_hi || key + size <= g.key_lo) return -1;
-        const int id = bt[key >> shift];
-        if (id >= 0 && id < p.num_pages) return id;
-        *holes = 1;                            // before the block is handed over
-        return -1;
-      };
-      int ids = page_of(first_key);
-      for (int b = 0; b < g.blocks; ++b, ++n) {
-        const int s = n % SC_STAGES, kb = first_key + b * AS_KEYS;
-        const int next_ids = b + 1 < g.blocks ? page_of(kb + AS_KEYS) : -1;
-        // the tiles that read this stage's last block are through with it
-        const uint32_t before = (used >> (2 * s)) & 3u;
-        int go = 1;
-        if (lane < 2 && ((before >> lane) & 1u))
-          go = ta_mbar_wait_idle(is_v ? v_empty(lane, s) : k_empty(lane, s), ((lane ? turn1 : turn0) >> s) & 1u, abort_flag, SC_ERR_KV_EMPTY) ? 1 : 0;
+    bool more = look_ahead();
+    while (more && ok) {
+      const int s = n % SC_STAGES, kb_now = kb, lo_now = lo, hi_now = hi, ids_now = ids;
+      const uint32_t tiles_now = tiles;
+      const uint8_t* head_now = head;
+      more = look_ahead();
+      // The tiles that read this stage's last block are through with it.  While that has to be waited for, whatever has been requested is handed over.
+      const uint32_t before = (used >> (2 * s)) & 3u;
+      const uint32_t bar = is_v ? v_empty(lane & 1, s) : k_empty(lane & 1, s), parity = ((lane & 1 ? turn1 : turn0) >> s) & 1u;
+      const bool mine = lane < 2 && ((before >> lane) & 1u);
+      if (__any_sync(0xffffffffu, mine && !ta_mbar_try_wait(bar, parity))) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        while (handed < n) hand_over();
+        const int go = !mine || ta_mbar_wait_idle(bar, parity, abort_flag, SC_ERR_KV_EMPTY) ? 1 : 0;
         if (__any_sync(0xffffffffu, go == 0)) { ok = false; break; }
-        turn0 ^= (before & 1u) << s;
-        turn1 ^= (before >> 1) << s;
-        used = (used & ~(3u << (2 * s))) | (tiles << (2 * s));
-        const uint32_t stage = ring + (uint32_t)s * L::KV_TILE;
-        switch (ps) {
-          case 8: sc_copy_block<8, D>(stage, xr, head, ids, kb, g.key_lo, g.key_hi, page_stride, rp, 0); break;
-          case 16: sc_copy_block<16, D>(stage, xr, head, ids, kb, g.key_lo, g.key_hi, page_stride, rp, 0); break;
-          case 32: sc_copy_block<32, D>(stage, xr, head, ids, kb, g.key_lo, g.key_hi, page_stride, rp, 0); break;
-          default: sc_copy_block<64, D>(stage, xr, head, ids, kb, g.key_lo, g.key_hi, page_stride, rp, kb & (ps - 1)); break;
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (n >= SC_IN_FLIGHT) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(SC_IN_FLIGHT) : "memory");
-          hand_over(n - SC_IN_FLIGHT);
-        }
-        ids = next_ids;
+      }
+      turn0 ^= (before & 1u) << s;
+      turn1 ^= (before >> 1) << s;
+      used = (used & ~(3u << (2 * s))) | (tiles_now << (2 * s));
+      const uint32_t stage = ring + (uint32_t)s * L::KV_TILE;
+      switch (ps) {
+        case 8: sc_copy_half<8, D>(stage, xr, head_now, ids_now, kb_now, lo_now, hi_now, page_stride, rp, 0); break;
+        case 16: sc_copy_half<16, D>(stage, xr, head_now, ids_now, kb_now, lo_now, hi_now, page_stride, rp, 0); break;
+        default: sc_copy_half<32, D>(stage, xr, head_now, ids_now, kb_now, lo_now, hi_now, page_stride, rp, kb_now & (ps - 1)); break;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      ++n;
+      if (n - handed > SC_IN_FLIGHT) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(SC_IN_FLIGHT) : "memory");
+        hand_over();
       }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (ok)
-      for (int i = max(n - SC_IN_FLIGHT, 0); i < n; ++i) hand_over(i);
-    if (is_v) as_write_records(p, plan, cta, gridDim.x, lane, 32);         // while the last blocks are worked on
+      while (handed < n) hand_over();
+    if (warp == 5) as_write_records(p, plan, cta, gridDim.x, lane, 32);    // while the last blocks are worked on
   } else if (warp == 1 || warp == 3) {
     // ---- products, one thread a tile -------------------------------------------------------------------------------------------------
     const int t = warp == 1 ? 0 : 1;
@@ -248,7 +261,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
           const uint32_t va = sbase + L::V_OFF + s * L::KV_TILE;
 #pragma unroll
           for (int k = 0; k < AS_KEYS / 16; ++k)
-            ta_umma_ts(o_col, s_col + (uint32_t)b * 64u + (uint32_t)(k >> 1) * 32u + (uint32_t)(k & 1) * 8u, ta_desc_mnmajor(va + (uint32_t)k * 16u * 128u, L::KV_HALF), idesc_pv, (i | k) != 0);
+            ta_umma_ts(o_col, s_col + (uint32_t)b * 64u + (uint32_t)k * 8u, ta_desc_mnmajor(va + (uint32_t)k * 16u * 128u, L::KV_HALF), idesc_pv, (i | k) != 0);
           ta_commit(pv_done(t, b));
           ta_commit(v_empty(t, s));
           if (i + 2 < g.blocks) ok = issue_qk(i + 2);          // where P(i) lies: the tensor cores finish P V(i) first
@@ -259,36 +272,23 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       }
     }
   } else {
-    // ---- softmax: two threads a query row, one for each half of a block's keys; warp w reads lanes (w % 4) * 32 .. + 31 of tensor memory ---
-    const int t = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;
+    // ---- softmax: thread = query row; warp w reads lanes (w % 4) * 32 .. + 31 of tensor memory ---------------------------------------------
+    const int t = (warp - SC_SOFTMAX) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t tlane = (uint32_t)(quarter * 32) << 16;
-    const uint32_t s_addr = tmem + tlane + (uint32_t)t * 128u + (uint32_t)half * 32u, o_addr = tmem + tlane + 256u + (uint32_t)t * 128u + (uint32_t)half * (D / 2);
+    const uint32_t s_addr = tmem + tlane + (uint32_t)t * 128u, o_addr = tmem + tlane + 256u + (uint32_t)t * 128u;
     const uint32_t q_rows = sbase + t * L::Q_TILE + (uint32_t)quarter * 32u * 128u;        // this warp's rows
-    const uint32_t my_pair = pair_bar(t, quarter);
-    float* told = reinterpret_cast<float*>(smem + L::PAIR_OFF) + t * 2 * TA_ROWS + r;      // [turn][.][half][row]
-    int turns = 0;
-    volatile ScWarp* mem = states + (warp - 4);
+    volatile ScWarp* mem = states + (warp - SC_SOFTMAX);
     if (lane == 0) {
       mem->way.x = way.x; mem->way.x_end = way.x_end; mem->way.kv_head = way.kv_head; mem->way.at = way.at; mem->way.tile = way.tile;
       mem->singles = 0;
     }
     __syncwarp();
     bool ok = true;
-    // Tells the row's other thread x and gets its.  Values of one turn are overwritten two turns later, when both have read them.
-    auto exchange = [&](float x) -> float {
-      float* at = told + (turns & 1) * 4 * TA_ROWS;
-      at[half * TA_ROWS] = x;
-      __syncwarp();
-      if (lane == 0) ta_mbar_arrive(my_pair);
-      if (!ta_mbar_wait(my_pair, (uint32_t)(turns & 1), abort_flag, SC_ERR_PAIR)) { ok = false; return x; }
-      ++turns;
-      return at[(half ^ 1) * TA_ROWS];
-    };
     // Of the segment at hand: blocks, the first one's first key, the first key and the end of those this row sees (of none, if there is no such
     // row), and the least end among the warp's rows.
     int blocks = 0, block_key = 0, lo = 0, hi = 0, hi_all = 0;
     bool valid = false, warp_valid = false;
-    // The next segment of this tile, if there is one: its queries are requested, half of a warp's rows by each of the two.
+    // The next segment of this tile, if there is one: its queries are requested.
     auto next_segment = [&]() -> bool {
       Walk at_now;
       at_now.x = mem->way.x; at_now.x_end = mem->way.x_end; at_now.kv_head = mem->way.kv_head; at_now.at = mem->way.at; at_now.tile = mem->way.tile;
@@ -324,8 +324,8 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         constexpr int CHUNKS = D / 8, RPI = 32 / CHUNKS;       // whole rows side by side
         const int c = lane % CHUNKS;
 #pragma unroll
-        for (int i = 0; i < 16 / RPI; ++i) {
-          const int rr = half * 16 + i * RPI + lane / CHUNKS, at = __shfl_sync(0xffffffffu, from, rr);
+        for (int i = 0; i < 32 / RPI; ++i) {
+          const int rr = i * RPI + lane / CHUNKS, at = __shfl_sync(0xffffffffu, from, rr);
           if (at >= 0)
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
                          ::"r"(q_rows + (uint32_t)rr * 128u + (uint32_t)(c >> 3) * TA_HALF_BYTES + (uint32_t)(((c & 7) ^ (rr & 7)) << 4)),
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       float m_ref = -INFINITY, l_run = 0.f;
       bool settled = false;                    // every row has a reference
       for (int i = 0; i < blocks; ++i, block_key += AS_KEYS) {
-        const int j = mine + i, b = j & 1, kb = block_key + half * 32;
+        const int j = mine + i, b = j & 1, kb = block_key;
         ok = ta_mbar_wait(s_full(t, b), (uint32_t)((j >> 1) & 1), abort_flag, SC_ERR_S_FULL);
         if (!ok) break;
         if (!warp_valid) {                     // no row of this warp: its rows of P are anything, and nobody reads what comes of them
@@ -356,13 +356,11 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
           continue;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        uint32_t seen = 0xffffffffu;           // which of this half's keys the row sees
-        bool masked = kb < lo || kb + 32 > hi_all;
-        if (masked) seen = sc_low_bits(hi - kb) & ~sc_low_bits(lo - kb);
+        bool masked = kb < lo || kb + AS_KEYS > hi_all;
+        unsigned long long seen = sc_low_bits(hi - kb) & ~sc_low_bits(lo - kb);        // which of the block's keys the row sees
         if (*holes) {                          // there are pages that are not: a look at this block's
-          const int size = min(p.page_size, 32);
-          const int key = kb + lane * size;
-          const bool here = lane * size < 32 && key < mem->key_hi && key + size > lo;
+          const int size = min(p.page_size, AS_KEYS), key = kb + lane * size;
+          const bool here = lane * size < AS_KEYS && key < mem->key_hi && key + size > lo;
           const int id = here ? p.table[(size_t)mem->request * p.max_pages + (key >> p.page_shift)] : 0;
           uint32_t absent = __ballot_sync(0xffffffffu, id < 0 || id >= p.num_pages);
           masked |= absent != 0;
@@ -371,33 +369,34 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
             seen &= ~(sc_low_bits(first + size) & ~sc_low_bits(first));
           }
         }
-        // Where every row has a reference, its maximum is not looked for: sums of 32 weights that stay below 2^14 say that no score is
+        // Where every row has a reference, its maximum is not looked for: a sum of 64 weights that stays below 2^15 says that no score is
         // far above the reference.  Otherwise the block is done again from the scores, which still lie in tensor memory, with the maximum.
-        uint32_t w[16];
+        uint32_t w[32];
         float sum;
         for (bool exact = !settled;; exact = true) {
-          float xs[32];
+          float xs[AS_KEYS];
           {
-            uint32_t v[32];
-            ta_tmem_ld32(s_addr + (uint32_t)b * 64u, v);
+            uint32_t v[AS_KEYS];
+            ta_tmem_ld64(s_addr + (uint32_t)b * 64u, v);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) xs[e] = __uint_as_float(v[e]);
+            for (int e = 0; e < AS_KEYS; ++e) xs[e] = __uint_as_float(v[e]);
           }
           if (masked) {
+            const uint32_t low = (uint32_t)seen, high = (uint32_t)(seen >> 32);
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((seen >> e) & 1u)) xs[e] = -INFINITY;
+            for (int e = 0; e < 32; ++e) {
+              if (!((low >> e) & 1u)) xs[e] = -INFINITY;
+              if (!((high >> e) & 1u)) xs[32 + e] = -INFINITY;
+            }
           }
           if (exact) {
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
+            for (int e = 0; e < AS_KEYS; e += 8) {
 #pragma unroll
               for (int u = 0; u < 4; ++u) mx4[u] = ta_max3(mx4[u], xs[e + 2 * u], xs[e + 2 * u + 1]);
             }
-            float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-            mx = fmaxf(mx, exchange(mx));
-            if (!ok) break;
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
             const float m_loc = mx * p.scale_log2;
             const bool grow = valid && m_loc > m_ref + TA_RESCALE_STEP;  // also true for the first finite maximum (m_ref = -inf)
             if (__any_sync(0xffffffffu, grow)) {
@@ -412,7 +411,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-                for (int c = 0; c < D / 2; c += 32) {          // half of the dimensions each
+                for (int c = 0; c < D; c += 32) {
                   uint32_t v[32];
                   ta_tmem_ld32(o_addr + (uint32_t)c, v);
 #pragma unroll
@@ -428,7 +427,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
           const uint64_t scale2 = ta_pack2(p.scale_log2, p.scale_log2), negm2 = ta_pack2(-m_use, -m_use);
           uint64_t sum2 = ta_pack2(0.f, 0.f);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
+          for (int e = 0; e < 32; ++e) {
             float y0, y1;
             ta_unpack2(ta_fma2(ta_pack2(xs[2 * e], xs[2 * e + 1]), scale2, negm2), y0, y1);
             const float p0 = exp2_approx(y0), p1 = exp2_approx(y1);      // 2^-inf = 0 for masked keys
@@ -440,13 +439,10 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
           ta_unpack2(sum2, s0, s1);
           sum = s0 + s1;
           if (exact) break;
-          // both halves of the keys, for all 32 rows
-          const bool far = __any_sync(0xffffffffu, valid && !(sum < 16384.f));
-          if (exchange(far ? 1.f : 0.f) == 0.f && !far) break;
-          if (!ok) break;
+          if (!__any_sync(0xffffffffu, valid && !(sum < 32768.f))) break;
         }
         if (!ok) break;
-        sc_tmem_st16(s_addr + (uint32_t)b * 64u, w);
+        ta_tmem_st32(s_addr + (uint32_t)b * 64u, w);
         ta_tmem_wait_st();
         l_run += sum;
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -464,12 +460,10 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (some_valid) {
-        l_run += exchange(l_run);
-        if (!ok) break;
-        if (row_valid && half == 0) *reinterpret_cast<float2*>(p.part_ml + (tile + row) * 2) = make_float2(m_ref, l_run);
-        float4* dst = reinterpret_cast<float4*>(p.part_o + tile * D) + (size_t)half * (D / 8) * rows + row;
+        if (row_valid) *reinterpret_cast<float2*>(p.part_ml + (tile + row) * 2) = make_float2(m_ref, l_run);
+        float4* dst = reinterpret_cast<float4*>(p.part_o + tile * D) + row;
 #pragma unroll 1
-        for (int c = 0; c < D / 2; c += 32) {
+        for (int c = 0; c < D; c += 32) {
           uint32_t v[32];
           ta_tmem_ld32(o_addr + (uint32_t)c, v);               // warp-wide: rows without a token take part and write nothing
           if (row_valid) {
@@ -497,7 +491,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
 template <int D>
 static cudaError_t sc_launch(const SharedParams& p, int ctas, cudaStream_t stream) {
   constexpr int smem = ScLayout<D>::BYTES + 1024;
-  static_assert(smem + sizeof(SharedPlan) + sizeof(ScWarp) * (SC_THREADS / 32 - 4) + 64 <= 227 * 1024, "shared memory of a CTA");
+  static_assert(smem + sizeof(SharedPlan) + sizeof(ScWarp) * (SC_THREADS / 32 - SC_SOFTMAX) + 64 <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<unsigned long long> configured{0ull};     // a bit a device
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);

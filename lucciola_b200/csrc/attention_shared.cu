@@ -13,6 +13,7 @@ namespace lb {
 
 constexpr int AP_THREADS = 256;
 constexpr int AP_ROWS = 32;
+constexpr int AS_FEW_BLOCKS = 296;
 
 __device__ __forceinline__ float4 ap_load4(const float* p) { return __ldcg(reinterpret_cast<const float4*>(p)); }
 __device__ __forceinline__ float4 ap_load4(const bf16* p) {
@@ -54,7 +55,7 @@ __global__ void __launch_bounds__(AP_THREADS) attention_shared_plain_kernel(Shar
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < rows && c < d) {
         int token, position;
-        as_token(plan, g, r / G, token, position);
+        as_token(plan, g.shared, g.request, g.first + r / G, token, position);
         v = ap_load4(q + ((size_t)token * p.heads + g.kv_head * G + r % G) * d + c);
       }
       *reinterpret_cast<float4*>(qs + r * D + c) = v;
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(AP_THREADS) attention_shared_plain_kernel(Shar
     for (int e = 0; e < 2; ++e) {
       int token;
       last[e] = -1;
-      if (2 * ty + e < rows) as_token(plan, g, (2 * ty + e) / G, token, last[e]);
+      if (2 * ty + e < rows) as_token(plan, g.shared, g.request, g.first + (2 * ty + e) / G, token, last[e]);
     }
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     float o[2][D / 64][4];
@@ -173,10 +174,11 @@ static int as_sms() {
 }
 
 // How a launch cuts its rows: kv heads that share a cached one, heads of a tile, tokens of a tile and of a part of one.
-struct SharedCut { bool tc; int share, group, tile_tokens, lane_tokens; };
+struct SharedCut { bool tc; int share, group, tile_tokens, lane_tokens, folds; };
 static SharedCut as_cut(int dtype, int group, int head_dim, int page_size) {
-  SharedCut c{attention_shared_tc_takes(dtype, group, head_dim, page_size), 1, group, 0, 0};
+  SharedCut c{attention_shared_tc_takes(dtype, group, head_dim, page_size), 1, group, 0, 0, 1};
   if (c.tc) {
+    c.folds = 4;
     attention_shared_tc_cut(group, c.tile_tokens, c.lane_tokens);
     return c;
   }
@@ -202,19 +204,22 @@ static cudaError_t ap_launch(const SharedParams& p, int ctas, cudaStream_t strea
 
 template <typename T>
 static cudaError_t as_combine(const SharedParams& p, cudaStream_t stream) {
-  return launch(as_combine_kernel<T>, dim3(p.T, p.kv_heads), dim3(AS_COMBINE_THREADS), 0, stream, p);
+  // Few rows: four threads share a row's partial results, so that one round of loads reads them all.
+  if ((long long)p.T * p.kv_heads <= AS_FEW_BLOCKS)
+    return launch(as_combine_kernel<T, 4>, dim3(p.T, p.kv_heads), dim3(4 * AS_COMBINE_THREADS), 0, stream, p);
+  return launch(as_combine_kernel<T, 1>, dim3(p.T, p.kv_heads), dim3(AS_COMBINE_THREADS), 0, stream, p);
 }
 
 }  // namespace lb
 
 // Elements of the two workspaces of a launch: partial results (float32) and the combining kernel's list (int32).
-LB_EXPORT int lb_attention_shared_workspace(int num_tokens, int num_q_heads, int num_kv_heads, int head_dim, int dtype, int page_size,
+LB_EXPORT int lb_attention_shared_workspace(int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int dtype, int page_size,
                                             long long* floats, long long* ints) {
   LB_CHECK_ARG(num_tokens >= 0 && num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0 && head_dim > 0, "attention_shared: bad sizes");
   const int ctas = lb::as_sms();
   LB_CHECK_ARG(ctas > 0, "attention_shared: no device");
   const lb::SharedCut cut = lb::as_cut(dtype, num_q_heads / num_kv_heads, head_dim, page_size);
-  const long long rows = 2ll * num_tokens * num_q_heads + (long long)ctas * cut.tile_tokens * cut.group;
+  const long long rows = lb::as_most_rows(num_tokens, num_seqs, cut.group, cut.folds) * num_kv_heads * cut.share + (long long)ctas * cut.tile_tokens * cut.group;
   *floats = rows * (head_dim + 2);
   *ints = (long long)num_tokens * lb::AS_REC + 8;
   return 0;
@@ -240,7 +245,7 @@ LB_EXPORT int lb_attention_shared(int dtype, const void* q, void* out, const voi
   LB_CHECK_ARG(((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)floats | (uintptr_t)ints) % 16 == 0,
                "attention_shared: operands must be 16-byte aligned");
   long long need_floats = 0, need_ints = 0;
-  if (lb_attention_shared_workspace(num_tokens, num_q_heads, num_kv_heads, head_dim, dtype, page_size, &need_floats, &need_ints)) return 1;
+  if (lb_attention_shared_workspace(num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, dtype, page_size, &need_floats, &need_ints)) return 1;
   LB_CHECK_ARG(floats && ints && num_floats >= need_floats && num_ints >= need_ints,
                "attention_shared: workspaces of %lld and %lld elements are needed, got %lld and %lld", need_floats, need_ints, num_floats, num_ints);
   const int ctas = lb::as_sms();
@@ -250,12 +255,12 @@ LB_EXPORT int lb_attention_shared(int dtype, const void* q, void* out, const voi
   p.cu = cu_tokens; p.ctx = context_lens; p.prefix_of = prefix_of; p.prefix_lens = prefix_lens;
   p.T = num_tokens; p.S = num_seqs; p.heads = num_q_heads; p.kv_heads = num_kv_heads * cut.share; p.group = cut.group; p.dim = head_dim;
   p.page_size = page_size; p.page_shift = -1; p.kv_share = cut.share; p.tile_tokens = cut.tile_tokens; p.lane_tokens = cut.lane_tokens;
-  p.min_span = cut.tc ? 2 : 1;
+  p.min_span = cut.tc ? 4 : 1; p.tile_start = cut.tc ? 2 : 0; p.folds = cut.folds;
   for (int b = 0; b < 31; ++b) if ((1 << b) == page_size) p.page_shift = b;
   p.scale_log2 = scale * 1.4426950408889634f;
   // units of the whole line, at most
   const long long tiles = 2ll * ((long long)num_tokens / p.tile_tokens + num_seqs), blocks = (long long)max_pages * page_size / lb::AS_KEYS + 1;
-  LB_CHECK_ARG(tiles * 2 * blocks * p.kv_heads < (1ll << 31) - 65536, "attention_shared: %d tokens of %d requests on tables of %d pages are too much for one launch",
+  LB_CHECK_ARG(tiles * (2 * blocks + 2) * p.kv_heads < (1ll << 31) - 65536, "attention_shared: %d tokens of %d requests on tables of %d pages are too much for one launch",
                num_tokens, num_seqs, max_pages);
   LB_CHECK_ARG(p.kv_heads <= 65535, "attention_shared: %d kv heads", p.kv_heads);
   const long long rows = (need_floats) / (head_dim + 2);

@@ -20,6 +20,7 @@ namespace lb {
 constexpr int AS_MAX_SEQS = 256;
 constexpr int AS_KEYS = 64;
 constexpr int AS_REC = 12;               // integers a token in the combining kernel's list
+constexpr int AS_FOLD_ROWS = 32;
 
 struct SharedParams {
   const void* q; void* out;              // [T, heads, dim]
@@ -30,6 +31,8 @@ struct SharedParams {
   int kv_share;                          // kv head j of this launch reads cache head j / kv_share
   int tile_tokens, lane_tokens;          // tokens of a tile; a tile of more than lane_tokens counts twice
   int min_span;                          // least units a CTA takes
+  int tile_start;                        // units that a tile costs beside its blocks
+  int folds;                             // a request's tile of at most AS_FOLD_ROWS rows leaves this many partial results, one behind the other
   float scale_log2;
   // Partial results: 4 consecutive dimensions of all rows of a tile, then the next 4 ([dim / 4][rows][4], so that threads with a row each
   // write, and threads with a head each read, side by side), and [rows][2]: the reference value (-inf: no key) and the sum.
@@ -60,13 +63,21 @@ struct SharedPlan {
 
 __device__ __forceinline__ int as_blocks(int lo, int hi) { return hi > lo ? (hi - (lo & ~(AS_KEYS - 1)) + AS_KEYS - 1) / AS_KEYS : 0; }
 
-// Units of `tokens` tokens in tiles with `blocks` blocks each.
+__device__ __forceinline__ int as_tile_units(const SharedParams& p, int tokens, int blocks) {
+  return p.tile_start + (tokens > p.lane_tokens ? 2 * blocks : blocks);
+}
+// Units of `tokens` tokens in tiles with `blocks` blocks each, and the rows of their partial results.
 __device__ __forceinline__ int as_units(const SharedParams& p, int tokens, int blocks) {
   if (tokens <= 0 || blocks <= 0) return 0;
-  const int twice = p.tile_tokens > p.lane_tokens ? 2 : 1;
-  if (tokens <= p.tile_tokens) return blocks * (tokens > p.lane_tokens ? 2 : 1);
-  const int full = (tokens - 1) / p.tile_tokens, last = tokens - full * p.tile_tokens;
-  return blocks * (full * twice + (last > p.lane_tokens ? 2 : 1));
+  if (tokens <= p.tile_tokens) return as_tile_units(p, tokens, blocks);
+  const int full = (tokens - 1) / p.tile_tokens;
+  return full * as_tile_units(p, p.tile_tokens, blocks) + as_tile_units(p, tokens - full * p.tile_tokens, blocks);
+}
+__device__ __forceinline__ int as_folds(const SharedParams& p, int rows) { return rows <= AS_FOLD_ROWS ? p.folds : 1; }
+__device__ __forceinline__ int as_rows(const SharedParams& p, int tokens) {        // of a request
+  if (tokens <= 0) return 0;
+  const int last = tokens <= p.tile_tokens ? tokens : tokens - (tokens - 1) / p.tile_tokens * p.tile_tokens;
+  return (tokens - last) * p.group + last * p.group * as_folds(p, last * p.group);
 }
 
 // An exclusive sum over `n` numbers by one warp, in place; returns the whole.  A lane has a run of them.
@@ -89,8 +100,6 @@ __device__ __forceinline__ int as_scan(int* a, int n) {
   }
   return total;
 }
-
-__device__ __forceinline__ int as_tile_units(const SharedParams& p, int blocks) { return p.tile_tokens > p.lane_tokens ? 2 * blocks : blocks; }
 
 // Made by all threads of a CTA (256 at least, a power of two of them or 384); ends with a barrier.  Reads lengths and groups only.
 __device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& pl, int cta, int ctas) {
@@ -136,7 +145,7 @@ __device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& 
       pl.first_member[s] = led;
       const int ua = leads ? as_units(p, led_tokens, as_blocks(0, me.w)) : 0, ub = as_units(p, me.y, as_blocks(shares ? prefix : 0, me.z));
       pl.unit[s] = ua; pl.unit[n + s] = ub;
-      pl.row[s] = leads ? led_tokens * p.group : 0; pl.row[n + s] = me.y * p.group;
+      pl.row[s] = leads ? led_tokens * p.group : 0; pl.row[n + s] = as_rows(p, me.y);
       pl.place[s] = ua > 0 ? 1 : 0; pl.place[n + s] = ub > 0 ? 1 : 0;
     }
   }
@@ -172,7 +181,7 @@ __device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& 
         const int nb = e < n ? as_blocks(0, pl.meta[e].w) : as_blocks(l >= 0 ? pl.meta[l].w : 0, pl.meta[e - n].z);
         pl.kv_head = kv;
         pl.at = at;
-        pl.tile = (int)((unsigned)(u - from) / (unsigned)as_tile_units(p, nb));
+        pl.tile = (int)((unsigned)(u - from) / (unsigned)as_tile_units(p, p.tile_tokens, nb));        // (only the last tile may be smaller)
       }
     }
   }
@@ -181,10 +190,14 @@ __device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& 
 }
 
 // cu_tokens that fall would make more rows than there is room for: nothing is done then.
-__device__ __forceinline__ bool as_sound(const SharedParams& p, const SharedPlan& pl) { return pl.rows <= 2 * p.T * p.group; }
+__host__ __device__ __forceinline__ long long as_most_rows(long long tokens, long long seqs, int group, int folds) {
+  const long long rows = tokens * group, folded = seqs * AS_FOLD_ROWS;      // a request's last tile may be folded
+  return 2 * rows + (folds - 1) * (folded < rows ? folded : rows);
+}
+__device__ __forceinline__ bool as_sound(const SharedParams& p, const SharedPlan& pl) { return pl.rows <= as_most_rows(p.T, p.S, p.group, p.folds); }
 
 // What the combining kernel has to know of every token, for the prefix and for the request's own keys: the first row of the token's
-// tile, the token's first row in the tile, the tile's rows, the unit of its first block, and how many units further the last block begins
+// tile, the token's first row in the tile, the tile's rows (not folded), the unit of its first block, and how many units further the last block begins
 // (-1: no block).  By `threads` threads of each CTA; the CTAs without work come first.
 __device__ __forceinline__ void as_write_records(const SharedParams& p, const SharedPlan& pl, int cta, int ctas, int thread, int threads) {
   if (cta == 0 && thread == 0) {
@@ -192,7 +205,6 @@ __device__ __forceinline__ void as_write_records(const SharedParams& p, const Sh
     p.head[3] = p.S > 0 ? pl.q0[0] : 0;
     p.head[4] = p.S > 0 ? pl.q0[p.S - 1] + pl.meta[p.S - 1].y : 0;
   }
-  const int twice = p.tile_tokens > p.lane_tokens ? 2 : 1;
   for (int s = ctas - 1 - cta; s < p.S; s += ctas) {
     const int4 me = pl.meta[s];
     const int t0 = pl.q0[s], q = me.y, l = pl.lead[s];
@@ -203,13 +215,13 @@ __device__ __forceinline__ void as_write_records(const SharedParams& p, const Sh
       if (l >= 0) {
         const int index = pl.rank[s] + i, tokens = pl.led[l], nb = as_blocks(0, prefix);
         const int tile = index / p.tile_tokens, first = tile * p.tile_tokens, here = min(tokens - first, p.tile_tokens);
-        a = make_int4(pl.row[l] + first * p.group, (index - first) * p.group, here * p.group, pl.unit[l] + tile * nb * twice);
+        a = make_int4(pl.row[l] + first * p.group, (index - first) * p.group, here * p.group, pl.unit[l] + tile * as_tile_units(p, p.tile_tokens, nb) + p.tile_start);
         a_last = (nb - 1) * (here > p.lane_tokens ? 2 : 1);
       }
       const int tile = i / p.tile_tokens, first = tile * p.tile_tokens, here = min(q - first, p.tile_tokens), e = p.S + s;
       const int nb = as_blocks(prefix, min(me.z, me.z - q + first + here));      // blocks that the tile's last token sees
       const int4 b = make_int4(pl.row[e] + first * p.group, (i - first) * p.group, here * p.group,
-                               pl.unit[e] + tile * as_blocks(prefix, me.z) * twice);
+                               pl.unit[e] + tile * as_tile_units(p, p.tile_tokens, as_blocks(prefix, me.z)) + p.tile_start);
       const int b_last = nb > 0 ? (nb - 1) * (here > p.lane_tokens ? 2 : 1) : -1;
       int4* dst = reinterpret_cast<int4*>(p.rec + (size_t)(t0 + i) * AS_REC);
       dst[0] = a; dst[1] = b; dst[2] = as_sound(p, pl) ? make_int4(a_last, b_last, 0, 0) : make_int4(-1, -1, 0, 0);
@@ -255,12 +267,12 @@ __device__ __forceinline__ Segment as_next(const SharedParams& p, const SharedPl
   g.tokens = min(tokens - g.first, p.tile_tokens);
   const int two = g.tokens > p.lane_tokens ? 1 : 0;              // units of a block: 1 << two
   g.key_hi = g.shared ? hi : min(hi, hi - tokens + g.first + g.tokens);
-  const int base = w.kv_head * pl.units + e.x + w.tile * as_tile_units(p, nb);
+  const int base = w.kv_head * pl.units + e.x + w.tile * as_tile_units(p, p.tile_tokens, nb) + p.tile_start;
   const int there = as_blocks(g.key_lo, g.key_hi);               // a portion's earlier tiles see fewer blocks than its last
   // a block belongs to the CTA in whose piece it begins
   const int tile_end = base + (nb << two), end = min(w.x_end, tile_end);
-  g.block = (w.x - base + two) >> two;
-  g.blocks = max(min((end - base + two) >> two, there) - g.block, 0);
+  g.block = max(w.x - base + two, 0) >> two;
+  g.blocks = max(min(max(end - base + two, 0) >> two, there) - g.block, 0);
   g.row = (long long)w.kv_head * pl.rows + pl.row[e.y] + g.first * p.group + (long long)cta * p.tile_tokens * p.group;
   w.x = end;
   if (end == tile_end) {
@@ -274,10 +286,9 @@ __device__ __forceinline__ Segment as_next(const SharedParams& p, const SharedPl
   return g;
 }
 
-// The i-th token of a segment: its place in the step, and the last key it sees.
-__device__ __forceinline__ void as_token(const SharedPlan& pl, const Segment& g, int i, int& token, int& position) {
-  int s = g.request, at = g.first + i;
-  if (g.shared) {                        // the member whose tokens these are: the last one whose first token is not behind
+// A token's place in the step, and the last key it sees: the `at`-th token of the group that row s leads, or of request s.
+__device__ __forceinline__ void as_token(const SharedPlan& pl, bool shared, int s, int at, int& token, int& position) {
+  if (shared) {                          // the member whose token it is: the last one whose first token is not behind
     int a = pl.first_member[s], b = pl.first_member[s + 1] - 1;
     while (a < b) {
       const int mid = (a + b + 1) >> 1;
@@ -297,16 +308,19 @@ __device__ __forceinline__ void as_store4(bf16* dst, float a, float b, float c, 
   *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
 }
 
-// out[t, h] = sum 2^(m - M) o / sum 2^(m - M) l over the partial results of a row, in the order of the line.  A block has one token and kv
-// head; a thread one head of the group (neighbouring threads neighbouring heads: rows that lie side by side) and four dimensions.  The
-// partial results are read eight at a time, all at once; one with m = -inf weighs nothing.
+// out[t, h] = sum 2^(m - M) o / sum 2^(m - M) l over the partial results of a row.  A block has one token and kv head; a thread one head
+// of the group (neighbouring threads neighbouring heads: rows that lie side by side), four dimensions, and every PARTS-th partial
+// result, eight of which are read at once; the threads' sums are added up in shared memory, in a fixed order.  A partial result with
+// m = -inf weighs nothing, and its o is not looked at.
 constexpr int AS_COMBINE_THREADS = 128;
-template <typename T>
-__global__ void __launch_bounds__(AS_COMBINE_THREADS) as_combine_kernel(SharedParams p) {
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(AS_COMBINE_THREADS * PARTS) as_combine_kernel(SharedParams p) {
+  __shared__ float4 sums[PARTS][128];
+  __shared__ float2 weights[PARTS][128];
   pdl_trigger();
   const int* rec = p.rec;
   const int* head = p.head;
-  const int t = blockIdx.x, kv = blockIdx.y;
+  const int t = blockIdx.x, kv = blockIdx.y, part = threadIdx.x >> 7, lane = threadIdx.x & 127;
   pdl_wait(rec, head);
   const int4* r = reinterpret_cast<const int4*>(rec + (size_t)t * AS_REC);
   const int4 a = __ldcg(r), b = __ldcg(r + 1), last = __ldcg(r + 2);
@@ -314,25 +328,38 @@ __global__ void __launch_bounds__(AS_COMBINE_THREADS) as_combine_kernel(SharedPa
   if (t < hd.w || t >= __ldcg(head + 4)) return;               // rows of no request stay as they were
   const unsigned line = (unsigned)kv * (unsigned)hd.x, span = (unsigned)hd.y;
   const long long step = (long long)p.tile_tokens * p.group;
+  const int fb = as_folds(p, b.z);
   const int ca = (int)((line + a.w) / span), cb = (int)((line + b.w) / span);
-  const int na = last.x < 0 ? 0 : (int)((line + a.w + last.x) / span) - ca + 1, total = na + (last.y < 0 ? 0 : (int)((line + b.w + last.y) / span) - cb + 1);
-  const long long row_a = (long long)kv * hd.z + a.x + ca * step, row_b = (long long)kv * hd.z + b.x + cb * step;
+  const int na = last.x < 0 ? 0 : (int)((line + a.w + last.x) / span) - ca + 1;
+  const int total = na + (last.y < 0 ? 0 : ((int)((line + b.w + last.y) / span) - cb + 1) * fb);
   const int chunks = p.dim / 4;
-  for (int i = threadIdx.x; i < p.group * chunks; i += AS_COMBINE_THREADS) {
-    const int h = i % p.group, c = i / p.group;
+  for (int i0 = 0; i0 < p.group * chunks; i0 += 128) {
+    const int i = i0 + lane, h = i % p.group, c = i / p.group;
+    const bool on = i < p.group * chunks;
+    // this thread's first partial result among the prefix's and among its own keys'
+    const long long tile_a = (long long)kv * hd.z + a.x + ca * step, tile_b = (long long)kv * hd.z + b.x + cb * step;
+    const float2* ml_a = reinterpret_cast<const float2*>(p.part_ml) + tile_a + a.y + h;
+    const float2* ml_b = reinterpret_cast<const float2*>(p.part_ml) + tile_b + b.y + h;
+    const float4* o_a = reinterpret_cast<const float4*>(p.part_o + tile_a * p.dim) + c * a.z + a.y + h;
+    const float4* o_b = reinterpret_cast<const float4*>(p.part_o + tile_b * p.dim) + c * b.z * fb + b.y + h;
     float M = -INFINITY, L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int z0 = 0; z0 < total; z0 += 8) {
+    for (int z0 = part; on && z0 < total; z0 += 8 * PARTS) {
       float2 ml[8];
       float4 o[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const int z = z0 + u;
-        const bool of_a = z < na;
-        const long long tile = of_a ? row_a + z * step : row_b + (z - na) * step;
-        const int in = (of_a ? a.y : b.y) + h, rows = of_a ? a.z : b.z;
-        ml[u] = z < total ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + (tile + in) * 2)) : make_float2(-INFINITY, 0.f);
-        o[u] = z < total ? __ldcg(reinterpret_cast<const float4*>(p.part_o + tile * p.dim + ((long long)c * rows + in) * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const int z = z0 + u * PARTS;
+        ml[u] = make_float2(-INFINITY, 0.f);
+        o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (z < na) {
+          ml[u] = __ldcg(ml_a + z * step);
+          o[u] = __ldcg(o_a + z * step * chunks);
+        } else if (z < total) {
+          const int at = z - na, cta = fb == 1 ? at : at >> 2, copy = fb == 1 ? 0 : at & 3;
+          ml[u] = __ldcg(ml_b + cta * step + copy * b.z);
+          o[u] = __ldcg(o_b + cta * step * chunks + copy * b.z);
+        }
       }
       float m = M;
 #pragma unroll
@@ -349,8 +376,30 @@ __global__ void __launch_bounds__(AS_COMBINE_THREADS) as_combine_kernel(SharedPa
         acc.x = fmaf(w, o[u].x, acc.x); acc.y = fmaf(w, o[u].y, acc.y); acc.z = fmaf(w, o[u].z, acc.z); acc.w = fmaf(w, o[u].w, acc.w);
       }
     }
+    if (PARTS > 1) {
+      __syncthreads();                                         // the last heads' sums have been read
+      sums[part][lane] = acc;
+      weights[part][lane] = make_float2(M, L);
+      __syncthreads();
+      if (part != 0) continue;
+      M = -INFINITY;
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q) M = fmaxf(M, weights[q][lane].x);
+      L = 0.f;
+      acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q) {
+        const float2 ml = weights[q][lane];
+        if (ml.x == -INFINITY) continue;
+        const float w = exp2f(ml.x - M);
+        const float4 o = sums[q][lane];
+        L = fmaf(w, ml.y, L);
+        acc.x = fmaf(w, o.x, acc.x); acc.y = fmaf(w, o.y, acc.y); acc.z = fmaf(w, o.z, acc.z); acc.w = fmaf(w, o.w, acc.w);
+      }
+    }
     const float inv = L > 0.f ? 1.f / L : 0.f;
-    as_store4(reinterpret_cast<T*>(p.out) + ((size_t)t * p.heads + (size_t)kv * p.group + h) * p.dim + 4 * c, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    if (on)
+      as_store4(reinterpret_cast<T*>(p.out) + ((size_t)t * p.heads + (size_t)kv * p.group + h) * p.dim + 4 * c, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
   }
 }
 

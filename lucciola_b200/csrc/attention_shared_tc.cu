@@ -16,8 +16,8 @@
 // lets the line be cut evenly.
 //
 // Warps: 0 and 4 copy keys, 2 and 5 values (cp.async, 16 bytes a thread, swizzled for the tensor cores; a warp has half of every block, and
-// three blocks in flight); 1 issues tile A's products and owns the tensor memory, 3 tile B's; 6..9 softmax of A, 10..13 of B.  Each walks the
-// same segments by itself.  Barriers tell one turn from the next only, so each tile has barriers of its own for the stages of the rings, and a
+// three blocks in flight); 1 issues tile A's products and owns the tensor memory, 3 tile B's; 6..9 softmax of A, 10..13 of B.  Each goes through the
+// segments, which warp 0 finds.  Barriers tell one turn from the next only, so each tile has barriers of its own for the stages of the rings, and a
 // copying warp speaks to the tiles that read a block.  All waits are bounded; when one gives up, the CTA records it and every role leaves.
 #include "attention_shared.cuh"
 #include "attention_tcgen05.cuh"
@@ -30,7 +30,7 @@ constexpr int SC_STAGES = 4;
 constexpr int SC_IN_FLIGHT = 2;                                // blocks a copying warp has requested beyond the one it waits for
 constexpr int SC_BARS = 4 * SC_STAGES + 8;                     // barriers of a tile
 constexpr int SC_THREADS = 448, SC_SOFTMAX = 6;                // the first of the softmax warps
-enum : int { SC_ERR_Q = 401, SC_ERR_KV_FULL = 402, SC_ERR_KV_EMPTY = 403, SC_ERR_S_FULL = 404, SC_ERR_P_FULL = 405, SC_ERR_O_FULL = 406, SC_ERR_O_FREE = 407 };
+enum : int { SC_ERR_Q = 401, SC_ERR_KV_FULL = 402, SC_ERR_KV_EMPTY = 403, SC_ERR_S_FULL = 404, SC_ERR_P_FULL = 405, SC_ERR_O_FULL = 406, SC_ERR_O_FREE = 407, SC_ERR_SEGMENT = 408 };
 
 // Shared memory: queries of A and B | ring of keys | ring of values | barriers.  Rows of 128 bytes (64 elements), 128-byte swizzle, the second
 // 64 elements of a head a half further on.
@@ -42,13 +42,16 @@ template <int D> struct ScLayout {
   static constexpr int BYTES = BAR_OFF + 2 * SC_BARS * 8 + 16;     // and the tensor memory's address and two flags
 };
 
-// What a softmax warp keeps of its way and of the segment at hand in shared memory: its registers are for a block's scores and weights (what
-// does not fit goes to local memory, of which little stays on the SM beside 220 KB of shared memory).
-struct ScWarp {
-  Walk way; int singles;
-  int request, key_hi, rows, row;        // row of the block table, end of the segment's keys; rows of its tile, this warp's first among them
-  long long tile;                        // where the tile's partial rows begin
+// A segment as all roles see it.  Warp 0, which copies keys, walks the line one segment ahead of its copies and leaves what it finds in a ring
+// of these; the others read them there.  A slot comes again after SC_SEGMENTS segments: the rings of keys and values hold warp 0 back to a
+// handful in front of whoever is last (a segment has a block at least, and a tile's next segment waits for the one before).
+struct ScSegment {
+  int kv_head, request, first, tokens;
+  int key_lo, key_hi, block, blocks;
+  long long row;
+  int shared, tiles;                     // the tiles that work on it, as bits (0: the line has ended)
 };
+constexpr int SC_SEGMENTS = 32;
 
 // Half of a block of 64 keys (or values) of a kv head from the pages into a stage of the ring, by one warp: a lane copies 16-byte chunk c of the
 // rows rp, rp + RPI, ... of the half.  `stage` is the half's address plus the lane's part of the head and row, xr[u] its swizzled chunk in rows
@@ -73,6 +76,36 @@ __device__ __forceinline__ void sc_copy_half(uint32_t stage, const uint32_t (&xr
   }
 }
 
+__device__ __forceinline__ void sc_tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// A count in shared memory that one thread raises when what it counts has been written, and the others wait for: more than n.
+__device__ __forceinline__ void sc_publish(uint32_t addr, int n) { asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(addr), "r"(n) : "memory"); }
+__device__ __forceinline__ bool sc_wait_count(uint32_t addr, int n, volatile int* abort_flag) {
+  long long t0 = 0;
+  for (unsigned it = 0;; ++it) {
+    int v;
+    asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    if (v > n) return true;
+    if (it == 0) t0 = clock64();
+    __nanosleep(40);
+    if ((it & 63u) == 63u) {
+      if (*abort_flag) return false;
+      if ((unsigned long long)(clock64() - t0) > TA_WAIT_CYCLES) {
+        *abort_flag = SC_ERR_SEGMENT;
+        atomicCAS(&g_attention_tc_error, 0, (int)SC_ERR_SEGMENT);
+        return false;
+      }
+    }
+  }
+}
+
 // The lowest n bits (none below 0, all from 64 on).
 __device__ __forceinline__ unsigned long long sc_low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 
@@ -81,7 +114,8 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   typedef ScLayout<D> L;
   extern __shared__ uint8_t smem_raw[];
   __shared__ SharedPlan plan;
-  __shared__ ScWarp states[SC_THREADS / 32 - SC_SOFTMAX];
+  __shared__ __align__(16) ScSegment ring_of_segments[SC_SEGMENTS];
+  __shared__ int segments_found;
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = ta_smem_u32(smem);
   const uint32_t bars = sbase + L::BAR_OFF;
@@ -112,6 +146,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     }
     *abort_flag = 0;
     *holes = 0;
+    segments_found = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -125,9 +160,18 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   const uint32_t tmem = *tmem_slot;            // columns: tile t's S buffers at t * 128 and t * 128 + 64 (P over their first 32), O at 256 + t * 128
 
   const int G = p.group, per = p.lane_tokens, cta = blockIdx.x;
-  Walk way = as_begin(p, plan, cta);
-  // the tiles that work on a segment, as bits: segments of one tile go to tile A and B in turn
-  auto tiles_of = [&](const Segment& g, int& singles) -> int { return g.tokens > per ? 3 : 1 << (singles++ & 1); };
+  const uint32_t found_addr = ta_smem_u32(&segments_found);
+  // The n-th segment, when it has been found; false at the end of the line (or when a wait gave up).
+  auto segment = [&](int n, ScSegment& g) -> bool {
+    if (!sc_wait_count(found_addr, n, abort_flag)) return false;
+    const int4* at = reinterpret_cast<const int4*>(&ring_of_segments[n % SC_SEGMENTS]);
+    const int4 a = at[0], b = at[1], c = at[2];
+    g.kv_head = a.x; g.request = a.y; g.first = a.z; g.tokens = a.w;
+    g.key_lo = b.x; g.key_hi = b.y; g.block = b.z; g.blocks = b.w;
+    g.row = (long long)(uint32_t)c.x | (long long)c.y << 32;
+    g.shared = c.z; g.tiles = c.w;
+    return g.tiles != 0;
+  };
 
   if (warp != 1 && warp != 3 && warp < SC_SOFTMAX) {
     // ---- copies: warps 0 and 4 the halves of every block of keys, 2 and 5 of values -----------------------------------------------------
@@ -143,7 +187,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     const int ps = p.page_size, shift = p.page_shift, size = min(ps, 32);
     const size_t page_stride = (size_t)p.kv_heads * ps * (D * 2);
     bool ok = true;
-    int n = 0, handed = 0, singles = 0;        // blocks requested, handed over; segments of one tile
+    int n = 0, handed = 0, seen = 0;           // blocks requested, handed over; segments looked at
     uint32_t used = 0, turn0 = 0, turn1 = 0;   // of stage s: the tiles that read its block (bits 2 s, 2 s + 1); of tiles A and B, bit s: the parity of the next wait
     // The block to come: its segment, this half's first key, lane i the id of the half's i-th page (-1: no page, or no key of the segment in it).
     // It is looked up before the one at hand is copied, across the ends of segments.
@@ -151,19 +195,31 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     uint32_t tiles = 0;
     const int* bt = nullptr;
     const uint8_t* head = nullptr;
+    Walk way = as_begin(p, plan, cta);
+    int singles = 0;                           // (of warp 0) segments of one tile so far: they go to tile A and B in turn
     auto look_ahead = [&]() -> bool {
       if (left == 0) {
-        for (;;) {
-          if (way.x >= way.x_end) return false;
-          const Segment g = as_next(p, plan, cta, way);
-          if (g.blocks == 0) continue;
-          tiles = (uint32_t)tiles_of(g, singles);
-          bt = p.table + (size_t)g.request * p.max_pages;
-          head = pool + (size_t)g.kv_head * ps * (D * 2);
-          left = g.blocks; lo = g.key_lo; hi = g.key_hi;
-          kb = (lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS + half * 32;
-          break;
+        if (warp == 0) {
+          Segment g;
+          g.blocks = 0;
+          while (g.blocks == 0 && way.x < way.x_end) g = as_next(p, plan, cta, way);
+          const int bits = g.blocks == 0 ? 0 : g.tokens > per ? 3 : 1 << (singles++ & 1);
+          if (lane == 0) {
+            int4* at = reinterpret_cast<int4*>(&ring_of_segments[seen % SC_SEGMENTS]);
+            at[0] = make_int4(g.kv_head, g.request, g.first, g.tokens);
+            at[1] = make_int4(g.key_lo, g.key_hi, g.block, g.blocks);
+            at[2] = make_int4((int)(uint32_t)g.row, (int)(g.row >> 32), g.shared ? 1 : 0, bits);
+            sc_publish(found_addr, seen + 1);
+          }
+          __syncwarp();
         }
+        ScSegment g;
+        if (!segment(seen++, g)) return false;
+        tiles = (uint32_t)g.tiles;
+        bt = p.table + (size_t)g.request * p.max_pages;
+        head = pool + (size_t)g.kv_head * ps * (D * 2);
+        left = g.blocks; lo = g.key_lo; hi = g.key_hi;
+        kb = (lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS + half * 32;
       } else {
         kb += AS_KEYS;
       }
@@ -226,13 +282,12 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       constexpr uint32_t idesc_qk = ta_idesc(0, AS_KEYS), idesc_pv = ta_idesc(1, D);
       const uint32_t s_col = tmem + (uint32_t)t * 128u, o_col = tmem + 256u + (uint32_t)t * 128u;
       const uint32_t qa = sbase + t * L::Q_TILE;
-      int n0 = 0, mine = 0, segments = 0, singles = 0;       // blocks of all segments so far, this tile's blocks and segments
+      int n0 = 0, mine = 0, segments = 0;      // blocks of all segments so far, this tile's blocks and segments
       uint32_t k_turn = 0, v_turn = 0;         // bit s: the parity of this tile's next wait for stage s
       bool ok = true;
-      while (way.x < way.x_end && ok) {
-        const Segment g = as_next(p, plan, cta, way);
-        if (g.blocks == 0) continue;
-        if (!((tiles_of(g, singles) >> t) & 1)) { n0 += g.blocks; continue; }
+      ScSegment g;
+      for (int seen = 0; ok && segment(seen, g); ++seen) {
+        if (!((g.tiles >> t) & 1)) { n0 += g.blocks; continue; }
         ok = ta_mbar_wait(q_full(t), (uint32_t)(segments & 1), abort_flag, SC_ERR_Q);
         // S(i) = Q K(i)^T into S buffer (mine + i) & 1
         auto issue_qk = [&](int i) -> bool {
@@ -277,62 +332,49 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     const uint32_t tlane = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_addr = tmem + tlane + (uint32_t)t * 128u, o_addr = tmem + tlane + 256u + (uint32_t)t * 128u;
     const uint32_t q_rows = sbase + t * L::Q_TILE + (uint32_t)quarter * 32u * 128u;        // this warp's rows
-    volatile ScWarp* mem = states + (warp - SC_SOFTMAX);
-    if (lane == 0) {
-      mem->way.x = way.x; mem->way.x_end = way.x_end; mem->way.kv_head = way.kv_head; mem->way.at = way.at; mem->way.tile = way.tile;
-      mem->singles = 0;
-    }
-    __syncwarp();
     bool ok = true;
-    // Of the segment at hand: blocks, the first one's first key, the first key and the end of those this row sees (of none, if there is no such
-    // row), and the least end among the warp's rows.
-    int blocks = 0, block_key = 0, lo = 0, hi = 0, hi_all = 0;
-    bool valid = false, warp_valid = false;
+    // Of the segment at hand: which it is, its blocks, the first one's first key, the first key and the end of those this row sees (of none, if
+    // there is no such row), and the least end among the warp's rows.  A request's tile of at most 32 rows is folded: all four warps have all its rows,
+    // and each a quarter of a block's keys (the tensor cores work on 128 rows anyway); each leaves a partial result of its own.
+    int at_segment = -1, blocks = 0, block_key = 0, lo = 0, hi = 0, hi_all = 0;
+    bool valid = false, warp_valid = false, folded = false;
     // The next segment of this tile, if there is one: its queries are requested.
     auto next_segment = [&]() -> bool {
-      Walk at_now;
-      at_now.x = mem->way.x; at_now.x_end = mem->way.x_end; at_now.kv_head = mem->way.kv_head; at_now.at = mem->way.at; at_now.tile = mem->way.tile;
-      int singles = mem->singles;
-      __syncwarp();
-      for (;;) {
-        if (at_now.x >= at_now.x_end) return false;
-        const Segment g = as_next(p, plan, cta, at_now);
-        if (g.blocks == 0) continue;
-        const int tiles = tiles_of(g, singles);
-        if (!((tiles >> t) & 1)) continue;
-        const int first = tiles == 3 ? t * per : 0, lane_rows = min(g.tokens - first, per) * G;
-        valid = r < lane_rows;
-        warp_valid = quarter * 32 < lane_rows;
+      ScSegment g;
+      do {
+        if (!segment(++at_segment, g)) return false;
+      } while (!((g.tiles >> t) & 1));
+      {
+        const int first = g.tiles == 3 ? t * per : 0, lane_rows = min(g.tokens - first, per) * G;
+        folded = !g.shared && g.tokens * G <= AS_FOLD_ROWS;
+        const int row = folded ? lane : r;     // of this tile's
+        valid = row < lane_rows;
+        warp_valid = folded || quarter * 32 < lane_rows;
         blocks = g.blocks;
         lo = g.key_lo;
         block_key = (lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS;
         hi = 0x7fffffff;
         int from = -1;                         // this row's place among all rows of the queries
         if (valid) {
-          const int i = r / G;
+          const int i = row / G;
           int token, position;
-          as_token(plan, g, first + i, token, position);
-          from = token * p.heads + g.kv_head * G + (r - i * G);
+          as_token(plan, g.shared != 0, g.request, g.first + first + i, token, position);
+          from = token * p.heads + g.kv_head * G + (row - i * G);
           hi = min(position + 1, g.key_hi);
         }
         hi_all = __reduce_min_sync(0xffffffffu, hi);
-        if (lane == 0) {
-          mem->way.x = at_now.x; mem->way.kv_head = at_now.kv_head; mem->way.at = at_now.at; mem->way.tile = at_now.tile; mem->singles = singles;
-          mem->request = g.request; mem->key_hi = g.key_hi; mem->rows = g.tokens * G; mem->row = first * G + quarter * 32; mem->tile = g.row;
-        }
-        __syncwarp();
         constexpr int CHUNKS = D / 8, RPI = 32 / CHUNKS;       // whole rows side by side
         const int c = lane % CHUNKS;
 #pragma unroll
         for (int i = 0; i < 32 / RPI; ++i) {
-          const int rr = i * RPI + lane / CHUNKS, at = __shfl_sync(0xffffffffu, from, rr);
-          if (at >= 0)
+          const int rr = i * RPI + lane / CHUNKS, row_at = __shfl_sync(0xffffffffu, from, rr);
+          if (row_at >= 0)
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
                          ::"r"(q_rows + (uint32_t)rr * 128u + (uint32_t)(c >> 3) * TA_HALF_BYTES + (uint32_t)(((c & 7) ^ (rr & 7)) << 4)),
-                           "l"((const uint8_t*)p.q + (size_t)at * (D * 2) + c * 16) : "memory");
+                           "l"((const uint8_t*)p.q + (size_t)row_at * (D * 2) + c * 16) : "memory");
         }
-        return true;
       }
+      return true;
     };
     auto hand_queries = [&]() {
       asm volatile("cp.async.wait_all;" ::: "memory");
@@ -345,8 +387,94 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     if (more) hand_queries();
     while (more) {
       float m_ref = -INFINITY, l_run = 0.f;
+      // O of this tile's rows times f, when P V of block j - 1 is complete
+      auto rescale = [&](int j, float f) -> bool {
+        if (!ta_mbar_wait(pv_done(t, (j - 1) & 1), (uint32_t)(((j - 1) >> 1) & 1), abort_flag, SC_ERR_O_FULL)) return false;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t v[32];
+          ta_tmem_ld32(o_addr + (uint32_t)c, v);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+          ta_tmem_st32(o_addr + (uint32_t)c, v);
+        }
+        ta_tmem_wait_st();
+        return true;
+      };
+      // the block's keys in pages that are not there, of `width` keys from kb on
+      auto absent_keys = [&](int kb, int width) -> unsigned long long {
+        const volatile ScSegment* g = &ring_of_segments[at_segment % SC_SEGMENTS];
+        const int size = min(p.page_size, width), key = kb + lane * size;
+        const bool here = lane * size < width && key < g->key_hi && key + size > lo;
+        const int id = here ? p.table[(size_t)g->request * p.max_pages + (key >> p.page_shift)] : 0;
+        unsigned long long keys = 0;
+        for (uint32_t absent = __ballot_sync(0xffffffffu, id < 0 || id >= p.num_pages); absent; absent &= absent - 1) {
+          const int first = (__ffs(absent) - 1) * size;
+          keys |= sc_low_bits(first + size) & ~sc_low_bits(first);
+        }
+        return keys;
+      };
+      if (folded) {
+        for (int i = 0; i < blocks; ++i, block_key += AS_KEYS) {
+          const int j = mine + i, b = j & 1, kb = block_key + quarter * 16;
+          ok = ta_mbar_wait(s_full(t, b), (uint32_t)((j >> 1) & 1), abort_flag, SC_ERR_S_FULL);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          float xs[16];
+          {
+            uint32_t v[16];
+            sc_tmem_ld16(s_addr + (uint32_t)b * 64u + (uint32_t)quarter * 16u, v);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) xs[e] = __uint_as_float(v[e]);
+          }
+          const bool some = *holes;
+          if (some || kb < lo || kb + 16 > hi_all) {
+            unsigned long long seen = sc_low_bits(hi - kb) & ~sc_low_bits(lo - kb);
+            if (some) seen &= ~absent_keys(kb, 16);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (!(((uint32_t)seen >> e) & 1u)) xs[e] = -INFINITY;
+          }
+          float mx = ta_max3(xs[0], xs[1], xs[2]);
+#pragma unroll
+          for (int e = 3; e < 15; e += 2) mx = ta_max3(mx, xs[e], xs[e + 1]);
+          mx = fmaxf(mx, xs[15]);
+          const float m_loc = mx * p.scale_log2;
+          const bool grow = valid && m_loc > m_ref + TA_RESCALE_STEP;    // also true for the first finite maximum (m_ref = -inf)
+          if (__any_sync(0xffffffffu, grow)) {
+            float f = 1.f;
+            if (grow) {
+              if (m_ref != -INFINITY) f = exp2f(m_ref - m_loc);
+              m_ref = m_loc;
+              l_run *= f;
+            }
+            if (i > 0) ok = rescale(j, f);
+            if (!ok) break;
+          }
+          const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+          uint32_t w[32];                      // the other warps' keys weigh nothing here
+          float sum = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float p0 = exp2_approx(fmaf(xs[2 * e], p.scale_log2, -m_use)), p1 = exp2_approx(fmaf(xs[2 * e + 1], p.scale_log2, -m_use));
+            sum += p0 + p1;
+            __nv_bfloat162 b2 = __floats2bfloat162_rn(p0, p1);
+            const uint32_t pair = *reinterpret_cast<uint32_t*>(&b2);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) w[8 * q + e] = q == quarter ? pair : 0u;
+          }
+          ta_tmem_st32(s_addr + (uint32_t)b * 64u, w);
+          ta_tmem_wait_st();
+          l_run += sum;
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) ta_mbar_arrive(p_full(t, b));
+        }
+        if (!ok) break;
+      }
       bool settled = false;                    // every row has a reference
-      for (int i = 0; i < blocks; ++i, block_key += AS_KEYS) {
+      for (int i = 0; i < blocks && !folded; ++i, block_key += AS_KEYS) {
         const int j = mine + i, b = j & 1, kb = block_key;
         ok = ta_mbar_wait(s_full(t, b), (uint32_t)((j >> 1) & 1), abort_flag, SC_ERR_S_FULL);
         if (!ok) break;
@@ -358,16 +486,10 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         bool masked = kb < lo || kb + AS_KEYS > hi_all;
         unsigned long long seen = sc_low_bits(hi - kb) & ~sc_low_bits(lo - kb);        // which of the block's keys the row sees
-        if (*holes) {                          // there are pages that are not: a look at this block's
-          const int size = min(p.page_size, AS_KEYS), key = kb + lane * size;
-          const bool here = lane * size < AS_KEYS && key < mem->key_hi && key + size > lo;
-          const int id = here ? p.table[(size_t)mem->request * p.max_pages + (key >> p.page_shift)] : 0;
-          uint32_t absent = __ballot_sync(0xffffffffu, id < 0 || id >= p.num_pages);
+        if (*holes) {
+          const unsigned long long absent = absent_keys(kb, AS_KEYS);
           masked |= absent != 0;
-          for (; absent; absent &= absent - 1) {
-            const int first = (__ffs(absent) - 1) * size;
-            seen &= ~(sc_low_bits(first + size) & ~sc_low_bits(first));
-          }
+          seen &= ~absent;
         }
         // Where every row has a reference, its maximum is not looked for: a sum of 64 weights that stays below 2^15 says that no score is
         // far above the reference.  Otherwise the block is done again from the scores, which still lie in tensor memory, with the maximum.
@@ -406,20 +528,8 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
                 m_ref = m_loc;
                 l_run *= f;
               }
-              if (i > 0) {
-                ok = ta_mbar_wait(pv_done(t, b ^ 1), (uint32_t)(((j - 1) >> 1) & 1), abort_flag, SC_ERR_O_FULL);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                  uint32_t v[32];
-                  ta_tmem_ld32(o_addr + (uint32_t)c, v);
-#pragma unroll
-                  for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                  ta_tmem_st32(o_addr + (uint32_t)c, v);
-                }
-                ta_tmem_wait_st();
-              }
+              if (i > 0) ok = rescale(j, f);
+              if (!ok) break;
             }
             settled = !__any_sync(0xffffffffu, valid && m_ref == -INFINITY);
           }
@@ -452,8 +562,10 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       if (!ok) break;
       mine += blocks;
       // All products with this tile's queries are done: the next segment's come while this one's result is awaited and written.
-      const long long tile = mem->tile;
-      const int rows = mem->rows, row = mem->row + lane;
+      const ScSegment* was = &ring_of_segments[at_segment % SC_SEGMENTS];
+      const long long tile = was->row;
+      const int tile_rows = was->tokens * G, rows = folded ? 4 * tile_rows : tile_rows;
+      const int row = folded ? quarter * tile_rows + lane : (was->tiles == 3 ? t * per * G : 0) + r;
       const bool row_valid = valid, some_valid = warp_valid;
       more = next_segment();
       ok = ta_mbar_wait(pv_done(t, (mine - 1) & 1), (uint32_t)(((mine - 1) >> 1) & 1), abort_flag, SC_ERR_O_FULL);
@@ -491,7 +603,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
 template <int D>
 static cudaError_t sc_launch(const SharedParams& p, int ctas, cudaStream_t stream) {
   constexpr int smem = ScLayout<D>::BYTES + 1024;
-  static_assert(smem + sizeof(SharedPlan) + sizeof(ScWarp) * (SC_THREADS / 32 - SC_SOFTMAX) + 64 <= 227 * 1024, "shared memory of a CTA");
+  static_assert(smem + sizeof(SharedPlan) + sizeof(ScSegment) * SC_SEGMENTS + 64 <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<unsigned long long> configured{0ull};     // a bit a device
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);

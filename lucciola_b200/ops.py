@@ -124,7 +124,7 @@ _SIGNATURES = {
                              c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_longlong, c_void_p, c_float, c_int, c_void_p,
                              c_void_p],
     "lb_attention_shared": [c_int] + [c_void_p] * 9 + [c_int] * 8 + [c_float, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p],
-    "lb_attention_shared_workspace": [c_int] * 6 + [c_void_p, c_void_p],
+    "lb_attention_shared_workspace": [c_int] * 7 + [c_void_p, c_void_p],
     "lb_latent_flash": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                         c_float, c_void_p, c_int, c_int, c_void_p, c_longlong, c_void_p],
     "lb_latent_gather": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
@@ -1520,7 +1520,7 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     if T == 0 or S == 0:
         return
     dt = dtype_code(q.dtype)
-    n_floats, n_ints = _shared_workspace(q.device.index, T, num_q_heads, num_kv_heads, head_dim, dt, page_size)
+    n_floats, n_ints = _shared_workspace(q.device.index, T, S, num_q_heads, num_kv_heads, head_dim, dt, page_size)
     floats = torch.empty(n_floats, dtype=torch.float32, device=q.device)
     ints = torch.empty(n_ints, dtype=torch.int32, device=q.device)
     if stream != torch.cuda.current_stream(q.device).cuda_stream:

@@ -174,11 +174,10 @@ static int as_sms() {
 }
 
 // How a launch cuts its rows: kv heads that share a cached one, heads of a tile, tokens of a tile and of a part of one.
-struct SharedCut { bool tc; int share, group, tile_tokens, lane_tokens, folds; };
+struct SharedCut { bool tc; int share, group, tile_tokens, lane_tokens; };
 static SharedCut as_cut(int dtype, int group, int head_dim, int page_size) {
-  SharedCut c{attention_shared_tc_takes(dtype, group, head_dim, page_size), 1, group, 0, 0, 1};
+  SharedCut c{attention_shared_tc_takes(dtype, group, head_dim, page_size), 1, group, 0, 0};
   if (c.tc) {
-    c.folds = 4;
     attention_shared_tc_cut(group, c.tile_tokens, c.lane_tokens);
     return c;
   }
@@ -219,7 +218,7 @@ LB_EXPORT int lb_attention_shared_workspace(int num_tokens, int num_seqs, int nu
   const int ctas = lb::as_sms();
   LB_CHECK_ARG(ctas > 0, "attention_shared: no device");
   const lb::SharedCut cut = lb::as_cut(dtype, num_q_heads / num_kv_heads, head_dim, page_size);
-  const long long rows = lb::as_most_rows(num_tokens, num_seqs, cut.group, cut.folds) * num_kv_heads * cut.share + (long long)ctas * cut.tile_tokens * cut.group;
+  const long long rows = lb::as_most_rows(num_tokens, num_seqs, cut.group, cut.tc) * num_kv_heads * cut.share + (long long)ctas * cut.tile_tokens * cut.group;
   *floats = rows * (head_dim + 2);
   *ints = (long long)num_tokens * lb::AS_REC + 8;
   return 0;
@@ -255,7 +254,7 @@ LB_EXPORT int lb_attention_shared(int dtype, const void* q, void* out, const voi
   p.cu = cu_tokens; p.ctx = context_lens; p.prefix_of = prefix_of; p.prefix_lens = prefix_lens;
   p.T = num_tokens; p.S = num_seqs; p.heads = num_q_heads; p.kv_heads = num_kv_heads * cut.share; p.group = cut.group; p.dim = head_dim;
   p.page_size = page_size; p.page_shift = -1; p.kv_share = cut.share; p.tile_tokens = cut.tile_tokens; p.lane_tokens = cut.lane_tokens;
-  p.min_span = cut.tc ? 4 : 1; p.tile_start = cut.tc ? 2 : 0; p.folds = cut.folds;
+  p.min_span = cut.tc ? 4 : 1; p.tile_start = cut.tc ? 2 : 0; p.folds = cut.tc;
   for (int b = 0; b < 31; ++b) if ((1 << b) == page_size) p.page_shift = b;
   p.scale_log2 = scale * 1.4426950408889634f;
   // units of the whole line, at most

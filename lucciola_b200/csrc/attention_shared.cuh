@@ -32,7 +32,7 @@ struct SharedParams {
   int tile_tokens, lane_tokens;          // tokens of a tile; a tile of more than lane_tokens counts twice
   int min_span;                          // least units a CTA takes
   int tile_start;                        // units that a tile costs beside its blocks
-  int folds;                             // a request's tile of at most AS_FOLD_ROWS rows leaves this many partial results, one behind the other
+  bool folds;                            // whether tiles of few rows leave several partial results (as_folds), one behind the other
   float scale_log2;
   // Partial results: 4 consecutive dimensions of all rows of a tile, then the next 4 ([dim / 4][rows][4], so that threads with a row each
   // write, and threads with a head each read, side by side), and [rows][2]: the reference value (-inf: no key) and the sum.
@@ -73,11 +73,15 @@ __device__ __forceinline__ int as_units(const SharedParams& p, int tokens, int b
   const int full = (tokens - 1) / p.tile_tokens;
   return full * as_tile_units(p, p.tile_tokens, blocks) + as_tile_units(p, tokens - full * p.tile_tokens, blocks);
 }
-__device__ __forceinline__ int as_folds(const SharedParams& p, int rows) { return rows <= AS_FOLD_ROWS ? p.folds : 1; }
-__device__ __forceinline__ int as_rows(const SharedParams& p, int tokens) {        // of a request
+// Partial results that each CTA leaves of a tile with this many rows: two of one that both halves of the tensor memory work on, a half of
+// the blocks each; four of a request's few rows, a quarter of every block's keys each.
+__host__ __device__ __forceinline__ int as_folds(const SharedParams& p, bool shared, int rows) {
+  return !p.folds || rows > p.lane_tokens * p.group ? 1 : !shared && rows <= AS_FOLD_ROWS ? 4 : 2;
+}
+__device__ __forceinline__ int as_rows(const SharedParams& p, bool shared, int tokens) {
   if (tokens <= 0) return 0;
   const int last = tokens <= p.tile_tokens ? tokens : tokens - (tokens - 1) / p.tile_tokens * p.tile_tokens;
-  return (tokens - last) * p.group + last * p.group * as_folds(p, last * p.group);
+  return (tokens - last) * p.group + last * p.group * as_folds(p, shared, last * p.group);
 }
 
 // An exclusive sum over `n` numbers by one warp, in place; returns the whole.  A lane has a run of them.
@@ -145,7 +149,7 @@ __device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& 
       pl.first_member[s] = led;
       const int ua = leads ? as_units(p, led_tokens, as_blocks(0, me.w)) : 0, ub = as_units(p, me.y, as_blocks(shares ? prefix : 0, me.z));
       pl.unit[s] = ua; pl.unit[n + s] = ub;
-      pl.row[s] = leads ? led_tokens * p.group : 0; pl.row[n + s] = as_rows(p, me.y);
+      pl.row[s] = leads ? as_rows(p, true, led_tokens) : 0; pl.row[n + s] = as_rows(p, false, me.y);
       pl.place[s] = ua > 0 ? 1 : 0; pl.place[n + s] = ub > 0 ? 1 : 0;
     }
   }
@@ -190,9 +194,9 @@ __device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& 
 }
 
 // cu_tokens that fall would make more rows than there is room for: nothing is done then.
-__host__ __device__ __forceinline__ long long as_most_rows(long long tokens, long long seqs, int group, int folds) {
-  const long long rows = tokens * group, folded = seqs * AS_FOLD_ROWS;      // a request's last tile may be folded
-  return 2 * rows + (folds - 1) * (folded < rows ? folded : rows);
+__host__ __device__ __forceinline__ long long as_most_rows(long long tokens, long long seqs, int group, bool folds) {
+  const long long rows = tokens * group, more = 256 * seqs;    // an entry's last tile may be folded
+  return 2 * rows + (!folds ? 0 : more < 4 * rows ? more : 4 * rows);
 }
 __device__ __forceinline__ bool as_sound(const SharedParams& p, const SharedPlan& pl) { return pl.rows <= as_most_rows(p.T, p.S, p.group, p.folds); }
 
@@ -328,10 +332,10 @@ __global__ void __launch_bounds__(AS_COMBINE_THREADS * PARTS) as_combine_kernel(
   if (t < hd.w || t >= __ldcg(head + 4)) return;               // rows of no request stay as they were
   const unsigned line = (unsigned)kv * (unsigned)hd.x, span = (unsigned)hd.y;
   const long long step = (long long)p.tile_tokens * p.group;
-  const int fb = as_folds(p, b.z);
+  const int fa = as_folds(p, true, a.z) - 1, fb = as_folds(p, false, b.z) - 1;       // 0, 1 or 3
   const int ca = (int)((line + a.w) / span), cb = (int)((line + b.w) / span);
-  const int na = last.x < 0 ? 0 : (int)((line + a.w + last.x) / span) - ca + 1;
-  const int total = na + (last.y < 0 ? 0 : ((int)((line + b.w + last.y) / span) - cb + 1) * fb);
+  const int na = last.x < 0 ? 0 : ((int)((line + a.w + last.x) / span) - ca + 1) * (fa + 1);
+  const int total = na + (last.y < 0 ? 0 : ((int)((line + b.w + last.y) / span) - cb + 1) * (fb + 1));
   const int chunks = p.dim / 4;
   for (int i0 = 0; i0 < p.group * chunks; i0 += 128) {
     const int i = i0 + lane, h = i % p.group, c = i / p.group;
@@ -340,8 +344,8 @@ __global__ void __launch_bounds__(AS_COMBINE_THREADS * PARTS) as_combine_kernel(
     const long long tile_a = (long long)kv * hd.z + a.x + ca * step, tile_b = (long long)kv * hd.z + b.x + cb * step;
     const float2* ml_a = reinterpret_cast<const float2*>(p.part_ml) + tile_a + a.y + h;
     const float2* ml_b = reinterpret_cast<const float2*>(p.part_ml) + tile_b + b.y + h;
-    const float4* o_a = reinterpret_cast<const float4*>(p.part_o + tile_a * p.dim) + c * a.z + a.y + h;
-    const float4* o_b = reinterpret_cast<const float4*>(p.part_o + tile_b * p.dim) + c * b.z * fb + b.y + h;
+    const float4* o_a = reinterpret_cast<const float4*>(p.part_o + tile_a * p.dim) + c * a.z * (fa + 1) + a.y + h;
+    const float4* o_b = reinterpret_cast<const float4*>(p.part_o + tile_b * p.dim) + c * b.z * (fb + 1) + b.y + h;
     float M = -INFINITY, L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int z0 = part; on && z0 < total; z0 += 8 * PARTS) {
@@ -352,13 +356,12 @@ __global__ void __launch_bounds__(AS_COMBINE_THREADS * PARTS) as_combine_kernel(
         const int z = z0 + u * PARTS;
         ml[u] = make_float2(-INFINITY, 0.f);
         o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (z < na) {
-          ml[u] = __ldcg(ml_a + z * step);
-          o[u] = __ldcg(o_a + z * step * chunks);
-        } else if (z < total) {
-          const int at = z - na, cta = fb == 1 ? at : at >> 2, copy = fb == 1 ? 0 : at & 3;
-          ml[u] = __ldcg(ml_b + cta * step + copy * b.z);
-          o[u] = __ldcg(o_b + cta * step * chunks + copy * b.z);
+        if (z < total) {
+          const bool of_a = z < na;
+          const int at = of_a ? z : z - na, f = of_a ? fa : fb, copy = (at & f) * (of_a ? a.z : b.z);
+          const long long cta = (at >> (f - (f >> 1))) * step;         // shifted by 0, 1 or 2
+          ml[u] = __ldcg((of_a ? ml_a : ml_b) + cta + copy);
+          o[u] = __ldcg((of_a ? o_a : o_b) + cta * chunks + copy);
         }
       }
       float m = M;

@@ -1,10 +1,9 @@
 // Attention of a step whose requests share prefixes, on the 5th-generation tensor cores (bfloat16, heads of 64 or 128, up to 128 query
 // heads a kv head, pages of 8 tokens and more that are powers of two).  The plan, the walk and the combination are attention_shared.cuh's.
 //
-// One CTA an SM walks its piece of the line of key blocks, segment after segment.  A segment has up to 256 query rows: two tiles, A and
-// B, of up to 128 rows each, on which two sets of warps and two halves of tensor memory work.  The rows of a group's members against its
-// prefix fill both; a segment of one tile (a request's own keys: a handful of rows) goes to A and B in turn, so that the start and the end
-// of one segment pass while the other's products run, and the copies of keys and values run on through all of them.
+// One CTA an SM walks its piece of the line of key blocks, segment after segment.  There are two tiles, A and B, of up to 128 query rows each,
+// on which two sets of warps and two halves of tensor memory work: on a segment with more rows both on every block, else on halves of a
+// segment's blocks, or on two requests' own keys (a handful of rows each) side by side.  Copies of keys and values run on through all segments.
 //     S = Q K^T      tcgen05.mma, operands from shared memory, two S buffers a tile
 //     P              one thread a query row, online softmax in 32 bits, P (bfloat16) written over S in tensor memory
 //     O += P V       tcgen05.mma, P from tensor memory, V as it lies in the pages; O stays in tensor memory
@@ -42,39 +41,20 @@ template <int D> struct ScLayout {
   static constexpr int BYTES = BAR_OFF + 2 * SC_BARS * 8 + 16;     // and the tensor memory's address and two flags
 };
 
-// A segment as all roles see it.  Warp 0, which copies keys, walks the line one segment ahead of its copies and leaves what it finds in a ring
-// of these; the others read them there.  A slot comes again after SC_SEGMENTS segments: the rings of keys and values hold warp 0 back to a
-// handful in front of whoever is last (a segment has a block at least, and a tile's next segment waits for the one before).
-struct ScSegment {
-  int kv_head, request, first, tokens;
-  int key_lo, key_hi, block, blocks;
-  long long row;
-  int shared, tiles;                     // the tiles that work on it, as bits (0: the line has ended)
+// What the two tiles work on side by side, a part each: halves of one segment's blocks, segments of two requests, or (both) the same blocks
+// with other rows.  The parts' blocks alternate in the rings of keys and values, so that neither tile waits for the other's to pass.
+// Warp 0, which copies keys, walks the line one step ahead of its copies and leaves what it finds in a ring of steps; the others read them there.
+// A slot comes again after SC_SEGMENTS steps: the rings of keys and values hold warp 0 back to a handful in front of whoever is last (a step
+// has a block at least, and a tile's next step waits for the one before).
+struct ScPart {
+  int kv_head, request, first, tokens;   // tokens 0: nothing for this tile
+  int key_lo, key_hi, block, blocks;     // blocks 0 of a part with tokens: it leaves an empty partial result
+  int row_low, row_high;                 // where the tile's partial rows begin
+  int shared, kind;
 };
+struct ScStep { ScPart part[2]; };
+enum : int { SC_END = 0, SC_PARTS = 1, SC_BOTH = 2, SC_HALVES = 3 };       // kind, of either part
 constexpr int SC_SEGMENTS = 32;
-
-// Half of a block of 64 keys (or values) of a kv head from the pages into a stage of the ring, by one warp: a lane copies 16-byte chunk c of the
-// rows rp, rp + RPI, ... of the half.  `stage` is the half's address plus the lane's part of the head and row, xr[u] its swizzled chunk in rows
-// rp + RPI u; `head` points at the lane's chunk and row of the head in page 0; lane i holds the id of the half's i-th page (-1: no page; pages of more
-// than 32 tokens: `sub` is where in the page the half begins).  Keys outside lo .. hi - 1 and of no page are filled with zeros.
-template <int PS, int D>
-__device__ __forceinline__ void sc_copy_half(uint32_t stage, const uint32_t (&xr)[4], const uint8_t* head, int ids, int kb, int lo, int hi,
-                                             size_t page_stride, int rp, int sub) {
-  constexpr int RPI = 32 / (D / 8), ROW = D * 2;
-  const bool inner = kb >= lo && kb + 32 <= hi;                // every key may be seen
-#pragma unroll
-  for (int pg = 0; pg < 32 / PS; ++pg) {
-    const int id = __shfl_sync(0xffffffffu, ids, pg);
-    const uint8_t* src = head + (size_t)max(id, 0) * page_stride + sub * ROW;
-#pragma unroll
-    for (int j = 0; j < PS / RPI; ++j) {
-      const int key = kb + pg * PS + rp + RPI * j;
-      const uint32_t bytes = (id >= 0 && (inner || (key >= lo && key < hi))) ? 16u : 0u;       // 0: sixteen zeros
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                   ::"r"(stage + xr[j & (8 / RPI - 1)] + (uint32_t)((pg * PS + RPI * j) * 128)), "l"(src + j * RPI * ROW), "r"(bytes) : "memory");
-    }
-  }
-}
 
 __device__ __forceinline__ void sc_tmem_ld16(uint32_t taddr, uint32_t* r) {
   asm volatile(
@@ -85,24 +65,33 @@ __device__ __forceinline__ void sc_tmem_ld16(uint32_t taddr, uint32_t* r) {
       : "memory");
 }
 
+// Waits, bounded like those of attention_tcgen05.cuh, in as few instructions as can be: the roles of this kernel are many, and what they
+// execute has to stay in the SM's instruction cache (with 138 KB of code most of the time went into fetching it).  What gave up is left in
+// shared memory, and reported at the kernel's end.
+constexpr unsigned SC_WAIT_CYCLES = 2000000000u;
+template <bool SLEEP>
+__device__ __forceinline__ bool sc_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
+  const unsigned t0 = (unsigned)clock();
+#pragma unroll 1
+  while (!ta_mbar_try_wait(bar, parity)) {
+    if (SLEEP) __nanosleep(40);
+    if (*abort_flag) return false;
+    if ((unsigned)clock() - t0 > SC_WAIT_CYCLES) { *abort_flag = code; return false; }
+  }
+  return true;
+}
 // A count in shared memory that one thread raises when what it counts has been written, and the others wait for: more than n.
 __device__ __forceinline__ void sc_publish(uint32_t addr, int n) { asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(addr), "r"(n) : "memory"); }
 __device__ __forceinline__ bool sc_wait_count(uint32_t addr, int n, volatile int* abort_flag) {
-  long long t0 = 0;
-  for (unsigned it = 0;; ++it) {
+  const unsigned t0 = (unsigned)clock();
+#pragma unroll 1
+  for (;;) {
     int v;
     asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     if (v > n) return true;
-    if (it == 0) t0 = clock64();
     __nanosleep(40);
-    if ((it & 63u) == 63u) {
-      if (*abort_flag) return false;
-      if ((unsigned long long)(clock64() - t0) > TA_WAIT_CYCLES) {
-        *abort_flag = SC_ERR_SEGMENT;
-        atomicCAS(&g_attention_tc_error, 0, (int)SC_ERR_SEGMENT);
-        return false;
-      }
-    }
+    if (*abort_flag) return false;
+    if ((unsigned)clock() - t0 > SC_WAIT_CYCLES) { *abort_flag = SC_ERR_SEGMENT; return false; }
   }
 }
 
@@ -114,8 +103,8 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   typedef ScLayout<D> L;
   extern __shared__ uint8_t smem_raw[];
   __shared__ SharedPlan plan;
-  __shared__ __align__(16) ScSegment ring_of_segments[SC_SEGMENTS];
-  __shared__ int segments_found;
+  __shared__ __align__(16) ScStep steps[SC_SEGMENTS];
+  __shared__ int steps_found;
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = ta_smem_u32(smem);
   const uint32_t bars = sbase + L::BAR_OFF;
@@ -146,7 +135,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     }
     *abort_flag = 0;
     *holes = 0;
-    segments_found = 0;
+    steps_found = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -160,120 +149,176 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   const uint32_t tmem = *tmem_slot;            // columns: tile t's S buffers at t * 128 and t * 128 + 64 (P over their first 32), O at 256 + t * 128
 
   const int G = p.group, per = p.lane_tokens, cta = blockIdx.x;
-  const uint32_t found_addr = ta_smem_u32(&segments_found);
-  // The n-th segment, when it has been found; false at the end of the line (or when a wait gave up).
-  auto segment = [&](int n, ScSegment& g) -> bool {
+  const uint32_t found_addr = ta_smem_u32(&steps_found);
+  // Tile t's part of the n-th step, when it has been found; false at the end of the line (or when a wait gave up).
+  auto step = [&](int n, int t, ScPart& g) -> bool {
     if (!sc_wait_count(found_addr, n, abort_flag)) return false;
-    const int4* at = reinterpret_cast<const int4*>(&ring_of_segments[n % SC_SEGMENTS]);
+    const int4* at = reinterpret_cast<const int4*>(&steps[n % SC_SEGMENTS].part[t]);
     const int4 a = at[0], b = at[1], c = at[2];
     g.kv_head = a.x; g.request = a.y; g.first = a.z; g.tokens = a.w;
     g.key_lo = b.x; g.key_hi = b.y; g.block = b.z; g.blocks = b.w;
-    g.row = (long long)(uint32_t)c.x | (long long)c.y << 32;
-    g.shared = c.z; g.tiles = c.w;
-    return g.tiles != 0;
+    g.row_low = c.x; g.row_high = c.y; g.shared = c.z; g.kind = c.w;
+    return g.kind != SC_END;
   };
+  // Where block i of tile t's part lies among the step's: A's and B's in turn, then what the longer part has more.
+  auto place = [](int t, int i, int others, int kind) { return kind == SC_BOTH ? i : i + min(t ? i + 1 : i, others); };
 
   if (warp != 1 && warp != 3 && warp < SC_SOFTMAX) {
     // ---- copies: warps 0 and 4 the halves of every block of keys, 2 and 5 of values -----------------------------------------------------
     const bool is_v = warp == 2 || warp == 5;
     const int half = warp >= 4 ? 1 : 0;
     constexpr int CHUNKS = D / 8, RPI = 32 / CHUNKS;           // 16-byte chunks of a row, rows an instruction
-    const int c = lane % CHUNKS, rp = lane / CHUNKS;
-    const uint8_t* pool = (const uint8_t*)(is_v ? p.v_cache : p.k_cache) + c * 16 + rp * (D * 2);
-    const uint32_t ring = sbase + (is_v ? L::V_OFF : L::K_OFF) + (uint32_t)(c >> 3) * L::KV_HALF + (uint32_t)(half * 32 + rp) * 128u;
-    uint32_t xr[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) xr[u] = (uint32_t)(((c & 7) ^ ((rp + RPI * u) & 7)) << 4);
-    const int ps = p.page_size, shift = p.page_shift, size = min(ps, 32);
+    const int c = lane % CHUNKS, rp = lane / CHUNKS;           // a lane copies chunk c of the rows rp, rp + RPI, ... of its half
+    const uint8_t* pool = (const uint8_t*)(is_v ? p.v_cache : p.k_cache) + c * 16;
+    const uint32_t ring = sbase + (is_v ? L::V_OFF : L::K_OFF) + (uint32_t)(c >> 3) * L::KV_HALF + (uint32_t)(half * 32) * 128u;
+    const uint32_t full0 = is_v ? v_full(0, 0) : k_full(0, 0), empty0 = is_v ? v_empty(0, 0) : k_empty(0, 0);
+    const int ps = p.page_size, shift = p.page_shift, size = min(ps, 32), bits = min(shift, 5);
     const size_t page_stride = (size_t)p.kv_heads * ps * (D * 2);
-    bool ok = true;
-    int n = 0, handed = 0, seen = 0;           // blocks requested, handed over; segments looked at
-    uint32_t used = 0, turn0 = 0, turn1 = 0;   // of stage s: the tiles that read its block (bits 2 s, 2 s + 1); of tiles A and B, bit s: the parity of the next wait
-    // The block to come: its segment, this half's first key, lane i the id of the half's i-th page (-1: no page, or no key of the segment in it).
-    // It is looked up before the one at hand is copied, across the ends of segments.
-    int left = 0, kb = 0, lo = 0, hi = 0, ids = -1;
-    uint32_t tiles = 0;
-    const int* bt = nullptr;
-    const uint8_t* head = nullptr;
+    int n = 0, handed = 0, seen = 0;           // blocks requested, handed over; steps looked at
+    uint32_t used = 0, turns = 0;              // bits 2 s + t: whether tile t reads stage s's block, and the parity of the next wait for it
+    // (Of warp 0) the way along the line, and a segment that has been found but is no part of a step yet.
     Walk way = as_begin(p, plan, cta);
-    int singles = 0;                           // (of warp 0) segments of one tile so far: they go to tile A and B in turn
-    auto look_ahead = [&]() -> bool {
-      if (left == 0) {
-        if (warp == 0) {
-          Segment g;
-          g.blocks = 0;
-          while (g.blocks == 0 && way.x < way.x_end) g = as_next(p, plan, cta, way);
-          const int bits = g.blocks == 0 ? 0 : g.tokens > per ? 3 : 1 << (singles++ & 1);
-          if (lane == 0) {
-            int4* at = reinterpret_cast<int4*>(&ring_of_segments[seen % SC_SEGMENTS]);
-            at[0] = make_int4(g.kv_head, g.request, g.first, g.tokens);
-            at[1] = make_int4(g.key_lo, g.key_hi, g.block, g.blocks);
-            at[2] = make_int4((int)(uint32_t)g.row, (int)(g.row >> 32), g.shared ? 1 : 0, bits);
-            sc_publish(found_addr, seen + 1);
-          }
-          __syncwarp();
+    Segment found;
+    found.blocks = 0;
+    auto find_step = [&]() {
+      int kind = SC_END;
+      // At most two segments: the second one if it is a request's few rows, as the first.
+#pragma unroll 1
+      for (int t = 0; t < 2; ++t) {
+        if (t == 0 || kind == SC_PARTS) {
+#pragma unroll 1
+          while (found.blocks == 0 && way.x < way.x_end) found = as_next(p, plan, cta, way);
         }
-        ScSegment g;
-        if (!segment(seen++, g)) return false;
-        tiles = (uint32_t)g.tiles;
-        bt = p.table + (size_t)g.request * p.max_pages;
-        head = pool + (size_t)g.kv_head * ps * (D * 2);
-        left = g.blocks; lo = g.key_lo; hi = g.key_hi;
-        kb = (lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS + half * 32;
-      } else {
-        kb += AS_KEYS;
+        const Segment& g = found;
+        const bool few = !g.shared && g.tokens * G <= AS_FOLD_ROWS;
+        int block = g.block, blocks = g.blocks, tokens = g.tokens;
+        bool keep = false;                     // for tile B, or for the step after this one
+        if (t == 0) {
+          kind = blocks == 0 ? SC_END : g.tokens > per ? SC_BOTH : few ? SC_PARTS : SC_HALVES;
+          if (kind == SC_HALVES) blocks = (blocks + 1) >> 1;
+          keep = kind >= SC_BOTH;
+        } else if (kind == SC_HALVES) {
+          block += (blocks + 1) >> 1;
+          blocks >>= 1;
+        } else if (kind == SC_PARTS && !(blocks > 0 && few)) {
+          keep = true;
+          blocks = tokens = 0;
+        }
+        if (lane == 0) {
+          int4* at = reinterpret_cast<int4*>(&steps[seen % SC_SEGMENTS].part[t]);
+          at[0] = make_int4(g.kv_head, g.request, g.first, tokens);
+          at[1] = make_int4(g.key_lo, g.key_hi, block, blocks);
+          at[2] = make_int4((int)(uint32_t)g.row, (int)(g.row >> 32), g.shared ? 1 : 0, kind);
+        }
+        if (!keep) found.blocks = 0;
       }
-      --left;
-      const int key = kb + lane * size;
-      ids = -1;
-      if (lane * size < 32 && key < hi && key + size > lo) {
-        const int id = bt[key >> shift];
-        if (id >= 0 && id < p.num_pages) ids = id;
-        else *holes = 1;                       // before the block is handed over
-      }
-      return true;
-    };
-    auto hand_over = [&]() {                   // the oldest block has landed: visible to the tensor cores, then said so to its tiles
-      const int s = handed++ % SC_STAGES;
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (lane == 0) sc_publish(found_addr, seen + 1);
       __syncwarp();
-      if (lane < 2 && ((used >> (2 * s + lane)) & 1u)) ta_mbar_arrive(is_v ? v_full(lane, s) : k_full(lane, s));
     };
-    bool more = look_ahead();
+    // The block to come: this half's first key, the keys of its part, lane i the id of the half's i-th page (-1: no page, or no key of the part in
+    // it).  It is looked up before the one at hand is copied, across the ends of steps.
+    int left0 = 0, left1 = 0, key0 = 0, key1 = 0, lo0 = 0, lo1 = 0, hi0 = 0, hi1 = 0, turn = 0;
+    int kb = 0, lo = 0, hi = 0, ids = -1;
+    uint32_t tiles = 0;
+    bool both = false, ok = true, more = true;
+    const int* bt0 = nullptr;
+    const int* bt1 = nullptr;
+    const uint8_t* head0 = nullptr;
+    const uint8_t* head1 = nullptr;
+    const uint8_t* head = nullptr;
+#pragma unroll 1
     while (more && ok) {
-      const int s = n % SC_STAGES, kb_now = kb, lo_now = lo, hi_now = hi, ids_now = ids;
+      // ---- the block at hand is the one that was looked up; the one after it
+      const int kb_now = kb, lo_now = lo, hi_now = hi, ids_now = ids;
       const uint32_t tiles_now = tiles;
       const uint8_t* head_now = head;
-      more = look_ahead();
-      // The tiles that read this stage's last block are through with it.  While that has to be waited for, whatever has been requested is handed over.
-      const uint32_t before = (used >> (2 * s)) & 3u;
-      const uint32_t bar = is_v ? v_empty(lane & 1, s) : k_empty(lane & 1, s), parity = ((lane & 1 ? turn1 : turn0) >> s) & 1u;
-      const bool mine = lane < 2 && ((before >> lane) & 1u);
-      if (__any_sync(0xffffffffu, mine && !ta_mbar_try_wait(bar, parity))) {
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        while (handed < n) hand_over();
-        const int go = !mine || ta_mbar_wait_idle(bar, parity, abort_flag, SC_ERR_KV_EMPTY) ? 1 : 0;
-        if (__any_sync(0xffffffffu, go == 0)) { ok = false; break; }
+      if (left0 + left1 == 0) {
+        if (warp == 0) find_step();
+        ScPart g;
+        more = step(seen, 1, g);
+        both = g.kind == SC_BOTH;
+        left1 = both ? 0 : g.blocks;
+        lo1 = g.key_lo; hi1 = g.key_hi;
+        key1 = (g.key_lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS + half * 32;
+        bt1 = p.table + (size_t)g.request * p.max_pages;
+        head1 = pool + (size_t)g.kv_head * ps * (D * 2);
+        more = more && step(seen, 0, g);
+        left0 = g.blocks;
+        lo0 = g.key_lo; hi0 = g.key_hi;
+        key0 = (g.key_lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS + half * 32;
+        bt0 = p.table + (size_t)g.request * p.max_pages;
+        head0 = pool + (size_t)g.kv_head * ps * (D * 2);
+        ++seen;
+        turn = 0;
       }
-      turn0 ^= (before & 1u) << s;
-      turn1 ^= (before >> 1) << s;
+      ids = -1;
+      if (more) {
+        const bool b = left0 == 0 || (turn && left1 > 0);
+        turn = !b;
+        lo = b ? lo1 : lo0; hi = b ? hi1 : hi0; kb = b ? key1 : key0;
+        head = b ? head1 : head0;
+        const int* bt = b ? bt1 : bt0;
+        tiles = both ? 3u : b ? 2u : 1u;
+        left0 -= !b; left1 -= b;
+        key0 += b ? 0 : AS_KEYS; key1 += b ? AS_KEYS : 0;
+        const int key = kb + lane * size;
+        if (lane * size < 32 && key < hi && key + size > lo) {
+          const int id = bt[key >> shift];
+          if (id >= 0 && id < p.num_pages) ids = id;
+          else *holes = 1;                     // before the block is handed over
+        }
+      }
+      if (tiles_now == 0) continue;            // nothing at hand yet
+      // ---- its stage: the tiles that read the last block there are through with it.  While that has to be waited for, whatever has been requested
+      // is handed over; else the oldest block when SC_IN_FLIGHT are behind it.
+      const int s = n % SC_STAGES;
+      const uint32_t before = (used >> (2 * s)) & 3u, bar = empty0 + 8u * (uint32_t)((lane & 1) * SC_BARS + s);
+      const bool mine = lane < 2 && ((before >> lane) & 1u);
+      const uint32_t parity = (turns >> (2 * s + (lane & 1))) & 1u;
+      const bool wait = __any_sync(0xffffffffu, mine && !ta_mbar_try_wait(bar, parity));
+      const int keep = wait ? 0 : SC_IN_FLIGHT;
+      if (n - handed > keep) {
+        if (wait) asm volatile("cp.async.wait_group 0;" ::: "memory");
+        else asm volatile("cp.async.wait_group %0;" ::"n"(SC_IN_FLIGHT) : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // visible to the tensor cores
+        __syncwarp();
+#pragma unroll 1
+        for (; n - handed > keep; ++handed) {
+          const int h = handed % SC_STAGES;
+          if (lane < 2 && ((used >> (2 * h + lane)) & 1u)) ta_mbar_arrive(full0 + 8u * (uint32_t)(lane * SC_BARS + h));
+        }
+      }
+      if (wait) {
+        const bool go = !mine || sc_wait<true>(bar, parity, abort_flag, SC_ERR_KV_EMPTY);
+        if (__any_sync(0xffffffffu, !go)) { ok = false; break; }
+      }
+      turns ^= before << (2 * s);
       used = (used & ~(3u << (2 * s))) | (tiles_now << (2 * s));
+      // ---- the copies.  Keys outside lo .. hi - 1 and of no page are filled with zeros.
       const uint32_t stage = ring + (uint32_t)s * L::KV_TILE;
-      switch (ps) {
-        case 8: sc_copy_half<8, D>(stage, xr, head_now, ids_now, kb_now, lo_now, hi_now, page_stride, rp, 0); break;
-        case 16: sc_copy_half<16, D>(stage, xr, head_now, ids_now, kb_now, lo_now, hi_now, page_stride, rp, 0); break;
-        default: sc_copy_half<32, D>(stage, xr, head_now, ids_now, kb_now, lo_now, hi_now, page_stride, rp, kb_now & (ps - 1)); break;
+      const bool inner = kb_now >= lo_now && kb_now + 32 <= hi_now;        // every key may be seen
+#pragma unroll 4
+      for (int j = 0; j < 32 / RPI; ++j) {
+        const int r = rp + RPI * j, key = kb_now + r;
+        const int id = __shfl_sync(0xffffffffu, ids_now, r >> bits);
+        const uint32_t bytes = (id >= 0 && (inner || (key >= lo_now && key < hi_now))) ? 16u : 0u;       // 0: sixteen zeros
+        const uint8_t* src = head_now + (size_t)max(id, 0) * page_stride + (uint32_t)(key & (ps - 1)) * (uint32_t)(D * 2);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                     ::"r"(stage + (uint32_t)r * 128u + (uint32_t)(((c & 7) ^ (r & 7)) << 4)), "l"(src), "r"(bytes) : "memory");
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
       ++n;
-      if (n - handed > SC_IN_FLIGHT) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(SC_IN_FLIGHT) : "memory");
-        hand_over();
-      }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (ok)
-      while (handed < n) hand_over();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (ok) {
+#pragma unroll 1
+      for (; handed < n; ++handed) {
+        const int h = handed % SC_STAGES;
+        if (lane < 2 && ((used >> (2 * h + lane)) & 1u)) ta_mbar_arrive(full0 + 8u * (uint32_t)(lane * SC_BARS + h));
+      }
+    }
     if (warp == 5) as_write_records(p, plan, cta, gridDim.x, lane, 32);    // while the last blocks are worked on
   } else if (warp == 1 || warp == 3) {
     // ---- products, one thread a tile -------------------------------------------------------------------------------------------------
@@ -285,45 +330,47 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       int n0 = 0, mine = 0, segments = 0;      // blocks of all segments so far, this tile's blocks and segments
       uint32_t k_turn = 0, v_turn = 0;         // bit s: the parity of this tile's next wait for stage s
       bool ok = true;
-      ScSegment g;
-      for (int seen = 0; ok && segment(seen, g); ++seen) {
-        if (!((g.tiles >> t) & 1)) { n0 += g.blocks; continue; }
-        ok = ta_mbar_wait(q_full(t), (uint32_t)(segments & 1), abort_flag, SC_ERR_Q);
-        // S(i) = Q K(i)^T into S buffer (mine + i) & 1
-        auto issue_qk = [&](int i) -> bool {
-          const int s = (n0 + i) % SC_STAGES, b = (mine + i) & 1;
-          if (!ta_mbar_wait(k_full(t, s), (k_turn >> s) & 1u, abort_flag, SC_ERR_KV_FULL)) return false;
-          k_turn ^= 1u << s;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t ka = sbase + L::K_OFF + s * L::KV_TILE;
+      ScPart g, other;
+#pragma unroll 1
+      for (int seen = 0; ok && step(seen, t, g) && step(seen, t ^ 1, other); ++seen) {
+        const int all = g.kind == SC_BOTH ? g.blocks : g.blocks + other.blocks;
+        if (g.blocks > 0) ok = sc_wait<false>(q_full(t), (uint32_t)(segments & 1), abort_flag, SC_ERR_Q);
+        // S(i) = Q K(i)^T into S buffer (mine + i) & 1, then O += P V(i - 1): S(i + 1) overwrites P(i - 1), whose product the tensor cores finish first
+#pragma unroll 1
+        for (int i = 0; i <= g.blocks && g.blocks > 0 && ok; ++i) {
+          if (i < g.blocks) {
+            const int s = (n0 + place(t, i, other.blocks, g.kind)) % SC_STAGES, b = (mine + i) & 1;
+            ok = sc_wait<false>(k_full(t, s), (k_turn >> s) & 1u, abort_flag, SC_ERR_KV_FULL);
+            if (!ok) break;
+            k_turn ^= 1u << s;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t ka = sbase + L::K_OFF + s * L::KV_TILE;
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            ta_umma(s_col + (uint32_t)b * 64u, ta_desc_kmajor(qa + (uint32_t)(k >> 2) * TA_HALF_BYTES + (uint32_t)(k & 3) * 32u),
-                    ta_desc_kmajor(ka + (uint32_t)(k >> 2) * L::KV_HALF + (uint32_t)(k & 3) * 32u), idesc_qk, k != 0);
-          ta_commit(s_full(t, b));
-          ta_commit(k_empty(t, s));
-          return true;
-        };
-        for (int i = 0; i < 2 && i < g.blocks && ok; ++i) ok = issue_qk(i);
-        for (int i = 0; i < g.blocks && ok; ++i) {
-          const int s = (n0 + i) % SC_STAGES, b = (mine + i) & 1;
-          ok = ta_mbar_wait(v_full(t, s), (v_turn >> s) & 1u, abort_flag, SC_ERR_KV_FULL);
-          if (ok && i == 0 && segments > 0) ok = ta_mbar_wait(o_free(t), (uint32_t)((segments - 1) & 1), abort_flag, SC_ERR_O_FREE);
-          ok = ok && ta_mbar_wait(p_full(t, b), (uint32_t)(((mine + i) >> 1) & 1), abort_flag, SC_ERR_P_FULL);
-          if (!ok) break;
-          v_turn ^= 1u << s;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t va = sbase + L::V_OFF + s * L::KV_TILE;
+            for (int k = 0; k < D / 16; ++k)
+              ta_umma(s_col + (uint32_t)b * 64u, ta_desc_kmajor(qa + (uint32_t)(k >> 2) * TA_HALF_BYTES + (uint32_t)(k & 3) * 32u),
+                      ta_desc_kmajor(ka + (uint32_t)(k >> 2) * L::KV_HALF + (uint32_t)(k & 3) * 32u), idesc_qk, k != 0);
+            ta_commit(s_full(t, b));
+            ta_commit(k_empty(t, s));
+          }
+          if (i > 0) {
+            const int h = i - 1, s = (n0 + place(t, h, other.blocks, g.kind)) % SC_STAGES, b = (mine + h) & 1;
+            ok = sc_wait<false>(v_full(t, s), (v_turn >> s) & 1u, abort_flag, SC_ERR_KV_FULL);
+            if (ok && h == 0 && segments > 0) ok = sc_wait<false>(o_free(t), (uint32_t)((segments - 1) & 1), abort_flag, SC_ERR_O_FREE);
+            ok = ok && sc_wait<false>(p_full(t, b), (uint32_t)(((mine + h) >> 1) & 1), abort_flag, SC_ERR_P_FULL);
+            if (!ok) break;
+            v_turn ^= 1u << s;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t va = sbase + L::V_OFF + s * L::KV_TILE;
 #pragma unroll
-          for (int k = 0; k < AS_KEYS / 16; ++k)
-            ta_umma_ts(o_col, s_col + (uint32_t)b * 64u + (uint32_t)k * 8u, ta_desc_mnmajor(va + (uint32_t)k * 16u * 128u, L::KV_HALF), idesc_pv, (i | k) != 0);
-          ta_commit(pv_done(t, b));
-          ta_commit(v_empty(t, s));
-          if (i + 2 < g.blocks) ok = issue_qk(i + 2);          // where P(i) lies: the tensor cores finish P V(i) first
+            for (int k = 0; k < AS_KEYS / 16; ++k)
+              ta_umma_ts(o_col, s_col + (uint32_t)b * 64u + (uint32_t)k * 8u, ta_desc_mnmajor(va + (uint32_t)k * 16u * 128u, L::KV_HALF), idesc_pv, (h | k) != 0);
+            ta_commit(pv_done(t, b));
+            ta_commit(v_empty(t, s));
+          }
         }
-        n0 += g.blocks;
+        n0 += all;
         mine += g.blocks;
-        ++segments;
+        if (g.blocks > 0) ++segments;
       }
     }
   } else {
@@ -332,20 +379,31 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     const uint32_t tlane = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_addr = tmem + tlane + (uint32_t)t * 128u, o_addr = tmem + tlane + 256u + (uint32_t)t * 128u;
     const uint32_t q_rows = sbase + t * L::Q_TILE + (uint32_t)quarter * 32u * 128u;        // this warp's rows
-    bool ok = true;
-    // Of the segment at hand: which it is, its blocks, the first one's first key, the first key and the end of those this row sees (of none, if
-    // there is no such row), and the least end among the warp's rows.  A request's tile of at most 32 rows is folded: all four warps have all its rows,
-    // and each a quarter of a block's keys (the tensor cores work on 128 rows anyway); each leaves a partial result of its own.
-    int at_segment = -1, blocks = 0, block_key = 0, lo = 0, hi = 0, hi_all = 0;
-    bool valid = false, warp_valid = false, folded = false;
-    // The next segment of this tile, if there is one: its queries are requested.
-    auto next_segment = [&]() -> bool {
-      ScSegment g;
-      do {
-        if (!segment(++at_segment, g)) return false;
-      } while (!((g.tiles >> t) & 1));
-      {
-        const int first = g.tiles == 3 ? t * per : 0, lane_rows = min(g.tokens - first, per) * G;
+    // Of the part at hand: the step, its blocks, the first one's first key, the first key and the end of those this row sees (of none, if there is
+    // no such row), and the least end among the warp's rows.  A request's tile of at most 32 rows is folded: all four warps have all its rows, and
+    // each a quarter of a block's keys (the tensor cores work on 128 rows anyway); each leaves a partial result of its own.
+    int at_step = -1, blocks = 0, block_key = 0, lo = 0, hi = 0, hi_all = 0, mine = 0;
+    bool valid = false, warp_valid = false, folded = false, ok = true;
+    float m_ref = -INFINITY, l_run = 0.f;
+    int done = -1;                             // the step of the part before
+#pragma unroll 1
+    for (;;) {
+      // ---- this tile's next part with blocks, if there is one: its queries are requested, whole rows side by side
+      bool more = true;
+      ScPart g;
+      int from = -1;                           // this row's place among all rows of the queries
+#pragma unroll 1
+      for (;;) {
+        more = step(++at_step, t, g);
+        if (!more) break;
+        if (g.tokens == 0) continue;
+        if (g.blocks > 0) break;
+        // the second half of a single block: an empty partial result
+        const long long tile = (long long)(uint32_t)g.row_low | (long long)g.row_high << 32;
+        if (r < g.tokens * G) *reinterpret_cast<float2*>(p.part_ml + (tile + g.tokens * G + r) * 2) = make_float2(-INFINITY, 0.f);
+      }
+      if (more) {
+        const int first = g.kind == SC_BOTH ? t * per : 0, lane_rows = min(g.tokens - first, per) * G;
         folded = !g.shared && g.tokens * G <= AS_FOLD_ROWS;
         const int row = folded ? lane : r;     // of this tile's
         valid = row < lane_rows;
@@ -354,7 +412,6 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         lo = g.key_lo;
         block_key = (lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS;
         hi = 0x7fffffff;
-        int from = -1;                         // this row's place among all rows of the queries
         if (valid) {
           const int i = row / G;
           int token, position;
@@ -363,9 +420,9 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
           hi = min(position + 1, g.key_hi);
         }
         hi_all = __reduce_min_sync(0xffffffffu, hi);
-        constexpr int CHUNKS = D / 8, RPI = 32 / CHUNKS;       // whole rows side by side
+        constexpr int CHUNKS = D / 8, RPI = 32 / CHUNKS;
         const int c = lane % CHUNKS;
-#pragma unroll
+#pragma unroll 4
         for (int i = 0; i < 32 / RPI; ++i) {
           const int rr = i * RPI + lane / CHUNKS, row_at = __shfl_sync(0xffffffffu, from, rr);
           if (row_at >= 0)
@@ -374,226 +431,188 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
                            "l"((const uint8_t*)p.q + (size_t)row_at * (D * 2) + c * 16) : "memory");
         }
       }
-      return true;
-    };
-    auto hand_queries = [&]() {
+      // ---- the part before it is complete meanwhile: its result is written
+      if (done >= 0) {
+        ok = sc_wait<false>(pv_done(t, (mine - 1) & 1), (uint32_t)(((mine - 1) >> 1) & 1), abort_flag, SC_ERR_O_FULL);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const volatile ScPart* was = &steps[done % SC_SEGMENTS].part[t];
+        const int tile_rows = was->tokens * G, kind = was->kind;
+        const long long tile = (long long)(uint32_t)was->row_low | (long long)was->row_high << 32;
+        const bool fold = !was->shared && tile_rows <= AS_FOLD_ROWS;
+        const int first_row = kind == SC_BOTH ? t * per * G : 0, rows = fold ? 4 * tile_rows : kind == SC_BOTH ? tile_rows : 2 * tile_rows;
+        const int in_tile = fold ? lane : r, left = min(tile_rows - first_row, per * G);             // this thread's row of the tile's `left`
+        if (fold || quarter * 32 < left) {
+          const bool on = in_tile < left;
+          const int row = fold ? quarter * tile_rows + lane : (kind == SC_BOTH ? first_row : t * tile_rows) + r;
+          if (on) *reinterpret_cast<float2*>(p.part_ml + (tile + row) * 2) = make_float2(m_ref, l_run);
+          float4* dst = reinterpret_cast<float4*>(p.part_o + tile * D) + row;
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t v[32];
+            ta_tmem_ld32(o_addr + (uint32_t)c, v);             // warp-wide: rows without a token take part and write nothing
+            if (on) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                dst[(size_t)((c >> 2) + e) * rows] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]), __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
+            }
+          }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) ta_mbar_arrive(o_free(t));
+      }
+      if (!more) break;
+      done = at_step;
       asm volatile("cp.async.wait_all;" ::: "memory");
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) ta_mbar_arrive(q_full(t));
-    };
-    int mine = 0;
-    bool more = next_segment();
-    if (more) hand_queries();
-    while (more) {
-      float m_ref = -INFINITY, l_run = 0.f;
-      // O of this tile's rows times f, when P V of block j - 1 is complete
-      auto rescale = [&](int j, float f) -> bool {
-        if (!ta_mbar_wait(pv_done(t, (j - 1) & 1), (uint32_t)(((j - 1) >> 1) & 1), abort_flag, SC_ERR_O_FULL)) return false;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      // ---- its blocks
+      m_ref = -INFINITY;
+      l_run = 0.f;
+      bool settled = false;                    // every row has a reference
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t v[32];
-          ta_tmem_ld32(o_addr + (uint32_t)c, v);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-          ta_tmem_st32(o_addr + (uint32_t)c, v);
-        }
-        ta_tmem_wait_st();
-        return true;
-      };
-      // the block's keys in pages that are not there, of `width` keys from kb on
-      auto absent_keys = [&](int kb, int width) -> unsigned long long {
-        const volatile ScSegment* g = &ring_of_segments[at_segment % SC_SEGMENTS];
-        const int size = min(p.page_size, width), key = kb + lane * size;
-        const bool here = lane * size < width && key < g->key_hi && key + size > lo;
-        const int id = here ? p.table[(size_t)g->request * p.max_pages + (key >> p.page_shift)] : 0;
-        unsigned long long keys = 0;
-        for (uint32_t absent = __ballot_sync(0xffffffffu, id < 0 || id >= p.num_pages); absent; absent &= absent - 1) {
-          const int first = (__ffs(absent) - 1) * size;
-          keys |= sc_low_bits(first + size) & ~sc_low_bits(first);
-        }
-        return keys;
-      };
-      if (folded) {
-        for (int i = 0; i < blocks; ++i, block_key += AS_KEYS) {
-          const int j = mine + i, b = j & 1, kb = block_key + quarter * 16;
-          ok = ta_mbar_wait(s_full(t, b), (uint32_t)((j >> 1) & 1), abort_flag, SC_ERR_S_FULL);
-          if (!ok) break;
+      for (int i = 0; i < blocks; ++i, block_key += AS_KEYS) {
+        const int j = mine + i, b = j & 1;
+        ok = sc_wait<false>(s_full(t, b), (uint32_t)((j >> 1) & 1), abort_flag, SC_ERR_S_FULL);
+        if (!ok) break;
+        if (warp_valid) {                      // (else its rows of P are anything, and nobody reads what comes of them)
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          float xs[16];
-          {
-            uint32_t v[16];
-            sc_tmem_ld16(s_addr + (uint32_t)b * 64u + (uint32_t)quarter * 16u, v);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) xs[e] = __uint_as_float(v[e]);
+          bool masked = block_key < lo || block_key + AS_KEYS > hi_all;
+          unsigned long long seen = sc_low_bits(hi - block_key) & ~sc_low_bits(lo - block_key);        // which of the block's keys the row sees
+          if (*holes) {                        // there are pages that are not: a look at this block's
+            const volatile ScPart* now = &steps[at_step % SC_SEGMENTS].part[t];
+            const int size = min(p.page_size, AS_KEYS), key = block_key + lane * size;
+            const bool here = lane * size < AS_KEYS && key < now->key_hi && key + size > lo;
+            const int id = here ? p.table[(size_t)now->request * p.max_pages + (key >> p.page_shift)] : 0;
+            uint32_t absent = __ballot_sync(0xffffffffu, id < 0 || id >= p.num_pages);
+            masked |= absent != 0;
+#pragma unroll 1
+            for (; absent; absent &= absent - 1) {
+              const int first = (__ffs(absent) - 1) * size;
+              seen &= ~(sc_low_bits(first + size) & ~sc_low_bits(first));
+            }
           }
-          const bool some = *holes;
-          if (some || kb < lo || kb + 16 > hi_all) {
-            unsigned long long seen = sc_low_bits(hi - kb) & ~sc_low_bits(lo - kb);
-            if (some) seen &= ~absent_keys(kb, 16);
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (!(((uint32_t)seen >> e) & 1u)) xs[e] = -INFINITY;
-          }
-          float mx = ta_max3(xs[0], xs[1], xs[2]);
-#pragma unroll
-          for (int e = 3; e < 15; e += 2) mx = ta_max3(mx, xs[e], xs[e + 1]);
-          mx = fmaxf(mx, xs[15]);
-          const float m_loc = mx * p.scale_log2;
-          const bool grow = valid && m_loc > m_ref + TA_RESCALE_STEP;    // also true for the first finite maximum (m_ref = -inf)
-          if (__any_sync(0xffffffffu, grow)) {
-            float f = 1.f;
+          uint32_t w[32];
+          float sum, f = 1.f;
+          bool rescale = false;
+          // A row's reference: its maximum so far when that has grown by 2^8.
+          auto follow = [&](float mx) {
+            const float m_loc = mx * p.scale_log2;
+            const bool grow = valid && m_loc > m_ref + TA_RESCALE_STEP;  // also true for the first finite maximum (m_ref = -inf)
+            rescale = __any_sync(0xffffffffu, grow);
             if (grow) {
               if (m_ref != -INFINITY) f = exp2f(m_ref - m_loc);
               m_ref = m_loc;
-              l_run *= f;
             }
-            if (i > 0) ok = rescale(j, f);
-            if (!ok) break;
+          };
+          if (folded) {
+            float xs[16];
+            {
+              uint32_t v[16];
+              sc_tmem_ld16(s_addr + (uint32_t)b * 64u + (uint32_t)quarter * 16u, v);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) xs[e] = __uint_as_float(v[e]);
+            }
+            if (masked) {
+              const uint32_t mask = (uint32_t)(seen >> (quarter * 16));
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (!((mask >> e) & 1u)) xs[e] = -INFINITY;
+            }
+            float mx = ta_max3(xs[0], xs[1], xs[2]);
+#pragma unroll
+            for (int e = 3; e < 15; e += 2) mx = ta_max3(mx, xs[e], xs[e + 1]);
+            follow(fmaxf(mx, xs[15]));
+            const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+            sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {      // the other warps' keys weigh nothing here
+              const float p0 = exp2_approx(fmaf(xs[2 * e], p.scale_log2, -m_use)), p1 = exp2_approx(fmaf(xs[2 * e + 1], p.scale_log2, -m_use));
+              sum += p0 + p1;
+              __nv_bfloat162 b2 = __floats2bfloat162_rn(p0, p1);
+              const uint32_t pair = *reinterpret_cast<uint32_t*>(&b2);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) w[8 * q + e] = q == quarter ? pair : 0u;
+            }
+          } else {
+            // Where every row has a reference, its maximum is not looked for: a sum of 64 weights that stays below 2^15 says that no score is
+            // far above the reference.  Otherwise the block is done again from the scores, which still lie in tensor memory, with the maximum.
+#pragma unroll 1
+            for (bool exact = !settled;; exact = true) {
+              float xs[AS_KEYS];
+              {
+                uint32_t v[AS_KEYS];
+                ta_tmem_ld64(s_addr + (uint32_t)b * 64u, v);
+#pragma unroll
+                for (int e = 0; e < AS_KEYS; ++e) xs[e] = __uint_as_float(v[e]);
+              }
+              if (masked) {
+                const uint32_t low = (uint32_t)seen, high = (uint32_t)(seen >> 32);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  if (!((low >> e) & 1u)) xs[e] = -INFINITY;
+                  if (!((high >> e) & 1u)) xs[32 + e] = -INFINITY;
+                }
+              }
+              if (exact) {
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < AS_KEYS; e += 8) {
+#pragma unroll
+                  for (int u = 0; u < 4; ++u) mx4[u] = ta_max3(mx4[u], xs[e + 2 * u], xs[e + 2 * u + 1]);
+                }
+                follow(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
+                settled = !__any_sync(0xffffffffu, valid && m_ref == -INFINITY);
+              }
+              const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+              const uint64_t scale2 = ta_pack2(p.scale_log2, p.scale_log2), negm2 = ta_pack2(-m_use, -m_use);
+              uint64_t sum2 = ta_pack2(0.f, 0.f);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                float y0, y1;
+                ta_unpack2(ta_fma2(ta_pack2(xs[2 * e], xs[2 * e + 1]), scale2, negm2), y0, y1);
+                const float p0 = exp2_approx(y0), p1 = exp2_approx(y1);  // 2^-inf = 0 for masked keys
+                sum2 = ta_add2(sum2, ta_pack2(p0, p1));
+                __nv_bfloat162 b2 = __floats2bfloat162_rn(p0, p1);
+                w[e] = *reinterpret_cast<uint32_t*>(&b2);
+              }
+              float s0, s1;
+              ta_unpack2(sum2, s0, s1);
+              sum = s0 + s1;
+              if (exact || !__any_sync(0xffffffffu, valid && !(sum < 32768.f))) break;
+            }
           }
-          const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-          uint32_t w[32];                      // the other warps' keys weigh nothing here
-          float sum = 0.f;
+          l_run = l_run * f + sum;
+          if (rescale && i > 0) {              // O in the new reference's units, when P V of the block before is complete
+            ok = sc_wait<false>(pv_done(t, b ^ 1), (uint32_t)(((j - 1) >> 1) & 1), abort_flag, SC_ERR_O_FULL);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t v[32];
+              ta_tmem_ld32(o_addr + (uint32_t)c, v);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float p0 = exp2_approx(fmaf(xs[2 * e], p.scale_log2, -m_use)), p1 = exp2_approx(fmaf(xs[2 * e + 1], p.scale_log2, -m_use));
-            sum += p0 + p1;
-            __nv_bfloat162 b2 = __floats2bfloat162_rn(p0, p1);
-            const uint32_t pair = *reinterpret_cast<uint32_t*>(&b2);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) w[8 * q + e] = q == quarter ? pair : 0u;
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+              ta_tmem_st32(o_addr + (uint32_t)c, v);
+            }
           }
           ta_tmem_st32(s_addr + (uint32_t)b * 64u, w);
           ta_tmem_wait_st();
-          l_run += sum;
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) ta_mbar_arrive(p_full(t, b));
         }
-        if (!ok) break;
-      }
-      bool settled = false;                    // every row has a reference
-      for (int i = 0; i < blocks && !folded; ++i, block_key += AS_KEYS) {
-        const int j = mine + i, b = j & 1, kb = block_key;
-        ok = ta_mbar_wait(s_full(t, b), (uint32_t)((j >> 1) & 1), abort_flag, SC_ERR_S_FULL);
-        if (!ok) break;
-        if (!warp_valid) {                     // no row of this warp: its rows of P are anything, and nobody reads what comes of them
-          __syncwarp();
-          if (lane == 0) ta_mbar_arrive(p_full(t, b));
-          continue;
-        }
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        bool masked = kb < lo || kb + AS_KEYS > hi_all;
-        unsigned long long seen = sc_low_bits(hi - kb) & ~sc_low_bits(lo - kb);        // which of the block's keys the row sees
-        if (*holes) {
-          const unsigned long long absent = absent_keys(kb, AS_KEYS);
-          masked |= absent != 0;
-          seen &= ~absent;
-        }
-        // Where every row has a reference, its maximum is not looked for: a sum of 64 weights that stays below 2^15 says that no score is
-        // far above the reference.  Otherwise the block is done again from the scores, which still lie in tensor memory, with the maximum.
-        uint32_t w[32];
-        float sum;
-        for (bool exact = !settled;; exact = true) {
-          float xs[AS_KEYS];
-          {
-            uint32_t v[AS_KEYS];
-            ta_tmem_ld64(s_addr + (uint32_t)b * 64u, v);
-#pragma unroll
-            for (int e = 0; e < AS_KEYS; ++e) xs[e] = __uint_as_float(v[e]);
-          }
-          if (masked) {
-            const uint32_t low = (uint32_t)seen, high = (uint32_t)(seen >> 32);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              if (!((low >> e) & 1u)) xs[e] = -INFINITY;
-              if (!((high >> e) & 1u)) xs[32 + e] = -INFINITY;
-            }
-          }
-          if (exact) {
-            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int e = 0; e < AS_KEYS; e += 8) {
-#pragma unroll
-              for (int u = 0; u < 4; ++u) mx4[u] = ta_max3(mx4[u], xs[e + 2 * u], xs[e + 2 * u + 1]);
-            }
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-            const float m_loc = mx * p.scale_log2;
-            const bool grow = valid && m_loc > m_ref + TA_RESCALE_STEP;  // also true for the first finite maximum (m_ref = -inf)
-            if (__any_sync(0xffffffffu, grow)) {
-              float f = 1.f;
-              if (grow) {
-                if (m_ref != -INFINITY) f = exp2f(m_ref - m_loc);
-                m_ref = m_loc;
-                l_run *= f;
-              }
-              if (i > 0) ok = rescale(j, f);
-              if (!ok) break;
-            }
-            settled = !__any_sync(0xffffffffu, valid && m_ref == -INFINITY);
-          }
-          const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-          const uint64_t scale2 = ta_pack2(p.scale_log2, p.scale_log2), negm2 = ta_pack2(-m_use, -m_use);
-          uint64_t sum2 = ta_pack2(0.f, 0.f);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            float y0, y1;
-            ta_unpack2(ta_fma2(ta_pack2(xs[2 * e], xs[2 * e + 1]), scale2, negm2), y0, y1);
-            const float p0 = exp2_approx(y0), p1 = exp2_approx(y1);      // 2^-inf = 0 for masked keys
-            sum2 = ta_add2(sum2, ta_pack2(p0, p1));
-            __nv_bfloat162 b2 = __floats2bfloat162_rn(p0, p1);
-            w[e] = *reinterpret_cast<uint32_t*>(&b2);
-          }
-          float s0, s1;
-          ta_unpack2(sum2, s0, s1);
-          sum = s0 + s1;
-          if (exact) break;
-          if (!__any_sync(0xffffffffu, valid && !(sum < 32768.f))) break;
-        }
-        if (!ok) break;
-        ta_tmem_st32(s_addr + (uint32_t)b * 64u, w);
-        ta_tmem_wait_st();
-        l_run += sum;
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
         if (lane == 0) ta_mbar_arrive(p_full(t, b));
       }
       if (!ok) break;
       mine += blocks;
-      // All products with this tile's queries are done: the next segment's come while this one's result is awaited and written.
-      const ScSegment* was = &ring_of_segments[at_segment % SC_SEGMENTS];
-      const long long tile = was->row;
-      const int tile_rows = was->tokens * G, rows = folded ? 4 * tile_rows : tile_rows;
-      const int row = folded ? quarter * tile_rows + lane : (was->tiles == 3 ? t * per * G : 0) + r;
-      const bool row_valid = valid, some_valid = warp_valid;
-      more = next_segment();
-      ok = ta_mbar_wait(pv_done(t, (mine - 1) & 1), (uint32_t)(((mine - 1) >> 1) & 1), abort_flag, SC_ERR_O_FULL);
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (some_valid) {
-        if (row_valid) *reinterpret_cast<float2*>(p.part_ml + (tile + row) * 2) = make_float2(m_ref, l_run);
-        float4* dst = reinterpret_cast<float4*>(p.part_o + tile * D) + row;
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t v[32];
-          ta_tmem_ld32(o_addr + (uint32_t)c, v);               // warp-wide: rows without a token take part and write nothing
-          if (row_valid) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              dst[(size_t)((c >> 2) + e) * rows] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]), __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
-          }
-        }
-      }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) ta_mbar_arrive(o_free(t));
-      if (more) hand_queries();
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) atomicCAS(&g_attention_tc_error, 0, (int)*abort_flag);
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
@@ -603,7 +622,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
 template <int D>
 static cudaError_t sc_launch(const SharedParams& p, int ctas, cudaStream_t stream) {
   constexpr int smem = ScLayout<D>::BYTES + 1024;
-  static_assert(smem + sizeof(SharedPlan) + sizeof(ScSegment) * SC_SEGMENTS + 64 <= 227 * 1024, "shared memory of a CTA");
+  static_assert(smem + sizeof(SharedPlan) + sizeof(ScStep) * SC_SEGMENTS + 64 <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<unsigned long long> configured{0ull};     // a bit a device
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);

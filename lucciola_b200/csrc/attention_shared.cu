@@ -29,33 +29,30 @@ template <int D> constexpr int ap_smem_bytes() { return (AP_ROWS * D + AS_KEYS *
 template <typename T, int D>
 __global__ void __launch_bounds__(AP_THREADS) attention_shared_plain_kernel(SharedParams p) {
   extern __shared__ __align__(16) float ap_smem[];
-  __shared__ SharedPlan plan;
   float* qs = ap_smem;
   float* ks = qs + AP_ROWS * D;
   float* vs = ks + AS_KEYS * (D + 4);
   float* ps = vs + AS_KEYS * D;
   int* page = reinterpret_cast<int*>(ps + AP_ROWS * (AS_KEYS + 4));      // offset of each key's row in the pool's page units, -1: not there
   pdl_trigger();
-  as_make_plan(p, plan, blockIdx.x, gridDim.x);                // lengths and groups were written before the kernel ahead began
   pdl_wait();
-  as_write_records(p, plan, blockIdx.x, gridDim.x, threadIdx.x, AP_THREADS);
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const T* q = reinterpret_cast<const T*>(p.q);
   const T* kc = reinterpret_cast<const T*>(p.k_cache);
   const T* vc = reinterpret_cast<const T*>(p.v_cache);
   const int d = p.dim, G = p.group, cache_heads = p.kv_heads / p.kv_share;
-  Walk way = as_begin(p, plan, blockIdx.x);
-  while (way.x < way.x_end) {
-    const Segment g = as_next(p, plan, blockIdx.x, way);
+  const int2 piece = __ldcg(p.pieces + blockIdx.x);
+  for (int at = piece.x; at <= piece.y; ++at) {
+    const Segment g = as_segment(p, at);
     if (g.blocks == 0) continue;
+    const long long first_row = (long long)(uint32_t)g.row_low | (long long)g.row_high << 32;
     const int rows = g.tokens * G;
     __syncthreads();
     for (int i = tid; i < AP_ROWS * (D / 4); i += AP_THREADS) {
       const int r = i / (D / 4), c = i % (D / 4) * 4;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < rows && c < d) {
-        int token, position;
-        as_token(plan, g.shared, g.request, g.first + r / G, token, position);
+        const int token = as_token(p, g.shared, g.first, g.position, r / G).x;
         v = ap_load4(q + ((size_t)token * p.heads + g.kv_head * G + r % G) * d + c);
       }
       *reinterpret_cast<float4*>(qs + r * D + c) = v;
@@ -63,9 +60,7 @@ __global__ void __launch_bounds__(AP_THREADS) attention_shared_plain_kernel(Shar
     int last[2];                         // the last key each row sees
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      int token;
-      last[e] = -1;
-      if (2 * ty + e < rows) as_token(plan, g.shared, g.request, g.first + (2 * ty + e) / G, token, last[e]);
+      last[e] = 2 * ty + e < rows ? as_token(p, g.shared, g.first, g.position, (2 * ty + e) / G).y : -1;
     }
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     float o[2][D / 64][4];
@@ -158,11 +153,60 @@ __global__ void __launch_bounds__(AP_THREADS) attention_shared_plain_kernel(Shar
     for (int e = 0; e < 2; ++e) {
       const int r = 2 * ty + e;
       if (r >= rows) continue;
-      if (tx == 0) *reinterpret_cast<float2*>(p.part_ml + (g.row + r) * 2) = make_float2(m[e], l[e]);
+      if (tx == 0) *reinterpret_cast<float2*>(p.part_ml + (first_row + r) * 2) = make_float2(m[e], l[e]);
 #pragma unroll
       for (int c = 0; c < D / 64; ++c)
         if (64 * c + 4 * tx < d)
-          *reinterpret_cast<float4*>(p.part_o + g.row * d + ((16 * c + tx) * rows + r) * 4) = make_float4(o[e][c][0], o[e][c][1], o[e][c][2], o[e][c][3]);
+          *reinterpret_cast<float4*>(p.part_o + first_row * d + ((16 * c + tx) * rows + r) * 4) = make_float4(o[e][c][0], o[e][c][1], o[e][c][2], o[e][c][3]);
+    }
+  }
+}
+
+// The plan of a step: every CTA makes all of it, and writes a part.
+__global__ void __launch_bounds__(AS_PLAN_THREADS) as_plan_kernel(SharedParams p, int ctas) {
+  __shared__ SharedPlan pl;
+  pdl_trigger();
+  as_make_plan(p, pl, ctas);             // lengths and groups were written before the kernel ahead began
+  pdl_wait();
+  as_write_records(p, pl, blockIdx.x, gridDim.x, threadIdx.x, AS_PLAN_THREADS);
+  const bool sound = as_sound(p, pl);
+  const int total = sound ? pl.units * p.kv_heads : 0, span = pl.span;
+  if (blockIdx.x == 0)
+    for (int c = threadIdx.x; c < ctas; c += AS_PLAN_THREADS)
+      if ((long long)c * span >= total) p.pieces[c] = make_int2(0, -1);
+  if (!sound) return;
+  // the segments: a thread has an entry and a kv head
+  for (int i = blockIdx.x * AS_PLAN_THREADS + threadIdx.x; i < 2 * p.S * p.kv_heads; i += gridDim.x * AS_PLAN_THREADS) {
+    const int kv = i / (2 * p.S), e = i - kv * (2 * p.S);
+    const bool shared = e < p.S;
+    const int s = shared ? e : e - p.S;
+    const int4 me = pl.meta[s];
+    const int end = e + 1 < 2 * p.S ? pl.unit[e + 1] : pl.units;
+    if (pl.unit[e] == end) continue;
+    const int lead = shared ? -1 : pl.lead[s], lo = lead >= 0 ? pl.meta[lead].w : 0, hi = shared ? me.w : me.z;
+    const int tokens = shared ? pl.led[s] : me.y, nb = as_blocks(lo, hi);
+    int base = kv * pl.units + pl.unit[e];
+#pragma unroll 1
+    for (int first = 0, tile = pl.tile[e]; first < tokens; first += p.tile_tokens, ++tile) {
+      const int here = min(tokens - first, p.tile_tokens), two = here > p.lane_tokens ? 1 : 0;             // units of a block: 1 << two
+      const int key_hi = shared ? hi : min(hi, hi - tokens + first + here), there = as_blocks(lo, key_hi);      // an earlier tile sees fewer blocks
+      const int b0 = base + p.tile_start, b1 = base + as_tile_units(p, here, nb);
+      const int c0 = (int)((unsigned)base / (unsigned)span), c1 = (int)((unsigned)(b1 - 1) / (unsigned)span);
+#pragma unroll 1
+      for (int c = c0; c <= c1; ++c) {
+        const int x0 = c * span, x1 = min(x0 + span, total);
+        // a block belongs to the CTA in whose piece it begins
+        const int block = max(x0 - b0 + two, 0) >> two, blocks = max(min(max(min(x1, b1) - b0 + two, 0) >> two, there) - block, 0);
+        const int at = kv * pl.tiles + tile + c;
+        const long long row = (long long)kv * pl.rows + pl.row[e] + (long long)first * p.group + (long long)c * p.tile_tokens * p.group;
+        int4* dst = p.segments + (size_t)at * 3;
+        dst[0] = make_int4(kv, s, (shared ? pl.first_member[s] : pl.q0[s]) + first, here);
+        dst[1] = make_int4(lo, key_hi, block, blocks);
+        dst[2] = make_int4((int)(uint32_t)row, (int)(row >> 32), shared ? 1 : 0, shared ? 0 : me.z - tokens + first);
+        if (x0 >= base) p.pieces[c].x = at;
+        if (x1 <= b1) p.pieces[c].y = at;
+      }
+      base = b1;
     }
   }
 }
@@ -209,62 +253,101 @@ static cudaError_t as_combine(const SharedParams& p, cudaStream_t stream) {
   return launch(as_combine_kernel<T, 1>, dim3(p.T, p.kv_heads), dim3(AS_COMBINE_THREADS), 0, stream, p);
 }
 
+
+// What all launches of one call have in common; false with the library's message when the arguments are refused.
+static bool as_params(SharedParams& p, SharedCut& cut, int& ctas, int dtype, int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
+                      int page_size, int max_pages) {
+#define AS_CHECK(cond, ...) do { if (!(cond)) { set_error(__VA_ARGS__); return false; } } while (0)
+  AS_CHECK(valid_dtype(dtype), "attention_shared: unknown element type %d", dtype);
+  AS_CHECK(num_tokens >= 0 && num_seqs >= 0 && num_seqs <= AS_MAX_SEQS, "attention_shared: %d tokens of %d requests, at most %d requests",
+           num_tokens, num_seqs, AS_MAX_SEQS);
+  AS_CHECK(num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0, "attention_shared: %d query heads on %d kv heads",
+           num_q_heads, num_kv_heads);
+  AS_CHECK(head_dim > 0 && head_dim <= 256 && head_dim % 8 == 0, "attention_shared: heads of %d, a multiple of 8 up to 256 is needed", head_dim);
+  AS_CHECK(page_size > 0 && max_pages > 0 && (long long)max_pages * page_size < (1ll << 31) - 64, "attention_shared: tables of %d pages of %d tokens",
+           max_pages, page_size);
+  AS_CHECK((long long)num_tokens * num_q_heads < (1ll << 30), "attention_shared: %d tokens of %d heads", num_tokens, num_q_heads);
+  ctas = as_sms();
+  AS_CHECK(ctas > 0, "attention_shared: no device");
+  cut = as_cut(dtype, num_q_heads / num_kv_heads, head_dim, page_size);
+  p = SharedParams{};
+  p.T = num_tokens; p.S = num_seqs; p.heads = num_q_heads; p.kv_heads = num_kv_heads * cut.share; p.group = cut.group; p.dim = head_dim;
+  p.page_size = page_size; p.max_pages = max_pages; p.page_shift = -1; p.kv_share = cut.share;
+  p.tile_tokens = cut.tile_tokens; p.lane_tokens = cut.lane_tokens;
+  p.min_span = cut.tc ? 4 : 1; p.tile_start = cut.tc ? 2 : 0; p.folds = cut.tc;
+  for (int b = 0; b < 31; ++b) if ((1 << b) == page_size) p.page_shift = b;
+  // units of the whole line, at most
+  const long long tiles = 2ll * ((long long)num_tokens / p.tile_tokens + num_seqs), blocks = (long long)max_pages * page_size / AS_KEYS + 1;
+  AS_CHECK(tiles * (2 * blocks + 2) * p.kv_heads < (1ll << 31) - 65536, "attention_shared: %d tokens of %d requests on tables of %d pages are too much for one launch",
+           num_tokens, num_seqs, max_pages);
+  AS_CHECK(p.kv_heads <= 65535, "attention_shared: %d kv heads", p.kv_heads);
+#undef AS_CHECK
+  return true;
+}
+
+static void as_plan_parts(SharedParams& p, int* plan, int ctas) {
+  const SharedPlanLayout at(p.T, p.S, p.kv_heads, p.tile_tokens, ctas);
+  p.head = plan; p.rec = plan + at.rec; p.pieces = reinterpret_cast<int2*>(plan + at.pieces);
+  p.segments = reinterpret_cast<int4*>(plan + at.segments); p.members = reinterpret_cast<int2*>(plan + at.members);
+}
+
 }  // namespace lb
 
-// Elements of the two workspaces of a launch: partial results (float32) and the combining kernel's list (int32).
-LB_EXPORT int lb_attention_shared_workspace(int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int dtype, int page_size,
-                                            long long* floats, long long* ints) {
-  LB_CHECK_ARG(num_tokens >= 0 && num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0 && head_dim > 0, "attention_shared: bad sizes");
-  const int ctas = lb::as_sms();
-  LB_CHECK_ARG(ctas > 0, "attention_shared: no device");
-  const lb::SharedCut cut = lb::as_cut(dtype, num_q_heads / num_kv_heads, head_dim, page_size);
-  const long long rows = lb::as_most_rows(num_tokens, num_seqs, cut.group, cut.tc) * num_kv_heads * cut.share + (long long)ctas * cut.tile_tokens * cut.group;
-  *floats = rows * (head_dim + 2);
-  *ints = (long long)num_tokens * lb::AS_REC + 8;
+// Elements that a call needs: of the plan (int32) and of the partial results (float32).
+LB_EXPORT int lb_attention_shared_sizes(int dtype, int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+                                        int max_pages, long long* ints, long long* floats) {
+  lb::SharedParams p;
+  lb::SharedCut cut;
+  int ctas = 0;
+  if (!lb::as_params(p, cut, ctas, dtype, num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, max_pages)) return 1;
+  *ints = lb::SharedPlanLayout(num_tokens, num_seqs, p.kv_heads, p.tile_tokens, ctas).total;
+  *floats = (lb::as_most_rows(num_tokens, num_seqs, cut.group, cut.tc) * p.kv_heads + (long long)ctas * cut.tile_tokens * cut.group) * (head_dim + 2);
   return 0;
 }
 
-// q, out: [T, heads, dim]; k_cache, v_cache: [pages, kv heads, page_size, dim]; table [S, max_pages], cu_tokens [S + 1], context_lens,
-// prefix_of and prefix_lens [S], all int32.  See attention_shared.cuh.
-LB_EXPORT int lb_attention_shared(int dtype, const void* q, void* out, const void* k_cache, const void* v_cache, const int* table,
-                                  const int* cu_tokens, const int* context_lens, const int* prefix_of, const int* prefix_lens, int num_tokens,
-                                  int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int page_size, int num_pages, int max_pages,
-                                  float scale, float* floats, long long num_floats, int* ints, long long num_ints, cudaStream_t stream) {
-  LB_CHECK_ARG(lb::valid_dtype(dtype), "attention_shared: unknown element type %d", dtype);
-  LB_CHECK_ARG(num_tokens >= 0 && num_seqs >= 0 && num_seqs <= lb::AS_MAX_SEQS, "attention_shared: %d tokens of %d requests, at most %d requests",
-               num_tokens, num_seqs, lb::AS_MAX_SEQS);
-  LB_CHECK_ARG(num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0, "attention_shared: %d query heads on %d kv heads",
-               num_q_heads, num_kv_heads);
-  LB_CHECK_ARG(head_dim > 0 && head_dim <= 256 && head_dim % 8 == 0, "attention_shared: heads of %d, a multiple of 8 up to 256 is needed", head_dim);
-  LB_CHECK_ARG(page_size > 0 && num_pages > 0 && max_pages > 0 && (long long)max_pages * page_size < (1ll << 31) - 64, "attention_shared: %d pages of %d tokens, tables of %d",
-               num_pages, page_size, max_pages);
+// The plan of a step for lb_attention_shared, from cu_tokens [S + 1], context_lens, prefix_of and prefix_lens [S], int32.
+LB_EXPORT int lb_attention_shared_plan(int dtype, int* plan, long long num_ints, const int* cu_tokens, const int* context_lens, const int* prefix_of,
+                                       const int* prefix_lens, int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
+                                       int page_size, int max_pages, cudaStream_t stream) {
+  lb::SharedParams p;
+  lb::SharedCut cut;
+  int ctas = 0;
+  if (!lb::as_params(p, cut, ctas, dtype, num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, max_pages)) return 1;
+  if (num_tokens == 0 || num_seqs == 0) return 0;
+  const long long need = lb::SharedPlanLayout(num_tokens, num_seqs, p.kv_heads, p.tile_tokens, ctas).total;
+  LB_CHECK_ARG(plan && (uintptr_t)plan % 16 == 0 && num_ints >= need, "attention_shared: a plan of %lld integers at a 16-byte boundary is needed, got %lld", need, num_ints);
+  p.cu = cu_tokens; p.ctx = context_lens; p.prefix_of = prefix_of; p.prefix_lens = prefix_lens;
+  lb::as_plan_parts(p, plan, ctas);
+  const long long tasks = 2ll * num_seqs * p.kv_heads;
+  const int blocks = (int)(tasks < 32 * 64 ? (tasks + 63) / 64 : 32);        // few tasks a CTA: each is a chain of lookups
+  lb::launch(lb::as_plan_kernel, dim3(blocks), dim3(lb::AS_PLAN_THREADS), 0, stream, p, ctas);
+  LB_CHECK_LAUNCH("attention_shared plan");
+  return 0;
+}
+
+// q, out: [T, heads, dim]; k_cache, v_cache: [pages, kv heads, page_size, dim]; table [S, max_pages] int32; a plan made for these sizes.
+// floats: the partial results.  See attention_shared.cuh.
+LB_EXPORT int lb_attention_shared(int dtype, const void* q, void* out, const void* k_cache, const void* v_cache, const int* table, int* plan,
+                                  long long num_ints, int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+                                  int num_pages, int max_pages, float scale, float* floats, long long num_floats, cudaStream_t stream) {
+  lb::SharedParams p;
+  lb::SharedCut cut;
+  int ctas = 0;
+  if (!lb::as_params(p, cut, ctas, dtype, num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, max_pages)) return 1;
+  LB_CHECK_ARG(num_pages > 0, "attention_shared: a pool of %d pages", num_pages);
   LB_CHECK_ARG(scale > 0.f && scale < 1e30f, "attention_shared: a scale of %f, a positive one is needed", (double)scale);
   if (num_tokens == 0 || num_seqs == 0) return 0;
-  LB_CHECK_ARG((long long)num_tokens * num_q_heads < (1ll << 30), "attention_shared: %d tokens of %d heads", num_tokens, num_q_heads);
-  LB_CHECK_ARG(((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)floats | (uintptr_t)ints) % 16 == 0,
+  LB_CHECK_ARG(((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)floats | (uintptr_t)plan) % 16 == 0,
                "attention_shared: operands must be 16-byte aligned");
-  long long need_floats = 0, need_ints = 0;
-  if (lb_attention_shared_workspace(num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, dtype, page_size, &need_floats, &need_ints)) return 1;
-  LB_CHECK_ARG(floats && ints && num_floats >= need_floats && num_ints >= need_ints,
-               "attention_shared: workspaces of %lld and %lld elements are needed, got %lld and %lld", need_floats, need_ints, num_floats, num_ints);
-  const int ctas = lb::as_sms();
-  const lb::SharedCut cut = lb::as_cut(dtype, num_q_heads / num_kv_heads, head_dim, page_size);
-  lb::SharedParams p;
-  p.q = q; p.out = out; p.k_cache = k_cache; p.v_cache = v_cache; p.table = table; p.max_pages = max_pages; p.num_pages = num_pages;
-  p.cu = cu_tokens; p.ctx = context_lens; p.prefix_of = prefix_of; p.prefix_lens = prefix_lens;
-  p.T = num_tokens; p.S = num_seqs; p.heads = num_q_heads; p.kv_heads = num_kv_heads * cut.share; p.group = cut.group; p.dim = head_dim;
-  p.page_size = page_size; p.page_shift = -1; p.kv_share = cut.share; p.tile_tokens = cut.tile_tokens; p.lane_tokens = cut.lane_tokens;
-  p.min_span = cut.tc ? 4 : 1; p.tile_start = cut.tc ? 2 : 0; p.folds = cut.tc;
-  for (int b = 0; b < 31; ++b) if ((1 << b) == page_size) p.page_shift = b;
+  const long long need = lb::SharedPlanLayout(num_tokens, num_seqs, p.kv_heads, p.tile_tokens, ctas).total;
+  const long long rows = lb::as_most_rows(num_tokens, num_seqs, cut.group, cut.tc) * p.kv_heads + (long long)ctas * cut.tile_tokens * cut.group;
+  LB_CHECK_ARG(plan && floats && num_ints >= need && num_floats >= rows * (head_dim + 2),
+               "attention_shared: a plan of %lld integers and a workspace of %lld floats are needed, got %lld and %lld", need, rows * (head_dim + 2),
+               num_ints, num_floats);
+  p.q = q; p.out = out; p.k_cache = k_cache; p.v_cache = v_cache; p.table = table; p.num_pages = num_pages;
   p.scale_log2 = scale * 1.4426950408889634f;
-  // units of the whole line, at most
-  const long long tiles = 2ll * ((long long)num_tokens / p.tile_tokens + num_seqs), blocks = (long long)max_pages * page_size / lb::AS_KEYS + 1;
-  LB_CHECK_ARG(tiles * (2 * blocks + 2) * p.kv_heads < (1ll << 31) - 65536, "attention_shared: %d tokens of %d requests on tables of %d pages are too much for one launch",
-               num_tokens, num_seqs, max_pages);
-  LB_CHECK_ARG(p.kv_heads <= 65535, "attention_shared: %d kv heads", p.kv_heads);
-  const long long rows = (need_floats) / (head_dim + 2);
   p.part_o = floats; p.part_ml = floats + rows * head_dim;
-  p.rec = ints; p.head = ints + (long long)num_tokens * lb::AS_REC;
+  lb::as_plan_parts(p, plan, ctas);
   cudaError_t e;
   if (cut.tc)
     e = lb::attention_shared_tc(p, ctas, stream);

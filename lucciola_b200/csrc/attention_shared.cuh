@@ -1,15 +1,18 @@
-// What the kernels of attention with shared prefixes have in common: the plan of a step, made by every CTA for itself from the requests'
-// lengths, the walk over a CTA's part of it, and the combination of the partial results.
+// What the kernels of attention with shared prefixes have in common: the plan of a step, which a kernel makes from the requests' lengths, and
+// the combination of the partial results.
 //
 // A step's requests fall into groups (prefix_of, prefix_lens): the members' first keys are the same pages.  The work is a list of tiles
 // of query rows (a row is a token and a head of a kv head's group of G query heads), each with a range of keys:
 //     the tokens of a group's members, up to `tile_tokens` of them, with the group's prefix       (one read of the prefix for all rows)
 //     up to `tile_tokens` tokens of one request with what the request has behind the prefix       (all its keys, if it shares none)
 // The keys of a tile are visited in blocks of 64.  All blocks of all tiles, once for every kv head, stand in one line, and each CTA
-// takes an equal piece of it: the cuts fall anywhere, so that every CTA has the same amount of work whatever the lengths are.  A tile
-// whose blocks fall to several CTAs has a partial result (m, l, o) of each, in 32 bits, which a second kernel adds up by token.
+// takes an equal piece of it: the cuts fall anywhere, so that every CTA has the same amount of work whatever the lengths are.  What a CTA has
+// of a tile is a segment; a tile has a partial result (m, l, o) of each of its segments, in 32 bits, and a last kernel adds them up by token.
 //
-// A group of a single member, or with less than a block of prefix, is none.  Nothing of this is kept or comes from the host: a step that is replayed from a recorded graph may have other groups and lengths.
+// A group of a single member, or with less than a block of prefix, is none.  Nothing of this comes from the host: a step that is replayed
+// from a recorded graph may have other groups and lengths.  The plan is a kernel of its own because the layers of a model share it, and because the
+// code that makes it would have to be fetched by every SM in front of its work (instructions are fetched anew by every launch: 9000 cycles
+// for the plan and the walk along it, of 45000 in all, at 64 requests behind 8192 keys).
 // Block ids outside the pool and keys past a request's table are not there; a row that sees no key gives zeros.
 #pragma once
 
@@ -17,7 +20,7 @@
 
 namespace lb {
 
-constexpr int AS_MAX_SEQS = 256;
+constexpr int AS_MAX_SEQS = 512;
 constexpr int AS_KEYS = 64;
 constexpr int AS_REC = 12;               // integers a token in the combining kernel's list
 constexpr int AS_FOLD_ROWS = 32;
@@ -37,7 +40,18 @@ struct SharedParams {
   // Partial results: 4 consecutive dimensions of all rows of a tile, then the next 4 ([dim / 4][rows][4], so that threads with a row each
   // write, and threads with a head each read, side by side), and [rows][2]: the reference value (-inf: no key) and the sum.
   float* part_o; float* part_ml;
-  int* rec; int* head;                   // [T][AS_REC], {units a kv head, units a CTA, rows a kv head, first token, end of the tokens}
+  // The plan.  head: {units a kv head, units a CTA, rows a kv head, first token, end of the tokens}; rec [T][AS_REC]: see as_write_records; pieces
+  // [CTAs]: the CTA's first and last segment; segments [..][12]: see Segment; members [T]: the groups' tokens, group by group, and the last key each sees
+  int* head; int* rec; int2* pieces; int4* segments; int2* members;
+};
+
+// Integers of a plan, and where its parts begin.
+struct SharedPlanLayout {
+  long long rec, pieces, segments, members, total;
+  __host__ SharedPlanLayout(long long tokens, long long seqs, int kv_heads, int tile_tokens, int ctas) {
+    const long long most = kv_heads * 2 * (tokens / tile_tokens + seqs) + ctas;        // a tile has one segment more than it has cuts
+    rec = 8; pieces = rec + tokens * AS_REC; segments = (pieces + 2 * ctas + 3) & ~3ll; members = segments + most * 12; total = members + 2 * tokens;
+  }
 };
 
 // The tensor-core kernel (attention_shared_tc.cu): what it takes, how it cuts rows, its launch.
@@ -45,20 +59,16 @@ bool attention_shared_tc_takes(int dtype, int group, int head_dim, int page_size
 void attention_shared_tc_cut(int group, int& tile_tokens, int& lane_tokens);
 cudaError_t attention_shared_tc(const SharedParams& p, int ctas, cudaStream_t stream);
 
-struct SharedPlan {
+struct SharedPlan {                      // in shared memory, while it is made
   int4 meta[AS_MAX_SEQS];                // prefix_of (-1: none), new tokens, context, tokens of the prefix in this row's table
   int q0[AS_MAX_SEQS];                   // first token
   int lead[AS_MAX_SEQS];                 // the row whose table holds the prefix that this request shares, -1: none
   int rank[AS_MAX_SEQS];                 // tokens of the group in front of this request's
-  int before[AS_MAX_SEQS];               // members of the group in front of it
   int led[AS_MAX_SEQS];                  // tokens of the group that this row leads
-  int member[AS_MAX_SEQS];               // the groups' members, group by group
-  int first_member[AS_MAX_SEQS + 1];     // of the group that this row leads
-  int unit[2 * AS_MAX_SEQS], row[2 * AS_MAX_SEQS], place[2 * AS_MAX_SEQS];     // of entry e (groups by their leader, then requests): where it
-                                         // begins in the line, in the list of rows and among the entries that are not empty
-  int2 entry[2 * AS_MAX_SEQS];           // of those: first unit, e
-  int entries, units, span, rows;        // how many; units and rows of a kv head, units of a CTA
-  int kv_head, at, tile;                 // where this CTA's piece begins
+  int unit[2 * AS_MAX_SEQS], row[2 * AS_MAX_SEQS], tile[2 * AS_MAX_SEQS];      // of entry e (groups by their leader, then requests): where it
+                                         // begins in the line, in the list of rows and among all tiles
+  int first_member[AS_MAX_SEQS];         // where the tokens of the group that this row leads begin among all groups'
+  int units, span, rows, tiles;          // units, rows and tiles of a kv head, units of a CTA
 };
 
 __device__ __forceinline__ int as_blocks(int lo, int hi) { return hi > lo ? (hi - (lo & ~(AS_KEYS - 1)) + AS_KEYS - 1) / AS_KEYS : 0; }
@@ -105,8 +115,9 @@ __device__ __forceinline__ int as_scan(int* a, int n) {
   return total;
 }
 
-// Made by all threads of a CTA (256 at least, a power of two of them or 384); ends with a barrier.  Reads lengths and groups only.
-__device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& pl, int cta, int ctas) {
+// Made by all AS_PLAN_THREADS threads of a CTA; ends with a barrier.  Reads lengths and groups only.
+constexpr int AS_PLAN_THREADS = 512;
+__device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& pl, int ctas) {
   const int tid = threadIdx.x, n = p.S;
   const int most = p.max_pages * p.page_size;
   if (tid < n) {
@@ -118,24 +129,24 @@ __device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& 
   }
   __syncthreads();
   // Who shares with whom: every request looks at all others (n is a few dozen, a few hundred at most), 1 << k lanes for each.
-  const int k = n <= (int)blockDim.x / 4 ? 2 : n <= (int)blockDim.x / 2 ? 1 : 0;
+  const int k = n <= AS_PLAN_THREADS / 8 ? 3 : n <= AS_PLAN_THREADS / 4 ? 2 : n <= AS_PLAN_THREADS / 2 ? 1 : 0;
   const int s = tid >> k, part = tid & ((1 << k) - 1);
   if ((s & ~(31 >> k)) < n) {            // whole warps
     const int4 me = s < n ? pl.meta[s] : make_int4(-1, 0, 0, 0);
     const int l = me.x;
-    int rank = 0, before = 0, all = 0, led = 0, led_tokens = 0;
+    int rank = 0, all = 0, led = 0, led_tokens = 0;
 #pragma unroll 4
     for (int j = part; j < n; j += 1 << k) {
       const int2 o = *reinterpret_cast<const int2*>(&pl.meta[j]);
       const bool same = o.x == l && l >= 0, mine = o.x == s;
       all += same ? 1 : 0;
-      before += same && j < s ? 1 : 0;
       rank += same && j < s ? o.y : 0;
       led += mine ? 1 : 0;
       led_tokens += mine ? o.y : 0;
     }
+#pragma unroll 1
     for (int o = (1 << k) >> 1; o > 0; o >>= 1) {
-      all += __shfl_xor_sync(0xffffffffu, all, o); before += __shfl_xor_sync(0xffffffffu, before, o); rank += __shfl_xor_sync(0xffffffffu, rank, o);
+      all += __shfl_xor_sync(0xffffffffu, all, o); rank += __shfl_xor_sync(0xffffffffu, rank, o);
       led += __shfl_xor_sync(0xffffffffu, led, o); led_tokens += __shfl_xor_sync(0xffffffffu, led_tokens, o);
     }
     if (part == 0 && s < n) {
@@ -144,52 +155,30 @@ __device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& 
       const bool shares = all >= 2 && prefix >= AS_KEYS, leads = led >= 2 && me.w >= AS_KEYS;
       pl.lead[s] = shares ? l : -1;
       pl.rank[s] = rank;
-      pl.before[s] = before;
       pl.led[s] = led_tokens;
-      pl.first_member[s] = led;
-      const int ua = leads ? as_units(p, led_tokens, as_blocks(0, me.w)) : 0, ub = as_units(p, me.y, as_blocks(shares ? prefix : 0, me.z));
-      pl.unit[s] = ua; pl.unit[n + s] = ub;
-      pl.row[s] = leads ? as_rows(p, true, led_tokens) : 0; pl.row[n + s] = as_rows(p, false, me.y);
-      pl.place[s] = ua > 0 ? 1 : 0; pl.place[n + s] = ub > 0 ? 1 : 0;
+      pl.first_member[s] = leads ? led_tokens : 0;
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        const int e = i * n + s, tokens = i ? me.y : leads ? led_tokens : 0, blocks = i ? as_blocks(shares ? prefix : 0, me.z) : as_blocks(0, me.w);
+        pl.unit[e] = as_units(p, tokens, blocks);
+        pl.row[e] = as_rows(p, i == 0, tokens);
+        pl.tile[e] = blocks > 0 ? (tokens + p.tile_tokens - 1) / p.tile_tokens : 0;
+      }
     }
   }
   __syncthreads();
   const int warp = tid >> 5;
-  if (warp == 0) {
-    const int u = as_scan(pl.unit, 2 * n);
-    if (tid == 0) {
-      pl.units = u;
-      pl.span = max((int)(((unsigned)u * (unsigned)p.kv_heads + (unsigned)ctas - 1u) / (unsigned)ctas), p.min_span);
-    }
-  } else if (warp == 1) {
-    const int r = as_scan(pl.row, 2 * n);
-    if ((tid & 31) == 0) pl.rows = r;
-  } else if (warp == 2) {
-    const int e = as_scan(pl.place, 2 * n);
-    if ((tid & 31) == 0) pl.entries = e;
-  } else if (warp == 3) {
-    const int m = as_scan(pl.first_member, n);
-    if ((tid & 31) == 0) pl.first_member[n] = m;
-  }
-  __syncthreads();
-  // where this CTA begins: the entry whose units hold its first one
-  const int units = pl.units, x = cta * pl.span;
-  const int kv = units > 0 ? (int)((unsigned)x / (unsigned)units) : 0, u = x - kv * units;
-  for (int e = tid; e < 2 * n; e += blockDim.x) {
-    const bool last = e + 1 == 2 * n;
-    const int at = pl.place[e], end = last ? units : pl.unit[e + 1], from = pl.unit[e];
-    if (at < (last ? pl.entries : pl.place[e + 1])) {
-      pl.entry[at] = make_int2(from, e);
-      if (from <= u && u < end) {
-        const int l = e < n ? -1 : pl.lead[e - n];
-        const int nb = e < n ? as_blocks(0, pl.meta[e].w) : as_blocks(l >= 0 ? pl.meta[l].w : 0, pl.meta[e - n].z);
-        pl.kv_head = kv;
-        pl.at = at;
-        pl.tile = (int)((unsigned)(u - from) / (unsigned)as_tile_units(p, p.tile_tokens, nb));        // (only the last tile may be smaller)
+  if (warp < 4) {
+    const int sum = as_scan(warp == 0 ? pl.unit : warp == 1 ? pl.row : warp == 2 ? pl.tile : pl.first_member, warp < 3 ? 2 * n : n);
+    if ((tid & 31) == 0) {
+      if (warp == 0) {
+        pl.units = sum;
+        pl.span = max((int)(((unsigned)sum * (unsigned)p.kv_heads + (unsigned)ctas - 1u) / (unsigned)ctas), p.min_span);
       }
+      if (warp == 1) pl.rows = sum;
+      if (warp == 2) pl.tiles = sum;
     }
   }
-  if (tid < n && pl.meta[tid].x >= 0) pl.member[pl.first_member[pl.meta[tid].x] + pl.before[tid]] = tid;
   __syncthreads();
 }
 
@@ -201,109 +190,56 @@ __host__ __device__ __forceinline__ long long as_most_rows(long long tokens, lon
 __device__ __forceinline__ bool as_sound(const SharedParams& p, const SharedPlan& pl) { return pl.rows <= as_most_rows(p.T, p.S, p.group, p.folds); }
 
 // What the combining kernel has to know of every token, for the prefix and for the request's own keys: the first row of the token's
-// tile, the token's first row in the tile, the tile's rows (not folded), the unit of its first block, and how many units further the last block begins
-// (-1: no block).  By `threads` threads of each CTA; the CTAs without work come first.
+// tile, the token's first row in the tile, the tile's rows (not folded), the unit of its first block, and how many units further the last block
+// begins (-1: no block).  And the groups' tokens.
 __device__ __forceinline__ void as_write_records(const SharedParams& p, const SharedPlan& pl, int cta, int ctas, int thread, int threads) {
   if (cta == 0 && thread == 0) {
     p.head[0] = pl.units; p.head[1] = pl.span; p.head[2] = pl.rows;
     p.head[3] = p.S > 0 ? pl.q0[0] : 0;
     p.head[4] = p.S > 0 ? pl.q0[p.S - 1] + pl.meta[p.S - 1].y : 0;
   }
-  for (int s = ctas - 1 - cta; s < p.S; s += ctas) {
+  for (int s = cta * (threads >> 5) + (thread >> 5); s < p.S; s += ctas * (threads >> 5)) {        // a warp a request
     const int4 me = pl.meta[s];
     const int t0 = pl.q0[s], q = me.y, l = pl.lead[s];
     const int prefix = l >= 0 ? pl.meta[l].w : 0;
-    for (int i = thread; i < q; i += threads) {
-      int4 a = make_int4(0, 0, 0, 0);
-      int a_last = -1;
-      if (l >= 0) {
-        const int index = pl.rank[s] + i, tokens = pl.led[l], nb = as_blocks(0, prefix);
-        const int tile = index / p.tile_tokens, first = tile * p.tile_tokens, here = min(tokens - first, p.tile_tokens);
-        a = make_int4(pl.row[l] + first * p.group, (index - first) * p.group, here * p.group, pl.unit[l] + tile * as_tile_units(p, p.tile_tokens, nb) + p.tile_start);
-        a_last = (nb - 1) * (here > p.lane_tokens ? 2 : 1);
-      }
-      const int tile = i / p.tile_tokens, first = tile * p.tile_tokens, here = min(q - first, p.tile_tokens), e = p.S + s;
-      const int nb = as_blocks(prefix, min(me.z, me.z - q + first + here));      // blocks that the tile's last token sees
-      const int4 b = make_int4(pl.row[e] + first * p.group, (i - first) * p.group, here * p.group,
-                               pl.unit[e] + tile * as_tile_units(p, p.tile_tokens, as_blocks(prefix, me.z)) + p.tile_start);
-      const int b_last = nb > 0 ? (nb - 1) * (here > p.lane_tokens ? 2 : 1) : -1;
+#pragma unroll 1
+    for (int i = thread & 31; i < q; i += 32) {
       int4* dst = reinterpret_cast<int4*>(p.rec + (size_t)(t0 + i) * AS_REC);
-      dst[0] = a; dst[1] = b; dst[2] = as_sound(p, pl) ? make_int4(a_last, b_last, 0, 0) : make_int4(-1, -1, 0, 0);
+      int last[2];
+#pragma unroll 1
+      for (int of = 0; of < 2; ++of) {   // the prefix, the request's own keys
+        const int e = of ? p.S + s : l, index = of ? i : pl.rank[s] + i, tokens = of ? q : l >= 0 ? pl.led[l] : 0;
+        const int tile = index / p.tile_tokens, first = tile * p.tile_tokens, here = min(tokens - first, p.tile_tokens);
+        const int lo = of ? prefix : 0, hi = of ? me.z : prefix;
+        const int blocks = as_blocks(lo, of ? min(hi, hi - q + first + here) : hi);            // that the tile's last token sees
+        const bool any = (of || l >= 0) && as_sound(p, pl);
+        dst[of] = any ? make_int4(pl.row[e] + first * p.group, (index - first) * p.group, here * p.group,
+                                  pl.unit[e] + tile * as_tile_units(p, p.tile_tokens, as_blocks(lo, hi)) + p.tile_start) : make_int4(0, 0, 0, 0);
+        last[of] = any && blocks > 0 ? (blocks - 1) * (here > p.lane_tokens ? 2 : 1) : -1;
+      }
+      dst[2] = make_int4(last[0], last[1], 0, 0);
+      if (l >= 0) p.members[pl.first_member[l] + pl.rank[s] + i] = make_int2(t0 + i, me.z - q + i);
     }
   }
 }
 
 // A run of blocks of one tile and one kv head.
 struct Segment {
-  int kv_head;
-  int request;                           // the row of the block table; whose tokens they are, if not shared
-  bool shared;                           // tokens of the members of the group that `request` leads
-  int first, tokens;                     // first token (of the group, of the request), and how many
+  int kv_head, request;                  // the row of the block table
+  int first, tokens;                     // first token (shared: its place among the groups' tokens), and how many
   int key_lo, key_hi;                    // keys of the tile (of all its rows together)
   int block, blocks;                     // first block of the run (of the tile's), and how many (0: none are there)
-  long long row;                         // where the tile's partial rows begin
+  int row_low, row_high;                 // where its partial rows begin, 64 bits
+  int shared, position;                  // rows of several requests; else the last key that the first token sees
 };
-
-// A CTA's way along the line: where it is, and which entry and tile that is in.
-struct Walk { int x, x_end, kv_head, at, tile; };
-
-__device__ __forceinline__ Walk as_begin(const SharedParams& p, const SharedPlan& pl, int cta) {
-  if (!as_sound(p, pl)) return Walk{0, 0, 0, 0, 0};
-  const int total = pl.units * p.kv_heads, x = min(cta * pl.span, total);
-  return Walk{x, min(x + pl.span, total), pl.kv_head, pl.at, pl.tile};
+__device__ __forceinline__ Segment as_segment(const SharedParams& p, int i) {
+  const int4* at = p.segments + (size_t)i * 3;
+  const int4 a = __ldcg(at), b = __ldcg(at + 1), c = __ldcg(at + 2);
+  return Segment{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w};
 }
-
-// The segment at w.x (< w.x_end); w moves behind it.
-__device__ __forceinline__ Segment as_next(const SharedParams& p, const SharedPlan& pl, int cta, Walk& w) {
-  Segment g;
-  const int2 e = pl.entry[w.at];
-  g.kv_head = w.kv_head;
-  g.shared = e.y < p.S;
-  const int s = g.shared ? e.y : e.y - p.S;
-  const int4 me = pl.meta[s];
-  const int tokens = g.shared ? pl.led[s] : me.y;
-  const int hi = g.shared ? me.w : me.z;
-  const int lead = g.shared ? -1 : pl.lead[s];
-  g.key_lo = lead >= 0 ? pl.meta[lead].w : 0;
-  const int nb = as_blocks(g.key_lo, hi);
-  g.request = s;
-  g.first = w.tile * p.tile_tokens;
-  g.tokens = min(tokens - g.first, p.tile_tokens);
-  const int two = g.tokens > p.lane_tokens ? 1 : 0;              // units of a block: 1 << two
-  g.key_hi = g.shared ? hi : min(hi, hi - tokens + g.first + g.tokens);
-  const int base = w.kv_head * pl.units + e.x + w.tile * as_tile_units(p, p.tile_tokens, nb) + p.tile_start;
-  const int there = as_blocks(g.key_lo, g.key_hi);               // a portion's earlier tiles see fewer blocks than its last
-  // a block belongs to the CTA in whose piece it begins
-  const int tile_end = base + (nb << two), end = min(w.x_end, tile_end);
-  g.block = max(w.x - base + two, 0) >> two;
-  g.blocks = max(min(max(end - base + two, 0) >> two, there) - g.block, 0);
-  g.row = (long long)w.kv_head * pl.rows + pl.row[e.y] + g.first * p.group + (long long)cta * p.tile_tokens * p.group;
-  w.x = end;
-  if (end == tile_end) {
-    if (g.first + g.tokens < tokens) {
-      ++w.tile;
-    } else {
-      w.tile = 0;
-      if (++w.at == pl.entries) { w.at = 0; ++w.kv_head; }
-    }
-  }
-  return g;
-}
-
-// A token's place in the step, and the last key it sees: the `at`-th token of the group that row s leads, or of request s.
-__device__ __forceinline__ void as_token(const SharedPlan& pl, bool shared, int s, int at, int& token, int& position) {
-  if (shared) {                          // the member whose token it is: the last one whose first token is not behind
-    int a = pl.first_member[s], b = pl.first_member[s + 1] - 1;
-    while (a < b) {
-      const int mid = (a + b + 1) >> 1;
-      if (pl.rank[pl.member[mid]] <= at) a = mid; else b = mid - 1;
-    }
-    s = pl.member[a];
-    at -= pl.rank[s];
-  }
-  token = pl.q0[s] + at;
-  const int4 me = pl.meta[s];
-  position = me.z - me.y + at;
+// A token of a segment: its place in the step, and the last key it sees.
+__device__ __forceinline__ int2 as_token(const SharedParams& p, int shared, int first, int position, int i) {
+  return shared ? __ldcg(p.members + first + i) : make_int2(first + i, position + i);
 }
 
 __device__ __forceinline__ void as_store4(float* dst, float a, float b, float c, float d) { *reinterpret_cast<float4*>(dst) = make_float4(a, b, c, d); }

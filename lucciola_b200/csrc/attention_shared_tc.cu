@@ -43,17 +43,17 @@ template <int D> struct ScLayout {
 
 // What the two tiles work on side by side, a part each: halves of one segment's blocks, segments of two requests, or (both) the same blocks
 // with other rows.  The parts' blocks alternate in the rings of keys and values, so that neither tile waits for the other's to pass.
-// Warp 0, which copies keys, walks the line one step ahead of its copies and leaves what it finds in a ring of steps; the others read them there.
+// Warp 0, which copies keys, makes steps of the CTA's segments, one ahead of its copies, and leaves them in a ring; the others read them there.
 // A slot comes again after SC_SEGMENTS steps: the rings of keys and values hold warp 0 back to a handful in front of whoever is last (a step
 // has a block at least, and a tile's next step waits for the one before).
-struct ScPart {
+struct ScPart {                          // a Segment, and
   int kv_head, request, first, tokens;   // tokens 0: nothing for this tile
   int key_lo, key_hi, block, blocks;     // blocks 0 of a part with tokens: it leaves an empty partial result
-  int row_low, row_high;                 // where the tile's partial rows begin
-  int shared, kind;
+  int row_low, row_high, position;
+  int kind;                              // one of the following, + SC_SHARED
 };
 struct ScStep { ScPart part[2]; };
-enum : int { SC_END = 0, SC_PARTS = 1, SC_BOTH = 2, SC_HALVES = 3 };       // kind, of either part
+enum : int { SC_END = 0, SC_PARTS = 1, SC_BOTH = 2, SC_HALVES = 3, SC_SHARED = 4 };      // of either part
 constexpr int SC_SEGMENTS = 32;
 
 __device__ __forceinline__ void sc_tmem_ld16(uint32_t taddr, uint32_t* r) {
@@ -102,7 +102,6 @@ template <int D>
 __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(SharedParams p) {
   typedef ScLayout<D> L;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ SharedPlan plan;
   __shared__ __align__(16) ScStep steps[SC_SEGMENTS];
   __shared__ int steps_found;
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -143,7 +142,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  as_make_plan(p, plan, blockIdx.x, gridDim.x);                // lengths and groups were written before the kernel ahead began
+  __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   pdl_wait();
   const uint32_t tmem = *tmem_slot;            // columns: tile t's S buffers at t * 128 and t * 128 + 64 (P over their first 32), O at 256 + t * 128
@@ -157,11 +156,11 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     const int4 a = at[0], b = at[1], c = at[2];
     g.kv_head = a.x; g.request = a.y; g.first = a.z; g.tokens = a.w;
     g.key_lo = b.x; g.key_hi = b.y; g.block = b.z; g.blocks = b.w;
-    g.row_low = c.x; g.row_high = c.y; g.shared = c.z; g.kind = c.w;
+    g.row_low = c.x; g.row_high = c.y; g.position = c.z; g.kind = c.w;
     return g.kind != SC_END;
   };
   // Where block i of tile t's part lies among the step's: A's and B's in turn, then what the longer part has more.
-  auto place = [](int t, int i, int others, int kind) { return kind == SC_BOTH ? i : i + min(t ? i + 1 : i, others); };
+  auto place = [](int t, int i, int others, int kind) { return (kind & 3) == SC_BOTH ? i : i + min(t ? i + 1 : i, others); };
 
   if (warp != 1 && warp != 3 && warp < SC_SOFTMAX) {
     // ---- copies: warps 0 and 4 the halves of every block of keys, 2 and 5 of values -----------------------------------------------------
@@ -169,26 +168,31 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     const int half = warp >= 4 ? 1 : 0;
     constexpr int CHUNKS = D / 8, RPI = 32 / CHUNKS;           // 16-byte chunks of a row, rows an instruction
     const int c = lane % CHUNKS, rp = lane / CHUNKS;           // a lane copies chunk c of the rows rp, rp + RPI, ... of its half
-    const uint8_t* pool = (const uint8_t*)(is_v ? p.v_cache : p.k_cache) + c * 16;
-    const uint32_t ring = sbase + (is_v ? L::V_OFF : L::K_OFF) + (uint32_t)(c >> 3) * L::KV_HALF + (uint32_t)(half * 32) * 128u;
+    const uint8_t* pool = (const uint8_t*)(is_v ? p.v_cache : p.k_cache) + c * 16 + rp * (D * 2);
+    const uint32_t ring = sbase + (is_v ? L::V_OFF : L::K_OFF) + (uint32_t)(c >> 3) * L::KV_HALF + (uint32_t)(half * 32 + rp) * 128u;
+    uint32_t swizzled[8 / RPI];                // this lane's chunk in its rows of eight
+#pragma unroll
+    for (int u = 0; u < 8 / RPI; ++u) swizzled[u] = (uint32_t)(RPI * u * 128 + (((c & 7) ^ (rp + RPI * u)) << 4));
     const uint32_t full0 = is_v ? v_full(0, 0) : k_full(0, 0), empty0 = is_v ? v_empty(0, 0) : k_empty(0, 0);
     const int ps = p.page_size, shift = p.page_shift, size = min(ps, 32), bits = min(shift, 5);
     const size_t page_stride = (size_t)p.kv_heads * ps * (D * 2);
     int n = 0, handed = 0, seen = 0;           // blocks requested, handed over; steps looked at
     uint32_t used = 0, turns = 0;              // bits 2 s + t: whether tile t reads stage s's block, and the parity of the next wait for it
-    // (Of warp 0) the way along the line, and a segment that has been found but is no part of a step yet.
-    Walk way = as_begin(p, plan, cta);
+    // (Of warp 0) the segment to come, fetched when the one before it was taken, and the one after it in the list.
+    const int2 piece = __ldcg(p.pieces + cta);
+    int at_segment = piece.x;
     Segment found;
-    found.blocks = 0;
+    auto fetch = [&]() {
+      found.blocks = 0;
+#pragma unroll 1
+      while (at_segment <= piece.y && found.blocks == 0) found = as_segment(p, at_segment++);
+    };
+    if (warp == 0) fetch();
     auto find_step = [&]() {
       int kind = SC_END;
       // At most two segments: the second one if it is a request's few rows, as the first.
 #pragma unroll 1
       for (int t = 0; t < 2; ++t) {
-        if (t == 0 || kind == SC_PARTS) {
-#pragma unroll 1
-          while (found.blocks == 0 && way.x < way.x_end) found = as_next(p, plan, cta, way);
-        }
         const Segment& g = found;
         const bool few = !g.shared && g.tokens * G <= AS_FOLD_ROWS;
         int block = g.block, blocks = g.blocks, tokens = g.tokens;
@@ -208,9 +212,9 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
           int4* at = reinterpret_cast<int4*>(&steps[seen % SC_SEGMENTS].part[t]);
           at[0] = make_int4(g.kv_head, g.request, g.first, tokens);
           at[1] = make_int4(g.key_lo, g.key_hi, block, blocks);
-          at[2] = make_int4((int)(uint32_t)g.row, (int)(g.row >> 32), g.shared ? 1 : 0, kind);
+          at[2] = make_int4(g.row_low, g.row_high, g.position, kind == SC_END ? SC_END : kind + (g.shared ? SC_SHARED : 0));
         }
-        if (!keep) found.blocks = 0;
+        if (!keep) fetch();
       }
       if (lane == 0) sc_publish(found_addr, seen + 1);
       __syncwarp();
@@ -236,7 +240,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         if (warp == 0) find_step();
         ScPart g;
         more = step(seen, 1, g);
-        both = g.kind == SC_BOTH;
+        both = (g.kind & 3) == SC_BOTH;
         left1 = both ? 0 : g.blocks;
         lo1 = g.key_lo; hi1 = g.key_hi;
         key1 = (g.key_lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS + half * 32;
@@ -297,14 +301,26 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       // ---- the copies.  Keys outside lo .. hi - 1 and of no page are filled with zeros.
       const uint32_t stage = ring + (uint32_t)s * L::KV_TILE;
       const bool inner = kb_now >= lo_now && kb_now + 32 <= hi_now;        // every key may be seen
-#pragma unroll 4
-      for (int j = 0; j < 32 / RPI; ++j) {
-        const int r = rp + RPI * j, key = kb_now + r;
-        const int id = __shfl_sync(0xffffffffu, ids_now, r >> bits);
-        const uint32_t bytes = (id >= 0 && (inner || (key >= lo_now && key < hi_now))) ? 16u : 0u;       // 0: sixteen zeros
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {            // eight rows at a time: they lie in one page
+        const int id = __shfl_sync(0xffffffffu, ids_now, (8 * e) >> bits), key = kb_now + 8 * e;
         const uint8_t* src = head_now + (size_t)max(id, 0) * page_stride + (uint32_t)(key & (ps - 1)) * (uint32_t)(D * 2);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                     ::"r"(stage + (uint32_t)r * 128u + (uint32_t)(((c & 7) ^ (r & 7)) << 4)), "l"(src), "r"(bytes) : "memory");
+        const uint32_t dst = stage + (uint32_t)e * 1024u;
+        if (inner) {
+          const uint32_t bytes = id >= 0 ? 16u : 0u;           // 0: sixteen zeros
+#pragma unroll
+          for (int u = 0; u < 8 / RPI; ++u)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                         ::"r"(dst + swizzled[u]), "l"(src + RPI * u * (D * 2)), "r"(bytes) : "memory");
+        } else {
+#pragma unroll
+          for (int u = 0; u < 8 / RPI; ++u) {
+            const int at = key + rp + RPI * u;
+            const uint32_t bytes = id >= 0 && at >= lo_now && at < hi_now ? 16u : 0u;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                         ::"r"(dst + swizzled[u]), "l"(src + RPI * u * (D * 2)), "r"(bytes) : "memory");
+          }
+        }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
       ++n;
@@ -319,7 +335,6 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         if (lane < 2 && ((used >> (2 * h + lane)) & 1u)) ta_mbar_arrive(full0 + 8u * (uint32_t)(lane * SC_BARS + h));
       }
     }
-    if (warp == 5) as_write_records(p, plan, cta, gridDim.x, lane, 32);    // while the last blocks are worked on
   } else if (warp == 1 || warp == 3) {
     // ---- products, one thread a tile -------------------------------------------------------------------------------------------------
     const int t = warp == 1 ? 0 : 1;
@@ -333,7 +348,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       ScPart g, other;
 #pragma unroll 1
       for (int seen = 0; ok && step(seen, t, g) && step(seen, t ^ 1, other); ++seen) {
-        const int all = g.kind == SC_BOTH ? g.blocks : g.blocks + other.blocks;
+        const int all = (g.kind & 3) == SC_BOTH ? g.blocks : g.blocks + other.blocks;
         if (g.blocks > 0) ok = sc_wait<false>(q_full(t), (uint32_t)(segments & 1), abort_flag, SC_ERR_Q);
         // S(i) = Q K(i)^T into S buffer (mine + i) & 1, then O += P V(i - 1): S(i + 1) overwrites P(i - 1), whose product the tensor cores finish first
 #pragma unroll 1
@@ -403,8 +418,8 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         if (r < g.tokens * G) *reinterpret_cast<float2*>(p.part_ml + (tile + g.tokens * G + r) * 2) = make_float2(-INFINITY, 0.f);
       }
       if (more) {
-        const int first = g.kind == SC_BOTH ? t * per : 0, lane_rows = min(g.tokens - first, per) * G;
-        folded = !g.shared && g.tokens * G <= AS_FOLD_ROWS;
+        const int first = (g.kind & 3) == SC_BOTH ? t * per : 0, lane_rows = min(g.tokens - first, per) * G;
+        folded = !(g.kind & SC_SHARED) && g.tokens * G <= AS_FOLD_ROWS;
         const int row = folded ? lane : r;     // of this tile's
         valid = row < lane_rows;
         warp_valid = folded || quarter * 32 < lane_rows;
@@ -414,10 +429,9 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         hi = 0x7fffffff;
         if (valid) {
           const int i = row / G;
-          int token, position;
-          as_token(plan, g.shared != 0, g.request, g.first + first + i, token, position);
-          from = token * p.heads + g.kv_head * G + (row - i * G);
-          hi = min(position + 1, g.key_hi);
+          const int2 token = as_token(p, g.kind & SC_SHARED, g.first, g.position, first + i);
+          from = token.x * p.heads + g.kv_head * G + (row - i * G);
+          hi = min(token.y + 1, g.key_hi);
         }
         hi_all = __reduce_min_sync(0xffffffffu, hi);
         constexpr int CHUNKS = D / 8, RPI = 32 / CHUNKS;
@@ -437,9 +451,9 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const volatile ScPart* was = &steps[done % SC_SEGMENTS].part[t];
-        const int tile_rows = was->tokens * G, kind = was->kind;
+        const int tile_rows = was->tokens * G, kind = was->kind & 3;
         const long long tile = (long long)(uint32_t)was->row_low | (long long)was->row_high << 32;
-        const bool fold = !was->shared && tile_rows <= AS_FOLD_ROWS;
+        const bool fold = !(was->kind & SC_SHARED) && tile_rows <= AS_FOLD_ROWS;
         const int first_row = kind == SC_BOTH ? t * per * G : 0, rows = fold ? 4 * tile_rows : kind == SC_BOTH ? tile_rows : 2 * tile_rows;
         const int in_tile = fold ? lane : r, left = min(tile_rows - first_row, per * G);             // this thread's row of the tile's `left`
         if (fold || quarter * 32 < left) {
@@ -622,7 +636,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
 template <int D>
 static cudaError_t sc_launch(const SharedParams& p, int ctas, cudaStream_t stream) {
   constexpr int smem = ScLayout<D>::BYTES + 1024;
-  static_assert(smem + sizeof(SharedPlan) + sizeof(ScStep) * SC_SEGMENTS + 64 <= 227 * 1024, "shared memory of a CTA");
+  static_assert(smem + sizeof(ScStep) * SC_SEGMENTS + 64 <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<unsigned long long> configured{0ull};     // a bit a device
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);

@@ -123,8 +123,9 @@ _SIGNATURES = {
     "lb_attention_tcgen05": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                              c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_longlong, c_void_p, c_float, c_int, c_void_p,
                              c_void_p],
-    "lb_attention_shared": [c_int] + [c_void_p] * 9 + [c_int] * 8 + [c_float, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p],
-    "lb_attention_shared_workspace": [c_int] * 7 + [c_void_p, c_void_p],
+    "lb_attention_shared": [c_int] + [c_void_p] * 6 + [c_longlong] + [c_int] * 8 + [c_float, c_void_p, c_longlong, c_void_p],
+    "lb_attention_shared_plan": [c_int, c_void_p, c_longlong] + [c_void_p] * 4 + [c_int] * 7 + [c_void_p],
+    "lb_attention_shared_sizes": [c_int] * 8 + [c_void_p, c_void_p],
     "lb_latent_flash": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                         c_float, c_void_p, c_int, c_int, c_void_p, c_longlong, c_void_p],
     "lb_latent_gather": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
@@ -219,7 +220,7 @@ def _check(t: torch.Tensor, what: str, dtype: torch.dtype | None = None) -> None
 
 def _on_current_device(t: torch.Tensor) -> None:
     """The library launches on the current device: a stream and pointers of another one are refused."""
-    if t.device.index != torch.cuda.current_device():
+    if t.get_device() != torch.cuda.current_device():
         raise KernelError(f"tensors on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
@@ -1475,60 +1476,84 @@ def _attention_workspace(device: torch.device, elems: int) -> torch.Tensor:
 
 
 @functools.lru_cache(maxsize=4096)
-def _shared_workspace(device: int, *sizes: int) -> tuple[int, int]:
-    """Elements of the workspaces of attention_shared on this device: float32, int32."""
-    floats, ints = c_longlong(0), c_longlong(0)
-    _call("lb_attention_shared_workspace", *sizes, ctypes.addressof(floats), ctypes.addressof(ints))
-    return floats.value, ints.value
+def _shared_sizes(device: int, *sizes: int) -> tuple[int, int]:
+    """Elements that attention_shared needs on this device: of a plan (int32), of partial results (float32)."""
+    ints, floats = c_longlong(0), c_longlong(0)
+    _call("lb_attention_shared_sizes", *sizes, ctypes.addressof(ints), ctypes.addressof(floats))
+    return ints.value, floats.value
+
+
+def _kept_for(stream: int, t: torch.Tensor) -> None:
+    """Tells torch's allocator that memory taken on the current stream is used on `stream`."""
+    if stream != torch.cuda.current_stream(t.device).cuda_stream:
+        t.record_stream(torch.cuda.ExternalStream(stream, device=t.device))
+
+
+def shared_plan(dtype: torch.dtype, num_tokens: int, cu_tokens: torch.Tensor, context_lens: torch.Tensor, prefix_of: torch.Tensor,
+                prefix_lens: torch.Tensor, num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int, pages_a_seq: int,
+                stream: int) -> torch.Tensor:
+    """What attention_shared has to know of a step of num_tokens tokens, made on the GPU from the requests' lengths and groups (its arguments of the same
+    names): once a step for all layers with these sizes.  Lengths and groups must not be written by the kernel of this library that is
+    launched right in front of this one (they are read while that may still run)."""
+    S = context_lens.shape[0]
+    for t, what, n in ((cu_tokens, "cu_tokens", S + 1), (context_lens, "context lengths", S), (prefix_of, "prefix_of", S), (prefix_lens, "prefix_lens", S)):
+        if not t.is_cuda or t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+            raise KernelError(f"{what} must be {n} int32 numbers on the GPU, is {tuple(t.shape)} of {t.dtype} on {t.device}")
+        if t.get_device() != cu_tokens.get_device():
+            raise KernelError(f"{what} is on {t.device}, cu_tokens on {cu_tokens.device}")
+    _on_current_device(cu_tokens)
+    dt = dtype_code(dtype)
+    sizes = (num_tokens, S, num_q_heads, num_kv_heads, head_dim, page_size, pages_a_seq)
+    n_ints, _ = _shared_sizes(cu_tokens.get_device(), dt, *sizes)
+    plan = cu_tokens.new_empty(n_ints)
+    _kept_for(stream, plan)
+    _call("lb_attention_shared_plan", dt, plan.data_ptr(), n_ints, cu_tokens.data_ptr(), context_lens.data_ptr(), prefix_of.data_ptr(),
+          prefix_lens.data_ptr(), *sizes, stream)
+    return plan
 
 
 def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                      cu_tokens: torch.Tensor, context_lens: torch.Tensor, prefix_of: torch.Tensor, prefix_lens: torch.Tensor, max_q_len: int,
-                     num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int, scale: float, stream: int) -> None:
+                     num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int, scale: float, stream: int,
+                     plan: torch.Tensor | None = None) -> None:
     """Causal attention of a step over paged keys and values, the keys that several requests share read once for all of them.
 
     q, out [T, heads, dim] (float32 or bfloat16); pools [pages, kv heads, page_size, dim]; block_table [S, pages a sequence],
     cu_tokens [S + 1] and context_lens [S] as in StepContext.  prefix_of[s] (int32 [S]) is the row of the batch whose block table
     holds the prefix that request s shares (its own row for that request itself, -1: none), prefix_lens[r] (int32 [S]) how many
     tokens the prefix of row r has: the first prefix_lens[prefix_of[s]] keys of s are read through that row's table, the others
-    through its own.  All of these are device values, read by the kernel, so that a recorded step is replayed with other groups and
-    lengths; `max_q_len` is the most tokens of a request.  Page ids outside the pool are not there: a row that sees no key gives
-    zeros, and rows of q that belong to no request (behind cu_tokens[S]) leave the output as it was.  S is at most 256, a head a multiple of
-    8 up to 256.  Partial results go through memory that the call
-    takes from torch's allocator on the current stream, so calls on several streams do not meet; a stream that is not the current
-    one is told to the allocator."""
-    _check(q, "q"); _check(out, "attention output", q.dtype); _check(k_cache, "k pool", q.dtype); _check(v_cache, "v pool", q.dtype)
+    through its own.  All of these are device values, read by the kernels, so that a recorded step is replayed with other groups and
+    lengths.  Page ids outside the pool are not there: a row that sees no key gives zeros, and rows of q that belong to no request
+    (behind cu_tokens[S]) leave the output as it was.  S is at most 512, a head a multiple of 8 up to 256, max_q_len the most tokens of a request.
+
+    `plan`: what shared_plan() made of these lengths, groups and sizes; without it the call makes one.  Partial results go through
+    memory that the call takes from torch's allocator, so calls on several streams do not meet."""
     T, S = q.shape[0], context_lens.shape[0]
-    for t, what, shape in ((cu_tokens, "cu_tokens", (S + 1,)), (context_lens, "context lengths", (S,)), (prefix_of, "prefix_of", (S,)),
-                           (prefix_lens, "prefix_lens", (S,))):
-        _check(t, what, torch.int32)
-        if tuple(t.shape) != shape:
-            raise KernelError(f"{what} is {tuple(t.shape)} for {S} requests")
-    _check(block_table, "block table", torch.int32)
+    if q.dim() != 3 or tuple(q.shape) != (T, num_q_heads, head_dim) or out.shape != q.shape:
+        raise KernelError(f"q is {tuple(q.shape)} and the output {tuple(out.shape)} for {num_q_heads} heads of {head_dim}")
+    if tuple(k_cache.shape[1:]) != (num_kv_heads, page_size, head_dim) or v_cache.shape != k_cache.shape:
+        raise KernelError(f"the pools are {tuple(k_cache.shape)} and {tuple(v_cache.shape)} for {num_kv_heads} heads of {head_dim} in pages of {page_size}")
     if block_table.dim() != 2 or block_table.shape[0] != S:
         raise KernelError(f"the block table is {tuple(block_table.shape)} for {S} requests")
-    if num_kv_heads <= 0 or num_q_heads % num_kv_heads:
-        raise KernelError(f"{num_q_heads} query heads are not a multiple of {num_kv_heads} kv heads")
-    if tuple(q.shape) != (T, num_q_heads, head_dim) or out.shape != q.shape:
-        raise KernelError(f"q is {tuple(q.shape)} and the output {tuple(out.shape)} for {num_q_heads} heads of {head_dim}")
-    if k_cache.dim() != 4 or tuple(k_cache.shape[1:]) != (num_kv_heads, page_size, head_dim) or v_cache.shape != k_cache.shape:
-        raise KernelError(f"the pools are {tuple(k_cache.shape)} and {tuple(v_cache.shape)} for {num_kv_heads} heads of {head_dim} in pages of {page_size}")
-    for t in (out, k_cache, v_cache, block_table, cu_tokens, context_lens, prefix_of, prefix_lens):
-        if t.device != q.device:
-            raise KernelError(f"operands on {q.device} and {t.device}")
+    device = q.get_device()
+    for t, what, dtype in ((q, "q", q.dtype), (out, "attention output", q.dtype), (k_cache, "k pool", q.dtype), (v_cache, "v pool", q.dtype),
+                           (block_table, "block table", torch.int32)):
+        _check(t, what, dtype)
+        if t.get_device() != device:
+            raise KernelError(f"{what} is on {t.device}, q on {q.device}")
     _on_current_device(q)
-    if T == 0 or S == 0:
-        return
+    P = block_table.shape[1]
+    if plan is None:
+        plan = shared_plan(q.dtype, T, cu_tokens, context_lens, prefix_of, prefix_lens, num_q_heads, num_kv_heads, head_dim, page_size, P, stream)
+    else:
+        _check(plan, "plan", torch.int32)
     dt = dtype_code(q.dtype)
-    n_floats, n_ints = _shared_workspace(q.device.index, T, S, num_q_heads, num_kv_heads, head_dim, dt, page_size)
+    _, n_floats = _shared_sizes(device, dt, T, S, num_q_heads, num_kv_heads, head_dim, page_size, P)
     floats = torch.empty(n_floats, dtype=torch.float32, device=q.device)
-    ints = torch.empty(n_ints, dtype=torch.int32, device=q.device)
-    if stream != torch.cuda.current_stream(q.device).cuda_stream:
-        other = torch.cuda.ExternalStream(stream, device=q.device)
-        floats.record_stream(other); ints.record_stream(other)
+    _kept_for(stream, floats)
     _call("lb_attention_shared", dt, q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-          cu_tokens.data_ptr(), context_lens.data_ptr(), prefix_of.data_ptr(), prefix_lens.data_ptr(), T, S, num_q_heads, num_kv_heads,
-          head_dim, page_size, k_cache.shape[0], block_table.shape[1], float(scale), floats.data_ptr(), n_floats, ints.data_ptr(), n_ints, stream)
+          plan.data_ptr(), plan.shape[0], T, S, num_q_heads, num_kv_heads, head_dim, page_size, k_cache.shape[0], P, float(scale),
+          floats.data_ptr(), n_floats, stream)
 
 
 def attention_flash_ok(q: torch.Tensor, num_q_heads: int, num_kv_heads: int, head_dim: int, v_dim: int = 0) -> bool:

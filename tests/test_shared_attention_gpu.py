@@ -260,9 +260,9 @@ def test_refusals(ops):
                 dict(page=8), dict(q=q.transpose(0, 1)), dict(out=out[:1]), dict(q=q.cpu())):
         with pytest.raises(ops.KernelError):
             call(**bad)
-    many = torch.zeros(300, dtype=torch.int32, device="cuda")
-    with pytest.raises(ops.KernelError, match="256"):
-        call(table=table[:1].expand(300, -1).contiguous(), cu=torch.zeros(301, dtype=torch.int32, device="cuda"), ctx=many, of=many, lens=many)
+    many = torch.zeros(600, dtype=torch.int32, device="cuda")
+    with pytest.raises(ops.KernelError, match="512"):
+        call(table=table[:1].expand(600, -1).contiguous(), cu=torch.zeros(601, dtype=torch.int32, device="cuda"), ctx=many, of=many, lens=many)
     wide = torch.empty(2, 1, 264, dtype=torch.bfloat16, device="cuda")
     pool = torch.empty(4, 1, 16, 264, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(ops.KernelError):

@@ -212,8 +212,13 @@ __global__ void __launch_bounds__(AS_PLAN_THREADS) as_plan_kernel(SharedParams p
 }
 
 static int as_sms() {
+  static std::atomic<int> known[64];                           // by device; 0: not asked yet
   int device = 0, n = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return 0;
+  std::atomic<int>& have = known[device & 63];
+  if (device < 64 && (n = have.load()) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
+  if (device < 64) have.store(n);
   return n;
 }
 
@@ -274,7 +279,9 @@ static bool as_params(SharedParams& p, SharedCut& cut, int& ctas, int dtype, int
   p.T = num_tokens; p.S = num_seqs; p.heads = num_q_heads; p.kv_heads = num_kv_heads * cut.share; p.group = cut.group; p.dim = head_dim;
   p.page_size = page_size; p.max_pages = max_pages; p.page_shift = -1; p.kv_share = cut.share;
   p.tile_tokens = cut.tile_tokens; p.lane_tokens = cut.lane_tokens;
-  p.min_span = cut.tc ? 4 : 1; p.tile_start = cut.tc ? 2 : 0; p.folds = cut.tc;
+  // Measured at 64 requests behind 8192 keys and at portions behind 2000 (us, recorded): tiles that cost nothing beside their blocks 44.8 and 46.4,
+  // 2 units 41.3 and 39.6, 3 units 39.7 and 38.6, 6 units 44.2 and 36.2.
+  p.min_span = cut.tc ? 5 : 1; p.tile_start = cut.tc ? 3 : 0; p.folds = cut.tc;
   for (int b = 0; b < 31; ++b) if ((1 << b) == page_size) p.page_shift = b;
   // units of the whole line, at most
   const long long tiles = 2ll * ((long long)num_tokens / p.tile_tokens + num_seqs), blocks = (long long)max_pages * page_size / AS_KEYS + 1;
@@ -305,6 +312,19 @@ LB_EXPORT int lb_attention_shared_sizes(int dtype, int num_tokens, int num_seqs,
   return 0;
 }
 
+static int as_plan(lb::SharedParams p, const lb::SharedCut& cut, int ctas, int* plan, long long num_ints, const int* cu_tokens, const int* context_lens,
+                   const int* prefix_of, const int* prefix_lens, cudaStream_t stream) {
+  const long long need = lb::SharedPlanLayout(p.T, p.S, p.kv_heads, p.tile_tokens, ctas).total;
+  LB_CHECK_ARG(plan && (uintptr_t)plan % 16 == 0 && num_ints >= need, "attention_shared: a plan of %lld integers at a 16-byte boundary is needed, got %lld", need, num_ints);
+  p.cu = cu_tokens; p.ctx = context_lens; p.prefix_of = prefix_of; p.prefix_lens = prefix_lens;
+  lb::as_plan_parts(p, plan, ctas);
+  const long long tasks = 2ll * p.S * p.kv_heads;
+  const int blocks = (int)(tasks < 32 * 64 ? (tasks + 63) / 64 : 32);        // few tasks a CTA: each is a chain of lookups
+  lb::launch(lb::as_plan_kernel, dim3(blocks), dim3(lb::AS_PLAN_THREADS), 0, stream, p, ctas);
+  LB_CHECK_LAUNCH("attention_shared plan");
+  return 0;
+}
+
 // The plan of a step for lb_attention_shared, from cu_tokens [S + 1], context_lens, prefix_of and prefix_lens [S], int32.
 LB_EXPORT int lb_attention_shared_plan(int dtype, int* plan, long long num_ints, const int* cu_tokens, const int* context_lens, const int* prefix_of,
                                        const int* prefix_lens, int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
@@ -314,21 +334,14 @@ LB_EXPORT int lb_attention_shared_plan(int dtype, int* plan, long long num_ints,
   int ctas = 0;
   if (!lb::as_params(p, cut, ctas, dtype, num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, max_pages)) return 1;
   if (num_tokens == 0 || num_seqs == 0) return 0;
-  const long long need = lb::SharedPlanLayout(num_tokens, num_seqs, p.kv_heads, p.tile_tokens, ctas).total;
-  LB_CHECK_ARG(plan && (uintptr_t)plan % 16 == 0 && num_ints >= need, "attention_shared: a plan of %lld integers at a 16-byte boundary is needed, got %lld", need, num_ints);
-  p.cu = cu_tokens; p.ctx = context_lens; p.prefix_of = prefix_of; p.prefix_lens = prefix_lens;
-  lb::as_plan_parts(p, plan, ctas);
-  const long long tasks = 2ll * num_seqs * p.kv_heads;
-  const int blocks = (int)(tasks < 32 * 64 ? (tasks + 63) / 64 : 32);        // few tasks a CTA: each is a chain of lookups
-  lb::launch(lb::as_plan_kernel, dim3(blocks), dim3(lb::AS_PLAN_THREADS), 0, stream, p, ctas);
-  LB_CHECK_LAUNCH("attention_shared plan");
-  return 0;
+  return as_plan(p, cut, ctas, plan, num_ints, cu_tokens, context_lens, prefix_of, prefix_lens, stream);
 }
 
-// q, out: [T, heads, dim]; k_cache, v_cache: [pages, kv heads, page_size, dim]; table [S, max_pages] int32; a plan made for these sizes.
-// floats: the partial results.  See attention_shared.cuh.
+// q, out: [T, heads, dim]; k_cache, v_cache: [pages, kv heads, page_size, dim]; table [S, max_pages] int32; a plan made for these sizes, or, with
+// cu_tokens (and the other three), memory for the plan that is made here.  floats: the partial results.  See attention_shared.cuh.
 LB_EXPORT int lb_attention_shared(int dtype, const void* q, void* out, const void* k_cache, const void* v_cache, const int* table, int* plan,
-                                  long long num_ints, int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+                                  long long num_ints, const int* cu_tokens, const int* context_lens, const int* prefix_of, const int* prefix_lens,
+                                  int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
                                   int num_pages, int max_pages, float scale, float* floats, long long num_floats, cudaStream_t stream) {
   lb::SharedParams p;
   lb::SharedCut cut;
@@ -344,6 +357,7 @@ LB_EXPORT int lb_attention_shared(int dtype, const void* q, void* out, const voi
   LB_CHECK_ARG(plan && floats && num_ints >= need && num_floats >= rows * (head_dim + 2),
                "attention_shared: a plan of %lld integers and a workspace of %lld floats are needed, got %lld and %lld", need, rows * (head_dim + 2),
                num_ints, num_floats);
+  if (cu_tokens && as_plan(p, cut, ctas, plan, num_ints, cu_tokens, context_lens, prefix_of, prefix_lens, stream)) return 2;
   p.q = q; p.out = out; p.k_cache = k_cache; p.v_cache = v_cache; p.table = table; p.num_pages = num_pages;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.part_o = floats; p.part_ml = floats + rows * head_dim;

@@ -25,9 +25,9 @@
 
 namespace lb {
 
-constexpr int SC_STAGES = 4;
+constexpr int SC_K_STAGES = 4, SC_V_STAGES = 5;                // a block of values stays until its keys' scores have become weights
 constexpr int SC_IN_FLIGHT = 2;                                // blocks a copying warp has requested beyond the one it waits for
-constexpr int SC_BARS = 4 * SC_STAGES + 8;                     // barriers of a tile
+constexpr int SC_BARS = 2 * (SC_K_STAGES + SC_V_STAGES) + 8;   // barriers of a tile
 constexpr int SC_THREADS = 448, SC_SOFTMAX = 6;                // the first of the softmax warps
 enum : int { SC_ERR_Q = 401, SC_ERR_KV_FULL = 402, SC_ERR_KV_EMPTY = 403, SC_ERR_S_FULL = 404, SC_ERR_P_FULL = 405, SC_ERR_O_FULL = 406, SC_ERR_O_FREE = 407, SC_ERR_SEGMENT = 408 };
 
@@ -37,7 +37,7 @@ template <int D> struct ScLayout {
   static constexpr int HALVES = D / 64;
   static constexpr int KV_HALF = AS_KEYS * 128, KV_TILE = HALVES * KV_HALF;
   static constexpr int Q_TILE = HALVES * TA_HALF_BYTES;
-  static constexpr int K_OFF = 2 * Q_TILE, V_OFF = K_OFF + SC_STAGES * KV_TILE, BAR_OFF = V_OFF + SC_STAGES * KV_TILE;
+  static constexpr int K_OFF = 2 * Q_TILE, V_OFF = K_OFF + SC_K_STAGES * KV_TILE, BAR_OFF = V_OFF + SC_V_STAGES * KV_TILE;
   static constexpr int BYTES = BAR_OFF + 2 * SC_BARS * 8 + 16;     // and the tensor memory's address and two flags
 };
 
@@ -109,14 +109,14 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   const uint32_t bars = sbase + L::BAR_OFF;
   // of tile t: keys (values) in stage s there, and read; of S buffer b: S complete, P written, P V complete; queries there, O read
   auto k_full = [&](int t, int s) { return bars + 8u * (t * SC_BARS + s); };
-  auto k_empty = [&](int t, int s) { return bars + 8u * (t * SC_BARS + SC_STAGES + s); };
-  auto v_full = [&](int t, int s) { return bars + 8u * (t * SC_BARS + 2 * SC_STAGES + s); };
-  auto v_empty = [&](int t, int s) { return bars + 8u * (t * SC_BARS + 3 * SC_STAGES + s); };
-  auto s_full = [&](int t, int b) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + b); };
-  auto p_full = [&](int t, int b) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + 2 + b); };
-  auto pv_done = [&](int t, int b) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + 4 + b); };
-  auto q_full = [&](int t) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + 6); };
-  auto o_free = [&](int t) { return bars + 8u * (t * SC_BARS + 4 * SC_STAGES + 7); };
+  auto k_empty = [&](int t, int s) { return bars + 8u * (t * SC_BARS + SC_K_STAGES + s); };
+  auto v_full = [&](int t, int s) { return bars + 8u * (t * SC_BARS + 2 * SC_K_STAGES + s); };
+  auto v_empty = [&](int t, int s) { return bars + 8u * (t * SC_BARS + 2 * SC_K_STAGES + SC_V_STAGES + s); };
+  auto s_full = [&](int t, int b) { return bars + 8u * (t * SC_BARS + SC_BARS - 8 + b); };
+  auto p_full = [&](int t, int b) { return bars + 8u * (t * SC_BARS + SC_BARS - 8 + 2 + b); };
+  auto pv_done = [&](int t, int b) { return bars + 8u * (t * SC_BARS + SC_BARS - 8 + 4 + b); };
+  auto q_full = [&](int t) { return bars + 8u * (t * SC_BARS + SC_BARS - 8 + 6); };
+  auto o_free = [&](int t) { return bars + 8u * (t * SC_BARS + SC_BARS - 8 + 7); };
   uint32_t* tmem_slot = (uint32_t*)(smem + L::BAR_OFF + 2 * SC_BARS * 8);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   volatile int* holes = (volatile int*)(tmem_slot + 2);       // some key of this CTA's segments lies in no page
@@ -125,10 +125,8 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
-      for (int i = 0; i < SC_STAGES; ++i) {
-        ta_mbar_init(k_full(t, i), 2); ta_mbar_init(k_empty(t, i), 1);     // two warps copy the halves of a block
-        ta_mbar_init(v_full(t, i), 2); ta_mbar_init(v_empty(t, i), 1);
-      }
+      for (int i = 0; i < SC_K_STAGES; ++i) { ta_mbar_init(k_full(t, i), 2); ta_mbar_init(k_empty(t, i), 1); }        // two warps copy the halves of a block
+      for (int i = 0; i < SC_V_STAGES; ++i) { ta_mbar_init(v_full(t, i), 2); ta_mbar_init(v_empty(t, i), 1); }
       for (int b = 0; b < 2; ++b) { ta_mbar_init(s_full(t, b), 1); ta_mbar_init(p_full(t, b), 4); ta_mbar_init(pv_done(t, b), 1); }
       ta_mbar_init(q_full(t), 4); ta_mbar_init(o_free(t), 4);
     }
@@ -176,7 +174,9 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     const uint32_t full0 = is_v ? v_full(0, 0) : k_full(0, 0), empty0 = is_v ? v_empty(0, 0) : k_empty(0, 0);
     const int ps = p.page_size, shift = p.page_shift, size = min(ps, 32), bits = min(shift, 5);
     const size_t page_stride = (size_t)p.kv_heads * ps * (D * 2);
+    const int stages = is_v ? SC_V_STAGES : SC_K_STAGES;
     int n = 0, handed = 0, seen = 0;           // blocks requested, handed over; steps looked at
+    int stage_n = 0, stage_h = 0;              // their stages
     uint32_t used = 0, turns = 0;              // bits 2 s + t: whether tile t reads stage s's block, and the parity of the next wait for it
     // (Of warp 0) the segment to come, fetched when the one before it was taken, and the one after it in the list.
     const int2 piece = __ldcg(p.pieces + cta);
@@ -275,21 +275,22 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       if (tiles_now == 0) continue;            // nothing at hand yet
       // ---- its stage: the tiles that read the last block there are through with it.  While that has to be waited for, whatever has been requested
       // is handed over; else the oldest block when SC_IN_FLIGHT are behind it.
-      const int s = n % SC_STAGES;
+      const int s = stage_n;
       const uint32_t before = (used >> (2 * s)) & 3u, bar = empty0 + 8u * (uint32_t)((lane & 1) * SC_BARS + s);
       const bool mine = lane < 2 && ((before >> lane) & 1u);
       const uint32_t parity = (turns >> (2 * s + (lane & 1))) & 1u;
       const bool wait = __any_sync(0xffffffffu, mine && !ta_mbar_try_wait(bar, parity));
-      const int keep = wait ? 0 : SC_IN_FLIGHT;
+      const int keep = wait ? 0 : n <= 2 ? 1 : SC_IN_FLIGHT;               // the first block is handed over early
       if (n - handed > keep) {
         if (wait) asm volatile("cp.async.wait_group 0;" ::: "memory");
+        else if (keep == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
         else asm volatile("cp.async.wait_group %0;" ::"n"(SC_IN_FLIGHT) : "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // visible to the tensor cores
         __syncwarp();
 #pragma unroll 1
         for (; n - handed > keep; ++handed) {
-          const int h = handed % SC_STAGES;
-          if (lane < 2 && ((used >> (2 * h + lane)) & 1u)) ta_mbar_arrive(full0 + 8u * (uint32_t)(lane * SC_BARS + h));
+          if (lane < 2 && ((used >> (2 * stage_h + lane)) & 1u)) ta_mbar_arrive(full0 + 8u * (uint32_t)(lane * SC_BARS + stage_h));
+          if (++stage_h == stages) stage_h = 0;
         }
       }
       if (wait) {
@@ -324,6 +325,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
       ++n;
+      if (++stage_n == stages) stage_n = 0;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -331,8 +333,8 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     if (ok) {
 #pragma unroll 1
       for (; handed < n; ++handed) {
-        const int h = handed % SC_STAGES;
-        if (lane < 2 && ((used >> (2 * h + lane)) & 1u)) ta_mbar_arrive(full0 + 8u * (uint32_t)(lane * SC_BARS + h));
+        if (lane < 2 && ((used >> (2 * stage_h + lane)) & 1u)) ta_mbar_arrive(full0 + 8u * (uint32_t)(lane * SC_BARS + stage_h));
+        if (++stage_h == stages) stage_h = 0;
       }
     }
   } else if (warp == 1 || warp == 3) {
@@ -354,7 +356,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
 #pragma unroll 1
         for (int i = 0; i <= g.blocks && g.blocks > 0 && ok; ++i) {
           if (i < g.blocks) {
-            const int s = (n0 + place(t, i, other.blocks, g.kind)) % SC_STAGES, b = (mine + i) & 1;
+            const int s = (n0 + place(t, i, other.blocks, g.kind)) % SC_K_STAGES, b = (mine + i) & 1;
             ok = sc_wait<false>(k_full(t, s), (k_turn >> s) & 1u, abort_flag, SC_ERR_KV_FULL);
             if (!ok) break;
             k_turn ^= 1u << s;
@@ -368,7 +370,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
             ta_commit(k_empty(t, s));
           }
           if (i > 0) {
-            const int h = i - 1, s = (n0 + place(t, h, other.blocks, g.kind)) % SC_STAGES, b = (mine + h) & 1;
+            const int h = i - 1, s = (n0 + place(t, h, other.blocks, g.kind)) % SC_V_STAGES, b = (mine + h) & 1;
             ok = sc_wait<false>(v_full(t, s), (v_turn >> s) & 1u, abort_flag, SC_ERR_KV_FULL);
             if (ok && h == 0 && segments > 0) ok = sc_wait<false>(o_free(t), (uint32_t)((segments - 1) & 1), abort_flag, SC_ERR_O_FREE);
             ok = ok && sc_wait<false>(p_full(t, b), (uint32_t)(((mine + h) >> 1) & 1), abort_flag, SC_ERR_P_FULL);
@@ -445,7 +447,13 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
                            "l"((const uint8_t*)p.q + (size_t)row_at * (D * 2) + c * 16) : "memory");
         }
       }
-      // ---- the part before it is complete meanwhile: its result is written
+      if (more) {                              // all products with the last part's queries are done: S of this part may come while that one's O is read
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) ta_mbar_arrive(q_full(t));
+      }
+      // ---- the part before it: its result is written
       if (done >= 0) {
         ok = sc_wait<false>(pv_done(t, (mine - 1) & 1), (uint32_t)(((mine - 1) >> 1) & 1), abort_flag, SC_ERR_O_FULL);
         if (!ok) break;
@@ -478,10 +486,6 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       }
       if (!more) break;
       done = at_step;
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) ta_mbar_arrive(q_full(t));
       // ---- its blocks
       m_ref = -INFINITY;
       l_run = 0.f;

@@ -123,7 +123,7 @@ _SIGNATURES = {
     "lb_attention_tcgen05": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                              c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_longlong, c_void_p, c_float, c_int, c_void_p,
                              c_void_p],
-    "lb_attention_shared": [c_int] + [c_void_p] * 6 + [c_longlong] + [c_int] * 8 + [c_float, c_void_p, c_longlong, c_void_p],
+    "lb_attention_shared": [c_int] + [c_void_p] * 6 + [c_longlong] + [c_void_p] * 4 + [c_int] * 8 + [c_float, c_void_p, c_longlong, c_void_p],
     "lb_attention_shared_plan": [c_int, c_void_p, c_longlong] + [c_void_p] * 4 + [c_int] * 7 + [c_void_p],
     "lb_attention_shared_sizes": [c_int] * 8 + [c_void_p, c_void_p],
     "lb_latent_flash": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
@@ -225,7 +225,8 @@ def _on_current_device(t: torch.Tensor) -> None:
 
 
 def current_stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The raw handle of torch's current stream on the current device (without the object that torch.cuda.current_stream() makes)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def embedding(out: torch.Tensor, ids: torch.Tensor, table: torch.Tensor, stream: int,
@@ -1006,15 +1007,13 @@ def sample(tokens: torch.Tensor, logits: torch.Tensor, stream: int, temperature:
     R, V = logits.shape
     if temperature is not None and (keys is None or counters is None):
         raise KernelError("a draw with temperature needs keys and counters")
+    device = logits.get_device()
     for t, what, dtype in ((tokens, "token output", torch.int32), (temperature, "temperature", torch.float32), (keys, "keys", torch.int64),
                            (counters, "counters", torch.int32), (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
                            (min_p, "min_p", torch.float32)):
-        if t is not None:
+        if t is not None and (t.dtype != dtype or t.shape != (R,) or t.get_device() != device or not t.is_contiguous()):
             _check(t, what, dtype)
-            if t.shape != (R,):
-                raise KernelError(f"{what} must be one number a row of {R}, is {tuple(t.shape)}")
-            if t.device != logits.device:
-                raise KernelError(f"{what} is on {t.device}, the logits on {logits.device}")
+            raise KernelError(f"{what} must be one number a row of {R} on {logits.device}, is {tuple(t.shape)} on {t.device}")
     _on_current_device(logits)
     _call("lb_sample_filtered", tokens.data_ptr(), logits.data_ptr(), logits.stride(0) if R > 1 else max(V, 1), _ptr(temperature), _ptr(keys),
           _ptr(counters), _ptr(top_k), _ptr(top_p), _ptr(min_p), R, V, stream)
@@ -1485,8 +1484,15 @@ def _shared_sizes(device: int, *sizes: int) -> tuple[int, int]:
 
 def _kept_for(stream: int, t: torch.Tensor) -> None:
     """Tells torch's allocator that memory taken on the current stream is used on `stream`."""
-    if stream != torch.cuda.current_stream(t.device).cuda_stream:
+    if stream != torch._C._cuda_getCurrentRawStream(t.get_device()):
         t.record_stream(torch.cuda.ExternalStream(stream, device=t.device))
+
+
+def _check_lengths(device: int, S: int, *lengths: torch.Tensor) -> None:
+    """cu_tokens, context lengths, prefix_of, prefix_lens of S requests."""
+    for t, what, n in zip(lengths, ("cu_tokens", "context lengths", "prefix_of", "prefix_lens"), (S + 1, S, S, S)):
+        if t.dtype != torch.int32 or t.get_device() != device or t.shape != (n,) or not t.is_contiguous():
+            raise KernelError(f"{what} must be {n} int32 numbers on cuda:{device}, is {tuple(t.shape)} of {t.dtype} on {t.device}")
 
 
 def shared_plan(dtype: torch.dtype, num_tokens: int, cu_tokens: torch.Tensor, context_lens: torch.Tensor, prefix_of: torch.Tensor,
@@ -1496,11 +1502,9 @@ def shared_plan(dtype: torch.dtype, num_tokens: int, cu_tokens: torch.Tensor, co
     names): once a step for all layers with these sizes.  Lengths and groups must not be written by the kernel of this library that is
     launched right in front of this one (they are read while that may still run)."""
     S = context_lens.shape[0]
-    for t, what, n in ((cu_tokens, "cu_tokens", S + 1), (context_lens, "context lengths", S), (prefix_of, "prefix_of", S), (prefix_lens, "prefix_lens", S)):
-        if not t.is_cuda or t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-            raise KernelError(f"{what} must be {n} int32 numbers on the GPU, is {tuple(t.shape)} of {t.dtype} on {t.device}")
-        if t.get_device() != cu_tokens.get_device():
-            raise KernelError(f"{what} is on {t.device}, cu_tokens on {cu_tokens.device}")
+    if not cu_tokens.is_cuda:
+        raise KernelError("cu_tokens must be on the GPU")
+    _check_lengths(cu_tokens.get_device(), S, cu_tokens, context_lens, prefix_of, prefix_lens)
     _on_current_device(cu_tokens)
     dt = dtype_code(dtype)
     sizes = (num_tokens, S, num_q_heads, num_kv_heads, head_dim, page_size, pages_a_seq)
@@ -1526,34 +1530,40 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     lengths.  Page ids outside the pool are not there: a row that sees no key gives zeros, and rows of q that belong to no request
     (behind cu_tokens[S]) leave the output as it was.  S is at most 512, a head a multiple of 8 up to 256, max_q_len the most tokens of a request.
 
-    `plan`: what shared_plan() made of these lengths, groups and sizes; without it the call makes one.  Partial results go through
-    memory that the call takes from torch's allocator, so calls on several streams do not meet."""
-    T, S = q.shape[0], context_lens.shape[0]
-    if q.dim() != 3 or tuple(q.shape) != (T, num_q_heads, head_dim) or out.shape != q.shape:
+    `plan`: what shared_plan() made of these lengths, groups and sizes; without it the call makes one (see there for when lengths and
+    groups may be written).  Partial results go through memory that the call takes from torch's allocator, so calls on several
+    streams do not meet."""
+    T, S, P = q.shape[0], context_lens.shape[0], block_table.shape[-1]
+    device, dtype = q.get_device(), q.dtype
+    if q.shape != (T, num_q_heads, head_dim) or out.shape != q.shape:
         raise KernelError(f"q is {tuple(q.shape)} and the output {tuple(out.shape)} for {num_q_heads} heads of {head_dim}")
-    if tuple(k_cache.shape[1:]) != (num_kv_heads, page_size, head_dim) or v_cache.shape != k_cache.shape:
+    if k_cache.shape[1:] != (num_kv_heads, page_size, head_dim) or v_cache.shape != k_cache.shape:
         raise KernelError(f"the pools are {tuple(k_cache.shape)} and {tuple(v_cache.shape)} for {num_kv_heads} heads of {head_dim} in pages of {page_size}")
-    if block_table.dim() != 2 or block_table.shape[0] != S:
+    if block_table.shape != (S, P):
         raise KernelError(f"the block table is {tuple(block_table.shape)} for {S} requests")
-    device = q.get_device()
-    for t, what, dtype in ((q, "q", q.dtype), (out, "attention output", q.dtype), (k_cache, "k pool", q.dtype), (v_cache, "v pool", q.dtype),
-                           (block_table, "block table", torch.int32)):
-        _check(t, what, dtype)
-        if t.get_device() != device:
+    for t, what, of in ((q, "q", dtype), (out, "attention output", dtype), (k_cache, "k pool", dtype), (v_cache, "v pool", dtype),
+                        (block_table, "block table", torch.int32)):
+        if t.dtype != of or t.get_device() != device or not t.is_contiguous():
+            _check(t, what, of)
             raise KernelError(f"{what} is on {t.device}, q on {q.device}")
+    if device < 0:
+        raise KernelError("q must be on the GPU")
     _on_current_device(q)
-    P = block_table.shape[1]
+    dt = dtype_code(dtype)
+    n_ints, n_floats = _shared_sizes(device, dt, T, S, num_q_heads, num_kv_heads, head_dim, page_size, P)
     if plan is None:
-        plan = shared_plan(q.dtype, T, cu_tokens, context_lens, prefix_of, prefix_lens, num_q_heads, num_kv_heads, head_dim, page_size, P, stream)
+        _check_lengths(device, S, cu_tokens, context_lens, prefix_of, prefix_lens)
+        lengths = cu_tokens.data_ptr(), context_lens.data_ptr(), prefix_of.data_ptr(), prefix_lens.data_ptr()
+        n_floats = (n_floats + 3) & ~3                     # the plan lies behind the partial results
+        floats = torch.empty(n_floats + n_ints, dtype=torch.float32, device=q.device)
+        plan_at = floats.data_ptr() + 4 * n_floats
     else:
         _check(plan, "plan", torch.int32)
-    dt = dtype_code(q.dtype)
-    _, n_floats = _shared_sizes(device, dt, T, S, num_q_heads, num_kv_heads, head_dim, page_size, P)
-    floats = torch.empty(n_floats, dtype=torch.float32, device=q.device)
+        lengths, plan_at, n_ints = (None, None, None, None), plan.data_ptr(), plan.shape[0]
+        floats = torch.empty(n_floats, dtype=torch.float32, device=q.device)
     _kept_for(stream, floats)
-    _call("lb_attention_shared", dt, q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-          plan.data_ptr(), plan.shape[0], T, S, num_q_heads, num_kv_heads, head_dim, page_size, k_cache.shape[0], P, float(scale),
-          floats.data_ptr(), n_floats, stream)
+    _call("lb_attention_shared", dt, q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), plan_at, n_ints,
+          *lengths, T, S, num_q_heads, num_kv_heads, head_dim, page_size, k_cache.shape[0], P, float(scale), floats.data_ptr(), n_floats, stream)
 
 
 def attention_flash_ok(q: torch.Tensor, num_q_heads: int, num_kv_heads: int, head_dim: int, v_dim: int = 0) -> bool:

@@ -67,6 +67,8 @@ class _RequestCache:
     tables: list[list[int]]          # per group: page of each logical page index, NO_PAGE once released
     length: int = 0                  # tokens whose keys are (or are about to be) in the cache
     version: int = 0                 # new, manager-wide unique number whenever a table changes (lets callers cache a converted copy)
+    family: int = 0                  # requests with the same number (not 0) have their first pages in common,
+    common: int = 0                  # this one so many of them with the family's first (-1: it is the first, all)
 
 
 class CacheManager:
@@ -79,6 +81,7 @@ class CacheManager:
         self._free_slots = list(range(num_slots - 1, -1, -1))
         self._requests: dict[Hashable, _RequestCache] = {}
         self._versions = 0
+        self._families = 0
 
     # ---- requests ------------------------------------------------------
     def has_request(self, rid: Hashable) -> bool:
@@ -106,6 +109,61 @@ class CacheManager:
                 if p != NO_PAGE:
                     self.pools[g].free(p)
         self._free_slots.append(rc.slot)
+
+    # ---- requests that begin alike ------------------------------------------
+    def can_share(self) -> bool:
+        """Whether requests may hold pages in common: every group keeps one entry for every token to the end, and nothing else is kept."""
+        return bool(self.groups) and all(g.window <= 0 and g.every <= 1 for g in self.groups)
+
+    def share_prefix(self, rid: Hashable, donor: Hashable, pages: int) -> None:
+        """The first `pages` pages of `donor`, which hold computed tokens, become the first of `rid`, which has been admitted and
+        has none yet: its length is that many pages then."""
+        if not self.can_share():
+            raise PagePoolError("requests of these cache groups cannot hold pages in common")
+        rc, dc = self._requests[rid], self._requests[donor]
+        if rc.length or any(rc.tables) or rid == donor:
+            raise PagePoolError(f"request {rid!r} cannot take over pages: it has some")
+        if not 0 < pages <= dc.length // self.page_size:
+            raise PagePoolError(f"{pages} pages of request {donor!r}, which has filled {dc.length // self.page_size}")
+        for g, table in enumerate(dc.tables):
+            for p in table[:pages]:
+                self.pools[g].share(p)
+            rc.tables[g].extend(table[:pages])
+        if not dc.family:
+            self._families += 1
+            dc.family, dc.common = self._families, -1
+        rc.family, rc.common = dc.family, pages if dc.common < 0 else min(pages, dc.common)
+        rc.length = pages * self.page_size
+        self._versions += 1
+        rc.version = self._versions
+
+    def prefix_groups(self, rids: Sequence[Hashable]) -> Optional[tuple[list[int], list[int]]]:
+        """Which of these requests begin with the same pages: for each the place in the list of the request whose pages stand for
+        its group's (-1: no group), and for that one how many tokens the group has in common (0 for the others).  Of a family's
+        requests those form a group for which (members x common pages) is largest.  None when there is no group."""
+        families: dict[int, list[int]] = {}
+        for i, rid in enumerate(rids):
+            rc = self._requests.get(rid)
+            if rc is not None and rc.family:
+                families.setdefault(rc.family, []).append(i)
+        found: Optional[tuple[list[int], list[int]]] = None
+        for members in families.values():
+            if len(members) < 2:
+                continue
+            whole = max(self._requests[rids[i]].length // self.page_size for i in members)
+            common = {i: whole if self._requests[rids[i]].common < 0 else self._requests[rids[i]].common for i in members}
+            # the family's first request has as many pages in common as anybody else has with it: cut where another's end
+            cuts = sorted({common[i] for i in members if self._requests[rids[i]].common >= 0})
+            pages = max(cuts, key=lambda c: sum(common[i] >= c for i in members) * c if sum(common[i] >= c for i in members) > 1 else 0)
+            group = [i for i in members if common[i] >= pages]
+            if len(group) < 2:
+                continue
+            if found is None:
+                found = [-1] * len(rids), [0] * len(rids)
+            for i in group:
+                found[0][i] = group[0]
+            found[1][group[0]] = pages * self.page_size
+        return found
 
     # ---- pages ---------------------------------------------------------
     def _first_needed_page(self, g: int, start: int) -> int:
@@ -225,16 +283,17 @@ class CacheManager:
         return len(self._requests)
 
     def check_invariants(self) -> None:
-        """No page lost, none held twice: every page is free or in exactly one table."""
+        """No page lost, none held twice: every page is free or in as many tables as it has holders, at the same place in all of them."""
         for g, pool in enumerate(self.pools):
-            seen: set[int] = set()
+            places: dict[int, list[int]] = {}
             for rid, rc in self._requests.items():
-                for p in rc.tables[g]:
-                    if p == NO_PAGE:
-                        continue
-                    if p in seen:
-                        raise PagePoolError(f"page {p} of group {g} is held twice")
-                    seen.add(p)
+                for i, p in enumerate(rc.tables[g]):
+                    if p != NO_PAGE:
+                        places.setdefault(p, []).append(i)
+            for p, at in places.items():
+                if len(at) != pool.holders(p) or len(set(at)) > 1:
+                    raise PagePoolError(f"page {p} of group {g} is held twice ({len(at)} tables, {pool.holders(p)} holders)")
+            seen = set(places)
             free = set(pool._free)
             if len(free) != len(pool._free):
                 raise PagePoolError(f"group {g}: a page is twice in the free list")

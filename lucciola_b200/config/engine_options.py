@@ -25,6 +25,8 @@ class EngineOptions:
     use_cuda_graph: bool = True        # record steps whose shape comes again as CUDA graphs and replay them
     graph_after: int = 2               # a step with portions of prompts is recorded when its shape has come this often
     max_shape_graphs: int = 32         # recordings of steps with portions kept at a time (least recently used goes)
+    share_prefixes: bool = False       # a request whose tokens begin like a running one's takes over the pages they have in common,
+                                       # and attention reads such pages once for all requests of a step that have them
     device: str = "cuda:0"
 
     def validate(self) -> None:

@@ -41,7 +41,7 @@ class Engine:
         self.options = runner.options
         self.scheduler = Scheduler(runner.manager, self.options.max_tokens_per_step, self.options.max_num_seqs,
                                    runner.max_model_len, self.options.prefill_chunk, runner.model.eos_token_ids,
-                                   release=runner.finish, token_tile=self.options.token_tile)
+                                   release=runner.finish, token_tile=self.options.token_tile, share_prefixes=self.options.share_prefixes)
         self.sampler = Sampler(runner.device)
         self._next_id = 1
         self._live: dict[int, Request] = {}              # requests that have not finished, by id
@@ -158,6 +158,7 @@ class Engine:
         sch = self.scheduler
         pools = self.runner.manager.pools
         return {"steps": sch.num_steps, "scheduled_tokens": sch.num_scheduled_tokens, "preemptions": sch.num_preemptions,
+                "shared_tokens": sch.num_shared_tokens,
                 "waiting": len(sch.waiting), "running": len(sch.running),
                 "free_pages": min(p.num_free for p in pools) if pools else 0,
                 "page_high_water": max(p.high_water for p in pools) if pools else 0}

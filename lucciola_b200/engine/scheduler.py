@@ -16,6 +16,9 @@ What it decides differently:
     generated, so its output is the same as without the preemption.  (lucciola moves such a
     request to a queue that nothing reads again, src/scheduler.cc:33-40: the request is lost.)
   * A request that could never fit the pool on its own is refused when it is added.
+  * With `share_prefixes` set, a request that is admitted while a running one begins with the same tokens takes over the whole pages
+    of these that have been computed (all but its last token, at most) and starts behind them.  While the running one is still
+    computing tokens that both begin with, the request waits for them.
   * With `token_tile` set, a portion that is not its prompt's last is shortened so that the step's tokens up to and
     including it are a multiple of the tile: the many-token products work on tiles of 128 tokens, and 32 decoded tokens
     beside a portion of 512 make them compute five tiles for 4.25 tiles of tokens.
@@ -41,7 +44,7 @@ class Scheduled:
 class Scheduler:
     def __init__(self, manager: CacheManager, max_tokens_per_step: int, max_num_seqs: int, max_model_len: int,
                  prefill_chunk: int = 0, eos_token_ids: Iterable[int] = (),
-                 release: Optional[Callable[[Hashable], None]] = None, token_tile: int = 0):
+                 release: Optional[Callable[[Hashable], None]] = None, token_tile: int = 0, share_prefixes: bool = False):
         """`release(rid)` gives back all that a request holds; whoever keeps more per request than the cache
         manager does (the runner's converted block tables) passes its own."""
         self.manager = manager
@@ -51,6 +54,7 @@ class Scheduler:
         self.max_model_len = max_model_len
         self.prefill_chunk = prefill_chunk
         self.token_tile = token_tile
+        self.share_prefixes = share_prefixes
         self.eos_token_ids = frozenset(eos_token_ids)
         self.waiting: deque[Request] = deque()
         self.running: list[Request] = []
@@ -59,6 +63,7 @@ class Scheduler:
         self.num_preemptions = 0
         self.num_steps = 0
         self.num_scheduled_tokens = 0
+        self.num_shared_tokens = 0             # tokens that were taken over instead of computed
 
     # ---- requests ----------------------------------------------------------
     def add_request(self, req: Request) -> None:
@@ -142,6 +147,38 @@ class Scheduler:
             self.running.remove(r)
         r.status, r.finish_reason = Status.FINISHED, reason
 
+    # ---- requests that begin alike ---------------------------------------------
+    @staticmethod
+    def _alike(a: Sequence[int], b: Sequence[int]) -> int:
+        """With how many equal tokens both begin."""
+        n = min(len(a), len(b))
+        if a[:n] == b[:n]:
+            return n
+        lo, hi = 0, n                          # a[:lo] == b[:lo], a[:hi] != b[:hi]
+        while hi - lo > 1:
+            mid = (lo + hi) // 2
+            if a[lo:mid] == b[lo:mid]:
+                lo = mid
+            else:
+                hi = mid
+        return lo
+
+    def _donor(self, r: Request) -> tuple[Optional[Request], int, bool]:
+        """The running request with which r has the most whole pages in common that have been computed, how many, and whether another
+        one is still computing more."""
+        ps = self.manager.page_size
+        best, pages, more = None, 0, 0
+        for d in self.running:
+            if d.tokens[0] != r.tokens[0]:
+                continue
+            alike = min(self._alike(r.tokens, d.tokens), r.length - 1)
+            have = min(alike, d.num_computed) // ps
+            if have > pages:
+                best, pages = d, have
+            if d.remaining > 1:
+                more = max(more, alike // ps)
+        return best, pages, more > pages
+
     # ---- one step ------------------------------------------------------------
     def schedule(self) -> list[Scheduled]:
         """The batch of the next step.  Empty only when there is nothing to do."""
@@ -213,8 +250,19 @@ class Scheduler:
         # before a preemption) are free now: admitting it earlier would only get it preempted again.
         while self.waiting and not blocked and budget > 0 and len(self.running) < self.max_num_seqs:
             r = self.waiting[0]
-            if not self._fits(self._pages_needed(r, r.length), reserved):
+            donor, pages = None, 0
+            if self.share_prefixes and self.running:
+                donor, pages, more = self._donor(r)
+                if more:
+                    break
+            need = self._pages_needed(r, r.length)
+            if not self._fits([k - pages for k in need], reserved):
                 break
+            if donor is not None:
+                self.manager.admit(r.rid)
+                self.manager.share_prefix(r.rid, donor.rid, pages)
+                r.num_computed = pages * self.manager.page_size
+                self.num_shared_tokens += r.num_computed
             most = min(budget, self.prefill_chunk or budget, r.remaining)
             n = self._aligned(most, r, budget)
             self.waiting.popleft()

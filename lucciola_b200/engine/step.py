@@ -138,6 +138,8 @@ class ModelRunner:
         self.cache = DeviceCache(requests, self.groups, self.page_size, counts, options.max_num_seqs, rt.act_dtype, self.device)
         self.max_pages_per_seq = -(-self.max_model_len // self.page_size)
         self._any_window = any(g.window > 0 for g in self.groups)
+        if options.share_prefixes and (self.state_cache_ids or not self.manager.can_share()):
+            raise ValueError("share_prefixes needs a model that keeps the keys and values of all tokens, and nothing else, of a request")
         self._arange_cache = np.arange(512, dtype=np.int32)
         # The parts that plan work on the host for every step: one for each distinct key.
         self._planners: dict[Hashable, object] = {}
@@ -369,7 +371,11 @@ class ModelRunner:
         max_ctx = max(s + n for s, n in zip(starts, q_lens))
         # A step that is recorded, or replayed from a recording, is padded: behind its leading single tokens come
         # entries that own no page (their keys and values are written nowhere and they attend to nothing).
+        # Requests that begin with the same pages; steps with and without such are recorded apart.
+        shared = self.manager.prefix_groups([e.rid for e in entries]) if self.options.share_prefixes else None
         shape = self._shape_of(entries, q_lens, max_ctx)
+        if shape is not None and shared:
+            shape += ("shared",)
         if shape is not None and not self._record_now(shape):
             shape = None
         lead = pad = 0
@@ -402,7 +408,7 @@ class ModelRunner:
             if plan is not None:
                 made[key] = plan
         has_state = bool(self.cache.states)
-        total = 3 * T + (S + 1) + 3 * S + R + G * S * P + sum(a.size + 3 for p in made.values() for a in p.arrays.values())
+        total = 3 * T + (S + 1) + 3 * S + R + G * S * P + (2 * S if shared else 0) + sum(a.size + 3 for p in made.values() for a in p.arrays.values())
         st = self._staging_for(total)
         hi, _ = st.next_host()
         h = st.host_np[hi]
@@ -415,6 +421,11 @@ class ModelRunner:
         tok, pos, seq = take(T), take(T), take(T)
         cu, ctx, slots, fresh, rows = take(S + 1), take(S), take(S), take(S), take(R)
         tables = [take(S * P).reshape(S, P) for _ in range(G)]
+        if shared:
+            of, lens = take(S), take(S)
+            of[:], lens[:] = -1, 0
+            for i, (leader, n) in enumerate(zip(*shared)):
+                of[place(i)], lens[place(i)] = place(leader) if leader >= 0 else -1, n
         for plan in made.values():
             for a in plan.arrays.values():
                 o = (o + 3) & ~3                      # kernels read a work item as one 16-byte word
@@ -510,6 +521,7 @@ class ModelRunner:
         d_tok, d_pos, d_seq = view(T), view(T), view(T)
         d_cu, d_ctx, d_slots, d_fresh, d_rows = view(S + 1), view(S), view(S), view(S), view(R)
         d_tables = [view(S * P).view(S, P) for _ in range(G)]
+        d_of, d_lens = (view(S), view(S)) if shared else (None, None)
         plans: dict[Hashable, PlanView] = {}
         for key, plan in made.items():
             arrays = {}
@@ -521,7 +533,8 @@ class ModelRunner:
         step = StepContext(
             num_tokens=T, num_seqs=S, positions=d_pos, token_seq=d_seq, cu_tokens=d_cu, context_lens=d_ctx,
             block_tables=d_tables, state_slots=d_slots, q_lens=q_lens, start_positions=starts,
-            max_q_len=batch.max_q_len, max_context_len=max_ctx, span_hint=batch.span_hint, plans=plans, token_ids=d_tok)
+            max_q_len=batch.max_q_len, max_context_len=max_ctx, span_hint=batch.span_hint, plans=plans, token_ids=d_tok,
+            prefix_of=d_of, prefix_lens=d_lens)
         self.rt.stream = self._stream()
         d_rows = d_rows if R else None
         d_fresh = d_fresh if has_state and (new_slots or shape is not None) else None

@@ -1495,6 +1495,11 @@ def _check_lengths(device: int, S: int, *lengths: torch.Tensor) -> None:
             raise KernelError(f"{what} must be {n} int32 numbers on cuda:{device}, is {tuple(t.shape)} of {t.dtype} on {t.device}")
 
 
+def attention_shared_ok(num_seqs: int, head_dim: int, scale: float) -> bool:
+    """The sizes that attention_shared takes."""
+    return num_seqs <= 512 and head_dim % 8 == 0 and 0 < head_dim <= 256 and scale > 0
+
+
 def shared_plan(dtype: torch.dtype, num_tokens: int, cu_tokens: torch.Tensor, context_lens: torch.Tensor, prefix_of: torch.Tensor,
                 prefix_lens: torch.Tensor, num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int, pages_a_seq: int,
                 stream: int) -> torch.Tensor:

@@ -155,6 +155,22 @@ class GQAttention(Mixer):
             return self.o.forward_into(out, sink)
         return self.o.forward(out)
 
+    def _attend(self, q: torch.Tensor, out: torch.Tensor, step: StepContext, cache: KVCacheView) -> None:
+        """The attention of the step's queries: where requests begin with the same pages, these are read once for all of them."""
+        nq, nkv, d = self.num_heads, self.num_kv_heads, self.head_dim
+        if step.prefix_of is not None and self.window == 0 and ops.attention_shared_ok(step.num_seqs, d, self.scale):
+            table = step.block_tables[cache.group]
+            key = ("shared prefixes", nq, nkv, d, cache.page_size, cache.group)       # one plan for all layers with these sizes
+            plan = step.memo.get(key)
+            if plan is None:
+                plan = step.memo[key] = ops.shared_plan(q.dtype, q.shape[0], step.cu_tokens, step.context_lens, step.prefix_of, step.prefix_lens,
+                                                        nq, nkv, d, cache.page_size, table.shape[1], self.rt.stream)
+            ops.attention_shared(q, out, cache.k, cache.v, table, step.cu_tokens, step.context_lens, step.prefix_of, step.prefix_lens,
+                                 step.max_q_len, nq, nkv, d, cache.page_size, self.scale, self.rt.stream, plan=plan)
+            return
+        ops.attention(q, out, cache.k, cache.v, step, cache.group, nq, nkv, d, cache.page_size, self.window,
+                      self.scale, self.rt.stream, plan=step.plans.get(self.plan_key()))
+
     def forward(self, h, step: StepContext, cache: KVCacheView, write_cache: bool = True, sink: Optional[NormSink] = None):
         rt = self.rt
         T = h.shape[0]
@@ -173,8 +189,7 @@ class GQAttention(Mixer):
                                    inv_freq=rotary[0] if rotary is not None else None,
                                    sumsq=scaled.sumsq if scaled is not None else None, row_eps=scaled.eps if scaled is not None else 0.0)
             out = rt.empty((T, nq, d))
-            ops.attention(q, out, cache.k, cache.v, step, cache.group, nq, nkv, d, cache.page_size, self.window,
-                          self.scale, rt.stream, plan=step.plans.get(self.plan_key()))
+            self._attend(q, out, step, cache)
             return self._project_out(out.view(T, self.q_size), sink)
         if scaled is not None and not self.qkv.row_scaled_ok(T):
             raise ops.KernelError("this mixer was handed rows without their norm factor for a step it cannot take them in")
@@ -205,8 +220,7 @@ class GQAttention(Mixer):
                             k_cache=cache.k, v_cache=cache.v, token_seq=step.token_seq, block_table=cache_table,
                             page_size=cache.page_size)
         out = rt.empty((T, nq, d))
-        ops.attention(q, out, cache.k, cache.v, step, cache.group, nq, nkv, d, cache.page_size, self.window,
-                      self.scale, rt.stream, plan=step.plans.get(self.plan_key()))
+        self._attend(q, out, step, cache)
         return self._project_out(out.view(T, self.q_size), sink)
 
 

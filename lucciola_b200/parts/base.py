@@ -152,6 +152,10 @@ class StepContext:
     # What the parts planned for this step, by their plan_key().
     plans: dict[Hashable, PlanView] = field(default_factory=dict)
     token_ids: Optional[torch.Tensor] = None    # [T]; for parts that choose by the token itself
+    # In a step some of whose requests begin with the same pages (else None), see ops.attention_shared: for each request the row whose
+    # table stands for its group's (-1: none), and that row's tokens in common.
+    prefix_of: Optional[torch.Tensor] = None    # [S]
+    prefix_lens: Optional[torch.Tensor] = None  # [S]
     # What a part wants to keep for its later calls in the same run of the model (a block that runs several times may use
     # again what depends on the tokens alone).  The model empties it before every run.
     memo: dict[Hashable, Any] = field(default_factory=dict)

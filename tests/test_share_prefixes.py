@@ -1,0 +1,262 @@
+"""Pages held by several requests: the pool's and the manager's bookkeeping, the scheduler that hands them over, the step function's groups."""
+import random
+
+import pytest
+import torch
+
+from lucciola_b200.cache import CacheGroup, CacheManager, PagePool, PagePoolError
+from lucciola_b200.config import EngineOptions
+from lucciola_b200.engine.request import Request
+from lucciola_b200.engine.scheduler import Scheduler
+from lucciola_b200.engine.step import StepEntry
+from lucciola_b200.sampling.params import SamplingParams
+from test_step_packing import HostRunner, StandInModel
+import test_step_packing as packing
+
+PS = 4
+
+
+def manager(pages=64, slots=8, groups=1):
+    return CacheManager([CacheGroup(2, 16, 0, (g,)) for g in range(groups)], PS, pages, slots)
+
+
+def test_a_page_goes_back_when_its_last_holder_gives_it_up():
+    pool = PagePool(3)
+    a = pool.allocate()
+    pool.share(a)
+    assert pool.holders(a) == 2
+    pool.free(a)
+    assert pool.num_free == 2
+    pool.free(a)
+    assert pool.num_free == 3
+    with pytest.raises(PagePoolError):
+        pool.free(a)
+    with pytest.raises(PagePoolError):
+        pool.share(a)
+    with pytest.raises(PagePoolError):
+        pool.share(7)
+
+
+def test_pages_are_taken_over_and_given_back():
+    m = manager(groups=2)
+    m.admit("a")
+    m.extend("a", 18)                                        # five pages, four of them full
+    m.admit("b")
+    m.share_prefix("b", "a", 4)
+    assert m.length("b") == 16 and all(m.block_table("b", g) == m.block_table("a", g)[:4] for g in range(2))
+    assert m.pages_needed("b", 19) == [1, 1]
+    m.extend("b", 19)
+    m.check_invariants()
+    assert m.pools[0].num_held == 6
+    m.release("a")
+    m.check_invariants()
+    assert m.pools[0].num_held == 5
+    m.admit("c")
+    m.share_prefix("c", "b", 4)
+    m.release("b")
+    m.release("c")
+    m.check_invariants()
+    assert m.pools[0].num_held == 0
+
+
+def test_what_cannot_be_taken_over_is_refused():
+    m = manager()
+    m.admit("a")
+    m.extend("a", 10)
+    m.admit("b")
+    for rid, donor, pages in (("b", "a", 3), ("b", "a", 0), ("a", "a", 1)):
+        with pytest.raises(PagePoolError):
+            m.share_prefix(rid, donor, pages)
+    m.extend("b", 1)
+    with pytest.raises(PagePoolError):
+        m.share_prefix("b", "a", 1)
+    w = CacheManager([CacheGroup(2, 16, 8, (0,))], PS, 8, 2)
+    w.admit("a")
+    w.extend("a", 8)
+    w.admit("b")
+    assert not w.can_share()
+    with pytest.raises(PagePoolError):
+        w.share_prefix("b", "a", 1)
+
+
+def test_groups_of_a_step():
+    m = manager(pages=200, slots=12)
+    m.admit("a")
+    m.extend("a", 41)                                        # ten full pages
+    for rid, donor, pages in (("b", "a", 10), ("c", "b", 10), ("d", "a", 3), ("e", "d", 3)):
+        m.admit(rid)
+        m.share_prefix(rid, donor, pages)
+        m.extend(rid, m.length(rid) + 5)
+    m.admit("x")
+    m.extend("x", 9)
+    assert m.prefix_groups(["x", "a"]) is None
+    assert m.prefix_groups(["x", "b", "a"]) == ([-1, 1, 1], [0, 40, 0])
+    assert m.prefix_groups(["d", "x", "e"]) == ([0, -1, 0], [12, 0, 0])
+    assert m.prefix_groups(["a", "b", "c", "d", "e"]) == ([0, 0, 0, -1, -1], [40, 0, 0, 0, 0])      # 3 x 10 pages are more than 5 x 3
+    assert m.prefix_groups(["b", "d"]) == ([0, 0], [12, 0])
+    m.release("a")
+    assert m.prefix_groups(["c", "b"]) == ([0, 0], [40, 0])
+    assert m.prefix_groups([]) is None
+
+
+def test_groups_name_pages_that_their_members_really_share():
+    """Random families: every member's table begins with the pages that the group's row stands for, and its tokens lie behind them."""
+    rng = random.Random(3)
+    for _ in range(200):
+        m = manager(pages=500, slots=16)
+        alive = []
+        for i in range(16):
+            m.admit(i)
+            if alive and rng.random() < 0.8:
+                donor = rng.choice(alive)
+                full = m.length(donor) // PS
+                if full:
+                    m.share_prefix(i, donor, rng.randint(1, full))
+            m.extend(i, m.length(i) + rng.randint(1, 30))
+            alive.append(i)
+            if rng.random() < 0.2:
+                m.release(alive.pop(rng.randrange(len(alive))))
+        m.check_invariants()
+        rng.shuffle(alive)
+        groups = m.prefix_groups(alive)
+        if groups is None:
+            continue
+        for i, leader in enumerate(groups[0]):
+            if leader >= 0:
+                n = groups[1][leader] // PS
+                assert groups[0][leader] == leader and n > 0
+                assert m.block_table(alive[i], 0)[:n] == m.block_table(alive[leader], 0)[:n]
+                assert m.length(alive[i]) >= n * PS
+
+
+def drive(s, m, steps=200):
+    """Runs the scheduler as the engine does; the next token is a function of the tokens so far.  Checks what each step computes."""
+    computed = 0
+    while s.has_unfinished() and steps:
+        steps -= 1
+        plan = s.schedule()
+        for e in plan:
+            r = e.request
+            if not m.has_request(r.rid):
+                m.admit(r.rid)
+            assert m.length(r.rid) == e.start == r.num_computed
+            assert m.extend(r.rid, e.start + e.num_tokens)
+            computed += e.num_tokens
+        m.check_invariants()
+        s.update(plan, [(sum(e.request.tokens) * 7 + len(e.request.tokens)) % 50 for e in plan if e.sample])
+    assert not s.has_unfinished()
+    assert m.pools[0].num_held == 0
+    return computed
+
+
+@pytest.mark.parametrize("pages", [200, 30])
+def test_the_scheduler_computes_a_common_beginning_once(pages):
+    """Eight answers to one prompt of 21 tokens, and two prompts that begin with half of it: the prompt is computed once, and the
+    tokens are those of requests that share nothing, preemptions or not."""
+    prompt = list(range(100, 121))
+    prompts = [prompt] * 8 + [prompt[:10] + [7, 8, 9], prompt[:10] + [3]]
+
+    def run(share):
+        m = manager(pages=pages, slots=12)
+        s = Scheduler(m, 64, 12, 200, share_prefixes=share)
+        reqs = [Request(i, list(p), SamplingParams(max_new_tokens=12)) for i, p in enumerate(prompts)]
+        for r in reqs:
+            s.add_request(r)
+        n = drive(s, m)
+        return [r.output for r in reqs], n, s
+    plain, n_plain, _ = run(False)
+    shared, n_shared, s = run(True)
+    assert shared == plain
+    if pages == 200:
+        assert s.num_shared_tokens == 7 * 20 + 2 * 8 and n_shared == n_plain - s.num_shared_tokens
+        assert s.num_preemptions == 0
+    else:
+        assert n_shared < n_plain
+
+
+def test_a_request_waits_for_a_beginning_that_is_being_computed():
+    m = manager(slots=4)
+    s = Scheduler(m, 8, 4, 200, share_prefixes=True)
+    prompt = list(range(1, 30))
+    for i in range(2):
+        s.add_request(Request(i, list(prompt), SamplingParams(max_new_tokens=2)))
+    seen = []
+    for _ in range(5):
+        plan = s.schedule()
+        seen.append([(e.request.rid, e.start, e.num_tokens) for e in plan])
+        for e in plan:
+            if not m.has_request(e.request.rid):
+                m.admit(e.request.rid)
+            m.extend(e.request.rid, e.start + e.num_tokens)
+        s.update(plan, [5] * sum(e.sample for e in plan))
+    assert seen == [[(0, 0, 8)], [(0, 8, 8)], [(0, 16, 8)], [(0, 24, 5)], [(0, 29, 1), (1, 28, 1)]]
+
+
+def test_the_last_token_of_a_prompt_is_always_computed():
+    m = manager()
+    s = Scheduler(m, 64, 4, 200, share_prefixes=True)
+    prompt = list(range(8))                                  # two whole pages
+    s.add_request(Request(0, list(prompt), SamplingParams(max_new_tokens=4)))
+    plan = s.schedule()
+    m.admit(0)
+    m.extend(0, 8)
+    s.update(plan, [9])
+    s.add_request(Request(1, list(prompt), SamplingParams(max_new_tokens=4)))
+    plan = s.schedule()
+    assert [(e.request.rid, e.start, e.num_tokens) for e in plan] == [(0, 8, 1), (1, 4, 4)]
+
+
+class SharingModel(StandInModel):
+    """Also hands out what the step says of its groups."""
+    def forward(self, tok, step, caches, rows):
+        out = super().forward(tok, step, caches, rows)
+        self.groups = None if step.prefix_of is None else (step.prefix_of.tolist(), step.prefix_lens.tolist())
+        return out
+
+
+def runner(monkeypatch, **kw):
+    monkeypatch.setattr(packing.step_mod, "_Staging", packing.HostStaging)
+    from lucciola_b200.parts.base import Runtime
+    monkeypatch.setattr(packing.step_mod, "DeviceCache", lambda *a, **k: type("C", (), {"states": {}, "views": []})())
+    rt = Runtime("cpu", torch.bfloat16)
+    return HostRunner(SharingModel(), rt, EngineOptions(max_blocks=100, max_num_seqs=8, use_cuda_graph=kw.pop("graph", False), share_prefixes=True, **kw))
+
+
+def test_the_step_function_names_the_groups(monkeypatch):
+    r = runner(monkeypatch)
+    r.step([StepEntry("a", list(range(40)), (39,))])
+    assert r.model.groups is None
+    r.manager.admit("b")
+    r.manager.share_prefix("b", "a", 2)
+    r.step([StepEntry("x", [1, 2], (1,)), StepEntry("a", [5], (0,)), StepEntry("b", [1, 2, 3], (2,))])
+    assert r.model.groups == ([-1, 1, 1], [0, 32, 0])
+    r.step([StepEntry("b", [5], (0,))])
+    assert r.model.groups is None
+
+
+def test_recordings_of_steps_with_groups(monkeypatch):
+    """A step with groups is recorded apart from one without, and a replay reads this step's groups; entries that pad belong to none."""
+    r = runner(monkeypatch, graph=True)
+    r.step([StepEntry("a", list(range(40)), (39,))])
+    for rid in "bcde":
+        r.manager.admit(rid)
+        r.manager.share_prefix(rid, "a", 2)
+        r.step([StepEntry(rid, [1, 2], (1,))])
+    r.step([StepEntry(i, [3], (0,)) for i in "abc"])
+    assert r.model.groups == ([0, 0, 0, -1], [32, 0, 0, 0])
+    r.step([StepEntry("x", [3, 4], (1,))])
+    before = r.graph_replays
+    r.step([StepEntry(i, [3], (0,)) for i in ("x", "d", "b")])
+    assert r.graph_replays == before + 1
+    assert r.model.groups == ([-1, 1, 1, -1], [0, 32, 0, 0])
+    assert sorted(len(k) for k in r._graphs if k[0] == 4) == [5]
+    r.step([StepEntry(i, [3], (0,)) for i in ("x", "d")])
+    assert r.model.groups is None
+
+
+def test_models_that_keep_more_than_all_keys_refuse(monkeypatch):
+    from lucciola_b200.parts.base import Runtime
+    monkeypatch.setattr(packing.step_mod, "_Staging", packing.HostStaging)
+    monkeypatch.setattr(packing.step_mod, "DeviceCache", lambda *a, **k: type("C", (), {"states": {}, "views": []})())
+    with pytest.raises(ValueError, match="share_prefixes"):
+        HostRunner(StandInModel(state=True), Runtime("cpu", torch.bfloat16), EngineOptions(max_blocks=10, max_num_seqs=2, share_prefixes=True))

@@ -23,6 +23,7 @@
 #include "sampling.cuh"
 
 #include <atomic>
+#include <cfloat>
 
 namespace lb {
 
@@ -206,9 +207,10 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(FilterPa
   const int per = (words + (int)g.size - 1) / (int)g.size;
   const int first = min(words, (int)g.rank * per), nq = min(words, first + per) - first;
   // word q of the slice from memory; places outside the row are not there (-inf)
+  auto whole = [&](int q) { const int v = 4 * (first + q) - skew; return v >= 0 && v + 4 <= p.vocab; };
   auto fetch = [&](int q) -> float4 {
+    if (whole(q)) return __ldcg(reinterpret_cast<const float4*>(base) + first + q);
     const int v = 4 * (first + q) - skew;
-    if (v >= 0 && v + 4 <= p.vocab) return __ldcg(reinterpret_cast<const float4*>(base) + first + q);
     float x[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = (v + e >= 0 && v + e < p.vocab) ? __ldcg(row_ptr + v + e) : -INFINITY;
@@ -221,34 +223,70 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(FilterPa
   float4* data4 = reinterpret_cast<float4*>(data);
   auto word = [&](int q) -> float4 { return IN_SMEM ? data4[q] : clean(fetch(q)); };
   auto index_of = [&](int q, int e) { return 4 * (first + q) - skew + e; };
+  // All of a thread's words are requested at once; only that thread reads them.
+  if (IN_SMEM) {
+#pragma unroll 4
+    for (int q = tid; q < nq; q += SF_THREADS) {
+      if (whole(q))
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(data4 + q)), "l"(base + 4ll * (first + q)) : "memory");
+      else
+        data4[q] = fetch(q);
+    }
+  }
+  const float temp = p.temperature ? __ldcg(p.temperature + row) : 0.f;
+  const int k_asked = p.top_k ? __ldcg(p.top_k + row) : 0;
+  const float top_p = p.top_p ? __ldcg(p.top_p + row) : 1.f, min_p = p.min_p ? __ldcg(p.min_p + row) : 0.f;
+  const bool by_k = k_asked > 0 && k_asked < p.vocab, by_p = top_p < 1.f, by_m = min_p > 0.f;
+  const double t64 = (double)fminf(temp, 1e30f);
+  const float inv_t = (float)fmin(1.0 / t64, 3e38);            // (M - M) / T stays 0 and -inf / T -inf
+  const float k2 = (float)fmin(1.4426950408889634 / t64, 3e38);
+  if (IN_SMEM) asm volatile("cp.async.wait_all;" ::: "memory");
 
-  // ---- largest logit ---------------------------------------------------------------------------------------------------------------
+  // ---- largest logit, and where sums are needed the sum of the weights against it, in one pass: each thread against its own largest ------------
+  const bool sums = temp > 0.f && !(by_k && k_asked <= SF_SHORT) && (by_p || by_m || by_k);
   float mine = -INFINITY;
+  double mine_sum = 0.0;
+#pragma unroll 2
   for (int q = tid; q < nq; q += SF_THREADS) {
-    const float4 x = clean(fetch(q));
-    if (IN_SMEM) data4[q] = x;
-    mine = fmaxf(fmaxf(mine, fmaxf(x.x, x.y)), fmaxf(x.z, x.w));
+    float4 x;
+    if (IN_SMEM) {
+      x = data4[q];
+      if (x.x != x.x || x.y != x.y || x.z != x.z || x.w != x.w) data4[q] = x = clean(x);
+    } else {
+      x = clean(fetch(q));
+    }
+    const float m = fmaxf(fmaxf(mine, fmaxf(x.x, x.y)), fmaxf(x.z, x.w));
+    if (sums && m > -INFINITY) {
+      if (m > mine) {
+        mine_sum *= (double)exp2_approx((mine - m) * k2);      // (0 before the first)
+        mine = m;
+      }
+      if (m < INFINITY)                                        // (+inf: no sum is asked for)
+        mine_sum += (double)((exp2_approx((x.x - m) * k2) + exp2_approx((x.y - m) * k2)) + (exp2_approx((x.z - m) * k2) + exp2_approx((x.w - m) * k2)));
+    }
+    mine = m;
   }
   sf_cluster_wait();
-  struct Most { float m, least; };                             // the largest, and the smallest of the threads' largest
-  const Most most = sf_reduce(g, Most{mine, mine > -INFINITY ? mine : INFINITY},
-                              [](Most a, Most b) { return Most{fmaxf(a.m, b.m), fminf(a.least, b.least)}; });
+  struct Most { double sum; float m, least; };                 // sum of the weights against the largest, the largest, and the smallest of the threads' largest
+  const Most most = sf_reduce(g, Most{mine_sum, mine, mine > -INFINITY ? mine : INFINITY}, [k2](Most a, Most b) {
+    const float m = fmaxf(a.m, b.m);
+    double sum = a.sum + b.sum;
+    if (a.m != b.m) sum = m == a.m ? a.sum + b.sum * (double)exp2_approx((b.m - m) * k2) : b.sum + a.sum * (double)exp2_approx((a.m - m) * k2);
+    return Most{sum, m, fminf(a.least, b.least)};
+  });
   const float M = most.m;
-  const float temp = p.temperature ? p.temperature[row] : 0.f;
-  const int k_asked = p.top_k ? p.top_k[row] : 0;
-  const float top_p = p.top_p ? p.top_p[row] : 1.f, min_p = p.min_p ? p.min_p[row] : 0.f;
-  const bool by_k = k_asked > 0 && k_asked < p.vocab, by_p = top_p < 1.f, by_m = min_p > 0.f;
   auto finish = [&](int token) { if (g.rank == 0 && tid == 0) p.tokens[row] = token; };
 
   if (!(M > -INFINITY)) { finish(0); return; }
   if (!(temp > 0.f) || M == INFINITY) {
     int at = 0x7fffffff;
-    for (int q = tid; q < nq; q += SF_THREADS) {
-      const float4 x = word(q);
-      const float v[4] = {x.x, x.y, x.z, x.w};
+    if (mine == M)
+      for (int q = tid; q < nq && at == 0x7fffffff; q += SF_THREADS) {
+        const float4 x = word(q);
+        const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-      for (int e = 3; e >= 0; --e) if (v[e] == M) at = min(at, index_of(q, e));
-    }
+        for (int e = 3; e >= 0; --e) if (v[e] == M) at = index_of(q, e);
+      }
     at = sf_reduce(g, at, [](int a, int b) { return min(a, b); });
     finish(at);
     return;
@@ -274,9 +312,6 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(FilterPa
     finish(b.i == 0x7fffffff ? 0 : b.i);
     return;
   }
-  const double t64 = (double)fminf(temp, 1e30f);
-  const float inv_t = (float)fmin(1.0 / t64, 3e38);            // (M - M) / T stays 0 and -inf / T -inf
-  const float k2 = (float)fmin(1.4426950408889634 / t64, 3e38);
   auto z64 = [&](float l) { return ((double)l - (double)M) / t64; };
   auto score64 = [&](float l, int i) {
     return z64(l) - log(-log(((double)hash_bits(hrow, (unsigned int)i) + 0.5) / 8388608.0));
@@ -408,7 +443,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(FilterPa
   auto sum_in_front = [&](const Border& b) {
     double s = 0.0;
     int n = 0;
-    for (int q = tid; q < nq; q += SF_THREADS) {
+    for (int q = tid; q < nq && mine >= b.l; q += SF_THREADS) {
       const float4 x = word(q);
       const float v[4] = {x.x, x.y, x.z, x.w};
       if (fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)) < b.l) continue;
@@ -439,8 +474,8 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(FilterPa
     return sf_reduce(g, s, [](Sum64 a, Sum64 c) { return Sum64{a.inner + c.inner, a.outer + c.outer}; });
   };
 
-  const Border whole = border;                                 // of all that top_k leaves
-  const double total = sum_in_front(whole).s;
+  const Border first_border = border;                          // of all that top_k leaves
+  const double total = by_k ? sum_in_front(first_border).s : most.sum;
   double sum = total;                                          // of what is in front of `border`
   for (;;) {
     Best best{-INFINITY, 0x7fffffff, 0.f, -INFINITY};
@@ -455,20 +490,29 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(FilterPa
       zc = fminf(zc, 0.f);                                     // the first is always kept
       const float l_cut = M + zc * fminf(temp, 1e30f) - 1e-5f * fabsf(M);
       const float reach = bounded ? exp2f(-bound * 1.4426951f) * 1.01f : INFINITY;       // -log u < w e^-bound for a score above the bound
-      for (int q = tid; q < nq; q += SF_THREADS) {
-        const float4 x = word(q);
-        const float v[4] = {x.x, x.y, x.z, x.w};
-        const float cut = fmaxf(l_cut, border.l);
+      // 32 logits at a time: which of them pass the cut is cheap to see, and only those are looked at one by one (a hash is thirty
+      // instructions, and where each lane takes its own, few lanes take many)
+      const float cut = fmaxf(fmaxf(l_cut, border.l), -FLT_MAX);
+      if (mine >= cut) {
+        for (int q0 = tid; q0 < nq; q0 += 8 * SF_THREADS) {
+          uint32_t pass = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (!(v[e] >= cut) || !(v[e] > -INFINITY)) continue;
-          const int i = index_of(q, e);
-          if (!in_front(v[e], i, border)) continue;
-          const float u = bits_to_uniform(hash_bits(hrow, (unsigned int)i));
-          if ((1.f - u) > weight(v[e]) * reach) continue;
-          const float s = (v[e] - M) * inv_t - logf(-logf(u));
-          if (s > best.s || (s == best.s && i < best.i)) { best.second = fmaxf(best.second, best.s); best.s = s; best.i = i; best.l = v[e]; }
-          else best.second = fmaxf(best.second, s);
+          for (int w = 0; w < 8; ++w) {
+            const int q = q0 + w * SF_THREADS;
+            if (q >= nq) break;
+            const float4 x = word(q);
+            pass |= (x.x >= cut ? 1u << (4 * w) : 0u) | (x.y >= cut ? 2u << (4 * w) : 0u) | (x.z >= cut ? 4u << (4 * w) : 0u) | (x.w >= cut ? 8u << (4 * w) : 0u);
+          }
+          for (; pass; pass &= pass - 1) {
+            const int bit = __ffs(pass) - 1, q = q0 + (bit >> 2) * SF_THREADS, i = index_of(q, bit & 3);
+            const float l = IN_SMEM ? data[4 * q + (bit & 3)] : __ldcg(row_ptr + i);
+            if (!in_front(l, i, border)) continue;
+            const float u = bits_to_uniform(hash_bits(hrow, (unsigned int)i));
+            if ((1.f - u) > weight(l) * reach) continue;
+            const float s = (l - M) * inv_t - logf(-logf(u));
+            if (s > best.s || (s == best.s && i < best.i)) { best.second = fmaxf(best.second, best.s); best.s = s; best.i = i; best.l = l; }
+            else best.second = fmaxf(best.second, s);
+          }
         }
       }
       auto better = [](Best a, Best c) {
@@ -508,7 +552,7 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(FilterPa
       if (fabs(before.s - room) > off) {
         kept = before.s < room;
       } else {
-        const Sum64 s = sums64(at, whole);
+        const Sum64 s = sums64(at, first_border);
         kept = (double)s.inner < (double)top_p * (double)s.outer;
       }
     }

@@ -23,8 +23,12 @@ __host__ __device__ __forceinline__ float bits_to_uniform(unsigned int bits23) {
 __host__ __device__ __forceinline__ unsigned long long hash_row(unsigned long long key, unsigned int counter) {
   return mix64(key + 0x9E3779B97F4A7C15ull * (unsigned long long)(counter + 1u));
 }
+// (mix64 without its last step, which changes the low 33 bits alone)
 __host__ __device__ __forceinline__ unsigned int hash_bits(unsigned long long row, unsigned int i) {
-  return (unsigned int)(mix64(row ^ (0xD6E8FEB86659FD93ull * (unsigned long long)(i + 1u))) >> 41);
+  unsigned long long x = row ^ (0xD6E8FEB86659FD93ull * (unsigned long long)(i + 1u));
+  x ^= x >> 30; x *= 0xBF58476D1CE4E5B9ull;
+  x ^= x >> 27; x *= 0x94D049BB133111EBull;
+  return (unsigned int)(x >> 41);
 }
 
 // Uniform in (0, 1) with 23 bits.

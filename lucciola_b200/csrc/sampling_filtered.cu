@@ -56,6 +56,29 @@ __device__ __forceinline__ uint32_t sf_remote(const void* local, uint32_t rank) 
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
   return a;
 }
+// A word into a peer's shared memory that is counted by a barrier there.  One way only: a barrier of the whole cluster around plain
+// stores is a way there and one back, and a row has four to eight of these (18.8 us against 16.5 for 8 rows of 151936).
+__device__ __forceinline__ void sf_send(uint32_t addr, uint32_t v, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];" ::"r"(addr), "r"(v), "r"(bar) : "memory");
+}
+__device__ __forceinline__ bool sf_try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+__device__ int g_sampling_error = 0;                  // 1 where a wait gave up (lb_sample_filtered_device_error)
+constexpr unsigned SF_WAIT_CYCLES = 2000000000u;
+__device__ __forceinline__ void sf_expect(unsigned long long* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(bar)), "r"(bytes) : "memory");
+}
+// Bounded (about a second): a wait that runs out is recorded, and the row goes on with what there is.
+__device__ __forceinline__ void sf_wait(unsigned long long* bar, uint32_t parity) {
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(bar);
+  const unsigned t0 = (unsigned)clock();
+  while (!sf_try_wait(at, parity))
+    if ((unsigned)clock() - t0 > SF_WAIT_CYCLES) { g_sampling_error = 1; break; }
+}
 __device__ __forceinline__ void sf_st_remote(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ uint32_t sf_ld_remote(uint32_t addr) {
   uint32_t v;
@@ -69,9 +92,10 @@ __device__ __forceinline__ uint32_t sf_add_remote(uint32_t addr, uint32_t v) {
 }
 
 // Values of up to SF_WORDS words a thread, reduced over the cluster; every thread gets the result.  Two sets of slots in turn: a CTA
-// writes a set again only after a barrier that its peers reach when they have read it.
+// writes a peer's set again only when it has that peer's values of the turn between, which the peer sends when it has read the set.
 constexpr int SF_WORDS = 6;
 struct FilterShared {
+  unsigned long long arrived[2];         // barriers of the two sets of slots
   uint32_t warp_part[SF_THREADS / 32][SF_WORDS];
   uint32_t slot[2][SF_MAX_CLUSTER][SF_WORDS];
   uint32_t hist[2][SF_BINS];
@@ -88,50 +112,50 @@ struct FilterGroup {                     // what a thread knows of its cluster
   int turn;
 };
 
-template <typename T, typename F>
-__device__ __forceinline__ T sf_reduce(FilterGroup& g, T v, F join) {
+// Floats as whole numbers of the same order, for the warp's one-instruction maxima and minima.
+__device__ __forceinline__ int sf_order(float x) { const int b = __float_as_int(x); return b ^ ((b >> 31) & 0x7fffffff); }
+__device__ __forceinline__ float sf_unorder(int o) { return __int_as_float(o ^ ((o >> 31) & 0x7fffffff)); }
+__device__ __forceinline__ double sf_warp_sum(double v, int lanes) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The cluster's value from the lanes' values: `lanes` joins the first 32 or SF_THREADS / 32 lanes of a warp (lane 0 has the result), `slots` the CTAs'.
+template <typename T, typename L, typename C>
+__device__ __forceinline__ T sf_reduce_by(FilterGroup& g, T v, L lanes, C slots) {
   static_assert(sizeof(T) % 4 == 0 && sizeof(T) / 4 <= SF_WORDS, "words of a slot");
   constexpr int W = sizeof(T) / 4;
   union U { T t; uint32_t w[W]; __device__ U() {} };
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    U a, b;
-    a.t = v;
-#pragma unroll
-    for (int i = 0; i < W; ++i) b.w[i] = __shfl_xor_sync(0xffffffffu, a.w[i], o);
-    v = join(v, b.t);
-  }
+  U a;
+  a.t = lanes(v, 32);
   if (lane == 0) {
-    U a;
-    a.t = v;
 #pragma unroll
     for (int i = 0; i < W; ++i) g.sh->warp_part[warp][i] = a.w[i];
   }
   __syncthreads();
-  uint32_t (*slot)[SF_WORDS] = g.sh->slot[g.turn & 1];
+  const int set = g.turn & 1;
+  const uint32_t parity = (g.turn >> 1) & 1;
+  uint32_t (*slot)[SF_WORDS] = g.sh->slot[set];
   ++g.turn;
   if (warp == 0) {
-    U a;
 #pragma unroll
     for (int i = 0; i < W; ++i) a.w[i] = g.sh->warp_part[lane & (SF_THREADS / 32 - 1)][i];
-    v = a.t;
+    a.t = lanes(a.t, SF_THREADS / 32);                         // (twice the same in the two halves of the warp)
+    // lane 0's value to all CTAs, a word a lane
+    uint32_t mine = 0;
 #pragma unroll
-    for (int o = SF_THREADS / 64; o > 0; o >>= 1) {
-      U b;
-      a.t = v;
-#pragma unroll
-      for (int i = 0; i < W; ++i) b.w[i] = __shfl_xor_sync(0xffffffffu, a.w[i], o);
-      v = join(v, b.t);
+    for (int i = 0; i < W; ++i) {
+      const uint32_t w = __shfl_sync(0xffffffffu, a.w[i], 0);
+      if (lane % W == i) mine = w;
     }
-    if (lane < g.size) {
-      a.t = v;
-#pragma unroll
-      for (int i = 0; i < W; ++i) sf_st_remote(sf_remote(&slot[g.rank][i], lane), a.w[i]);
-    }
+    if (lane == 0) sf_expect(&g.sh->arrived[set], g.size * W * 4);
+    for (uint32_t c = lane / W; c < g.size; c += 32 / W)
+      if (lane < 32 / W * W) sf_send(sf_remote(&slot[g.rank][lane % W], c), mine, sf_remote(&g.sh->arrived[set], c));
   }
-  sf_cluster_sync();
-  U a;
+  sf_wait(&g.sh->arrived[set], parity);
 #pragma unroll
   for (int i = 0; i < W; ++i) a.w[i] = slot[0][i];
   T out = a.t;
@@ -139,9 +163,26 @@ __device__ __forceinline__ T sf_reduce(FilterGroup& g, T v, F join) {
     U b;
 #pragma unroll
     for (int i = 0; i < W; ++i) b.w[i] = slot[c][i];
-    out = join(out, b.t);
+    out = slots(out, b.t);
   }
   return out;
+}
+// The same with one way of joining two values.
+template <typename T, typename F>
+__device__ __forceinline__ T sf_reduce(FilterGroup& g, T v, F join) {
+  constexpr int W = sizeof(T) / 4;
+  union U { T t; uint32_t w[W]; __device__ U() {} };
+  return sf_reduce_by(g, v, [&](T x, int n) {
+#pragma unroll 1
+    for (int o = n >> 1; o > 0; o >>= 1) {
+      U a, b;
+      a.t = x;
+#pragma unroll
+      for (int i = 0; i < W; ++i) b.w[i] = __shfl_xor_sync(0xffffffffu, a.w[i], o);
+      x = join(x, b.t);
+    }
+    return x;
+  }, join);
 }
 
 // A histogram of the CTA's threads becomes the cluster's, and the first bin with `want` entries in it or in front of it is found:
@@ -195,7 +236,12 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(FilterPa
   const int tid = threadIdx.x;
   const int row = blockIdx.x / g.size;
   for (int b = tid; b < 2 * SF_BINS; b += SF_THREADS) sh.hist[0][b] = 0;
-  if (tid == 0) sh.list_n = 0;
+  if (tid == 0) {
+    sh.list_n = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(&sh.arrived[i])));
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   sf_cluster_arrive();
   pdl_wait(p.logits, p.temperature, p.keys, p.counters, p.top_k, p.top_p, p.min_p);
 
@@ -268,11 +314,13 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(FilterPa
   }
   sf_cluster_wait();
   struct Most { double sum; float m, least; };                 // sum of the weights against the largest, the largest, and the smallest of the threads' largest
-  const Most most = sf_reduce(g, Most{mine_sum, mine, mine > -INFINITY ? mine : INFINITY}, [k2](Most a, Most b) {
+  const auto scaled = [k2](double sum, float from, float to) { return from == to ? sum : sum * (double)exp2_approx((from - to) * k2); };      // (from -inf: 0)
+  const Most most = sf_reduce_by(g, Most{mine_sum, mine, mine > -INFINITY ? mine : INFINITY}, [scaled](Most a, int n) {
+    const float m = sf_unorder(__reduce_max_sync(0xffffffffu, sf_order(a.m)));
+    return Most{sf_warp_sum(scaled(a.sum, a.m, m), n), m, sf_unorder(__reduce_min_sync(0xffffffffu, sf_order(a.least)))};
+  }, [scaled](Most a, Most b) {
     const float m = fmaxf(a.m, b.m);
-    double sum = a.sum + b.sum;
-    if (a.m != b.m) sum = m == a.m ? a.sum + b.sum * (double)exp2_approx((b.m - m) * k2) : b.sum + a.sum * (double)exp2_approx((a.m - m) * k2);
-    return Most{sum, m, fminf(a.least, b.least)};
+    return Most{scaled(a.sum, a.m, m) + scaled(b.sum, b.m, m), m, fminf(a.least, b.least)};
   });
   const float M = most.m;
   auto finish = [&](int token) { if (g.rank == 0 && tid == 0) p.tokens[row] = token; };
@@ -453,7 +501,11 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(FilterPa
         if (in_front(v[e], index_of(q, e), b)) { w4 += weight(v[e]); ++n; }
       s += (double)w4;
     }
-    return sf_reduce(g, Sum{s, n, 0}, [](Sum a, Sum c) { return Sum{a.s + c.s, a.n + c.n, 0}; });
+    return sf_reduce_by(g, Sum{s, n, 0}, [](Sum a, int lanes) {
+      // (both halves of warp 0 have the same when it joins the warps' sums: their number is not added up twice)
+      const int n = __reduce_add_sync(0xffffffffu, a.n);
+      return Sum{sf_warp_sum(a.s, lanes), lanes < 32 ? n / (32 / lanes) : n, 0};
+    }, [](Sum a, Sum c) { return Sum{a.s + c.s, a.n + c.n, 0}; });
   };
   // the same of two borders in whole numbers, for what the above cannot tell: units of 2^-unit, the sum of a row below 2^63
   struct Sum64 { unsigned long long inner, outer; };
@@ -490,13 +542,23 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(FilterPa
       zc = fminf(zc, 0.f);                                     // the first is always kept
       const float l_cut = M + zc * fminf(temp, 1e30f) - 1e-5f * fabsf(M);
       const float reach = bounded ? exp2f(-bound * 1.4426951f) * 1.01f : INFINITY;       // -log u < w e^-bound for a score above the bound
-      // 32 logits at a time: which of them pass the cut is cheap to see, and only those are looked at one by one (a hash is thirty
-      // instructions, and where each lane takes its own, few lanes take many)
       const float cut = fmaxf(fmaxf(l_cut, border.l), -FLT_MAX);
-      if (mine >= cut) {
+      const bool inside = border.l > -INFINITY;
+      auto score = [&](float l, int i) {
+        // 1 - u = 2 - 2^-24 - (1 + b / 2^23), the bits b as a mantissa
+        const uint32_t b = hash_bits(hrow, (unsigned int)i);
+        if ((2.f - __uint_as_float(0x3f800000u | b)) - 1.f / 16777216.f <= weight(l) * reach && (!inside || in_front(l, i, border))) {
+          const float s = (l - M) * inv_t - logf(-logf(bits_to_uniform(b)));
+          if (s > best.s || (s == best.s && i < best.i)) { best.second = fmaxf(best.second, best.s); best.s = s; best.i = i; best.l = l; }
+          else best.second = fmaxf(best.second, s);
+        }
+      };
+      // 32 logits at a time: which of them pass the cut is cheap to see, and only those are looked at one by one (a hash is twenty
+      // instructions, and where each lane takes its own, few lanes take many).  Scoring all four of a word instead where most pass, and
+      // queues that a warp takes 32 from at a time, were both slower: 65 and 77 us for 64 rows of 151936, against 64.
+      if (mine >= cut)
         for (int q0 = tid; q0 < nq; q0 += 8 * SF_THREADS) {
           uint32_t pass = 0;
-#pragma unroll
           for (int w = 0; w < 8; ++w) {
             const int q = q0 + w * SF_THREADS;
             if (q >= nq) break;
@@ -505,22 +567,22 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(FilterPa
           }
           for (; pass; pass &= pass - 1) {
             const int bit = __ffs(pass) - 1, q = q0 + (bit >> 2) * SF_THREADS, i = index_of(q, bit & 3);
-            const float l = IN_SMEM ? data[4 * q + (bit & 3)] : __ldcg(row_ptr + i);
-            if (!in_front(l, i, border)) continue;
-            const float u = bits_to_uniform(hash_bits(hrow, (unsigned int)i));
-            if ((1.f - u) > weight(l) * reach) continue;
-            const float s = (l - M) * inv_t - logf(-logf(u));
-            if (s > best.s || (s == best.s && i < best.i)) { best.second = fmaxf(best.second, best.s); best.s = s; best.i = i; best.l = l; }
-            else best.second = fmaxf(best.second, s);
+            score(IN_SMEM ? data[4 * q + (bit & 3)] : __ldcg(row_ptr + i), i);
           }
         }
-      }
       auto better = [](Best a, Best c) {
         const bool swap = c.s > a.s || (c.s == a.s && c.i < a.i);
         const float second = fmaxf(fmaxf(a.second, c.second), fminf(a.s, c.s));
         return swap ? Best{c.s, c.i, c.l, second} : Best{a.s, a.i, a.l, second};
       };
-      best = sf_reduce(g, best, better);
+      best = sf_reduce_by(g, best, [](Best a, int) {
+        const int order = sf_order(a.s), top = __reduce_max_sync(0xffffffffu, order);
+        const int i = __reduce_min_sync(0xffffffffu, order == top ? a.i : 0x7fffffff);
+        const bool won = order == top && a.i == i;
+        const int from = __ffs(__ballot_sync(0xffffffffu, won)) - 1;
+        const int second = __reduce_max_sync(0xffffffffu, sf_order(won ? a.second : a.s));
+        return Best{sf_unorder(top), i, __shfl_sync(0xffffffffu, a.l, from), sf_unorder(second)};
+      }, better);
       if (bounded && !(best.s >= bound)) best.i = 0x7fffffff;          // what was left out may be better
       if (best.i != 0x7fffffff && best.second > best.s - SF_SCORE_MARGIN) {
         // two scores too near to tell apart: in 64 bits, all that come near the best
@@ -608,4 +670,12 @@ LB_EXPORT int lb_sample_filtered(int* tokens, const float* logits, long long row
   if (e != cudaSuccess) { lb::set_error("sample_filtered: launch failed: %s", cudaGetErrorString(e)); return 2; }
   lb::count_launch();
   return 0;
+}
+
+// Reads and clears the flag a bounded wait of this kernel sets when it gives up (0: none).
+LB_EXPORT int lb_sample_filtered_device_error() {
+  int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, lb::g_sampling_error, sizeof(int)) != cudaSuccess) return -1;
+  if (v != 0) cudaMemcpyToSymbol(lb::g_sampling_error, &zero, sizeof(int));
+  return v;
 }

@@ -1436,10 +1436,11 @@ def device_error() -> int:
     lib.lb_latent_prefill_device_error.restype = c_int
     lib.lb_chunk_device_error.restype = c_int
     lib.lb_attention_shared_device_error.restype = c_int
+    lib.lb_sample_filtered_device_error.restype = c_int
     return (int(lib.lb_device_error()) or int(lib.lb_attention_tcgen05_device_error())
             or int(lib.lb_attention_flash_device_error()) or int(lib.lb_latent_flash_device_error())
             or int(lib.lb_latent_prefill_device_error()) or int(lib.lb_chunk_device_error())
-            or int(lib.lb_attention_shared_device_error()))
+            or int(lib.lb_attention_shared_device_error()) or int(lib.lb_sample_filtered_device_error()))
 
 
 def linear(y: torch.Tensor, x: torch.Tensor, w: torch.Tensor, stream: int, fast: bool, post: str | None = None, post_c: float = 0.0) -> None:

@@ -166,10 +166,10 @@ __global__ void __launch_bounds__(AP_THREADS) attention_shared_plain_kernel(Shar
 __global__ void __launch_bounds__(AS_PLAN_THREADS) as_plan_kernel(SharedParams p, int ctas) {
   __shared__ SharedPlan pl;
   pdl_trigger();
-  as_make_plan(p, pl, ctas);             // lengths and groups were written before the kernel ahead began
   pdl_wait();
+  as_make_plan(p, pl, ctas);
   as_write_records(p, pl, blockIdx.x, gridDim.x, threadIdx.x, AS_PLAN_THREADS);
-  const bool sound = as_sound(p, pl);
+  const bool sound = pl.sound;
   const int total = sound ? pl.units * p.kv_heads : 0, span = pl.span;
   if (blockIdx.x == 0)
     for (int c = threadIdx.x; c < ctas; c += AS_PLAN_THREADS)

@@ -69,6 +69,7 @@ struct SharedPlan {                      // in shared memory, while it is made
                                          // begins in the line, in the list of rows and among all tiles
   int first_member[AS_MAX_SEQS];         // where the tokens of the group that this row leads begin among all groups'
   int units, span, rows, tiles;          // units, rows and tiles of a kv head, units of a CTA
+  bool sound;                            // cu_tokens rise: every token belongs to one request at most
 };
 
 __device__ __forceinline__ int as_blocks(int lo, int hi) { return hi > lo ? (hi - (lo & ~(AS_KEYS - 1)) + AS_KEYS - 1) / AS_KEYS : 0; }
@@ -115,19 +116,22 @@ __device__ __forceinline__ int as_scan(int* a, int n) {
   return total;
 }
 
-// Made by all AS_PLAN_THREADS threads of a CTA; ends with a barrier.  Reads lengths and groups only.
+// Made by all AS_PLAN_THREADS threads of a CTA; ends with a barrier.
 constexpr int AS_PLAN_THREADS = 512;
 __device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& pl, int ctas) {
   const int tid = threadIdx.x, n = p.S;
   const int most = p.max_pages * p.page_size;
+  bool falls = false;
   if (tid < n) {
     const int s = tid;
     const int a = __ldcg(p.cu + s), b = __ldcg(p.cu + s + 1), c = __ldcg(p.ctx + s), l = __ldcg(p.prefix_of + s), f = __ldcg(p.prefix_lens + s);
     const int q0 = min(max(a, 0), p.T);
+    falls = b < a;
     pl.q0[s] = q0;
-    pl.meta[s] = make_int4(l >= 0 && l < n ? l : -1, max(min(b, p.T) - q0, 0), min(max(c, 0), most), min(max(f, 0), most));
+    pl.meta[s] = make_int4(l >= 0 && l < n ? l : -1, max(min(b, p.T), q0) - q0, min(max(c, 0), most), min(max(f, 0), most));
   }
-  __syncthreads();
+  const bool sound = __syncthreads_or(falls) == 0;
+  if (tid == 0) pl.sound = sound;
   // Who shares with whom: every request looks at all others (n is a few dozen, a few hundred at most), 1 << k lanes for each.
   const int k = n <= AS_PLAN_THREADS / 8 ? 3 : n <= AS_PLAN_THREADS / 4 ? 2 : n <= AS_PLAN_THREADS / 2 ? 1 : 0;
   const int s = tid >> k, part = tid & ((1 << k) - 1);
@@ -182,23 +186,23 @@ __device__ __forceinline__ void as_make_plan(const SharedParams& p, SharedPlan& 
   __syncthreads();
 }
 
-// cu_tokens that fall would make more rows than there is room for: nothing is done then.
+// Rows of partial results of a kv head, at most: a token has its own and those with its prefix, and the last tile of an entry (one a request, one
+// a group of two or more) may be folded, into four with up to 32 rows each or two with up to 128.
+// Where cu_tokens fall, requests' tokens overlap and there may be more of everything than there is room for: the plan is empty then, and the output stays as it was.
 __host__ __device__ __forceinline__ long long as_most_rows(long long tokens, long long seqs, int group, bool folds) {
-  const long long rows = tokens * group, more = 256 * seqs;    // an entry's last tile may be folded
+  const long long rows = tokens * group, more = 256 * seqs;
   return 2 * rows + (!folds ? 0 : more < 4 * rows ? more : 4 * rows);
 }
-__device__ __forceinline__ bool as_sound(const SharedParams& p, const SharedPlan& pl) { return pl.rows <= as_most_rows(p.T, p.S, p.group, p.folds); }
-
 // What the combining kernel has to know of every token, for the prefix and for the request's own keys: the first row of the token's
 // tile, the token's first row in the tile, the tile's rows (not folded), the unit of its first block, and how many units further the last block
 // begins (-1: no block).  And the groups' tokens.
 __device__ __forceinline__ void as_write_records(const SharedParams& p, const SharedPlan& pl, int cta, int ctas, int thread, int threads) {
   if (cta == 0 && thread == 0) {
     p.head[0] = pl.units; p.head[1] = pl.span; p.head[2] = pl.rows;
-    p.head[3] = p.S > 0 ? pl.q0[0] : 0;
-    p.head[4] = p.S > 0 ? pl.q0[p.S - 1] + pl.meta[p.S - 1].y : 0;
+    p.head[3] = pl.sound ? pl.q0[0] : 0;
+    p.head[4] = pl.sound ? pl.q0[p.S - 1] + pl.meta[p.S - 1].y : 0;
   }
-  for (int s = cta * (threads >> 5) + (thread >> 5); s < p.S; s += ctas * (threads >> 5)) {        // a warp a request
+  for (int s = cta * (threads >> 5) + (thread >> 5); pl.sound && s < p.S; s += ctas * (threads >> 5)) {        // a warp a request
     const int4 me = pl.meta[s];
     const int t0 = pl.q0[s], q = me.y, l = pl.lead[s];
     const int prefix = l >= 0 ? pl.meta[l].w : 0;
@@ -212,7 +216,7 @@ __device__ __forceinline__ void as_write_records(const SharedParams& p, const Sh
         const int tile = index / p.tile_tokens, first = tile * p.tile_tokens, here = min(tokens - first, p.tile_tokens);
         const int lo = of ? prefix : 0, hi = of ? me.z : prefix;
         const int blocks = as_blocks(lo, of ? min(hi, hi - q + first + here) : hi);            // that the tile's last token sees
-        const bool any = (of || l >= 0) && as_sound(p, pl);
+        const bool any = of || l >= 0;
         dst[of] = any ? make_int4(pl.row[e] + first * p.group, (index - first) * p.group, here * p.group,
                                   pl.unit[e] + tile * as_tile_units(p, p.tile_tokens, as_blocks(lo, hi)) + p.tile_start) : make_int4(0, 0, 0, 0);
         last[of] = any && blocks > 0 ? (blocks - 1) * (here > p.lane_tokens ? 2 : 1) : -1;

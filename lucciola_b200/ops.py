@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 from ctypes import c_float, c_int, c_longlong, c_uint, c_ulonglong, c_void_p
+from typing import NamedTuple
 
 import torch
 
@@ -1501,12 +1502,25 @@ def attention_shared_ok(num_seqs: int, head_dim: int, scale: float) -> bool:
     return num_seqs <= 512 and head_dim % 8 == 0 and 0 < head_dim <= 256 and scale > 0
 
 
+def attention_shared_tensor_cores(dtype: torch.dtype, num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int) -> bool:
+    """Whether attention_shared runs on the tensor cores for these sizes: bfloat16 heads of 64 or 128, at most 128 query heads a kv
+    head, pages of 8 tokens or more that are a power of two."""
+    return (dtype == torch.bfloat16 and head_dim in (64, 128) and num_q_heads // num_kv_heads <= 128 and page_size >= 8
+            and page_size & (page_size - 1) == 0)
+
+
+class SharedPlan(NamedTuple):
+    """A step's plan for attention_shared: the integers, and the element type and sizes (tokens, requests, query heads, kv heads, head size,
+    page size, pages a request) that they were made for."""
+    data: torch.Tensor
+    sizes: tuple
+
+
 def shared_plan(dtype: torch.dtype, num_tokens: int, cu_tokens: torch.Tensor, context_lens: torch.Tensor, prefix_of: torch.Tensor,
                 prefix_lens: torch.Tensor, num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int, pages_a_seq: int,
-                stream: int) -> torch.Tensor:
-    """What attention_shared has to know of a step of num_tokens tokens, made on the GPU from the requests' lengths and groups (its arguments of the same
-    names): once a step for all layers with these sizes.  Lengths and groups must not be written by the kernel of this library that is
-    launched right in front of this one (they are read while that may still run)."""
+                stream: int) -> SharedPlan:
+    """What attention_shared has to know of a step of num_tokens tokens, made on the GPU from the requests' lengths and groups (its arguments
+    of the same names): once a step for all layers with these sizes."""
     S = context_lens.shape[0]
     if not cu_tokens.is_cuda:
         raise KernelError("cu_tokens must be on the GPU")
@@ -1519,13 +1533,13 @@ def shared_plan(dtype: torch.dtype, num_tokens: int, cu_tokens: torch.Tensor, co
     _kept_for(stream, plan)
     _call("lb_attention_shared_plan", dt, plan.data_ptr(), n_ints, cu_tokens.data_ptr(), context_lens.data_ptr(), prefix_of.data_ptr(),
           prefix_lens.data_ptr(), *sizes, stream)
-    return plan
+    return SharedPlan(plan, (dt, *sizes))
 
 
 def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                      cu_tokens: torch.Tensor, context_lens: torch.Tensor, prefix_of: torch.Tensor, prefix_lens: torch.Tensor, max_q_len: int,
                      num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int, scale: float, stream: int,
-                     plan: torch.Tensor | None = None) -> None:
+                     plan: SharedPlan | None = None) -> None:
     """Causal attention of a step over paged keys and values, the keys that several requests share read once for all of them.
 
     q, out [T, heads, dim] (float32 or bfloat16); pools [pages, kv heads, page_size, dim]; block_table [S, pages a sequence],
@@ -1534,11 +1548,12 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     tokens the prefix of row r has: the first prefix_lens[prefix_of[s]] keys of s are read through that row's table, the others
     through its own.  All of these are device values, read by the kernels, so that a recorded step is replayed with other groups and
     lengths.  Page ids outside the pool are not there: a row that sees no key gives zeros, and rows of q that belong to no request
-    (behind cu_tokens[S]) leave the output as it was.  S is at most 512, a head a multiple of 8 up to 256, max_q_len the most tokens of a request.
+    (behind cu_tokens[S]) leave the output as it was.  Where cu_tokens fall, all of the output stays as it was.
+    Keys and values past a request's end may be anything; those of its own later tokens have to be finite (they are multiplied by
+    weights of 0).  S is at most 512, a head a multiple of 8 up to 256, max_q_len the most tokens of a request.
 
-    `plan`: what shared_plan() made of these lengths, groups and sizes; without it the call makes one (see there for when lengths and
-    groups may be written).  Partial results go through memory that the call takes from torch's allocator, so calls on several
-    streams do not meet."""
+    `plan`: what shared_plan() made of these lengths, groups and sizes; without it the call makes one.  Partial results go through memory
+    that the call takes from torch's allocator, so calls on several streams do not meet."""
     T, S, P = q.shape[0], context_lens.shape[0], block_table.shape[-1]
     device, dtype = q.get_device(), q.dtype
     if q.shape != (T, num_q_heads, head_dim) or out.shape != q.shape:
@@ -1564,8 +1579,9 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
         floats = torch.empty(n_floats + n_ints, dtype=torch.float32, device=q.device)
         plan_at = floats.data_ptr() + 4 * n_floats
     else:
-        _check(plan, "plan", torch.int32)
-        lengths, plan_at, n_ints = (None, None, None, None), plan.data_ptr(), plan.shape[0]
+        if plan.sizes != (dt, T, S, num_q_heads, num_kv_heads, head_dim, page_size, P) or plan.data.get_device() != device:
+            raise KernelError(f"the plan was made for other sizes, {plan.sizes}, or another device, {plan.data.device}")
+        lengths, plan_at, n_ints = (None, None, None, None), plan.data.data_ptr(), plan.data.shape[0]
         floats = torch.empty(n_floats, dtype=torch.float32, device=q.device)
     _kept_for(stream, floats)
     _call("lb_attention_shared", dt, q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), plan_at, n_ints,

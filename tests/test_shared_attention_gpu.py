@@ -2,9 +2,9 @@
 
 Tolerances.  float32: sums of up to a few hundred products in 32 bits; a score is off by less than 2^-20 (|q . k| scale is a few), a weight
 as much relatively, a result (a mean of values of size 1 to 4) by less than 2^-18.  bfloat16: the same where the products run on the ordinary
-pipes; on the tensor cores each weight is rounded to bfloat16, by at most 2^-9 of itself, so the mean of values |v| <= V moves by at most
-2^-9 V (and its denominator, summed before the rounding, not at all); and the output is rounded once, by at most 2^-9 of itself, also V at
-most.  Together 2^-8 V, and 2^-18."""
+pipes; on the tensor cores each weight is rounded to bfloat16, by at most half a step, 2^-8 of itself, so the mean of values |v| <= V moves by
+at most 2^-8 V (and its denominator, summed before the rounding, not at all); and the output is rounded once, by at most 2^-8 of itself, also
+V at most.  Together 2^-7 V, and 2^-18."""
 import random
 
 import pytest
@@ -82,7 +82,7 @@ class Batch:
         n = self.cu[-1]
         got, want = got[:n].double().cpu(), want[:n]
         top = float(self.v[~self.v.isnan()].abs().max())
-        off = 2 ** -18 * max(top, 1) + (2 ** -8 * top if self.dtype == torch.bfloat16 else 0)
+        off = 2 ** -18 * max(top, 1) + (2 ** -7 * top if self.dtype == torch.bfloat16 else 0)
         assert got.isfinite().all()
         assert (got - want).abs().max() <= off
 
@@ -268,3 +268,64 @@ def test_refusals(ops):
     with pytest.raises(ops.KernelError):
         call(q=wide, out=wide.clone(), k=pool, v=pool, heads=1, kv_heads=1, dim=264)
     call(q=q[:0], out=out[:0])                                                 # no tokens: nothing to do
+
+
+def a_batch():
+    return Batch(8, 2, 128, 16, [(0, 1, 193), (0, 3, 260), (-1, 5, 40), (0, 1, 400)], [192], torch.bfloat16)
+
+
+def plan_of(ops, b, dev, **other):
+    q, k, v, table, cu, ctx, of, lens = dev
+    sizes = dict(dtype=b.dtype, num_tokens=b.T, num_q_heads=b.heads, num_kv_heads=b.kv_heads, head_dim=b.dim, page_size=b.page,
+                 pages_a_seq=table.shape[1], stream=ops.current_stream())
+    return ops.shared_plan(cu_tokens=cu, context_lens=ctx, prefix_of=of, prefix_lens=lens, **{**sizes, **other})
+
+
+def with_plan(ops, b, dev, plan):
+    q, k, v, table, cu, ctx, of, lens = dev
+    out = torch.empty_like(q)
+    ops.attention_shared(q, out, k, v, table, cu, ctx, of, lens, b.max_new, b.heads, b.kv_heads, b.dim, b.page, b.scale, ops.current_stream(), plan=plan)
+    return out
+
+
+def test_a_plan_serves_calls_of_its_sizes_only(ops):
+    b = a_batch()
+    dev = b.device()
+    plan = plan_of(ops, b, dev)
+    first = with_plan(ops, b, dev, plan)
+    b.compare(first)
+    assert torch.equal(first, with_plan(ops, b, dev, plan)) and torch.equal(first, b.launch(ops, dev, torch.empty_like(dev[0])))
+    for other in (dict(dtype=torch.float32), dict(num_tokens=b.T + 1), dict(num_q_heads=16), dict(num_kv_heads=4), dict(head_dim=64),
+                  dict(page_size=32), dict(pages_a_seq=dev[3].shape[1] + 1)):
+        with pytest.raises(ops.KernelError, match="other sizes"):
+            with_plan(ops, b, dev, plan_of(ops, b, dev, **other))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_tokens_that_belong_to_two_requests(ops, dtype):
+    """cu_tokens that fall: there is no room for what would come of it, and nothing is computed."""
+    b = Batch(8, 2, 128, 16, [(0, 4, 300)] * 8, [192], dtype)
+    dev = b.device()
+    for cu in ([0, 32] * 4 + [32], [0, 30, 2, 31, 3, 32, 0, 32, 32], [32, 28, 24, 20, 16, 12, 8, 4, 0], [0, -5, 2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 0, 40, 5, 32]):
+        dev[4] = torch.tensor(cu, dtype=torch.int32, device="cuda")
+        out = b.launch(ops, dev, torch.full_like(dev[0], 7.0))
+        assert (out == 7).all()
+    assert ops.device_error() == 0
+
+
+def test_lengths_written_right_in_front(ops):
+    """Lengths and groups that kernels on the same stream write directly ahead of the call, through a chain of the library's own launches."""
+    b = a_batch()
+    dev = b.device()
+    ints = [t.clone() for t in dev[4:]]
+    want = b.launch(ops, dev, torch.empty_like(dev[0]))
+    alone = b.launch(ops, dev[:6] + [torch.full_like(ints[2], -1), torch.zeros_like(ints[3])], torch.empty_like(dev[0]))
+    for turn in range(30):
+        for t, keep in zip(dev[4:], ints):
+            t.zero_()
+        b.launch(ops, dev, torch.empty_like(dev[0]))
+        for t, keep in zip(dev[4:], ints):
+            t.copy_(keep)
+        if turn % 2:
+            dev[6].fill_(-1)
+        assert torch.equal(b.launch(ops, dev, torch.empty_like(dev[0])), alone if turn % 2 else want)

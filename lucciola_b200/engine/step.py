@@ -37,7 +37,7 @@ from ..cache.device_cache import DeviceCache, pages_that_fit
 from ..cache.manager import NO_PAGE, CacheManager, plan_groups
 from ..config.engine_options import EngineOptions
 from ..models.decoder import DecoderModel
-from ..parts.base import BatchShape, Mixer, PlanView, Runtime, StepContext, StepPlan
+from ..parts.base import BatchShape, KVPages, Mixer, PlanView, Runtime, StepContext, StepPlan
 
 
 # Numbers of leading single tokens for which steps are recorded; a step is padded to the next one.
@@ -49,6 +49,16 @@ _RECORD_PORTIONS = 4
 # A recording of a portion of which some logits are wanted computes those of all its tokens; not worth it for
 # a long portion of which few are wanted.
 _ALL_ROWS = 64
+# Requests that begin with the same pages go through the kernels for shared prefixes when these spare so many elements of keys in a layer (8 kv heads
+# of 128: 16 K keys).  Requests of 8 kv heads of 128, each with a new token, us a layer ordinarily and with the keys read once: 16 behind 512 common
+# keys (8 M elements) 13.5 and 16.2, 16 behind 1024 (16 M) 18.4 and 17.1, 16 behind 2048 (31 M) 27.5 and 18.6, 32 behind 4096 (130 M) 80 and 28; and the
+# plan, 4 us a step.  In 32 bits the keys are read once by better kernels in any case.
+SHARED_ELEMENTS = 1 << 24
+
+
+def _elements_saved(prefix_of: Sequence[int], prefix_lens: Sequence[int], a_key: int) -> int:
+    """Elements of keys that are not read again when every group (prefix_of, prefix_lens) reads its prefix once."""
+    return sum((prefix_of.count(r) - 1) * n * a_key for r, n in enumerate(prefix_lens) if n)
 
 
 class OutOfPages(RuntimeError):
@@ -138,6 +148,7 @@ class ModelRunner:
         self.cache = DeviceCache(requests, self.groups, self.page_size, counts, options.max_num_seqs, rt.act_dtype, self.device)
         self.max_pages_per_seq = -(-self.max_model_len // self.page_size)
         self._any_window = any(g.window > 0 for g in self.groups)
+        self._key_elements = max([r.num_kv_heads * r.head_dim for r in requests if isinstance(r, KVPages) and not r.shared], default=0)      # of a key in a layer
         if options.share_prefixes and (self.state_cache_ids or not self.manager.can_share()):
             raise ValueError("share_prefixes needs a model that keeps the keys and values of all tokens, and nothing else, of a request")
         self._arange_cache = np.arange(512, dtype=np.int32)
@@ -373,6 +384,8 @@ class ModelRunner:
         # entries that own no page (their keys and values are written nowhere and they attend to nothing).
         # Requests that begin with the same pages; steps with and without such are recorded apart.
         shared = self.manager.prefix_groups([e.rid for e in entries]) if self.options.share_prefixes else None
+        if shared and self.rt.fast_kernels and _elements_saved(*shared, self._key_elements) < SHARED_ELEMENTS:
+            shared = None
         shape = self._shape_of(entries, q_lens, max_ctx)
         if shape is not None and shared:
             shape += ("shared",)

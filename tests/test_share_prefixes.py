@@ -224,6 +224,7 @@ def runner(monkeypatch, **kw):
 
 def test_the_step_function_names_the_groups(monkeypatch):
     r = runner(monkeypatch)
+    monkeypatch.setattr(packing.step_mod, "SHARED_ELEMENTS", 0)
     r.step([StepEntry("a", list(range(40)), (39,))])
     assert r.model.groups is None
     r.manager.admit("b")
@@ -237,6 +238,7 @@ def test_the_step_function_names_the_groups(monkeypatch):
 def test_recordings_of_steps_with_groups(monkeypatch):
     """A step with groups is recorded apart from one without, and a replay reads this step's groups; entries that pad belong to none."""
     r = runner(monkeypatch, graph=True)
+    monkeypatch.setattr(packing.step_mod, "SHARED_ELEMENTS", 0)
     r.step([StepEntry("a", list(range(40)), (39,))])
     for rid in "bcde":
         r.manager.admit(rid)
@@ -260,3 +262,9 @@ def test_models_that_keep_more_than_all_keys_refuse(monkeypatch):
     monkeypatch.setattr(packing.step_mod, "DeviceCache", lambda *a, **k: type("C", (), {"states": {}, "views": []})())
     with pytest.raises(ValueError, match="share_prefixes"):
         HostRunner(StandInModel(state=True), Runtime("cpu", torch.bfloat16), EngineOptions(max_blocks=10, max_num_seqs=2, share_prefixes=True))
+
+
+def test_elements_that_groups_spare():
+    from lucciola_b200.engine.step import _elements_saved
+    assert _elements_saved([0, 0, -1, 3, 0, 3], [32, 0, 0, 16, 0, 0], 10) == (2 * 32 + 1 * 16) * 10
+    assert _elements_saved([-1, -1], [0, 0], 10) == 0

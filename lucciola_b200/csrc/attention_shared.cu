@@ -34,16 +34,17 @@ __global__ void __launch_bounds__(AP_THREADS) attention_shared_plain_kernel(Shar
   float* vs = ks + AS_KEYS * (D + 4);
   float* ps = vs + AS_KEYS * D;
   int* page = reinterpret_cast<int*>(ps + AP_ROWS * (AS_KEYS + 4));      // offset of each key's row in the pool's page units, -1: not there
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();                         // behind the wait: the combining kernel reads the plan before its own
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const T* q = reinterpret_cast<const T*>(p.q);
   const T* kc = reinterpret_cast<const T*>(p.k_cache);
   const T* vc = reinterpret_cast<const T*>(p.v_cache);
   const int d = p.dim, G = p.group, cache_heads = p.kv_heads / p.kv_share;
-  const int2 piece = __ldcg(p.pieces + blockIdx.x);
+  Segment g;
+  const int2 piece = as_piece(p, blockIdx.x, g);
   for (int at = piece.x; at <= piece.y; ++at) {
-    const Segment g = as_segment(p, at);
+    if (at != piece.x) g = as_segment(p, at);
     if (g.blocks == 0) continue;
     const long long first_row = (long long)(uint32_t)g.row_low | (long long)g.row_high << 32;
     const int rows = g.tokens * G;
@@ -173,10 +174,10 @@ __global__ void __launch_bounds__(AS_PLAN_THREADS) as_plan_kernel(SharedParams p
   const int total = sound ? pl.units * p.kv_heads : 0, span = pl.span;
   if (blockIdx.x == 0)
     for (int c = threadIdx.x; c < ctas; c += AS_PLAN_THREADS)
-      if ((long long)c * span >= total) p.pieces[c] = make_int2(0, -1);
+      if ((long long)c * span >= total) p.pieces[c * (AS_PIECE / 4)] = make_int4(0, -1, 0, 0);
   if (!sound) return;
-  // the segments: a thread has an entry and a kv head
-  for (int i = blockIdx.x * AS_PLAN_THREADS + threadIdx.x; i < 2 * p.S * p.kv_heads; i += gridDim.x * AS_PLAN_THREADS) {
+  // the segments: eight threads have an entry and a kv head, every eighth tile each, or, of a few tiles, every eighth segment
+  for (int i = (blockIdx.x * AS_PLAN_THREADS + threadIdx.x) >> 3; i < 2 * p.S * p.kv_heads; i += gridDim.x * AS_PLAN_THREADS >> 3) {
     const int kv = i / (2 * p.S), e = i - kv * (2 * p.S);
     const bool shared = e < p.S;
     const int s = shared ? e : e - p.S;
@@ -185,28 +186,36 @@ __global__ void __launch_bounds__(AS_PLAN_THREADS) as_plan_kernel(SharedParams p
     if (pl.unit[e] == end) continue;
     const int lead = shared ? -1 : pl.lead[s], lo = lead >= 0 ? pl.meta[lead].w : 0, hi = shared ? me.w : me.z;
     const int tokens = shared ? pl.led[s] : me.y, nb = as_blocks(lo, hi);
-    int base = kv * pl.units + pl.unit[e];
+    const int units = as_tile_units(p, p.tile_tokens, nb);     // of every tile but the last
+    const bool by_tile = tokens > 4 * p.tile_tokens;
+    const int mine = threadIdx.x & 7, tile_step = by_tile ? 8 : 1, step = by_tile ? 1 : 8;
 #pragma unroll 1
-    for (int first = 0, tile = pl.tile[e]; first < tokens; first += p.tile_tokens, ++tile) {
+    for (int i_tile = by_tile ? mine : 0; i_tile * p.tile_tokens < tokens; i_tile += tile_step) {
+      const int first = i_tile * p.tile_tokens, tile = pl.tile[e] + i_tile, base = kv * pl.units + pl.unit[e] + i_tile * units;
       const int here = min(tokens - first, p.tile_tokens), two = here > p.lane_tokens ? 1 : 0;             // units of a block: 1 << two
       const int key_hi = shared ? hi : min(hi, hi - tokens + first + here), there = as_blocks(lo, key_hi);      // an earlier tile sees fewer blocks
       const int b0 = base + p.tile_start, b1 = base + as_tile_units(p, here, nb);
       const int c0 = (int)((unsigned)base / (unsigned)span), c1 = (int)((unsigned)(b1 - 1) / (unsigned)span);
 #pragma unroll 1
-      for (int c = c0; c <= c1; ++c) {
+      for (int c = c0 + (by_tile ? 0 : mine); c <= c1; c += step) {
         const int x0 = c * span, x1 = min(x0 + span, total);
         // a block belongs to the CTA in whose piece it begins
         const int block = max(x0 - b0 + two, 0) >> two, blocks = max(min(max(min(x1, b1) - b0 + two, 0) >> two, there) - block, 0);
         const int at = kv * pl.tiles + tile + c;
         const long long row = (long long)kv * pl.rows + pl.row[e] + (long long)first * p.group + (long long)c * p.tile_tokens * p.group;
         int4* dst = p.segments + (size_t)at * 3;
-        dst[0] = make_int4(kv, s, (shared ? pl.first_member[s] : pl.q0[s]) + first, here);
-        dst[1] = make_int4(lo, key_hi, block, blocks);
-        dst[2] = make_int4((int)(uint32_t)row, (int)(row >> 32), shared ? 1 : 0, shared ? 0 : me.z - tokens + first);
-        if (x0 >= base) p.pieces[c].x = at;
-        if (x1 <= b1) p.pieces[c].y = at;
+        int4* piece = p.pieces + c * (AS_PIECE / 4);
+        const int4 segment[3] = {make_int4(kv, s, (shared ? pl.first_member[s] : pl.q0[s]) + first, here), make_int4(lo, key_hi, block, blocks),
+                                 make_int4((int)(uint32_t)row, (int)(row >> 32), shared ? 1 : 0, shared ? 0 : me.z - tokens + first)};
+#pragma unroll
+        for (int u = 0; u < 3; ++u) dst[u] = segment[u];
+        if (x0 >= base) {
+          piece->x = at;
+#pragma unroll
+          for (int u = 0; u < 3; ++u) piece[1 + u] = segment[u];
+        }
+        if (x1 <= b1) piece->y = at;
       }
-      base = b1;
     }
   }
 }
@@ -294,7 +303,7 @@ static bool as_params(SharedParams& p, SharedCut& cut, int& ctas, int dtype, int
 
 static void as_plan_parts(SharedParams& p, int* plan, int ctas) {
   const SharedPlanLayout at(p.T, p.S, p.kv_heads, p.tile_tokens, ctas);
-  p.head = plan; p.rec = plan + at.rec; p.pieces = reinterpret_cast<int2*>(plan + at.pieces);
+  p.head = plan; p.rec = plan + at.rec; p.pieces = reinterpret_cast<int4*>(plan + at.pieces);
   p.segments = reinterpret_cast<int4*>(plan + at.segments); p.members = reinterpret_cast<int2*>(plan + at.members);
 }
 
@@ -318,8 +327,9 @@ static int as_plan(lb::SharedParams p, const lb::SharedCut& cut, int ctas, int* 
   LB_CHECK_ARG(plan && (uintptr_t)plan % 16 == 0 && num_ints >= need, "attention_shared: a plan of %lld integers at a 16-byte boundary is needed, got %lld", need, num_ints);
   p.cu = cu_tokens; p.ctx = context_lens; p.prefix_of = prefix_of; p.prefix_lens = prefix_lens;
   lb::as_plan_parts(p, plan, ctas);
-  const long long tasks = 2ll * p.S * p.kv_heads;
-  const int blocks = (int)(tasks < 32 * 64 ? (tasks + 63) / 64 : 32);        // few tasks a CTA: each is a chain of lookups
+  // A round of segments and of tokens for every thread, up to 32 CTAs (each makes the whole plan first).
+  const long long tasks = 2ll * p.S * p.kv_heads * 8, most = tasks > p.T ? tasks : p.T;
+  const int blocks = (int)(most < 32 * lb::AS_PLAN_THREADS ? (most + lb::AS_PLAN_THREADS - 1) / lb::AS_PLAN_THREADS : 32);
   lb::launch(lb::as_plan_kernel, dim3(blocks), dim3(lb::AS_PLAN_THREADS), 0, stream, p, ctas);
   LB_CHECK_LAUNCH("attention_shared plan");
   return 0;

@@ -23,6 +23,7 @@ namespace lb {
 constexpr int AS_MAX_SEQS = 512;
 constexpr int AS_KEYS = 64;
 constexpr int AS_REC = 12;               // integers a token in the combining kernel's list
+constexpr int AS_PIECE = 16;             // integers a CTA in the list of their pieces
 constexpr int AS_FOLD_ROWS = 32;
 
 struct SharedParams {
@@ -41,8 +42,8 @@ struct SharedParams {
   // write, and threads with a head each read, side by side), and [rows][2]: the reference value (-inf: no key) and the sum.
   float* part_o; float* part_ml;
   // The plan.  head: {units a kv head, units a CTA, rows a kv head, first token, end of the tokens}; rec [T][AS_REC]: see as_write_records; pieces
-  // [CTAs]: the CTA's first and last segment; segments [..][12]: see Segment; members [T]: the groups' tokens, group by group, and the last key each sees
-  int* head; int* rec; int2* pieces; int4* segments; int2* members;
+  // [CTAs][AS_PIECE]: the CTA's first and last segment, two of nothing, and the first segment itself; segments [..][12]: see Segment; members [T]: the groups' tokens, group by group, and the last key each sees
+  int* head; int* rec; int4* pieces; int4* segments; int2* members;
 };
 
 // Integers of a plan, and where its parts begin.
@@ -50,7 +51,7 @@ struct SharedPlanLayout {
   long long rec, pieces, segments, members, total;
   __host__ SharedPlanLayout(long long tokens, long long seqs, int kv_heads, int tile_tokens, int ctas) {
     const long long most = kv_heads * 2 * (tokens / tile_tokens + seqs) + ctas;        // a tile has one segment more than it has cuts
-    rec = 8; pieces = rec + tokens * AS_REC; segments = (pieces + 2 * ctas + 3) & ~3ll; members = segments + most * 12; total = members + 2 * tokens;
+    rec = 8; pieces = rec + tokens * AS_REC; segments = pieces + AS_PIECE * ctas; members = segments + most * 12; total = members + 2 * tokens;
   }
 };
 
@@ -202,12 +203,21 @@ __device__ __forceinline__ void as_write_records(const SharedParams& p, const Sh
     p.head[3] = pl.sound ? pl.q0[0] : 0;
     p.head[4] = pl.sound ? pl.q0[p.S - 1] + pl.meta[p.S - 1].y : 0;
   }
-  for (int s = cta * (threads >> 5) + (thread >> 5); pl.sound && s < p.S; s += ctas * (threads >> 5)) {        // a warp a request
-    const int4 me = pl.meta[s];
-    const int t0 = pl.q0[s], q = me.y, l = pl.lead[s];
-    const int prefix = l >= 0 ? pl.meta[l].w : 0;
+  if (!pl.sound) return;
+  // Token by token: the request of a token is the last one that begins at it or in front of it and has any.
+  const int begin = pl.q0[0], end = pl.q0[p.S - 1] + pl.meta[p.S - 1].y;
+  for (int t = begin + cta * threads + thread; t < end; t += ctas * threads) {
+    int s = 0;
 #pragma unroll 1
-    for (int i = thread & 31; i < q; i += 32) {
+    for (int lo = 0, hi = p.S; hi - lo > 1;) {
+      const int mid = (lo + hi) >> 1;
+      if (pl.q0[mid] <= t) lo = mid; else hi = mid;
+      s = lo;
+    }
+    const int4 me = pl.meta[s];
+    const int t0 = pl.q0[s], q = me.y, l = pl.lead[s], i = t - t0;
+    const int prefix = l >= 0 ? pl.meta[l].w : 0;
+    {
       int4* dst = reinterpret_cast<int4*>(p.rec + (size_t)(t0 + i) * AS_REC);
       int last[2];
 #pragma unroll 1
@@ -236,10 +246,19 @@ struct Segment {
   int row_low, row_high;                 // where its partial rows begin, 64 bits
   int shared, position;                  // rows of several requests; else the last key that the first token sees
 };
-__device__ __forceinline__ Segment as_segment(const SharedParams& p, int i) {
-  const int4* at = p.segments + (size_t)i * 3;
+__device__ __forceinline__ Segment as_segment(const int4* at) {
   const int4 a = __ldcg(at), b = __ldcg(at + 1), c = __ldcg(at + 2);
   return Segment{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w};
+}
+__device__ __forceinline__ Segment as_segment(const SharedParams& p, int i) { return as_segment(p.segments + (size_t)i * 3); }
+// The first and the last segment of a CTA's piece of the line, and the first itself (nothing, if there is none): one access to memory in
+// front of the first keys less.
+__device__ __forceinline__ int2 as_piece(const SharedParams& p, int cta, Segment& first) {
+  const int4* at = p.pieces + (size_t)cta * (AS_PIECE / 4);
+  const int4 piece = __ldcg(at);
+  first = as_segment(at + 1);
+  if (piece.y < piece.x) first.blocks = 0;
+  return make_int2(piece.x, piece.y);
 }
 // A token of a segment: its place in the step, and the last key it sees.
 __device__ __forceinline__ int2 as_token(const SharedParams& p, int shared, int first, int position, int i) {
@@ -262,14 +281,14 @@ __global__ void __launch_bounds__(AS_COMBINE_THREADS * PARTS) as_combine_kernel(
   __shared__ float4 sums[PARTS][128];
   __shared__ float2 weights[PARTS][128];
   pdl_trigger();
-  const int* rec = p.rec;
-  const int* head = p.head;
   const int t = blockIdx.x, kv = blockIdx.y, part = threadIdx.x >> 7, lane = threadIdx.x & 127;
-  pdl_wait(rec, head);
-  const int4* r = reinterpret_cast<const int4*>(rec + (size_t)t * AS_REC);
+  // The plan was complete when the kernel ahead let this one begin (it waits for the plan first), and is read while that kernel still runs.
+  const int4* r = reinterpret_cast<const int4*>(p.rec + (size_t)t * AS_REC);
   const int4 a = __ldcg(r), b = __ldcg(r + 1), last = __ldcg(r + 2);
-  const int4 hd = __ldcg(reinterpret_cast<const int4*>(head));
-  if (t < hd.w || t >= __ldcg(head + 4)) return;               // rows of no request stay as they were
+  const int4 hd = __ldcg(reinterpret_cast<const int4*>(p.head));
+  const int end = __ldcg(p.head + 4);
+  pdl_wait(p.part_o, p.part_ml);
+  if (t < hd.w || t >= end) return;                            // rows of no request stay as they were
   const unsigned line = (unsigned)kv * (unsigned)hd.x, span = (unsigned)hd.y;
   const long long step = (long long)p.tile_tokens * p.group;
   const int fa = as_folds(p, true, a.z) - 1, fb = as_folds(p, false, b.z) - 1;       // 0, 1 or 3

@@ -121,7 +121,6 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   volatile int* holes = (volatile int*)(tmem_slot + 2);       // some key of this CTA's segments lies in no page
 
-  pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
@@ -143,6 +142,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   pdl_wait();
+  pdl_trigger();                               // behind the wait: the combining kernel reads the plan before its own
   const uint32_t tmem = *tmem_slot;            // columns: tile t's S buffers at t * 128 and t * 128 + 64 (P over their first 32), O at 256 + t * 128
 
   const int G = p.group, per = p.lane_tokens, cta = blockIdx.x;
@@ -179,15 +179,15 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     int stage_n = 0, stage_h = 0;              // their stages
     uint32_t used = 0, turns = 0;              // bits 2 s + t: whether tile t reads stage s's block, and the parity of the next wait for it
     // (Of warp 0) the segment to come, fetched when the one before it was taken, and the one after it in the list.
-    const int2 piece = __ldcg(p.pieces + cta);
-    int at_segment = piece.x;
     Segment found;
+    const int2 piece = as_piece(p, cta, found);
+    int at_segment = piece.x + 1;
     auto fetch = [&]() {
       found.blocks = 0;
 #pragma unroll 1
       while (at_segment <= piece.y && found.blocks == 0) found = as_segment(p, at_segment++);
     };
-    if (warp == 0) fetch();
+    if (warp == 0 && found.blocks == 0) fetch();
     auto find_step = [&]() {
       int kind = SC_END;
       // At most two segments: the second one if it is a request's few rows, as the first.

@@ -31,8 +31,9 @@ constexpr int SF_THREADS = 512;
 constexpr int SF_BINS = 256;
 constexpr int SF_SHORT = 256;            // most top_k of the short way
 constexpr int SF_LIST = 512;             // logits the first CTA ranks, one a thread
-constexpr int SF_MAX_CLUSTER = 8;
+constexpr int SF_MAX_LOG2 = 3, SF_MAX_CLUSTER = 1 << SF_MAX_LOG2;
 constexpr int SF_SLICE_BYTES = 200 * 1024;     // most logits of a CTA; longer rows are read again where they lie
+constexpr int SF_PAIR_BYTES = 100 * 1024;      // with as many, two CTAs share an SM
 constexpr float SF_SCORE_MARGIN = 1.f / 32768.f;     // 32-bit scores z + g lie in [-20, 20] and are off by less than 2^-17
 constexpr float SF_SUM_MARGIN = 1.f / 32768.f;       // 32-bit sums of w, relative: w within 2^-18 where it counts, four at a time in 32 bits
 constexpr float SF_BELOW = 60.f;                     // weights below e^-60 of the largest change no sum of 64 bits
@@ -624,29 +625,70 @@ __global__ void __launch_bounds__(SF_THREADS, 2) sample_filtered_kernel(FilterPa
   }
 }
 
-template <bool IN_SMEM>
-static cudaError_t sf_launch(const FilterParams& p, int rows, int cluster, size_t smem, cudaStream_t stream) {
-  if (IN_SMEM) {
-    static std::atomic<unsigned long long> configured{0ull};   // a bit a device
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e != cudaSuccess) return e;
-    if (!(configured.load() >> (device & 63) & 1ull)) {
-      e = cudaFuncSetAttribute(sample_filtered_kernel<IN_SMEM>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_SLICE_BYTES);
-      if (e != cudaSuccess) return e;
-      configured.fetch_or(1ull << (device & 63));
-    }
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)rows * cluster); cfg.blockDim = dim3(SF_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
+static void sf_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, int ctas, int cluster, size_t smem, cudaStream_t stream) {
+  cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas); cfg.blockDim = dim3(SF_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = g_pdl_enabled ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, sample_filtered_kernel<IN_SMEM>, p);
+}
+
+// How many clusters of 1 << log2 CTAs the GPU has room for at a time, with `per_sm` CTAs on an SM.  (A cluster lies within one of the GPU's parts of
+// some 18 SMs: 32 clusters of 8, two CTAs an SM, on 148 SMs.)
+static cudaError_t sf_room(int device, int log2, int per_sm, int& room) {
+  static std::atomic<int> known[64][4][2];                     // 0: not asked yet
+  room = device < 64 ? known[device][log2][per_sm - 1].load() : 0;
+  if (room > 0) return cudaSuccess;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  sf_config(cfg, attr, 1 << log2, 1 << log2, per_sm == 2 ? SF_PAIR_BYTES : SF_SLICE_BYTES, nullptr);
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaOccupancyMaxActiveClusters(&room, sample_filtered_kernel<true>, &cfg);
+  if (e != cudaSuccess) return e;
+  if (room < 1) room = 1;
+  if (device < 64) known[device][log2][per_sm - 1].store(room);
+  return cudaSuccess;
+}
+
+// The cluster of a row: the one for which the rounds of rows that there is room for take least time, a round of slices of n logits
+// 8.5 us + n x 0.4 ns, or 0.62 ns where two CTAs share an SM; with a word a thread at least, and slices that fit shared memory.  Measured (us,
+// clusters of 8, 4, 2, 1): 37 rows of 50003 23.4, 17.0, 19.0, 28.9; 128 rows of 32000 48, 32, 25, 34; 64 rows of 151936 50, 60, 222, 431; 8 rows
+// of 100000 14.3, 18.9, 30, 167 (slices that do not fit are read from memory each time).
+static cudaError_t sf_launch(const FilterParams& p, int rows, cudaStream_t stream) {
+  static std::atomic<unsigned long long> configured{0ull};     // a bit a device
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  if (!(configured.load() >> (device & 63) & 1ull)) {
+    e = cudaFuncSetAttribute(sample_filtered_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SF_SLICE_BYTES);
+    if (e != cudaSuccess) return e;
+    configured.fetch_or(1ull << (device & 63));
+  }
+  const int words = (p.vocab + 3 + 3) / 4;
+  int cluster = 0;
+  float least = 0.f;
+  for (int log2 = 0; log2 <= SF_MAX_LOG2; ++log2) {
+    const int slice = (words + (1 << log2) - 1) >> log2;
+    if (slice * 16 > SF_SLICE_BYTES) continue;
+    const int per_sm = slice * 16 <= SF_PAIR_BYTES ? 2 : 1;
+    int room = 0;
+    e = sf_room(device, log2, per_sm, room);
+    if (e != cudaSuccess) return e;
+    const float time = (float)((rows + room - 1) / room) * (8.5f + (float)slice * (per_sm == 2 ? 4 * 0.62e-3f : 4 * 0.4e-3f));
+    if (cluster == 0 || time < least) { cluster = 1 << log2; least = time; }
+    if (slice <= SF_THREADS) break;
+  }
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  if (cluster == 0) {
+    sf_config(cfg, attr, rows << SF_MAX_LOG2, 1 << SF_MAX_LOG2, 0, stream);
+    return cudaLaunchKernelEx(&cfg, sample_filtered_kernel<false>, p);
+  }
+  sf_config(cfg, attr, rows * cluster, cluster, (size_t)((words + cluster - 1) / cluster) * 16, stream);
+  return cudaLaunchKernelEx(&cfg, sample_filtered_kernel<true>, p);
 }
 
 }  // namespace lb
@@ -661,12 +703,7 @@ LB_EXPORT int lb_sample_filtered(int* tokens, const float* logits, long long row
   if (num_rows == 0) return 0;
   LB_CHECK_ARG(num_rows <= (1 << 24), "sample_filtered: %d rows, at most %d a launch", num_rows, 1 << 24);
   const lb::FilterParams p{tokens, logits, temperature, keys, counters, top_k, top_p, min_p, row_stride, vocab};
-  const int words = (vocab + 3 + 3) / 4;
-  int cluster = 1;
-  while (cluster < lb::SF_MAX_CLUSTER && words / cluster > lb::SF_THREADS) cluster *= 2;
-  const size_t smem = (size_t)((words + cluster - 1) / cluster) * 16;
-  const bool fits = smem <= lb::SF_SLICE_BYTES;
-  const cudaError_t e = fits ? lb::sf_launch<true>(p, num_rows, cluster, smem, stream) : lb::sf_launch<false>(p, num_rows, cluster, 0, stream);
+  const cudaError_t e = lb::sf_launch(p, num_rows, stream);
   if (e != cudaSuccess) { lb::set_error("sample_filtered: launch failed: %s", cudaGetErrorString(e)); return 2; }
   lb::count_launch();
   return 0;

@@ -247,3 +247,21 @@ def test_engine_generates_with_filters(ops, tiny_models):
              SamplingParams(max_new_tokens=6, ignore_eos=True),
              SamplingParams(max_new_tokens=6, ignore_eos=True, temperature=0.7, seed=2, min_p=0.1, top_k=30)]
     assert engine.generate(prompts, mixed)[1] == greedy[1]
+
+
+@pytest.mark.parametrize("vocab", [4097, 20011, 70001])
+def test_a_row_draws_the_same_among_many(ops, vocab):
+    """Batches so large that a row has fewer and fewer CTAs."""
+    gen = torch.Generator().manual_seed(vocab)
+    rows = 6
+    x = (torch.randn(rows, vocab, generator=gen) * 2).cuda()
+    t, keys = torch.tensor([0.7, 1.0, 1.3, 0.9, 1.0, 0.0]).cuda(), torch.arange(rows).cuda()
+    counters, k = torch.arange(rows, dtype=torch.int32).cuda(), torch.tensor([0, 40, 0, vocab // 3, 0, 5], dtype=torch.int32).cuda()
+    p, m = torch.tensor([0.95, 0.9, 1.0, 0.999, 0.5, 0.9]).cuda(), torch.tensor([0.0, 0.01, 0.02, 0.0, 0.0, 0.0]).cuda()
+    draws = []
+    for times in (1, 5, 10, 25, 60, 120):
+        out = torch.full((rows * times,), -1, dtype=torch.int32, device="cuda")
+        many = [a.repeat(times) for a in (t, keys, counters, k, p, m)]
+        ops.sample(out, x.repeat(times, 1), ops.current_stream(), *many[:3], top_k=many[3], top_p=many[4], min_p=many[5])
+        draws.append(out.view(times, rows))
+    assert all(torch.equal(d, draws[0].expand_as(d)) for d in draws)

@@ -1,10 +1,12 @@
-// Attention of a step whose requests share prefixes: the entry point, and the kernel on the ordinary pipes for 32-bit queries, keys and values, and bfloat16 ones that the
-// tensor-core kernel does not take.  The plan, the walk and the combination are attention_shared.cuh's.
+// Attention of a step whose requests share prefixes: the entry point, the plan, and the kernel on the ordinary pipes for 32-bit queries, keys
+// and values, and bfloat16 ones that the tensor-core kernel does not take.  The plan's layout and the combination are attention_shared.cuh's.
 //
 // A tile has up to 32 query rows (tokens x heads of a kv head's group; a group of more heads is cut into equal parts that read the same
 // cached head).  Queries, a block of 64 keys and its values lie in shared memory as 32-bit numbers.  256 threads: thread (ty, tx) has
 // rows 2 ty and 2 ty + 1; of the scores the keys tx, tx + 16, tx + 32, tx + 48, of the result the dimensions 4 tx + 64 c .. + 3.  Sixteen
-// threads share a row: its maximum and sum are four shuffles.
+// threads share a row: its maximum and sum are four shuffles.  Bound by the multiplications: 32 requests behind 4096 common keys, 32 heads of
+// 128 on 8 in 32 bits, 243 us (2.2 GFLOP, 9 TFLOP/s); 6 requests behind 1000, 16 heads of 64 on 4, with plan and combination 15.9 us, most of it
+// three kernels' beginnings and ends.
 #include "attention_shared.cuh"
 
 #include <atomic>
@@ -163,7 +165,8 @@ __global__ void __launch_bounds__(AP_THREADS) attention_shared_plain_kernel(Shar
   }
 }
 
-// The plan of a step: every CTA makes all of it, and writes a part.
+// The plan of a step: every CTA makes all of it, and writes a part.  A chain of lookups, not bytes: 3.3 us at 2 requests, 4.4 at 64, 8.4 at 32 of
+// which one has 2048 new tokens.
 __global__ void __launch_bounds__(AS_PLAN_THREADS) as_plan_kernel(SharedParams p, int ctas) {
   __shared__ SharedPlan pl;
   pdl_trigger();
@@ -261,7 +264,8 @@ static cudaError_t ap_launch(const SharedParams& p, int ctas, cudaStream_t strea
 
 template <typename T>
 static cudaError_t as_combine(const SharedParams& p, cudaStream_t stream) {
-  // Few rows: four threads share a row's partial results, so that one round of loads reads them all.
+  // Few rows: four threads share a row's partial results, so that one round of loads reads them all.  (8 requests behind 8192 keys 24.0 us against
+  // 30.4; 64 requests, which are above the border, 39.8 against 44.8 with four, portions 38 against 61.)
   if ((long long)p.T * p.kv_heads <= AS_FEW_BLOCKS)
     return launch(as_combine_kernel<T, 4>, dim3(p.T, p.kv_heads), dim3(4 * AS_COMBINE_THREADS), 0, stream, p);
   return launch(as_combine_kernel<T, 1>, dim3(p.T, p.kv_heads), dim3(AS_COMBINE_THREADS), 0, stream, p);
@@ -288,8 +292,9 @@ static bool as_params(SharedParams& p, SharedCut& cut, int& ctas, int dtype, int
   p.T = num_tokens; p.S = num_seqs; p.heads = num_q_heads; p.kv_heads = num_kv_heads * cut.share; p.group = cut.group; p.dim = head_dim;
   p.page_size = page_size; p.max_pages = max_pages; p.page_shift = -1; p.kv_share = cut.share;
   p.tile_tokens = cut.tile_tokens; p.lane_tokens = cut.lane_tokens;
-  // Measured at 64 requests behind 8192 keys and at portions behind 2000 (us, recorded): tiles that cost nothing beside their blocks 44.8 and 46.4,
-  // 2 units 41.3 and 39.6, 3 units 39.7 and 38.6, 6 units 44.2 and 36.2.
+  // Measured at 64 requests behind 8192 keys, at portions behind 2000 and at 2 requests behind 256 (us, recorded): tiles that cost 2 units beside
+  // their blocks 39.1, 38.3 and 17.1, 3 units 38.7, 36.7 and 14.3, 4 units 39.1, 35.5 and 15.4; pieces of at least 4 units 38.5, 36.9 and 15.2, of 8
+  // 38.5, 36.8 and 18.2.
   p.min_span = cut.tc ? 5 : 1; p.tile_start = cut.tc ? 3 : 0; p.folds = cut.tc;
   for (int b = 0; b < 31; ++b) if ((1 << b) == page_size) p.page_shift = b;
   // units of the whole line, at most

@@ -10,12 +10,18 @@
 // The sum of a row's weights is taken before they are rounded to bfloat16 for P V.  A row's reference value is the maximum of its first
 // block, and moves (O is rescaled then) when a block's weights against it sum up to 2^15: what the maximum was does not matter to the quotient.
 //
+// What bounds it: the way of a block through barriers, tensor memory and registers.  A block that both tiles work on takes 2080 cycles, of
+// which the tensor cores are at work for 1000 and the exponentials take 1024 (two warps a quarter of the SM); taking the exponentials out
+// leaves 1800.  64 requests with a token each behind 8192 common keys, up to 256 keys of their own, 32 heads of 128 on 8: 26 us of the 38.7 that
+// the call takes (plan 4.4, combination 6 to 8; recorded), 66 MB read; by the counters the tensor cores are busy for 23 % of the cycles (36 % on
+// the SMs that have the prefix), the issue slots for 35 %, DRAM for 23 %.  8 requests: 23.2 us in all; 2 requests behind 256: 14.3.
+//
 // Why 128-row tiles even for one request's few rows: a block of 64 keys takes the tensor cores some 500 cycles whatever the rows, and the
 // memory 1400 cycles at its full rate shared by all SMs, so rows that are not there cost nothing; one kernel for both kinds of work is what
 // lets the line be cut evenly.
 //
 // Warps: 0 and 4 copy keys, 2 and 5 values (cp.async, 16 bytes a thread, swizzled for the tensor cores; a warp has half of every block, and
-// three blocks in flight); 1 issues tile A's products and owns the tensor memory, 3 tile B's; 6..9 softmax of A, 10..13 of B.  Each goes through the
+// two blocks in flight); 1 issues tile A's products and owns the tensor memory, 3 tile B's; 6..9 softmax of A, 10..13 of B.  Each goes through the
 // segments, which warp 0 finds.  Barriers tell one turn from the next only, so each tile has barriers of its own for the stages of the rings, and a
 // copying warp speaks to the tiles that read a block.  All waits are bounded; when one gives up, the CTA records it and every role leaves.
 #include "attention_shared.cuh"
@@ -26,7 +32,6 @@
 namespace lb {
 
 constexpr int SC_K_STAGES = 4, SC_V_STAGES = 5;                // a block of values stays until its keys' scores have become weights
-constexpr int SC_IN_FLIGHT = 2;                                // blocks a copying warp has requested beyond the one it waits for
 constexpr int SC_BARS = 2 * (SC_K_STAGES + SC_V_STAGES) + 8;   // barriers of a tile
 constexpr int SC_THREADS = 448, SC_SOFTMAX = 6;                // the first of the softmax warps
 enum : int { SC_ERR_Q = 401, SC_ERR_KV_FULL = 402, SC_ERR_KV_EMPTY = 403, SC_ERR_S_FULL = 404, SC_ERR_P_FULL = 405, SC_ERR_O_FULL = 406, SC_ERR_O_FREE = 407, SC_ERR_SEGMENT = 408 };
@@ -274,17 +279,17 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       }
       if (tiles_now == 0) continue;            // nothing at hand yet
       // ---- its stage: the tiles that read the last block there are through with it.  While that has to be waited for, whatever has been requested
-      // is handed over; else the oldest block when SC_IN_FLIGHT are behind it.
+      // is handed over; else the block before the one that was requested last.  (With one more in flight blocks come a block's time later: 64
+      // requests behind 8192 common keys 39.9 us against 38.9.)
       const int s = stage_n;
       const uint32_t before = (used >> (2 * s)) & 3u, bar = empty0 + 8u * (uint32_t)((lane & 1) * SC_BARS + s);
       const bool mine = lane < 2 && ((before >> lane) & 1u);
       const uint32_t parity = (turns >> (2 * s + (lane & 1))) & 1u;
       const bool wait = __any_sync(0xffffffffu, mine && !ta_mbar_try_wait(bar, parity));
-      const int keep = wait ? 0 : n <= 2 ? 1 : SC_IN_FLIGHT;               // the first block is handed over early
+      const int keep = wait ? 0 : 1;
       if (n - handed > keep) {
         if (wait) asm volatile("cp.async.wait_group 0;" ::: "memory");
-        else if (keep == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-        else asm volatile("cp.async.wait_group %0;" ::"n"(SC_IN_FLIGHT) : "memory");
+        else asm volatile("cp.async.wait_group 1;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // visible to the tensor cores
         __syncwarp();
 #pragma unroll 1

@@ -183,25 +183,27 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     int n = 0, handed = 0, seen = 0;           // blocks requested, handed over; steps looked at
     int stage_n = 0, stage_h = 0;              // their stages
     uint32_t used = 0, turns = 0;              // bits 2 s + t: whether tile t reads stage s's block, and the parity of the next wait for it
-    // (Of warp 0) the segment to come, fetched when the one before it was taken, and the one after it in the list.
+    // (Of warp 0) the segment to come, requested when the one before it was taken (and looked at when it is needed), and the one after it in the list.
     Segment found;
     const int2 piece = as_piece(p, cta, found);
     int at_segment = piece.x + 1;
-    auto fetch = [&]() {
-      found.blocks = 0;
-#pragma unroll 1
-      while (at_segment <= piece.y && found.blocks == 0) found = as_segment(p, at_segment++);
+    auto request = [&]() {
+      if (at_segment <= piece.y) found = as_segment(p, at_segment++);
+      else found.blocks = 0;
     };
-    if (warp == 0 && found.blocks == 0) fetch();
     auto find_step = [&]() {
       int kind = SC_END;
+      bool keep = false;                       // whether the segment at hand is for tile B too, or for the step after this one
       // At most two segments: the second one if it is a request's few rows, as the first.
 #pragma unroll 1
       for (int t = 0; t < 2; ++t) {
+        if (t == 1 && !keep) request();
+#pragma unroll 1
+        while (found.blocks == 0 && at_segment <= piece.y) request();
         const Segment& g = found;
         const bool few = !g.shared && g.tokens * G <= AS_FOLD_ROWS;
         int block = g.block, blocks = g.blocks, tokens = g.tokens;
-        bool keep = false;                     // for tile B, or for the step after this one
+        keep = false;
         if (t == 0) {
           kind = blocks == 0 ? SC_END : g.tokens > per ? SC_BOTH : few ? SC_PARTS : SC_HALVES;
           if (kind == SC_HALVES) blocks = (blocks + 1) >> 1;
@@ -219,15 +221,16 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
           at[1] = make_int4(g.key_lo, g.key_hi, block, blocks);
           at[2] = make_int4(g.row_low, g.row_high, g.position, kind == SC_END ? SC_END : kind + (g.shared ? SC_SHARED : 0));
         }
-        if (!keep) fetch();
       }
       if (lane == 0) sc_publish(found_addr, seen + 1);
+      if (!keep) request();
       __syncwarp();
     };
     // The block to come: this half's first key, the keys of its part, lane i the id of the half's i-th page (-1: no page, or no key of the part in
     // it).  It is looked up before the one at hand is copied, across the ends of steps.
     int left0 = 0, left1 = 0, key0 = 0, key1 = 0, lo0 = 0, lo1 = 0, hi0 = 0, hi1 = 0, turn = 0;
-    int kb = 0, lo = 0, hi = 0, ids = -1;
+    int kb = 0, lo = 0, hi = 0, id = -1;
+    bool looked_up = false;                    // whether id has been read from the table; it is looked at a block later
     uint32_t tiles = 0;
     bool both = false, ok = true, more = true;
     const int* bt0 = nullptr;
@@ -238,7 +241,8 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
 #pragma unroll 1
     while (more && ok) {
       // ---- the block at hand is the one that was looked up; the one after it
-      const int kb_now = kb, lo_now = lo, hi_now = hi, ids_now = ids;
+      const int kb_now = kb, lo_now = lo, hi_now = hi, ids_now = looked_up && id >= 0 && id < p.num_pages ? id : -1;
+      if (looked_up && ids_now < 0) *holes = 1;                // before the block is handed over
       const uint32_t tiles_now = tiles;
       const uint8_t* head_now = head;
       if (left0 + left1 == 0) {
@@ -260,7 +264,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         ++seen;
         turn = 0;
       }
-      ids = -1;
+      looked_up = false;
       if (more) {
         const bool b = left0 == 0 || (turn && left1 > 0);
         turn = !b;
@@ -271,11 +275,8 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         left0 -= !b; left1 -= b;
         key0 += b ? 0 : AS_KEYS; key1 += b ? AS_KEYS : 0;
         const int key = kb + lane * size;
-        if (lane * size < 32 && key < hi && key + size > lo) {
-          const int id = bt[key >> shift];
-          if (id >= 0 && id < p.num_pages) ids = id;
-          else *holes = 1;                     // before the block is handed over
-        }
+        looked_up = lane * size < 32 && key < hi && key + size > lo;
+        if (looked_up) id = bt[key >> shift];
       }
       if (tiles_now == 0) continue;            // nothing at hand yet
       // ---- its stage: the tiles that read the last block there are through with it.  While that has to be waited for, whatever has been requested

@@ -85,6 +85,13 @@ __device__ __forceinline__ bool sc_wait(uint32_t bar, uint32_t parity, volatile 
   }
   return true;
 }
+// Whether a wait would be over, without any waiting.
+__device__ __forceinline__ bool sc_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
 // A count in shared memory that one thread raises when what it counts has been written, and the others wait for: more than n.
 __device__ __forceinline__ void sc_publish(uint32_t addr, int n) { asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(addr), "r"(n) : "memory"); }
 __device__ __forceinline__ bool sc_wait_count(uint32_t addr, int n, volatile int* abort_flag) {
@@ -226,6 +233,16 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       if (!keep) request();
       __syncwarp();
     };
+    // Tells the tiles that read them that the blocks in front of the `end`-th are there.
+    auto hand_over = [&](int end) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // visible to the tensor cores
+      __syncwarp();
+#pragma unroll 1
+      for (; handed < end; ++handed) {
+        if (lane < 2 && ((used >> (2 * stage_h + lane)) & 1u)) ta_mbar_arrive(full0 + 8u * (uint32_t)(lane * SC_BARS + stage_h));
+        if (++stage_h == stages) stage_h = 0;
+      }
+    };
     // The block to come: this half's first key, the keys of its part, lane i the id of the half's i-th page (-1: no page, or no key of the part in
     // it).  It is looked up before the one at hand is copied, across the ends of steps.
     int left0 = 0, left1 = 0, key0 = 0, key1 = 0, lo0 = 0, lo1 = 0, hi0 = 0, hi1 = 0, turn = 0;
@@ -280,26 +297,16 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       }
       if (tiles_now == 0) continue;            // nothing at hand yet
       // ---- its stage: the tiles that read the last block there are through with it.  While that has to be waited for, whatever has been requested
-      // is handed over; else the block before the one that was requested last.  (With one more in flight blocks come a block's time later: 64
-      // requests behind 8192 common keys 39.9 us against 38.9.)
+      // is handed over.
       const int s = stage_n;
       const uint32_t before = (used >> (2 * s)) & 3u, bar = empty0 + 8u * (uint32_t)((lane & 1) * SC_BARS + s);
       const bool mine = lane < 2 && ((before >> lane) & 1u);
       const uint32_t parity = (turns >> (2 * s + (lane & 1))) & 1u;
-      const bool wait = __any_sync(0xffffffffu, mine && !ta_mbar_try_wait(bar, parity));
-      const int keep = wait ? 0 : 1;
-      if (n - handed > keep) {
-        if (wait) asm volatile("cp.async.wait_group 0;" ::: "memory");
-        else asm volatile("cp.async.wait_group 1;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // visible to the tensor cores
-        __syncwarp();
-#pragma unroll 1
-        for (; n - handed > keep; ++handed) {
-          if (lane < 2 && ((used >> (2 * stage_h + lane)) & 1u)) ta_mbar_arrive(full0 + 8u * (uint32_t)(lane * SC_BARS + stage_h));
-          if (++stage_h == stages) stage_h = 0;
+      if (__any_sync(0xffffffffu, mine && !sc_test(bar, parity))) {
+        if (n > handed) {
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
+          hand_over(n);
         }
-      }
-      if (wait) {
         const bool go = !mine || sc_wait<true>(bar, parity, abort_flag, SC_ERR_KV_EMPTY);
         if (__any_sync(0xffffffffu, !go)) { ok = false; break; }
       }
@@ -308,41 +315,45 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       // ---- the copies.  Keys outside lo .. hi - 1 and of no page are filled with zeros.
       const uint32_t stage = ring + (uint32_t)s * L::KV_TILE;
       const bool inner = kb_now >= lo_now && kb_now + 32 <= hi_now;        // every key may be seen
+      const uint8_t* src[4];
+      uint32_t there = 0;                      // bit e: whether those eight rows' page is
 #pragma unroll
       for (int e = 0; e < 4; ++e) {            // eight rows at a time: they lie in one page
-        const int id = __shfl_sync(0xffffffffu, ids_now, (8 * e) >> bits), key = kb_now + 8 * e;
-        const uint8_t* src = head_now + (size_t)max(id, 0) * page_stride + (uint32_t)(key & (ps - 1)) * (uint32_t)(D * 2);
-        const uint32_t dst = stage + (uint32_t)e * 1024u;
-        if (inner) {
-          const uint32_t bytes = id >= 0 ? 16u : 0u;           // 0: sixteen zeros
+        const int of = __shfl_sync(0xffffffffu, ids_now, (8 * e) >> bits);
+        src[e] = head_now + (size_t)max(of, 0) * page_stride + (uint32_t)((kb_now + 8 * e) & (ps - 1)) * (uint32_t)(D * 2);
+        there |= of >= 0 ? 1u << e : 0u;
+      }
+      if (inner && there == 15u) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
 #pragma unroll
           for (int u = 0; u < 8 / RPI; ++u)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                         ::"r"(dst + swizzled[u]), "l"(src + RPI * u * (D * 2)), "r"(bytes) : "memory");
-        } else {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(stage + (uint32_t)e * 1024u + swizzled[u]), "l"(src[e] + RPI * u * (D * 2)) : "memory");
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
 #pragma unroll
           for (int u = 0; u < 8 / RPI; ++u) {
-            const int at = key + rp + RPI * u;
-            const uint32_t bytes = id >= 0 && at >= lo_now && at < hi_now ? 16u : 0u;
+            const int at = kb_now + 8 * e + rp + RPI * u;
+            const uint32_t bytes = (there >> e & 1u) && at >= lo_now && at < hi_now ? 16u : 0u;        // 0: sixteen zeros
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                         ::"r"(dst + swizzled[u]), "l"(src + RPI * u * (D * 2)), "r"(bytes) : "memory");
+                         ::"r"(stage + (uint32_t)e * 1024u + swizzled[u]), "l"(src[e] + RPI * u * (D * 2)), "r"(bytes) : "memory");
           }
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
       ++n;
       if (++stage_n == stages) stage_n = 0;
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncwarp();
-    if (ok) {
-#pragma unroll 1
-      for (; handed < n; ++handed) {
-        if (lane < 2 && ((used >> (2 * stage_h + lane)) & 1u)) ta_mbar_arrive(full0 + 8u * (uint32_t)(lane * SC_BARS + stage_h));
-        if (++stage_h == stages) stage_h = 0;
+      // ---- the block before it is handed over.  (With one or two more in flight blocks come that much later: 64 requests behind 8192 common keys
+      // 39.9 and 43.0 us against 38.9.)
+      if (n - handed > 1) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        hand_over(n - 1);
       }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (ok) hand_over(n);
   } else if (warp == 1 || warp == 3) {
     // ---- products, one thread a tile -------------------------------------------------------------------------------------------------
     const int t = warp == 1 ? 0 : 1;

@@ -329,3 +329,20 @@ def test_lengths_written_right_in_front(ops):
         if turn % 2:
             dev[6].fill_(-1)
         assert torch.equal(b.launch(ops, dev, torch.empty_like(dev[0])), alone if turn % 2 else want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_pages_behind_four_gigabytes(ops, dtype):
+    """The same keys at the beginning and at the end of pools whose offsets pass 32 bits: the same result."""
+    b = Batch(8, 2, 128, 16, [(0, 1, 193), (0, 3, 260), (-1, 5, 40), (0, 1, 400)], [192], dtype)
+    dev = b.device()
+    near = b.launch(ops, dev, torch.empty_like(dev[0]))
+    b.compare(near)
+    pages = dev[1].shape[0]
+    total = 2 ** 32 // (2 * 16 * 128 * dev[1].element_size()) + 2 * pages
+    k, v = torch.empty(total, 2, 16, 128, dtype=dtype, device="cuda"), torch.empty(total, 2, 16, 128, dtype=dtype, device="cuda")
+    k[-pages:], v[-pages:] = dev[1], dev[2]
+    k[:2 * pages], v[:2 * pages] = float("nan"), float("nan")
+    table = torch.where(dev[3] >= 0, dev[3] + (total - pages), dev[3]).to(torch.int32)
+    far = b.launch(ops, [dev[0], k, v, table] + dev[4:], torch.empty_like(dev[0]))
+    assert torch.equal(near, far)

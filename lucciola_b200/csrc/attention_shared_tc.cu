@@ -22,8 +22,9 @@
 // memory 1400 cycles at its full rate shared by all SMs, so rows that are not there cost nothing; one kernel for both kinds of work is what
 // lets the line be cut evenly.
 //
-// Warps: 0 and 4 copy keys, 2 and 5 values (cp.async, 16 bytes a thread, swizzled for the tensor cores; a warp has half of every block, and
-// two blocks in flight); 1 issues tile A's products and owns the tensor memory, 3 tile B's; 6..9 softmax of A, 10..13 of B.  Each goes through the
+// Warps: 0 and 3 copy keys, 2 and 5 values (cp.async, 16 bytes a thread, swizzled for the tensor cores; a warp has half of every block, two
+// blocks in flight, and a quarter of the SM that no other copying warp has: three groups of 11 behind 2352 keys 37.2 us against 39.1); 1 issues tile
+// A's products and owns the tensor memory, 4 tile B's; 6..9 softmax of A, 10..13 of B.  Each goes through the
 // segments, which warp 0 finds.  Barriers tell one turn from the next only, so each tile has barriers of its own for the stages of the rings, and a
 // copying warp speaks to the tiles that read a block.  All waits are bounded; when one gives up, the CTA records it and every role leaves.
 #include "attention_shared.cuh"
@@ -174,10 +175,10 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   // Where block i of tile t's part lies among the step's: A's and B's in turn, then what the longer part has more.
   auto place = [](int t, int i, int others, int kind) { return (kind & 3) == SC_BOTH ? i : i + min(t ? i + 1 : i, others); };
 
-  if (warp != 1 && warp != 3 && warp < SC_SOFTMAX) {
-    // ---- copies: warps 0 and 4 the halves of every block of keys, 2 and 5 of values -----------------------------------------------------
+  if (warp != 1 && warp != 4 && warp < SC_SOFTMAX) {
+    // ---- copies: warps 0 and 3 the halves of every block of keys, 2 and 5 of values -----------------------------------------------------
     const bool is_v = warp == 2 || warp == 5;
-    const int half = warp >= 4 ? 1 : 0;
+    const int half = warp >= 3 ? 1 : 0;
     constexpr int CHUNKS = D / 8, RPI = 32 / CHUNKS;           // 16-byte chunks of a row, rows an instruction
     const int c = lane % CHUNKS, rp = lane / CHUNKS;           // a lane copies chunk c of the rows rp, rp + RPI, ... of its half
     const uint8_t* pool = (const uint8_t*)(is_v ? p.v_cache : p.k_cache) + c * 16 + rp * (D * 2);
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (ok) hand_over(n);
-  } else if (warp == 1 || warp == 3) {
+  } else if (warp == 1 || warp == 4) {
     // ---- products, one thread a tile -------------------------------------------------------------------------------------------------
     const int t = warp == 1 ? 0 : 1;
     if (elect_one()) {

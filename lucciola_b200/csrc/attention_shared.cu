@@ -5,7 +5,7 @@
 // cached head).  Queries, a block of 64 keys and its values lie in shared memory as 32-bit numbers.  256 threads: thread (ty, tx) has
 // rows 2 ty and 2 ty + 1; of the scores the keys tx, tx + 16, tx + 32, tx + 48, of the result the dimensions 4 tx + 64 c .. + 3.  Sixteen
 // threads share a row: its maximum and sum are four shuffles.  Bound by the multiplications: 32 requests behind 4096 common keys, 32 heads of
-// 128 on 8 in 32 bits, 243 us (2.2 GFLOP, 9 TFLOP/s); 6 requests behind 1000, 16 heads of 64 on 4, with plan and combination 15.9 us, most of it
+// 128 on 8 in 32 bits, 246 us (2.2 GFLOP, 9 TFLOP/s); 6 requests behind 1000, 16 heads of 64 on 4, with plan and combination 15.9 us, most of it
 // three kernels' beginnings and ends.
 #include "attention_shared.cuh"
 
@@ -165,8 +165,8 @@ __global__ void __launch_bounds__(AP_THREADS) attention_shared_plain_kernel(Shar
   }
 }
 
-// The plan of a step: every CTA makes all of it, and writes a part.  A chain of lookups, not bytes: 3.3 us at 2 requests, 4.4 at 64, 8.4 at 32 of
-// which one has 2048 new tokens.
+// The plan of a step: every CTA makes all of it, and writes a part.  A chain of lookups, not bytes: 5 us at 2 requests and at 32, 7 to 8 where one of them has 2048
+// new tokens (plan after plan; in front of the attention a part of it is hidden).
 __global__ void __launch_bounds__(AS_PLAN_THREADS) as_plan_kernel(SharedParams p, int ctas) {
   __shared__ SharedPlan pl;
   pdl_trigger();

@@ -50,10 +50,11 @@ _RECORD_PORTIONS = 4
 # a long portion of which few are wanted.
 _ALL_ROWS = 64
 # Requests that begin with the same pages go through the kernels for shared prefixes when these spare so many elements of keys in a layer (8 kv heads
-# of 128: 16 K keys).  Requests of 8 kv heads of 128, each with a new token, us a layer ordinarily and with the keys read once: 16 behind 512 common
-# keys (8 M elements) 13.5 and 16.2, 16 behind 1024 (16 M) 18.4 and 17.1, 16 behind 2048 (31 M) 27.5 and 18.6, 32 behind 4096 (130 M) 80 and 28; and the
-# plan, 4 us a step.  In 32 bits the keys are read once by better kernels in any case.
-SHARED_ELEMENTS = 1 << 24
+# of 128: 8 K keys).  Requests of 8 kv heads of 128, each with a new token, us a layer ordinarily and with the keys read once: 4 behind 2048 common
+# keys (6 M elements) 12.3 and 12.6, 16 behind 512 (8 M) 13.5 and 13.8, 4 behind 4096 (13 M) 17.0 and 15.1, 16 behind 2048 (31 M) 26.9 and 15.0, 32
+# behind 4096 (130 M) 80 and 24; and the plan, 5 us a step.  (Many requests behind few keys gain least: 32 behind 512, 16 M, 16.4 and 21.2.)  In 32 bits
+# the keys are read once by better kernels in any case.
+SHARED_ELEMENTS = 1 << 23
 
 
 def _elements_saved(prefix_of: Sequence[int], prefix_lens: Sequence[int], a_key: int) -> int:

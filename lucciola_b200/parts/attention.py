@@ -27,7 +27,7 @@ from .rope import NeighbourRotary
 # Entries with at least this many tokens in a step go to the tensor-memory attention kernel (128-row tiles).
 BIG_PORTION = 16
 # Portions of more tokens stay with their own kernel although other requests of the step share prefixes: 16 requests behind 2048 common tokens, heads of
-# 128, one of them with 512 new tokens, take 73 us by either way; with 2048 new tokens 168 us on the ordinary kernels, 313 on those for shared prefixes.
+# 128, one of them with 512 new tokens, take 73 us on the ordinary kernels and 58 on those for shared prefixes; with 2048 new tokens 166 and 228.
 SHARED_PORTION = 512
 # Query rows (heads of a group x tokens) of a tile of the mma.sync kernels; tiles of at most DECODE_ROWS rows have
 # a kernel of their own, which a launch uses only if all of its tiles are such.
@@ -161,8 +161,8 @@ class GQAttention(Mixer):
     def _attend_shared(self, q: torch.Tensor, step: StepContext, cache: KVCacheView) -> bool:
         """Whether the kernels for requests that share prefixes take this step.  Where they run on the tensor cores: unless there is a
         portion of a prompt that the kernel for such takes and that has more than SHARED_PORTION tokens.  Where they do not: if the other
-        choice is the plain kernel (32 tokens behind 4096 common keys, 32 heads on 8: float32 heads of 128 243 us against 3381, bfloat16
-        heads of 256 172 against 4308; but bfloat16 heads of 96 239 against 80 on the mma.sync kernels)."""
+        choice is the plain kernel (32 tokens behind 4096 common keys, 32 heads on 8: float32 heads of 128 246 us against 3382, bfloat16
+        heads of 256 169 against 4305; but bfloat16 heads of 96 239 against 80 on the mma.sync kernels)."""
         nq, nkv, d = self.num_heads, self.num_kv_heads, self.head_dim
         if step.prefix_of is None or self.window != 0 or not ops.attention_shared_ok(step.num_seqs, d, self.scale):
             return False

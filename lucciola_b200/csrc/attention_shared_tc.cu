@@ -52,8 +52,10 @@ template <int D> struct ScLayout {
 // What the two tiles work on side by side, a part each: halves of one segment's blocks, segments of two requests, or (both) the same blocks
 // with other rows.  The parts' blocks alternate in the rings of keys and values, so that neither tile waits for the other's to pass.
 // Warp 0, which copies keys, makes steps of the CTA's segments, one ahead of its copies, and leaves them in a ring; the others read them there.
-// A slot comes again after SC_SEGMENTS steps: the rings of keys and values hold warp 0 back to a handful in front of whoever is last (a step
-// has a block at least, and a tile's next step waits for the one before).
+// A slot comes again after SC_SEGMENTS steps.  The rings of keys and values do not hold warp 0 back for a tile that the steps leave out (tile B has
+// no block of a segment of one block, nor beside a request's few rows without a partner: 83 such steps in a row at 256 requests in pairs behind
+// 64 keys, 32 kv heads).  So every warp that reads the steps gives each half of the ring back when it is through with it, and warp 0 waits for all of them
+// before it writes that half again.  It cannot wait for itself: the steps of that half lie SC_SEGMENTS / 2 behind, and all their blocks are handed over.
 struct ScPart {                          // a Segment, and
   int kv_head, request, first, tokens;   // tokens 0: nothing for this tile
   int key_lo, key_hi, block, blocks;     // blocks 0 of a part with tokens: it leaves an empty partial result
@@ -62,7 +64,8 @@ struct ScPart {                          // a Segment, and
 };
 struct ScStep { ScPart part[2]; };
 enum : int { SC_END = 0, SC_PARTS = 1, SC_BOTH = 2, SC_HALVES = 3, SC_SHARED = 4 };      // of either part
-constexpr int SC_SEGMENTS = 32;
+constexpr int SC_SEGMENTS = 32, SC_SEGMENTS_HALF = SC_SEGMENTS / 2;
+constexpr int SC_STEP_READERS = 13;      // warps 1 to 13
 
 __device__ __forceinline__ void sc_tmem_ld16(uint32_t taddr, uint32_t* r) {
   asm volatile(
@@ -119,6 +122,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(16) ScStep steps[SC_SEGMENTS];
   __shared__ int steps_found;
+  __shared__ unsigned long long steps_read[2];                // barriers of the ring's halves
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = ta_smem_u32(smem);
   const uint32_t bars = sbase + L::BAR_OFF;
@@ -144,6 +148,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       for (int b = 0; b < 2; ++b) { ta_mbar_init(s_full(t, b), 1); ta_mbar_init(p_full(t, b), 4); ta_mbar_init(pv_done(t, b), 1); }
       ta_mbar_init(q_full(t), 4); ta_mbar_init(o_free(t), 4);
     }
+    for (int h = 0; h < 2; ++h) ta_mbar_init(ta_smem_u32(&steps_read[h]), SC_STEP_READERS);
     *abort_flag = 0;
     *holes = 0;
     steps_found = 0;
@@ -171,6 +176,11 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     g.key_lo = b.x; g.key_hi = b.y; g.block = b.z; g.blocks = b.w;
     g.row_low = c.x; g.row_high = c.y; g.position = c.z; g.kind = c.w;
     return g.kind != SC_END;
+  };
+  auto half_read = [&](int n) { return ta_smem_u32(&steps_read[(n / SC_SEGMENTS_HALF) & 1]); };      // of step n's half
+  // One thread of a reading warp that needs no step in front of the n-th any more: where that ends a half, the half goes back.
+  auto give_back = [&](int n) {
+    if (n > 0 && n % SC_SEGMENTS_HALF == 0) ta_mbar_arrive(half_read(n - 1));
   };
   // Where block i of tile t's part lies among the step's: A's and B's in turn, then what the longer part has more.
   auto place = [](int t, int i, int others, int kind) { return (kind & 3) == SC_BOTH ? i : i + min(t ? i + 1 : i, others); };
@@ -202,6 +212,10 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       else found.blocks = 0;
     };
     auto find_step = [&]() {
+      if (seen >= SC_SEGMENTS && seen % SC_SEGMENTS_HALF == 0) {
+        const bool go = sc_wait<true>(half_read(seen), (uint32_t)(seen / SC_SEGMENTS - 1) & 1u, abort_flag, SC_ERR_SEGMENT);
+        if (__any_sync(0xffffffffu, !go)) return;              // nothing is found: step() sees the flag
+      }
       int kind = SC_END;
       bool keep = false;                       // whether the segment at hand is for tile B too, or for the step after this one
       // At most two segments: the second one if it is a request's few rows, as the first.
@@ -282,6 +296,8 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         bt0 = p.table + (size_t)g.request * p.max_pages;
         head0 = pool + (size_t)g.kv_head * ps * (D * 2);
         ++seen;
+        __syncwarp();
+        if (warp != 0 && lane == 0) give_back(seen);
         turn = 0;
       }
       looked_up = false;
@@ -370,6 +386,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       ScPart g, other;
 #pragma unroll 1
       for (int seen = 0; ok && step(seen, t, g) && step(seen, t ^ 1, other); ++seen) {
+        give_back(seen + 1);
         const int all = (g.kind & 3) == SC_BOTH ? g.blocks : g.blocks + other.blocks;
         if (g.blocks > 0) ok = sc_wait<false>(q_full(t), (uint32_t)(segments & 1), abort_flag, SC_ERR_Q);
         // S(i) = Q K(i)^T into S buffer (mine + i) & 1, then O += P V(i - 1): S(i + 1) overwrites P(i - 1), whose product the tensor cores finish first
@@ -422,30 +439,25 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
     int at_step = -1, blocks = 0, block_key = 0, lo = 0, hi = 0, hi_all = 0, mine = 0;
     bool valid = false, warp_valid = false, folded = false, ok = true;
     float m_ref = -INFINITY, l_run = 0.f;
-    int done = -1;                             // the step of the part before
+    bool pending = false;                      // whether the result of the step before has yet to be written
 #pragma unroll 1
     for (;;) {
-      // ---- this tile's next part with blocks, if there is one: its queries are requested, whole rows side by side
-      bool more = true;
+      // ---- the next step.  If this tile's part has blocks, its queries are requested, whole rows side by side.
       ScPart g;
       int from = -1;                           // this row's place among all rows of the queries
-#pragma unroll 1
-      for (;;) {
-        more = step(++at_step, t, g);
-        if (!more) break;
-        if (g.tokens == 0) continue;
-        if (g.blocks > 0) break;
-        // the second half of a single block: an empty partial result
+      const bool more = step(++at_step, t, g);
+      blocks = more ? g.blocks : 0;
+      const bool work = blocks > 0;
+      if (more && !work && r < g.tokens * G) { // the second half of a single block: an empty partial result
         const long long tile = (long long)(uint32_t)g.row_low | (long long)g.row_high << 32;
-        if (r < g.tokens * G) *reinterpret_cast<float2*>(p.part_ml + (tile + g.tokens * G + r) * 2) = make_float2(-INFINITY, 0.f);
+        *reinterpret_cast<float2*>(p.part_ml + (tile + g.tokens * G + r) * 2) = make_float2(-INFINITY, 0.f);
       }
-      if (more) {
+      if (work) {
         const int first = (g.kind & 3) == SC_BOTH ? t * per : 0, lane_rows = min(g.tokens - first, per) * G;
         folded = !(g.kind & SC_SHARED) && g.tokens * G <= AS_FOLD_ROWS;
         const int row = folded ? lane : r;     // of this tile's
         valid = row < lane_rows;
         warp_valid = folded || quarter * 32 < lane_rows;
-        blocks = g.blocks;
         lo = g.key_lo;
         block_key = (lo & ~(AS_KEYS - 1)) + g.block * AS_KEYS;
         hi = 0x7fffffff;
@@ -467,18 +479,18 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
                            "l"((const uint8_t*)p.q + (size_t)row_at * (D * 2) + c * 16) : "memory");
         }
       }
-      if (more) {                              // all products with the last part's queries are done: S of this part may come while that one's O is read
+      if (work) {                              // all products with the last part's queries are done: S of this part may come while that one's O is read
         asm volatile("cp.async.wait_all;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) ta_mbar_arrive(q_full(t));
       }
-      // ---- the part before it: its result is written
-      if (done >= 0) {
+      // ---- the part of the step before, if it had blocks: its result is written before any later step is looked at
+      if (pending) {
         ok = sc_wait<false>(pv_done(t, (mine - 1) & 1), (uint32_t)(((mine - 1) >> 1) & 1), abort_flag, SC_ERR_O_FULL);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const volatile ScPart* was = &steps[done % SC_SEGMENTS].part[t];
+        const volatile ScPart* was = &steps[(at_step - 1) % SC_SEGMENTS].part[t];
         const int tile_rows = was->tokens * G, kind = was->kind & 3;
         const long long tile = (long long)(uint32_t)was->row_low | (long long)was->row_high << 32;
         const bool fold = !(was->kind & SC_SHARED) && tile_rows <= AS_FOLD_ROWS;
@@ -504,8 +516,11 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         __syncwarp();
         if (lane == 0) ta_mbar_arrive(o_free(t));
       }
+      __syncwarp();
+      if (lane == 0) give_back(at_step);
       if (!more) break;
-      done = at_step;
+      pending = work;
+      if (!work) continue;
       // ---- its blocks
       m_ref = -INFINITY;
       l_run = 0.f;

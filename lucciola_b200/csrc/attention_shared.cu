@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(AS_PLAN_THREADS) as_plan_kernel(SharedParams p
       const int c0 = (int)((unsigned)base / (unsigned)span), c1 = (int)((unsigned)(b1 - 1) / (unsigned)span);
 #pragma unroll 1
       for (int c = c0 + (by_tile ? 0 : mine); c <= c1; c += step) {
-        const int x0 = c * span, x1 = min(x0 + span, total);
+        const int x0 = c * span, x1 = (int)min((unsigned)x0 + (unsigned)span, (unsigned)total);
         // a block belongs to the CTA in whose piece it begins
         const int block = max(x0 - b0 + two, 0) >> two, blocks = max(min(max(min(x1, b1) - b0 + two, 0) >> two, there) - block, 0);
         const int at = kv * pl.tiles + tile + c;
@@ -285,8 +285,6 @@ static bool as_params(SharedParams& p, SharedCut& cut, int& ctas, int dtype, int
   AS_CHECK(page_size > 0 && max_pages > 0 && (long long)max_pages * page_size < (1ll << 31) - 64, "attention_shared: tables of %d pages of %d tokens",
            max_pages, page_size);
   AS_CHECK((long long)num_tokens * num_q_heads < (1ll << 30), "attention_shared: %d tokens of %d heads", num_tokens, num_q_heads);
-  ctas = as_sms();
-  AS_CHECK(ctas > 0, "attention_shared: no device");
   cut = as_cut(dtype, num_q_heads / num_kv_heads, head_dim, page_size);
   p = SharedParams{};
   p.T = num_tokens; p.S = num_seqs; p.heads = num_q_heads; p.kv_heads = num_kv_heads * cut.share; p.group = cut.group; p.dim = head_dim;
@@ -297,11 +295,13 @@ static bool as_params(SharedParams& p, SharedCut& cut, int& ctas, int dtype, int
   // 38.5, 36.8 and 18.2.
   p.min_span = cut.tc ? 5 : 1; p.tile_start = cut.tc ? 3 : 0; p.folds = cut.tc;
   for (int b = 0; b < 31; ++b) if ((1 << b) == page_size) p.page_shift = b;
-  // units of the whole line, at most
-  const long long tiles = 2ll * ((long long)num_tokens / p.tile_tokens + num_seqs), blocks = (long long)max_pages * page_size / AS_KEYS + 1;
-  AS_CHECK(tiles * (2 * blocks + 2) * p.kv_heads < (1ll << 31) - 65536, "attention_shared: %d tokens of %d requests on tables of %d pages are too much for one launch",
+  // units of the whole line, at most (as_tile_units; places in the line are 32-bit numbers, an end of a CTA's piece may lie a piece further)
+  const long long tiles = 2ll * ((long long)num_tokens / p.tile_tokens + num_seqs), blocks = ((long long)max_pages * page_size + AS_KEYS - 1) / AS_KEYS;
+  AS_CHECK(tiles * (2 * blocks + p.tile_start) * p.kv_heads < (1ll << 31) - 65536, "attention_shared: %d tokens of %d requests on tables of %d pages are too much for one launch",
            num_tokens, num_seqs, max_pages);
   AS_CHECK(p.kv_heads <= 65535, "attention_shared: %d kv heads", p.kv_heads);
+  ctas = as_sms();
+  AS_CHECK(ctas > 0, "attention_shared: no device");
 #undef AS_CHECK
   return true;
 }

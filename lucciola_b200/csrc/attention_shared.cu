@@ -272,10 +272,10 @@ static cudaError_t as_combine(const SharedParams& p, cudaStream_t stream) {
 }
 
 
-// What all launches of one call have in common; false with the library's message when the arguments are refused.
-static bool as_params(SharedParams& p, SharedCut& cut, int& ctas, int dtype, int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
-                      int page_size, int max_pages) {
 #define AS_CHECK(cond, ...) do { if (!(cond)) { set_error(__VA_ARGS__); return false; } } while (0)
+// What all launches of one call have in common; false with the library's message when the sizes are refused.
+static bool as_sizes(SharedParams& p, SharedCut& cut, int dtype, int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
+                      int page_size, int max_pages) {
   AS_CHECK(valid_dtype(dtype), "attention_shared: unknown element type %d", dtype);
   AS_CHECK(num_tokens >= 0 && num_seqs >= 0 && num_seqs <= AS_MAX_SEQS, "attention_shared: %d tokens of %d requests, at most %d requests",
            num_tokens, num_seqs, AS_MAX_SEQS);
@@ -300,11 +300,17 @@ static bool as_params(SharedParams& p, SharedCut& cut, int& ctas, int dtype, int
   AS_CHECK(tiles * (2 * blocks + p.tile_start) * p.kv_heads < (1ll << 31) - 65536, "attention_shared: %d tokens of %d requests on tables of %d pages are too much for one launch",
            num_tokens, num_seqs, max_pages);
   AS_CHECK(p.kv_heads <= 65535, "attention_shared: %d kv heads", p.kv_heads);
-  ctas = as_sms();
-  AS_CHECK(ctas > 0, "attention_shared: no device");
-#undef AS_CHECK
   return true;
 }
+// The same on the current device.
+static bool as_params(SharedParams& p, SharedCut& cut, int& ctas, int dtype, int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
+                      int page_size, int max_pages) {
+  if (!as_sizes(p, cut, dtype, num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, max_pages)) return false;
+  ctas = as_sms();
+  AS_CHECK(ctas > 0, "attention_shared: no device");
+  return true;
+}
+#undef AS_CHECK
 
 static void as_plan_parts(SharedParams& p, int* plan, int ctas) {
   const SharedPlanLayout at(p.T, p.S, p.kv_heads, p.tile_tokens, ctas);
@@ -313,6 +319,13 @@ static void as_plan_parts(SharedParams& p, int* plan, int ctas) {
 }
 
 }  // namespace lb
+
+// 0 if calls of these sizes are taken, else 1 with the message; needs no GPU.
+LB_EXPORT int lb_attention_shared_refused(int dtype, int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int page_size, int max_pages) {
+  lb::SharedParams p;
+  lb::SharedCut cut;
+  return lb::as_sizes(p, cut, dtype, num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, max_pages) ? 0 : 1;
+}
 
 // Elements that a call needs: of the plan (int32) and of the partial results (float32).
 LB_EXPORT int lb_attention_shared_sizes(int dtype, int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int page_size,

@@ -126,6 +126,7 @@ _SIGNATURES = {
                              c_void_p],
     "lb_attention_shared": [c_int] + [c_void_p] * 6 + [c_longlong] + [c_void_p] * 4 + [c_int] * 8 + [c_float, c_void_p, c_longlong, c_void_p],
     "lb_attention_shared_plan": [c_int, c_void_p, c_longlong] + [c_void_p] * 4 + [c_int] * 7 + [c_void_p],
+    "lb_attention_shared_refused": [c_int] * 8,
     "lb_attention_shared_sizes": [c_int] * 8 + [c_void_p, c_void_p],
     "lb_latent_flash": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                         c_float, c_void_p, c_int, c_int, c_void_p, c_longlong, c_void_p],
@@ -1498,8 +1499,15 @@ def _check_lengths(device: int, S: int, *lengths: torch.Tensor) -> None:
 
 
 def attention_shared_ok(num_seqs: int, head_dim: int, scale: float) -> bool:
-    """The sizes that attention_shared takes."""
-    return num_seqs <= 512 and head_dim % 8 == 0 and 0 < head_dim <= 256 and scale > 0
+    """The requests and heads that attention_shared takes."""
+    return num_seqs <= 512 and head_dim % 8 == 0 and 0 < head_dim <= 256 and 0 < scale < 1e30
+
+
+@functools.lru_cache(maxsize=4096)
+def attention_shared_fits(dtype: torch.dtype, num_tokens: int, num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
+                          pages_a_seq: int) -> bool:
+    """Whether attention_shared takes a step of these sizes (many requests on tables of millions of keys are too much for one launch)."""
+    return _invoke("lb_attention_shared_refused", dtype_code(dtype), num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, pages_a_seq) == 0
 
 
 def attention_shared_tensor_cores(dtype: torch.dtype, num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int) -> bool:

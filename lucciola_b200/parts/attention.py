@@ -173,7 +173,8 @@ class GQAttention(Mixer):
     def _attend(self, q: torch.Tensor, out: torch.Tensor, step: StepContext, cache: KVCacheView) -> None:
         """The attention of the step's queries: where requests begin with the same pages, these are read once for all of them."""
         nq, nkv, d = self.num_heads, self.num_kv_heads, self.head_dim
-        if self._attend_shared(q, step, cache):
+        if self._attend_shared(q, step, cache) and ops.attention_shared_fits(q.dtype, q.shape[0], step.num_seqs, nq, nkv, d, cache.page_size,
+                                                                             step.block_tables[cache.group].shape[1]):
             table = step.block_tables[cache.group]
             key = ("shared prefixes", nq, nkv, d, cache.page_size, cache.group)       # one plan for all layers with these sizes
             plan = step.memo.get(key)

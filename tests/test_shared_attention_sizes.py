@@ -33,3 +33,21 @@ def test_the_line_of_blocks_fits_32_bits(seqs, kv_heads, page):
     for pages in range(max(lo - 4, 1), lo + 1):
         tiles = 2 * (tokens // 256 + seqs)
         assert tiles * (3 + 2 * -(-pages * page // 64)) * kv_heads < 2 ** 31
+
+
+@pytest.mark.parametrize("pages,shared", [(1 << 13, True), (1 << 17, False)])
+def test_a_step_that_is_too_much_for_a_launch_takes_the_ordinary_kernels(monkeypatch, pages, shared):
+    """512 requests of 64 kv heads on tables of 2^17 and of 2^21 keys: the second step is none that attention_shared takes."""
+    from types import SimpleNamespace as N
+    from lucciola_b200.parts.attention import GQAttention
+    called = []
+    monkeypatch.setattr(ops, "attention", lambda *a, **k: called.append("ordinary"))
+    monkeypatch.setattr(ops, "shared_plan", lambda *a, **k: called.append("plan"))
+    monkeypatch.setattr(ops, "attention_shared", lambda *a, **k: called.append("shared"))
+    part = N(num_heads=64, num_kv_heads=64, head_dim=128, window=0, scale=0.1, plan_key=lambda: ("attention tiles", 1), rt=N(stream=0))
+    part._attend_shared = lambda *a: GQAttention._attend_shared(part, *a)
+    q = torch.empty(512, 64, 128, dtype=torch.bfloat16)
+    step = N(prefix_of=q, prefix_lens=q, num_seqs=512, max_q_len=1, cu_tokens=None, context_lens=None, memo={}, plans={},
+             block_tables=[torch.empty(512, 1, dtype=torch.int32).expand(512, pages)])
+    GQAttention._attend(part, q, q, step, N(page_size=16, group=0, k=None, v=None))
+    assert called == (["plan", "shared"] if shared else ["ordinary"])

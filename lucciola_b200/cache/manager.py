@@ -14,7 +14,7 @@ device_cache.py.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Optional, Hashable, Sequence
 
 from ..parts.base import KVPages, StateSlot
@@ -67,8 +67,20 @@ class _RequestCache:
     tables: list[list[int]]          # per group: page of each logical page index, NO_PAGE once released
     length: int = 0                  # tokens whose keys are (or are about to be) in the cache
     version: int = 0                 # new, manager-wide unique number whenever a table changes (lets callers cache a converted copy)
-    family: int = 0                  # requests with the same number (not 0) have their first pages in common,
-    common: int = 0                  # this one so many of them with the family's first (-1: it is the first, all)
+    cuts: set[int] = field(default_factory=set)      # numbers of first pages that it has, or had, in common with others
+
+
+@dataclass(eq=False)
+class _Alike:
+    """Requests of a step (by their places in it) that have their first pages in common, and the groups chosen among them."""
+    members: list[int]
+    spared: int                      # pages that need not be read again
+    groups: list[tuple[list[int], int]]              # members and pages
+    rest: list[int]                  # members of no group
+
+
+# Keys that attention reads at a time (ops.attention_shared): a group with fewer in common reads nothing less.
+_BLOCK_KEYS = 64
 
 
 class CacheManager:
@@ -81,7 +93,8 @@ class CacheManager:
         self._free_slots = list(range(num_slots - 1, -1, -1))
         self._requests: dict[Hashable, _RequestCache] = {}
         self._versions = 0
-        self._families = 0
+        self._shares = 0                 # changes whenever a request takes over pages, or one that has some in common with others ends
+        self._groups_of: tuple = (None, None, None)          # requests, self._shares and the answer of the last prefix_groups
 
     # ---- requests ------------------------------------------------------
     def has_request(self, rid: Hashable) -> bool:
@@ -104,6 +117,7 @@ class CacheManager:
     def release(self, rid: Hashable) -> None:
         """Give back everything a request holds (it ended or is preempted)."""
         rc = self._requests.pop(rid)
+        self._shares += bool(rc.cuts)
         for g, table in enumerate(rc.tables):
             for p in table:
                 if p != NO_PAGE:
@@ -129,41 +143,68 @@ class CacheManager:
             for p in table[:pages]:
                 self.pools[g].share(p)
             rc.tables[g].extend(table[:pages])
-        if not dc.family:
-            self._families += 1
-            dc.family, dc.common = self._families, -1
-        rc.family, rc.common = dc.family, pages if dc.common < 0 else min(pages, dc.common)
+        # Whoever has these pages has them as its first: a page has the same place in all tables.
+        last = dc.tables[0][pages - 1]
+        for other in self._requests.values():
+            if len(other.tables[0]) >= pages and other.tables[0][pages - 1] == last:
+                other.cuts.add(pages)
+        rc.cuts |= {c for c in dc.cuts if c < pages}
+        self._shares += 1
         rc.length = pages * self.page_size
         self._versions += 1
         rc.version = self._versions
 
     def prefix_groups(self, rids: Sequence[Hashable]) -> Optional[tuple[list[int], list[int]]]:
         """Which of these requests begin with the same pages: for each the place in the list of the request whose pages stand for
-        its group's (-1: no group), and for that one how many tokens the group has in common (0 for the others).  Of a family's
-        requests those form a group for which (members x common pages) is largest.  None when there is no group."""
-        families: dict[int, list[int]] = {}
+        its group's (-1: no group), and for that one how many tokens the group has in common (0 for the others).  Where requests share a
+        short beginning and some of them a long one, there are as many groups as spare most keys.  None when there is no group."""
+        rids = tuple(rids)
+        if self._groups_of[:2] != (rids, self._shares):
+            self._groups_of = rids, self._shares, self._find_groups(rids)
+        found = self._groups_of[2]
+        return None if found is None else (list(found[0]), list(found[1]))
+
+    def _find_groups(self, rids: Sequence[Hashable]) -> Optional[tuple[list[int], list[int]]]:
+        # Requests with the same page in front of a cut have all pages up to there in common.  Two sets of such requests are one inside the
+        # other, or have nobody in common: a tree, in which a deeper set has more pages.
+        sets: dict[tuple[int, int], list[int]] = {}
         for i, rid in enumerate(rids):
             rc = self._requests.get(rid)
-            if rc is not None and rc.family:
-                families.setdefault(rc.family, []).append(i)
-        found: Optional[tuple[list[int], list[int]]] = None
-        for members in families.values():
-            if len(members) < 2:
-                continue
-            whole = max(self._requests[rids[i]].length // self.page_size for i in members)
-            common = {i: whole if self._requests[rids[i]].common < 0 else self._requests[rids[i]].common for i in members}
-            # the family's first request has as many pages in common as anybody else has with it: cut where another's end
-            cuts = sorted({common[i] for i in members if self._requests[rids[i]].common >= 0})
-            pages = max(cuts, key=lambda c: sum(common[i] >= c for i in members) * c if sum(common[i] >= c for i in members) > 1 else 0)
-            group = [i for i in members if common[i] >= pages]
-            if len(group) < 2:
-                continue
-            if found is None:
-                found = [-1] * len(rids), [0] * len(rids)
-            for i in group:
-                found[0][i] = group[0]
-            found[1][group[0]] = pages * self.page_size
-        return found
+            if rc is not None and rc.cuts:
+                rc.cuts = {c for c in rc.cuts if self.pools[0].holders(rc.tables[0][c - 1]) > 1}
+                for c in rc.cuts:
+                    sets.setdefault((c, rc.tables[0][c - 1]), []).append(i)
+        innermost: dict[int, _Alike] = {}                     # of each member the last set that went by
+        for (pages, _), members in sorted(sets.items(), key=lambda kv: -kv[0][0]):
+            if len(members) > 1:
+                below = {id(innermost[i]): innermost[i] for i in members if i in innermost}
+                node = self._alike(pages, members, [i for i in members if i not in innermost], list(below.values()))
+                innermost.update(dict.fromkeys(members, node))
+        groups = [g for node in {id(n): n for n in innermost.values()}.values() for g in node.groups]
+        if not groups:
+            return None
+        prefix_of, prefix_lens = [-1] * len(rids), [0] * len(rids)
+        for members, pages in groups:
+            leader = min(members)
+            prefix_lens[leader] = pages * self.page_size
+            for i in members:
+                prefix_of[i] = leader
+        return prefix_of, prefix_lens
+
+    def _alike(self, pages: int, members: list[int], direct: list[int], below: list["_Alike"]) -> "_Alike":
+        """The best of three for a set of requests: the groups of the sets in it alone; all in one group; a group of those whom these
+        leave over (and of sets whose members gain more that way), if they have a block of the kernels' in common."""
+        groups = [g for n in below for g in n.groups]
+        best = _Alike(members, sum(n.spared for n in below), groups, direct + [i for n in below for i in n.rest])
+        whole = (len(members) - 1) * pages
+        if whole > best.spared:
+            best = _Alike(members, whole, [(members, pages)], [])
+        kept = [n for n in below if n.spared + len(n.rest) * pages >= len(n.members) * pages]
+        rest = direct + [i for n in below for i in (n.rest if n in kept else n.members)]
+        spared = sum(n.spared for n in kept) + (len(rest) - 1) * pages
+        if kept and len(rest) > 1 and pages * self.page_size >= _BLOCK_KEYS and spared > best.spared:
+            best = _Alike(members, spared, [g for n in kept for g in n.groups] + [(rest, pages)], [])
+        return best
 
     # ---- pages ---------------------------------------------------------
     def _first_needed_page(self, g: int, start: int) -> int:

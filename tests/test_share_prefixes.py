@@ -268,3 +268,96 @@ def test_elements_that_groups_spare():
     from lucciola_b200.engine.step import _elements_saved
     assert _elements_saved([0, 0, -1, 3, 0, 3], [32, 0, 0, 16, 0, 0], 10) == (2 * 32 + 1 * 16) * 10
     assert _elements_saved([-1, -1], [0, 0], 10) == 0
+
+
+def documents(m, first, docs, pages, each):
+    """`docs` documents of `pages` pages that begin with the same `first` pages, `each` requests behind every one: (rid, document)."""
+    out = []
+    for d in range(docs):
+        for i in range(each):
+            rid = (d, i)
+            m.admit(rid)
+            if i:
+                m.share_prefix(rid, (d, 0), pages)
+            elif d and first:
+                m.share_prefix(rid, (0, 0), first)
+            m.extend(rid, pages * PS + 1 + i)
+            out.append((rid, d))
+    return out
+
+
+@pytest.mark.parametrize("first", [0, 1, 4, 16, 50])
+def test_documents_behind_a_common_beginning(first):
+    """Requests on several long documents, all of which begin with the same system prompt: a group for every document, with all that its
+    requests have in common."""
+    m = manager(pages=4000, slots=40)
+    rids = documents(m, first, 4, 64, 8)
+    random.Random(first).shuffle(rids)
+    of, lens = m.prefix_groups([r for r, _ in rids])
+    for i, (_, d) in enumerate(rids):
+        leader = of[i]
+        assert leader >= 0 and rids[leader][1] == d and lens[leader] == 64 * PS
+    assert sum(n > 0 for n in lens) == 4
+    m.release((2, 0))
+    of, lens = m.prefix_groups([r for r, _ in rids if r != (2, 0)])
+    assert sorted(lens)[-4:] == [64 * PS] * 4 and of.count(-1) == 0
+
+
+def test_what_deeper_groups_leave_over():
+    """Two requests on a document each and six more behind the system prompt alone: these share the system prompt, if it is a block long."""
+    for first, grouped in ((20, True), (15, False)):
+        m = manager(pages=4000, slots=40)
+        rids = [r for r, _ in documents(m, first, 2, 200, 2)]
+        for i in range(6):
+            m.admit(i)
+            m.share_prefix(i, (0, 0), first)
+            m.extend(i, first * PS + 3)
+            rids.append(i)
+        of, lens = m.prefix_groups(rids)
+        assert of == [0, 0, 2, 2] + ([4] * 6 if grouped else [-1] * 6)
+        assert lens == [200 * PS, 0, 200 * PS, 0] + ([first * PS] if grouped else [0]) + [0] * 5
+
+
+def spared(m, rids, groups):
+    of, lens = groups
+    return sum((of.count(r) - 1) * n for r, n in enumerate(lens) if n)
+
+
+def test_groups_of_nested_families():
+    """Random trees of shared beginnings: groups name pages that their members share, and spare no less than one group of the best length would;
+    the answer is the same when it is asked for again, and follows requests that end."""
+    rng = random.Random(11)
+    for turn in range(150):
+        m = CacheManager([CacheGroup(2, 16, 0, (0,))], PS, 3000, 24)
+        alive = []
+        for i in range(24):
+            m.admit(i)
+            if alive and rng.random() < 0.85:
+                donor = rng.choice(alive)
+                full = m.length(donor) // PS
+                m.share_prefix(i, donor, rng.choice([full, max(1, full // 2), rng.randint(1, full)]))
+            m.extend(i, m.length(i) + rng.choice([rng.randint(PS, 30), rng.randint(100, 300)]))
+            alive.append(i)
+            if rng.random() < 0.1:
+                m.release(alive.pop(rng.randrange(len(alive))))
+            if rng.random() < 0.3:
+                m.prefix_groups(alive)
+        rng.shuffle(alive)
+        groups = m.prefix_groups(alive)
+        tables = [m.block_table(i, 0) for i in alive]
+        one = 0
+        for t in tables:
+            for n in range(1, len(t) + 1):
+                k = sum(u[:n] == t[:n] for u in tables)
+                if k > 1:
+                    one = max(one, (k - 1) * n * PS)
+        assert (groups is None) == (one == 0)
+        if groups is None:
+            continue
+        assert spared(m, alive, groups) >= one
+        assert m.prefix_groups(list(alive)) == groups
+        for i, leader in enumerate(groups[0]):
+            if leader >= 0:
+                n = groups[1][leader] // PS
+                assert groups[0][leader] == leader and n > 0 and tables[i][:n] == tables[leader][:n]
+                assert min(j for j, x in enumerate(groups[0]) if x == leader) == leader

@@ -30,6 +30,7 @@ from dataclasses import dataclass
 from typing import Callable, Hashable, Iterable, Optional, Sequence
 
 from ..cache.manager import CacheManager
+from .prefixes import PrefixTree
 from .request import Request, Status
 
 
@@ -59,6 +60,9 @@ class Scheduler:
         self.waiting: deque[Request] = deque()
         self.running: list[Request] = []
         self._admissions = 0
+        self._prefixes = PrefixTree(manager.page_size)         # of the running requests, with share_prefixes
+        self._changes = 0                      # requests that were admitted or ended, and portions that were computed
+        self._blocked: Optional[tuple] = None  # the request that had to wait for pages, self._changes then, and how many it needs
         # counters
         self.num_preemptions = 0
         self.num_steps = 0
@@ -135,6 +139,7 @@ class Scheduler:
     def _preempt(self, r: Request) -> None:
         self._release(r.rid)
         self.running.remove(r)
+        self._forget(r)
         r.status = Status.WAITING
         r.num_computed = 0
         r.preemptions += 1
@@ -145,38 +150,33 @@ class Scheduler:
         self._release(r.rid)
         if r in self.running:
             self.running.remove(r)
+            self._forget(r)
         r.status, r.finish_reason = Status.FINISHED, reason
 
     # ---- requests that begin alike ---------------------------------------------
-    @staticmethod
-    def _alike(a: Sequence[int], b: Sequence[int]) -> int:
-        """With how many equal tokens both begin."""
-        n = min(len(a), len(b))
-        if a[:n] == b[:n]:
-            return n
-        lo, hi = 0, n                          # a[:lo] == b[:lo], a[:hi] != b[:hi]
-        while hi - lo > 1:
-            mid = (lo + hi) // 2
-            if a[lo:mid] == b[lo:mid]:
-                lo = mid
-            else:
-                hi = mid
-        return lo
+    def _forget(self, r: Request) -> None:
+        """A request that does not run any more."""
+        self._prefixes.remove(r.rid)
+        self._changes += 1
 
     def _donor(self, r: Request) -> tuple[Optional[Request], int, bool]:
         """The running request with which r has the most whole pages in common that have been computed, how many, and whether another
         one is still computing more."""
         ps = self.manager.page_size
         best, pages, more = None, 0, 0
-        for d in self.running:
-            if d.tokens[0] != r.tokens[0]:
-                continue
-            alike = min(self._alike(r.tokens, d.tokens), r.length - 1)
-            have = min(alike, d.num_computed) // ps
-            if have > pages:
-                best, pages = d, have
-            if d.remaining > 1:
-                more = max(more, alike // ps)
+        seen: set[Hashable] = set()
+        for run, alike in reversed(self._prefixes.walk(r.tokens, (r.length - 1) // ps)):       # those with most in common first
+            for d in run.holders.values():
+                if d.rid in seen:
+                    continue
+                seen.add(d.rid)
+                have = min(alike, d.num_computed // ps)
+                if have > pages:
+                    best, pages = d, have
+                if d.remaining > 1:
+                    more = max(more, alike)
+            if pages >= alike:
+                break                          # nobody else has as much
         return best, pages, more > pages
 
     # ---- one step ------------------------------------------------------------
@@ -251,12 +251,16 @@ class Scheduler:
         while self.waiting and not blocked and budget > 0 and len(self.running) < self.max_num_seqs:
             r = self.waiting[0]
             donor, pages = None, 0
-            if self.share_prefixes and self.running:
+            if self.share_prefixes:
+                # It had to wait for pages, and since then nobody began, ended or computed what it could take over.
+                if self._blocked is not None and self._blocked[:2] == (r.rid, self._changes) and not self._fits(self._blocked[2], reserved):
+                    break
                 donor, pages, more = self._donor(r)
                 if more:
                     break
             need = self._pages_needed(r, r.length)
             if not self._fits([k - pages for k in need], reserved):
+                self._blocked = r.rid, self._changes, [k - pages for k in need]
                 break
             if donor is not None:
                 self.manager.admit(r.rid)
@@ -270,6 +274,9 @@ class Scheduler:
             r.admitted_at = self._admissions
             self._admissions += 1
             self.running.append(r)
+            if self.share_prefixes:
+                self._prefixes.add(r)
+                self._changes += 1
             take(r, n)
             if n < most:
                 budget = 0
@@ -286,10 +293,14 @@ class Scheduler:
         for s in plan:
             r = s.request
             r.num_computed += s.num_tokens
+            if s.num_tokens > 1 or not s.sample:
+                self._changes += 1
             if not s.sample:
                 continue
             tok = int(next(it))
             r.append(tok)
+            if self.share_prefixes and r.status is Status.RUNNING and r.length % self.manager.page_size == 0:
+                self._prefixes.add(r)
             reason = None
             if tok in self.eos_token_ids and not r.params.ignore_eos:
                 reason = "stop"

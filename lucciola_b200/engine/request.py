@@ -15,7 +15,7 @@ class Status(enum.Enum):
     FINISHED = "finished"
 
 
-@dataclass
+@dataclass(eq=False)                   # a request is itself: lists of them are searched in every step
 class Request:
     rid: int
     prompt: list[int]

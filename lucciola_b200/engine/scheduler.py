@@ -215,7 +215,7 @@ class Scheduler:
         preempted = False
         # 1. Requests that decode: one token each, whatever the budget says.
         for r in sorted((r for r in self.running if r.remaining == 1), key=lambda r: r.admitted_at):
-            if r not in self.running:
+            if r.status is not Status.RUNNING:
                 continue                      # it was a victim a moment ago
             need = self._pages_needed(r, r.num_computed + 1)
             while not self._fits(need, reserved):
@@ -226,7 +226,7 @@ class Scheduler:
                 preempted = True
                 if victim is r:
                     break
-            if r in self.running:
+            if r.status is Status.RUNNING:
                 take(r, 1, need)
 
         # 2. Prompts under way (and requests that are recomputed), oldest first.  After a preemption

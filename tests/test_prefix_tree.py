@@ -147,3 +147,11 @@ def test_requests_that_ended_leave_the_tree():
     assert b.status is Status.RUNNING and len(s._prefixes) == 1
     s.abort(1)
     assert len(s._prefixes) == 0 and s._prefixes.num_runs() == 0
+
+
+def test_requests_are_themselves():
+    """Searching the running requests looks at no tokens: two requests of the same content are two."""
+    a, b = request(0, [Token(1)] * 5), request(0, [Token(1)] * 5)
+    Token.compared = 0
+    assert a != b and a in [b, a] and a not in [b] and len({a, b}) == 2
+    assert Token.compared == 0

@@ -18,7 +18,7 @@ What it decides differently:
   * A request that could never fit the pool on its own is refused when it is added.
   * With `share_prefixes` set, a request that is admitted while a running one begins with the same tokens takes over the whole pages
     of these that have been computed (all but its last token, at most) and starts behind them.  While the running one is still
-    computing tokens that both begin with, the request waits for them.
+    computing tokens that both begin with, the request waits for them, and those behind it that do not may pass.
   * With `token_tile` set, a portion that is not its prompt's last is shortened so that the step's tokens up to and
     including it are a multiple of the tile: the many-token products work on tiles of 128 tokens, and 32 decoded tokens
     beside a portion of 512 make them compute five tiles for 4.25 tiles of tokens.
@@ -42,6 +42,10 @@ class Scheduled:
     sample: bool           # the portion reaches the request's last token: sample after the step
 
 
+# Requests that a step may find to wait for a beginning that is being computed, before it looks no further.
+_LOOK_PAST = 8
+
+
 class Scheduler:
     def __init__(self, manager: CacheManager, max_tokens_per_step: int, max_num_seqs: int, max_model_len: int,
                  prefill_chunk: int = 0, eos_token_ids: Iterable[int] = (),
@@ -62,6 +66,8 @@ class Scheduler:
         self._admissions = 0
         self._prefixes = PrefixTree(manager.page_size)         # of the running requests, with share_prefixes
         self._changes = 0                      # requests that were admitted or ended, and portions that were computed
+        self._awaited: dict[Hashable, tuple[Request, int, int]] = {}       # by request: the one that computes what it waits for, the
+                                               # latter's admission, and how many pages that is
         self._blocked: Optional[tuple] = None  # the request that had to wait for pages, self._changes then, and how many it needs
         # counters
         self.num_preemptions = 0
@@ -97,6 +103,7 @@ class Scheduler:
         for r in list(self.waiting):
             if r.rid == rid:
                 self.waiting.remove(r)
+                self._awaited.pop(rid, None)
                 r.status, r.finish_reason = Status.FINISHED, "abort"
                 return True
         return False
@@ -161,9 +168,9 @@ class Scheduler:
 
     def _donor(self, r: Request) -> tuple[Optional[Request], int, bool]:
         """The running request with which r has the most whole pages in common that have been computed, how many, and whether another
-        one is still computing more."""
+        one is still computing more (self._awaited says which)."""
         ps = self.manager.page_size
-        best, pages, more = None, 0, 0
+        best, pages, awaited, more = None, 0, None, 0
         seen: set[Hashable] = set()
         for run, alike in reversed(self._prefixes.walk(r.tokens, (r.length - 1) // ps)):       # those with most in common first
             for d in run.holders.values():
@@ -173,11 +180,22 @@ class Scheduler:
                 have = min(alike, d.num_computed // ps)
                 if have > pages:
                     best, pages = d, have
-                if d.remaining > 1:
-                    more = max(more, alike)
+                if d.remaining > 1 and alike > more:
+                    awaited, more = d, alike
             if pages >= alike:
                 break                          # nobody else has as much
+        if more > pages:
+            self._awaited[r.rid] = awaited, awaited.admitted_at, more
         return best, pages, more > pages
+
+    def _waits(self, r: Request) -> bool:
+        """Whether what r was found to wait for is still being computed."""
+        if r.rid in self._awaited:
+            d, admitted_at, pages = self._awaited[r.rid]
+            if d.status is Status.RUNNING and d.admitted_at == admitted_at and d.remaining > 1 and d.num_computed // self.manager.page_size < pages:
+                return True
+            del self._awaited[r.rid]
+        return False
 
     # ---- one step ------------------------------------------------------------
     def schedule(self) -> list[Scheduled]:
@@ -248,16 +266,24 @@ class Scheduler:
         # 3. New requests, first come first served, while there is budget and a slot.  A request is
         # admitted only when the pages for all it has to run (its prompt, and what it had generated
         # before a preemption) are free now: admitting it earlier would only get it preempted again.
-        while self.waiting and not blocked and budget > 0 and len(self.running) < self.max_num_seqs:
-            r = self.waiting[0]
+        at = found_to_wait = 0
+        while at < len(self.waiting) and not blocked and budget > 0 and len(self.running) < self.max_num_seqs and found_to_wait < _LOOK_PAST:
+            r = self.waiting[at]
             donor, pages = None, 0
             if self.share_prefixes:
+                # Whoever waits for a beginning lets the next ones pass.  These do not make it wait longer: one that has more in common with it
+                # than has been computed would wait for the same.
+                if self._waits(r):
+                    at += 1
+                    continue
                 # It had to wait for pages, and since then nobody began, ended or computed what it could take over.
                 if self._blocked is not None and self._blocked[:2] == (r.rid, self._changes) and not self._fits(self._blocked[2], reserved):
                     break
                 donor, pages, more = self._donor(r)
                 if more:
-                    break
+                    at += 1
+                    found_to_wait += 1
+                    continue
             need = self._pages_needed(r, r.length)
             if not self._fits([k - pages for k in need], reserved):
                 self._blocked = r.rid, self._changes, [k - pages for k in need]
@@ -269,7 +295,7 @@ class Scheduler:
                 self.num_shared_tokens += r.num_computed
             most = min(budget, self.prefill_chunk or budget, r.remaining)
             n = self._aligned(most, r, budget)
-            self.waiting.popleft()
+            del self.waiting[at]
             r.status = Status.RUNNING
             r.admitted_at = self._admissions
             self._admissions += 1

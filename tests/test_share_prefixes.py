@@ -192,6 +192,69 @@ def test_a_request_waits_for_a_beginning_that_is_being_computed():
     assert seen == [[(0, 0, 8)], [(0, 8, 8)], [(0, 16, 8)], [(0, 24, 5)], [(0, 29, 1), (1, 28, 1)]]
 
 
+def test_others_pass_a_request_that_waits_for_a_beginning():
+    """Behind a request that waits for a prompt that is being computed stand one that waits for the same and two that share nothing: these
+    start at once, and the waiting ones as soon as the beginning is there."""
+    m = manager(pages=200, slots=8)
+    s = Scheduler(m, 16, 8, 200, prefill_chunk=8, share_prefixes=True)
+    prompt = list(range(1, 30))
+    for i, p in enumerate([prompt, prompt, [60, 61, 62], prompt[:25], [70, 71]]):
+        s.add_request(Request(i, list(p), SamplingParams(max_new_tokens=9)))
+    seen = []
+    for _ in range(6):
+        plan = s.schedule()
+        seen.append([(e.request.rid, e.start, e.num_tokens) for e in plan])
+        for e in plan:
+            if not m.has_request(e.request.rid):
+                m.admit(e.request.rid)
+            m.extend(e.request.rid, e.start + e.num_tokens)
+        s.update(plan, [5] * sum(e.sample for e in plan))
+    assert seen[0] == [(0, 0, 8), (2, 0, 3), (4, 0, 2)]
+    assert seen[1] == [(2, 3, 1), (4, 2, 1), (0, 8, 8)]
+    assert seen[3] == [(2, 5, 1), (4, 4, 1), (0, 24, 5), (3, 24, 1)]         # what 3 waits for is there; 1 waits for one page more
+    assert seen[4] == [(0, 29, 1), (2, 6, 1), (4, 5, 1), (3, 25, 1), (1, 28, 1)]
+
+
+def test_many_that_wait_are_not_looked_for_in_every_step(monkeypatch):
+    """A hundred requests that wait for the same prompt: each is looked for once while it is computed, a few a step."""
+    m = manager(pages=400, slots=200)
+    s = Scheduler(m, 4, 200, 200, share_prefixes=True)
+    looked = []
+    donor = Scheduler._donor
+    monkeypatch.setattr(Scheduler, "_donor", lambda self, r: looked.append(r.rid) or donor(self, r))
+    for i in range(100):
+        s.add_request(Request(i, list(range(60)), SamplingParams(max_new_tokens=2)))
+    steps = 0
+    while s.running[0].num_computed < 56 if s.running else True:
+        run = s.schedule()
+        steps += 1
+        assert [e.request.rid for e in run] == [0]
+        for e in run:
+            if not m.has_request(0):
+                m.admit(0)
+            m.extend(0, e.start + e.num_tokens)
+        s.update(run, [])
+    assert len(looked) == len(set(looked)) <= 8 * steps
+    assert s.abort(99) and 99 not in s._awaited
+    n = drive_on(s, m)
+    assert n == 100 - 1
+
+
+def drive_on(s, m):
+    """To the end, with token 5 every time; how many requests ended."""
+    ended = 0
+    while s.has_unfinished():
+        plan = s.schedule()
+        for e in plan:
+            if not m.has_request(e.request.rid):
+                m.admit(e.request.rid)
+            assert m.extend(e.request.rid, e.start + e.num_tokens)
+        ended += sum(done for _, _, done in s.update(plan, [5] * sum(e.sample for e in plan)))
+        m.check_invariants()
+    assert not s._awaited
+    return ended
+
+
 def test_the_last_token_of_a_prompt_is_always_computed():
     m = manager()
     s = Scheduler(m, 64, 4, 200, share_prefixes=True)

@@ -50,11 +50,26 @@ _RECORD_PORTIONS = 4
 # a long portion of which few are wanted.
 _ALL_ROWS = 64
 # Requests that begin with the same pages go through the kernels for shared prefixes when these spare so many elements of keys in a layer (8 kv heads
-# of 128: 8 K keys).  Requests of 8 kv heads of 128, each with a new token, us a layer ordinarily and with the keys read once: 4 behind 2048 common
-# keys (6 M elements) 12.3 and 12.6, 16 behind 512 (8 M) 13.5 and 13.8, 4 behind 4096 (13 M) 17.0 and 15.1, 16 behind 2048 (31 M) 26.9 and 15.0, 32
-# behind 4096 (130 M) 80 and 24; and the plan, 5 us a step.  (Many requests behind few keys gain least: 32 behind 512, 16 M, 16.4 and 21.2.)  In 32 bits
-# the keys are read once by better kernels in any case.
+# of 128: 8 K keys), in 32 bits always (the keys are read once by better kernels there).  In a step of single tokens it has to be more the more requests and
+# groups there are, whose rows and first blocks cost their part.  8 kv heads of 128, 100 keys of their own, keys not in L2, us a layer ordinarily and
+# with the keys read once, the plan (5 us a step) apart:
+#     one group, behind         512            1024           2048           4096               16 groups of 2, behind 1024: 26 and 33, 2048: 46 and 44
+#      4 requests           7.4 and 12.9    9.8 and 13.1   12.0 and 13.2   16.8 and 14.9        8 groups of 8, behind 256: 22 and 26, 512: 31 and 29
+#     16 requests          12.7 and 13.8   17.3 and 14.1   26.3 and 15.2   44.6 and 16.6        128 groups of 2, behind 512: 114 and 125, 1024: 179 and 162
+#     32 requests          15.4 and 21.2   24.6 and 20.5   42.8 and 22.4   79.6 and 23.8
+#     64 requests          30.9 and 23.3   49.0 and 23.0   85.5 and 25.2
+# Of 281 such steps (heads of 64 and 128, 1 to 16 kv heads, 2 to 256 requests, 256 to 8192 keys in common) the rule takes the slower way in 14 by more than
+# 8 %; a border of 8 M alone did in 39.  Beside a portion of a prompt the ordinary kernels lose more: 4 requests behind 2048, one with 64 new tokens, 34 and 21.
 SHARED_ELEMENTS = 1 << 23
+
+
+def _worth_sharing(prefix_of: Sequence[int], prefix_lens: Sequence[int], heads: int, a_key: int, single_tokens: bool) -> bool:
+    """Whether the kernels for shared prefixes are the faster ones for these groups of a step, with so many kv heads and elements a key."""
+    border = SHARED_ELEMENTS
+    if single_tokens:
+        groups = sum(n > 0 for n in prefix_lens)
+        border *= 1 + min(len(prefix_of), 40) / 27 + groups * heads / 107
+    return _elements_saved(prefix_of, prefix_lens, a_key) >= border
 
 
 def _elements_saved(prefix_of: Sequence[int], prefix_lens: Sequence[int], a_key: int) -> int:
@@ -149,7 +164,9 @@ class ModelRunner:
         self.cache = DeviceCache(requests, self.groups, self.page_size, counts, options.max_num_seqs, rt.act_dtype, self.device)
         self.max_pages_per_seq = -(-self.max_model_len // self.page_size)
         self._any_window = any(g.window > 0 for g in self.groups)
-        self._key_elements = max([r.num_kv_heads * r.head_dim for r in requests if isinstance(r, KVPages) and not r.shared], default=0)      # of a key in a layer
+        # kv heads and elements of a key, in the layer with most
+        self._key_elements, self._key_heads = max([(r.num_kv_heads * r.head_dim, r.num_kv_heads) for r in requests if isinstance(r, KVPages) and not r.shared],
+                                                  default=(0, 0))
         if options.share_prefixes and (self.state_cache_ids or not self.manager.can_share()):
             raise ValueError("share_prefixes needs a model that keeps the keys and values of all tokens, and nothing else, of a request")
         self._arange_cache = np.arange(512, dtype=np.int32)
@@ -385,7 +402,7 @@ class ModelRunner:
         # entries that own no page (their keys and values are written nowhere and they attend to nothing).
         # Requests that begin with the same pages; steps with and without such are recorded apart.
         shared = self.manager.prefix_groups([e.rid for e in entries]) if self.options.share_prefixes else None
-        if shared and self.rt.fast_kernels and _elements_saved(*shared, self._key_elements) < SHARED_ELEMENTS:
+        if shared and self.rt.fast_kernels and not _worth_sharing(*shared, self._key_heads, self._key_elements, max(q_lens) == 1):
             shared = None
         shape = self._shape_of(entries, q_lens, max_ctx)
         if shape is not None and shared:

@@ -424,3 +424,33 @@ def test_groups_of_nested_families():
                 n = groups[1][leader] // PS
                 assert groups[0][leader] == leader and n > 0 and tables[i][:n] == tables[leader][:n]
                 assert min(j for j, x in enumerate(groups[0]) if x == leader) == leader
+
+
+@pytest.mark.parametrize("groups,members,prefix,heads,dim,single,faster", [
+    # what was measured, see SHARED_ELEMENTS
+    (1, 4, 2048, 8, 128, True, False), (1, 4, 4096, 8, 128, True, True), (1, 16, 512, 8, 128, True, False), (1, 16, 1024, 8, 128, True, True),
+    (1, 32, 512, 8, 128, True, False), (1, 32, 1024, 8, 128, True, True), (1, 64, 512, 8, 128, True, True), (1, 32, 512, 8, 128, False, True),
+    (16, 2, 1024, 8, 128, True, False), (16, 2, 2048, 8, 128, True, True), (8, 8, 256, 8, 128, True, False), (8, 8, 512, 8, 128, True, True),
+    (128, 2, 512, 8, 128, True, False), (128, 2, 1024, 8, 128, True, True), (128, 2, 256, 16, 128, True, False), (16, 2, 1024, 8, 64, True, False),
+    (16, 2, 4096, 8, 64, True, True), (1, 2, 8192, 8, 128, True, False)])
+def test_steps_take_the_faster_way(groups, members, prefix, heads, dim, single, faster):
+    from lucciola_b200.engine import step
+    of = [s // members * members for s in range(groups * members)]
+    lens = [0 if s % members else prefix for s in range(groups * members)]
+    assert step._worth_sharing(of, lens, heads, heads * dim, single) == faster
+
+
+def test_the_runner_asks_which_way_is_faster(monkeypatch):
+    r = runner(monkeypatch)
+    asked = []
+    monkeypatch.setattr(packing.step_mod, "_worth_sharing", lambda *a: asked.append(a) or len(asked) > 1)
+    r.rt.fast_kernels = True
+    r.step([StepEntry("a", list(range(40)), (39,))])
+    r.manager.admit("b")
+    r.manager.share_prefix("b", "a", 2)
+    r.step([StepEntry("b", [1, 2], (1,)), StepEntry("a", [3], (0,))])
+    assert r.model.groups is None
+    r.step([StepEntry("a", [3], (0,)), StepEntry("b", [1], (0,))])
+    assert r.model.groups == ([0, 0], [32, 0])
+    heads = r.groups[0].num_kv_heads
+    assert asked == [([0, 0], [32, 0], heads, heads * r.groups[0].head_dim, False), ([0, 0], [32, 0], heads, heads * r.groups[0].head_dim, True)]

@@ -73,12 +73,24 @@ constexpr unsigned SF_WAIT_CYCLES = 2000000000u;
 __device__ __forceinline__ void sf_expect(unsigned long long* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(bar)), "r"(bytes) : "memory");
 }
-// Bounded (about a second): a wait that runs out is recorded, and the row goes on with what there is.
+// A CTA one of whose waits ran out records it and leaves the row's token as it is.  Not at once: its peers may still write to its shared memory or
+// read there.  They get no more values from it, so that each of them ends, or gives up its next wait and comes here too; until then a peer passes the
+// cluster's barrier SF_BARRIERS times at most, which this CTA passes with it, and then once more.  (CTAs that have ended count as arrived.)
+constexpr int SF_BARRIERS = 10;          // between two exchanges of values: one a digit of top_k's border, three of the short way in front of them
+__device__ __noinline__ void sf_leave() {
+  g_sampling_error = 1;
+#pragma unroll 1
+  for (int i = 0; i <= SF_BARRIERS; ++i) sf_cluster_sync();
+  asm volatile("exit;");
+}
+// By all threads of a CTA, bounded (about a second); a barrier of the CTA too.
 __device__ __forceinline__ void sf_wait(unsigned long long* bar, uint32_t parity) {
   const uint32_t at = (uint32_t)__cvta_generic_to_shared(bar);
   const unsigned t0 = (unsigned)clock();
+  bool lost = false;
   while (!sf_try_wait(at, parity))
-    if ((unsigned)clock() - t0 > SF_WAIT_CYCLES) { g_sampling_error = 1; break; }
+    if ((unsigned)clock() - t0 > SF_WAIT_CYCLES) { lost = true; break; }
+  if (__syncthreads_or(lost)) sf_leave();
 }
 __device__ __forceinline__ void sf_st_remote(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ uint32_t sf_ld_remote(uint32_t addr) {

@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
   __shared__ __align__(16) ScStep steps[SC_SEGMENTS];
   __shared__ int steps_found;
   __shared__ unsigned long long steps_read[2];                // barriers of the ring's halves
+  __shared__ unsigned long long products_done[2];             // of the tiles: all products there are
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = ta_smem_u32(smem);
   const uint32_t bars = sbase + L::BAR_OFF;
@@ -148,7 +149,7 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
       for (int b = 0; b < 2; ++b) { ta_mbar_init(s_full(t, b), 1); ta_mbar_init(p_full(t, b), 4); ta_mbar_init(pv_done(t, b), 1); }
       ta_mbar_init(q_full(t), 4); ta_mbar_init(o_free(t), 4);
     }
-    for (int h = 0; h < 2; ++h) ta_mbar_init(ta_smem_u32(&steps_read[h]), SC_STEP_READERS);
+    for (int h = 0; h < 2; ++h) { ta_mbar_init(ta_smem_u32(&steps_read[h]), SC_STEP_READERS); ta_mbar_init(ta_smem_u32(&products_done[h]), 1); }
     *abort_flag = 0;
     *holes = 0;
     steps_found = 0;
@@ -426,6 +427,9 @@ __global__ void __launch_bounds__(SC_THREADS, 1) attention_shared_tc_kernel(Shar
         mine += g.blocks;
         if (g.blocks > 0) ++segments;
       }
+      // Whatever ended this (the line, or a wait that ran out), the CTA's memory is given away behind its last product.
+      ta_commit(ta_smem_u32(&products_done[t]));
+      ta_mbar_drain(ta_smem_u32(&products_done[t]), 0);
     }
   } else {
     // ---- softmax: thread = query row; warp w reads lanes (w % 4) * 32 .. + 31 of tensor memory ---------------------------------------------

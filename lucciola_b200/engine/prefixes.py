@@ -67,6 +67,7 @@ class PrefixTree:
                 if at < below.end:
                     below = self._split(below, at)
             below.holders[r.rid] = r
+            self._join(run)
             run = below
         self._last[r.rid] = run
 
@@ -86,18 +87,25 @@ class PrefixTree:
             above, page = run.above, self._page(run.tokens, run.start)
             if not run.holders:
                 del above.below[page]
-            elif len(run.below) == 1:
-                (only,) = run.below.values()
-                if len(only.holders) == len(run.holders):      # nobody ends between the two
-                    only.start, only.above = run.start, above
-                    above.below[page] = only
+            else:
+                self._join(run)
             run = above
+
+    def _join(self, run: _Run) -> None:
+        """A run behind which only one lies, with the same holders, becomes a part of that one."""
+        if run is not self._root and len(run.below) == 1:
+            (only,) = run.below.values()
+            if len(only.holders) == len(run.holders):
+                only.start, only.above = run.start, run.above
+                run.above.below[self._page(run.tokens, run.start)] = only
 
     def __len__(self) -> int:
         """Requests that are in the tree."""
         return len(self._last)
 
     def num_runs(self) -> int:
-        def under(run: _Run) -> int:
-            return sum(1 + under(b) for b in run.below.values())
-        return under(self._root)
+        n, runs = 0, list(self._root.below.values())
+        while runs:
+            n += 1
+            runs.extend(runs.pop().below.values())
+        return n

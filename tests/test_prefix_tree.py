@@ -155,3 +155,22 @@ def test_requests_are_themselves():
     Token.compared = 0
     assert a != b and a in [b, a] and a not in [b] and len({a, b}) == 2
     assert Token.compared == 0
+
+
+def test_requests_that_grow_alike_stay_one_run():
+    tree = PrefixTree(PS)
+    rs = [request(i, range(10)) for i in range(3)]
+    for n in range(10, 400):
+        for r in rs:
+            tree.add(r)
+            r.append(n)
+        assert tree.num_runs() == 1
+    rs[0].append(-1)
+    for n in range(8):
+        for r in rs:
+            r.append(n)
+            tree.add(r)
+    assert tree.num_runs() == 3
+    assert tree.walk(rs[1].tokens, 90)[-1][1] == 90
+    tree.remove(0)
+    assert tree.num_runs() == 1

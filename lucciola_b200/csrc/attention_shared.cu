@@ -4,9 +4,10 @@
 // A tile has up to 32 query rows (tokens x heads of a kv head's group; a group of more heads is cut into equal parts that read the same
 // cached head).  Queries, a block of 64 keys and its values lie in shared memory as 32-bit numbers.  256 threads: thread (ty, tx) has
 // rows 2 ty and 2 ty + 1; of the scores the keys tx, tx + 16, tx + 32, tx + 48, of the result the dimensions 4 tx + 64 c .. + 3.  Sixteen
-// threads share a row: its maximum and sum are four shuffles.  Bound by the multiplications: 32 requests behind 4096 common keys, 32 heads of
-// 128 on 8 in 32 bits, 246 us (2.2 GFLOP, 9 TFLOP/s); 6 requests behind 1000, 16 heads of 64 on 4, with plan and combination 15.9 us, most of it
-// three kernels' beginnings and ends.
+// threads share a row: its maximum and sum are four shuffles.  Bound by a block's copy and its products, which take turns, and by reads of shared memory (a
+// thread reads six 16-byte words for 32 multiplications): 32 requests behind 4096 common keys, 32 heads of 128 on 8 in 32 bits, 246 us (2.2 GFLOP,
+// 9 TFLOP/s of the pipes' 70 or so); 6 requests behind 1000, 16 heads of 64 on 4, with plan and combination 15.9 us, most of it three kernels'
+// beginnings and ends.
 #include "attention_shared.cuh"
 
 #include <atomic>

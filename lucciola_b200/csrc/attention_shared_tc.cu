@@ -12,9 +12,9 @@
 //
 // What bounds it: the way of a block through barriers, tensor memory and registers.  A block that both tiles work on takes 2080 cycles, of
 // which the tensor cores are at work for 1000 and the exponentials take 1024 (two warps a quarter of the SM); taking the exponentials out
-// leaves 1800.  64 requests with a token each behind 8192 common keys, up to 256 keys of their own, 32 heads of 128 on 8: 25 us of the 37.7 that
+// leaves 1800.  64 requests with a token each behind 8192 common keys, up to 256 keys of their own, 32 heads of 128 on 8: 25 us of the 38.5 that
 // the call takes (plan 4.4, combination 6 to 8; recorded), 66 MB read; by the counters the tensor cores are busy for 26 % of the cycles (41 % on
-// the SMs that have the prefix), the issue slots for 38 %, DRAM for 25 %.  8 requests: 21.6 us in all; 2 requests behind 256: 13.9.
+// the SMs that have the prefix), the issue slots for 38 %, DRAM for 25 %.  8 requests: 22.2 us in all; 2 requests behind 256: 14.3.
 // Where only one tile works on a block, the copying warps set the pace, 1300 to 1500 cycles a block: their instructions, not the memory (copies that
 // read nothing take as long), which is why their loop looks nothing up that it waits for and makes all addresses before the first copy.
 //

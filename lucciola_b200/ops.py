@@ -1557,8 +1557,8 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     through its own.  All of these are device values, read by the kernels, so that a recorded step is replayed with other groups and
     lengths.  Page ids outside the pool are not there: a row that sees no key gives zeros, and rows of q that belong to no request
     (behind cu_tokens[S]) leave the output as it was.  Where cu_tokens fall, all of the output stays as it was.
-    Keys and values past a request's end may be anything; those of its own later tokens have to be finite (they are multiplied by
-    weights of 0).  S is at most 512, a head a multiple of 8 up to 256.  max_q_len, the most tokens of a request, is there for the
+    Keys and values that no request of the step has may be anything; those of a request's own later tokens, and of a prefix that is longer
+    than what some member sees, have to be finite (they are multiplied by weights of 0).  S is at most 512, a head a multiple of 8 up to 256.  max_q_len, the most tokens of a request, is there for the
     kernels' relatives, which need it: nothing here depends on it.
 
     `plan`: what shared_plan() made of these lengths, groups and sizes; without it the call makes one.  Partial results go through memory
